@@ -5,9 +5,9 @@ A generation cache in pages: ``k, v`` ``(P, H, S, 64)`` and ``b`` ``(P, H, S, 32
 a dict of plain values; its ``"kind"`` names the operator:
 
 * ``write``   -- new positions of every sequence into the pages: position ``start[n] + m`` for ``m < count[n]``;
-* ``decode``  -- one new token per sequence against its cached positions, ``s_j = q.k_j / 8 + lam exp(min(g - g_j, 0))
-                 (c.b_j) + (F - F_j)``, ``out = softmax(s) v``; with ``tracked``, the token's softmax weights are added
-                 to every position's accumulated weight;
+* ``decode``  -- one new token per sequence against its cached positions, ``s_j = q.k_j / 8 + lam exp(g - g_j) (c.b_j) +
+                 (F - F_j)``, ``out = softmax(s) v``; with ``tracked``, the token's softmax weights are added to every
+                 position's accumulated weight;
 * ``weights`` -- what each position of a prompt has received: the sum, over the last ``window`` queries of the sequence
                  (0: all of them), of the softmax weights that they give it;
 * ``evict``   -- a cache cut down to ``keep`` positions per head: the last ``recent`` ones and, of the others, those of
@@ -273,7 +273,7 @@ def _decode(s):
     N, n = s["case"]["longest"], s["lengths"].long()
     there = (torch.arange(N, device=DEVICE) < n[:, None])[:, None, None]
     k, v, b, g, f = (_rows_of(s["pages"][x], s["table"])[:, :, :N].float() for x in ("k", "v", "b", "g", "f"))
-    decay = torch.exp((s["g"] - g).clamp(max=0.0))[:, :, None]
+    decay = torch.exp(s["g"] - torch.where(there[:, :, 0], g, s["g"]))[:, :, None]
     score = (s["q"].float() @ k.mT) / 8.0 + s["lam"][:, None, None] * decay * (s["c"].float() @ b.mT)
     score = torch.where(there, score + (s["f"] - f)[:, :, None], float("-inf"))
     p = torch.exp(score - score.amax(-1, keepdim=True))
@@ -293,7 +293,7 @@ def _weights(s):
     c = s["c"].gather(2, row[..., None].expand(-1, -1, -1, D_STATE)).float()
     g, f = s["g"].gather(2, row), s["f"].gather(2, row)
     seen = torch.arange(L, device=DEVICE) <= row[..., None]
-    decay = torch.exp((g[..., None] - s["g"][:, :, None]).clamp(max=0.0))
+    decay = torch.exp(torch.where(seen, g[..., None] - s["g"][:, :, None], 0.0))
     score = (q @ s["k"].float().mT) / 8.0 + s["lam"][:, None, None] * decay * (c @ s["b"].float().mT)
     score = torch.where(seen, score + (f[..., None] - s["f"][:, :, None]), float("-inf"))
     p = torch.exp(score - score.amax(-1, keepdim=True))
