@@ -147,6 +147,38 @@ class CacheFillArgs(Structure):
                 ("g", View), ("f", View), ("phi", c_void_p)]
 
 
+class PagePoolArgs(Structure):
+    _fields_ = [("pages", c_int32), ("heads", c_int32), ("page_size", c_int32), ("dtype", c_int32),
+                ("k", View), ("v", View), ("b", View), ("g", View), ("f", View)]
+
+
+class PagedWriteArgs(Structure):
+    _fields_ = [("B", c_int32), ("M", c_int32), ("W", c_int32), ("reserved", c_int32), ("pool", PagePoolArgs),
+                ("table", c_void_p), ("s_table", c_int64), ("start", c_void_p), ("count", c_void_p),
+                ("k", View), ("v", View), ("b", View), ("g", View), ("f", View)]
+
+
+class PagedDecodeArgs(Structure):
+    _fields_ = [("B", c_int32), ("M", c_int32), ("W", c_int32), ("max_len", c_int32), ("pool", PagePoolArgs),
+                ("table", c_void_p), ("s_table", c_int64), ("lengths", c_void_p), ("q", View), ("c", View),
+                ("gq", View), ("fq", View), ("lam", c_void_p), ("s_lam", c_int64), ("w_in", View), ("w_out", View),
+                ("out", c_void_p), ("workspace", c_void_p)]
+
+
+class AttnWeightsArgs(Structure):
+    _fields_ = [("B", c_int32), ("H", c_int32), ("L", c_int32), ("window", c_int32), ("dtype", c_int32),
+                ("reserved", c_int32), ("q", View), ("k", View), ("c", View), ("b", View), ("g", View), ("f", View),
+                ("lam", c_void_p), ("s_lam", c_int64), ("lengths", c_void_p), ("out", c_void_p),
+                ("workspace", c_void_p)]
+
+
+class CacheEvictArgs(Structure):
+    _fields_ = [("B", c_int32), ("W", c_int32), ("W_new", c_int32), ("max_len", c_int32), ("keep", c_int32),
+                ("recent", c_int32), ("from_", PagePoolArgs), ("to", PagePoolArgs), ("table", c_void_p),
+                ("s_table", c_int64), ("new_table", c_void_p), ("s_new", c_int64), ("lengths", c_void_p),
+                ("weights", View), ("new_lengths", c_void_p), ("new_weights", c_void_p), ("positions", c_void_p)]
+
+
 class Round16Args(Structure):
     _fields_ = [("n", c_int64), ("dtype", c_int32), ("x", c_void_p), ("y", c_void_p), ("back", c_void_p)]
 
@@ -203,6 +235,16 @@ CE_SIGNATURES = {
     "sisa_ce_mean_wide": ([c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p], c_int),
 }
 
+# caches in pages (include/sisa_hip_cache.h)
+CACHE_SIGNATURES = {
+    "sisa_paged_write": ([POINTER(PagedWriteArgs), c_void_p], c_int),
+    "sisa_paged_decode_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32, c_int32], c_int64),
+    "sisa_paged_decode": ([POINTER(PagedDecodeArgs), c_void_p], c_int),
+    "sisa_attn_weights_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32], c_int64),
+    "sisa_attn_weights": ([POINTER(AttnWeightsArgs), c_void_p], c_int),
+    "sisa_cache_evict": ([POINTER(CacheEvictArgs), c_void_p], c_int),
+}
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -219,7 +261,7 @@ def load() -> ctypes.CDLL:
             raise RuntimeError(f"SISA HIP library not built: {LIB_PATH} is missing (run sisa_amd.build.build())")
         lib = ctypes.CDLL(LIB_PATH)
         for name, (argtypes, restype) in (*SIGNATURES.items(), *STEP_SIGNATURES.items(),
-                                           *CE_SIGNATURES.items()):
+                                           *CE_SIGNATURES.items(), *CACHE_SIGNATURES.items()):
             fn = getattr(lib, name)
             fn.argtypes = argtypes
             fn.restype = restype

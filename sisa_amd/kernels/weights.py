@@ -1,0 +1,57 @@
+"""What the positions of a prompt have received from its queries, on the HIP kernels of csrc/attn_weights.hip
+(``include/sisa_hip_cache.h``): the accumulated softmax weights from which :func:`sisa_amd.kernels.paged.
+sisa_cache_evict_hip` chooses what stays in a cache. Inference only; no counterpart in the reference."""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from ..config import HIP_D_HEAD, HIP_D_STATE
+from . import _lib
+from .paged import _DTYPES, _int32, no_grad_wanted, readable
+
+__all__ = ["sisa_attention_weights_hip"]
+
+
+def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor,
+                               fgate: Tensor | None = None, *, lengths: Tensor | None = None,
+                               window: int | None = None) -> Tensor:
+    """The softmax weights of SISA attention summed over its queries: ``out[n, h, j]`` is the sum, over the last ``window``
+    queries ``i >= j`` of sequence ``n`` (default: all of its queries), of the weight that query ``i`` gives position ``j``.
+
+    ``q, k`` ``(B, H, L, 64)`` and ``c, b`` ``(B, H, L, 32)`` in bf16, fp16 or fp32, ``g, fgate`` ``(B, H, L)`` and ``lam``
+    ``(H,)`` float32, as :func:`sisa_amd.kernels.attention.sisa_attention_hip` takes them. ``lengths`` ``(B,)`` int32: the
+    positions of each sequence of a right-padded batch (default ``L``; values outside ``0 .. L`` count as the nearer of the
+    two); what lies behind is not looked at and receives 0. Returns ``(B, H, L)`` float32. The scores are formed twice and
+    never stored."""
+    name = "sisa_attention_weights_hip"
+    no_grad_wanted(name, q, k, c, b, g, lam, fgate)
+    if q.dim() != 4 or q.shape[-1] != HIP_D_HEAD or k.shape != q.shape:
+        raise ValueError(f"{name}: q and k must be (B, H, L, {HIP_D_HEAD}), got {tuple(q.shape)} and {tuple(k.shape)}")
+    B, H, L, _ = q.shape
+    if c.shape != (B, H, L, HIP_D_STATE) or b.shape != c.shape:
+        raise ValueError(f"{name}: c and b must be {(B, H, L, HIP_D_STATE)}, got {tuple(c.shape)} and {tuple(b.shape)}")
+    if g.shape != (B, H, L) or (fgate is not None and fgate.shape != g.shape) or lam.shape != (H,):
+        raise ValueError(f"{name}: g and fgate must be {(B, H, L)} and lam ({H},)")
+    if q.dtype not in _DTYPES or not (q.dtype == k.dtype == c.dtype == b.dtype):
+        raise TypeError(f"{name}: q, k, c, b must share one of bf16, fp16, fp32")
+    if g.dtype is not torch.float32 or lam.dtype is not torch.float32 or (fgate is not None
+                                                                         and fgate.dtype is not torch.float32):
+        raise TypeError(f"{name}: g, fgate and lam must be float32")
+    device = _lib.device_index(q)
+    if any(t is not None and t.get_device() != device for t in (k, c, b, g, lam, fgate)):
+        raise ValueError(f"{name}: the tensors are on different devices")
+    if window is not None and window < 1:
+        raise ValueError(f"{name}: window = {window} must be positive or None")
+    if lengths is not None:
+        _int32(name, "lengths", lengths, (B,), device)
+    out = torch.empty((B, H, L), device=q.device, dtype=torch.float32)
+    if not out.numel():
+        return out
+    q, k, c, b = (readable(t) for t in (q, k, c, b))
+    window = 0 if window is None or window >= L else window
+    ws = torch.empty(_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window), device=q.device, dtype=torch.uint8)
+    _lib.call("sisa_attn_weights", _lib.AttnWeightsArgs(
+        B, H, L, window, _lib.dtype_code(q.dtype), 0, _lib.view(q), _lib.view(k), _lib.view(c), _lib.view(b), _lib.view(g),
+        _lib.view(fgate), lam.data_ptr(), lam.stride(0), _lib.ptr(lengths), out.data_ptr(), ws.data_ptr()), q)
+    return out
