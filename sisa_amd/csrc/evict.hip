@@ -4,12 +4,14 @@
 // The selection is a radix select on the weights' bit patterns, mapped so that they order as unsigned integers: one
 // workgroup per (sequence, head) counts the digits of eight bits from the top in LDS (integer counts: their order does not
 // matter), narrows to the digit that holds the last position to keep, and after four digits knows the smallest weight that
-// stays and how many of its equals do. Waves own contiguous ranges of positions, so positions come out in order.
+// stays and how many of its equals do. Waves own contiguous ranges of positions, so positions come out in order. The keys
+// stay in registers (up to 24 a thread: 24,576 positions; longer caches are read again for every digit). Accumulated
+// weights share their leading bits, so that the lanes of a wave count the same few digits: eight copies of the counters,
+// one per lane modulo 8, keep a count from waiting for 63 others.
 #include "pages.h"
 
 namespace {
 
-constexpr int DH = 64, DS = 32;
 constexpr int SW = 16;                // waves of the selection
 
 // Orders as the weight does: NaN above all, both zeros alike.
@@ -22,8 +24,12 @@ SISA_DEV unsigned order_of(float x) {
 SISA_DEV int count_of(uint64_t lanes) { return __builtin_popcountll(lanes); }
 SISA_DEV int below(uint64_t lanes, int lane) { return __builtin_popcountll(lanes & ((1ull << lane) - 1)); }
 
+constexpr int COPIES = 8, COPY = 257;  // counters' copies, and from one to the next (a digit's copies on banks of their own)
+
+// NK keys a thread in registers, or 0: read from memory each time they are needed.
+template <int NK>
 __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_args a, int shift, int new_shift) {
-    __shared__ unsigned hist[256];
+    __shared__ unsigned hist[COPIES * COPY];
     __shared__ unsigned found, left;                   // the digit with the last one to keep, and how many to keep in it
     __shared__ int gt[SW], eq[SW];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -43,24 +49,64 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
         return;
     }
     const int old = len - recent, pick = keep - recent;        // pick of the first `old`, then the recent ones
+    // the wave's range of positions, 64 at a time
+    const int steps = ((old + SW - 1) / SW + 63) / 64, i0 = w * steps * 64;
+    float x[NK ? NK : 1];
+    if constexpr (NK > 0) {
+#pragma unroll
+        for (int s = 0; s < NK; ++s)
+            if (s < steps && i0 + 64 * s + lane < old) x[s] = W[(i0 + 64 * s + lane) * sl];
+    }
     for (int i = tid; i < recent; i += 64 * SW) pos[pick + i] = old + i, neww[pick + i] = W[(old + i) * sl];
     if (pick == 0) return;
+    // f(position, weight) for each of the wave's positions in order, all lanes together; position -1 where there is none
+    auto each = [&](auto&& f) {
+        if constexpr (NK > 0) {
+#pragma unroll
+            for (int s = 0; s < NK; ++s)
+                if (s < steps) {
+                    const int i = i0 + 64 * s + lane;
+                    f(i < old ? i : -1, x[s]);
+                }
+        } else {
+            for (int s0 = 0; s0 < steps; s0 += 8) {            // eight loads under way
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int i = i0 + 64 * (s0 + e) + lane;
+                    y[e] = s0 + e < steps && i < old ? W[i * sl] : 0.f;
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (s0 + e < steps) {
+                        const int i = i0 + 64 * (s0 + e) + lane;
+                        f(i < old ? i : -1, y[e]);
+                    }
+            }
+        }
+    };
 
     // The smallest key that stays, digit by digit; `want` of the keys with the digits so far are still to be picked.
     unsigned prefix = 0, want = pick;
     for (int d = 24; d >= 0; d -= 8) {
-        if (tid < 256) hist[tid] = 0;
+        for (int i = tid; i < COPIES * COPY; i += 64 * SW) hist[i] = 0;
         __syncthreads();
-        for (int i = tid; i < old; i += 64 * SW) {
-            const unsigned k = order_of(W[i * sl]);
-            if (d == 24 || (k >> (d + 8)) == (prefix >> (d + 8))) atomicAdd(&hist[(k >> d) & 255], 1u);
-        }
+        const unsigned high = d == 24 ? 0u : prefix >> (d + 8);
+        each([&](int i, float v) {
+            const unsigned k = order_of(v);
+            if (i >= 0 && (d == 24 || k >> (d + 8) == high)) atomicAdd(&hist[(lane & (COPIES - 1)) * COPY + (k >> d & 255)], 1u);
+        });
         __syncthreads();
         if (w == 0) {
             // lane l: digits 255 - 4 l down to 252 - 4 l; above: how many keys have a larger digit
             unsigned c[4], mine = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[e] = hist[255 - 4 * lane - e], mine += c[e];
+            for (int e = 0; e < 4; ++e) {
+                c[e] = 0;
+#pragma unroll
+                for (int k = 0; k < COPIES; ++k) c[e] += hist[k * COPY + 255 - 4 * lane - e];
+                mine += c[e];
+            }
             unsigned incl = mine;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -77,18 +123,15 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
         __syncthreads();
         prefix |= found << d;
         want = left;
-        __syncthreads();
     }
 
-    // A wave's range of positions: those above the smallest key, and its equals from the lowest position on.
-    const int per = ((old + SW - 1) / SW + 63) / 64 * 64, i0 = w * per, i1 = i0 + per < old ? i0 + per : old;
+    // Those above the smallest key, and its equals from the lowest position on.
     int ng = 0, ne = 0;
-    for (int i = i0; i < i1; i += 64) {
-        const bool in = i + lane < i1;
-        const unsigned k = in ? order_of(W[(i + lane) * sl]) : 0;
-        ng += count_of(__ballot(in && k > prefix));
-        ne += count_of(__ballot(in && k == prefix));
-    }
+    each([&](int i, float v) {
+        const unsigned k = order_of(v);
+        ng += count_of(__ballot(i >= 0 && k > prefix));
+        ne += count_of(__ballot(i >= 0 && k == prefix));
+    });
     if (lane == 0) gt[w] = ng, eq[w] = ne;
     __syncthreads();
     int at = 0, equals = 0;
@@ -97,54 +140,47 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
         at += gt[k] + (take < 0 ? 0 : take < eq[k] ? take : eq[k]);
         equals += eq[k];
     }
-    for (int i = i0; i < i1; i += 64) {
-        const bool in = i + lane < i1;
-        const float x = in ? W[(i + lane) * sl] : 0.f;
-        const unsigned k = order_of(x);
-        const uint64_t same = __ballot(in && k == prefix);
-        const bool stay = in && (k > prefix || (k == prefix && equals + below(same, lane) < (int)want));
+    each([&](int i, float v) {
+        const unsigned k = order_of(v);
+        const uint64_t same = __ballot(i >= 0 && k == prefix);
+        const bool stay = i >= 0 && (k > prefix || (k == prefix && equals + below(same, lane) < (int)want));
         const uint64_t stays = __ballot(stay);
         if (stay) {
             const int to = at + below(stays, lane);
-            pos[to] = i + lane;
-            neww[to] = x;
+            pos[to] = i;
+            neww[to] = v;
         }
         at += count_of(stays);
         equals += count_of(same);
-    }
+    });
 }
 
-// 32 threads per (sequence, head, kept row), as the write of new positions. A row without a page marks its sequence.
-template <class T>
+// A wave moves ROWS kept rows. A row without a page marks its sequence.
+template <class T, int ROWS>
 __global__ __launch_bounds__(256) void evict_copy_kernel(sisa_cache_evict_args a, int shift, int new_shift) {
-    const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int t = threadIdx.x & 31, H = a.from.heads;
-    if (id >= (int64_t)a.B * H * a.keep) return;
-    const int i = (int)(id % a.keep);
-    const int64_t nh = id / a.keep;
-    const int h = (int)(nh % H), n = (int)(nh / H);
-    const int j = a.positions[id];
-    if (j < 0) return;
-    const int src = page_of(a.table + n * a.s_table, a.W, shift, a.from.pages, j);
-    const int dst = page_of(a.new_table + n * a.s_new, a.W_new, new_shift, a.to.pages, i);
-    if (src < 0 || dst < 0) {
-        if (t == 0) a.new_lengths[n] = -1;
-        return;
+    const int lane = threadIdx.x & 63;
+    const unsigned id = (blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS + lane, keep = a.keep, H = a.from.heads;
+    const unsigned nh = id / keep, h = nh % H;
+    const int i = id % keep;
+    const int64_t n = nh / H;
+    const int j = lane < ROWS && n < a.B ? a.positions[id] : -1;
+    int src = -1, dst = -1;
+    if (j >= 0) {
+        src = page_of(a.table + n * a.s_table, a.W, shift, a.from.pages, j);
+        dst = page_of(a.new_table + n * a.s_new, a.W_new, new_shift, a.to.pages, i);
+        if (src < 0 || dst < 0) a.new_lengths[n] = -1;
     }
-    const int64_t sslot = j & (a.from.page_size - 1), dslot = i & (a.to.page_size - 1);
-    if (t < 20) {
-        const sisa_view& s = t < 8 ? a.from.k : t < 16 ? a.from.v : a.from.b;
-        const sisa_view& d = t < 8 ? a.to.k : t < 16 ? a.to.v : a.to.b;
-        const int e = 8 * (t < 16 ? t & 7 : t - 16);
-        *reinterpret_cast<frag8<T>*>((T*)d.ptr + dst * d.sb + h * d.sh + dslot * d.sl + e) =
-            load8<T>((const T*)s.ptr + src * s.sb + h * s.sh + sslot * s.sl + e);
-    } else if (t < 22) {
-        const sisa_view& s = t == 20 ? a.from.g : a.from.f;
-        const sisa_view& d = t == 20 ? a.to.g : a.to.f;
-        if (s.ptr)
-            ((float*)d.ptr)[dst * d.sb + h * d.sh + dslot * d.sl] =
-                ((const float*)s.ptr)[src * s.sb + h * s.sh + sslot * s.sl];
-    }
+    move_rows<T, ROWS>(rows_of_pool(a.from), rows_of_pool(a.to), src >= 0 && dst >= 0, src, dst, h,
+                       j & (a.from.page_size - 1), i & (a.to.page_size - 1), lane);
+}
+
+template <class T>
+void launch_copy(const sisa_cache_evict_args* a, int64_t rows, hipStream_t st) {
+    const int shift = sisa::log2_of(a->from.page_size), new_shift = sisa::log2_of(a->to.page_size);
+    const int per = 4 * sisa::rows_per_wave(rows);
+    const unsigned grid = (unsigned)sisa::cdiv(rows, per);
+    if (per == 256) evict_copy_kernel<T, 64><<<grid, 256, 0, st>>>(*a, shift, new_shift);
+    else evict_copy_kernel<T, 8><<<grid, 256, 0, st>>>(*a, shift, new_shift);
 }
 
 }  // namespace
@@ -165,17 +201,21 @@ extern "C" int sisa_cache_evict(const sisa_cache_evict_args* a, void* stream) {
     if (a->B == 0) return SISA_OK;
     SISA_REQUIRE(a->table && a->new_table && a->lengths && a->weights.ptr && a->new_lengths && a->new_weights && a->positions,
                  "sisa_cache_evict: null pointer");
-    const int64_t heads = (int64_t)a->B * a->from.heads, groups = sisa::cdiv(heads * a->keep, 8);
-    SISA_REQUIRE(groups < ((int64_t)1 << 31), "sisa_cache_evict: B*H*keep too large for one launch");
+    const int64_t heads = (int64_t)a->B * a->from.heads, rows = heads * a->keep;
+    SISA_REQUIRE(rows < ((int64_t)1 << 31), "sisa_cache_evict: B*H*keep must be below 2^31");
     const int shift = sisa::log2_of(a->from.page_size), new_shift = sisa::log2_of(a->to.page_size);
     hipStream_t st = (hipStream_t)stream;
-    evict_select_kernel<<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
+    const int64_t per = sisa::cdiv(a->max_len, 64 * SW);       // keys a thread
+    if (per <= 4) evict_select_kernel<4><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
+    else if (per <= 16) evict_select_kernel<16><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
+    else if (per <= 24) evict_select_kernel<24><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
+    else evict_select_kernel<0><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
     const int rc = sisa::launch_status("sisa_cache_evict (selection)");
     if (rc) return rc;
     switch (a->from.dtype) {
-        case SISA_BF16: evict_copy_kernel<__bf16><<<(unsigned)groups, 256, 0, st>>>(*a, shift, new_shift); break;
-        case SISA_F16: evict_copy_kernel<_Float16><<<(unsigned)groups, 256, 0, st>>>(*a, shift, new_shift); break;
-        default: evict_copy_kernel<float><<<(unsigned)groups, 256, 0, st>>>(*a, shift, new_shift);
+        case SISA_BF16: launch_copy<__bf16>(a, rows, st); break;
+        case SISA_F16: launch_copy<_Float16>(a, rows, st); break;
+        default: launch_copy<float>(a, rows, st);
     }
     return sisa::launch_status("sisa_cache_evict (copy)");
 }

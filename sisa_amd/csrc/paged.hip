@@ -11,33 +11,30 @@ namespace {
 constexpr int DH = 64, DS = 32;
 
 // ------------------------------------------------------------------------------------------------ write
-// 32 threads per (sequence, row, head): 16-byte pieces (8 elements) of k (8), v (8) and b~ (4), and the two gates. The
-// heads of a row are neighbours in the sources that a projection leaves, so the row's threads read whole lines.
-template <class T>
+// A wave moves ROWS rows, numbered with the positions of a head as neighbours: a prompt's rows of a head become neighbours
+// in a page.
+template <class T, int ROWS>
 __global__ __launch_bounds__(256) void paged_write_kernel(sisa_paged_write_args a, int shift) {
-    const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int t = threadIdx.x & 31, H = a.pool.heads;
-    if (id >= (int64_t)a.B * a.M * H) return;
-    const int h = (int)(id % H);
-    const int64_t bm = id / H;
-    const int m = (int)(bm % a.M), n = (int)(bm / a.M);
-    if (a.count && m >= a.count[n]) return;
-    const int64_t pos = (int64_t)a.start[n] + m;
-    const int page = page_of(a.table + n * a.s_table, a.W, shift, a.pool.pages, pos);
-    if (page < 0) return;
-    const int64_t slot = pos & (a.pool.page_size - 1);
-    if (t < 20) {
-        const sisa_view& s = t < 8 ? a.k : t < 16 ? a.v : a.b;
-        const sisa_view& d = t < 8 ? a.pool.k : t < 16 ? a.pool.v : a.pool.b;
-        const int e = 8 * (t < 16 ? t & 7 : t - 16);
-        *reinterpret_cast<frag8<T>*>((T*)d.ptr + page * d.sb + h * d.sh + slot * d.sl + e) =
-            load8<T>((const T*)s.ptr + n * s.sb + h * s.sh + m * s.sl + e);
-    } else if (t < 22) {
-        const sisa_view& s = t == 20 ? a.g : a.f;
-        const sisa_view& d = t == 20 ? a.pool.g : a.pool.f;
-        if (s.ptr)
-            ((float*)d.ptr)[page * d.sb + h * d.sh + slot * d.sl] = ((const float*)s.ptr)[n * s.sb + h * s.sh + m * s.sl];
+    const int lane = threadIdx.x & 63;
+    const unsigned id = (blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS + lane, M = a.M, H = a.pool.heads;
+    const unsigned m = id % M, nh = id / M, h = nh % H;
+    const int64_t n = nh / H;
+    int64_t pos = 0;
+    int page = -1;
+    if (lane < ROWS && n < a.B && (!a.count || (int)m < a.count[n])) {
+        pos = (int64_t)a.start[n] + m;
+        page = page_of(a.table + n * a.s_table, a.W, shift, a.pool.pages, pos);
     }
+    move_rows<T, ROWS>(RowViews{a.k, a.v, a.b, a.g, a.f}, rows_of_pool(a.pool), page >= 0, n, page, h, m,
+                       pos & (a.pool.page_size - 1), lane);
+}
+
+template <class T>
+void launch_write(const sisa_paged_write_args* a, int64_t rows, hipStream_t st) {
+    const int shift = sisa::log2_of(a->pool.page_size), per = 4 * sisa::rows_per_wave(rows);
+    const unsigned grid = (unsigned)sisa::cdiv(rows, per);
+    if (per == 256) paged_write_kernel<T, 64><<<grid, 256, 0, st>>>(*a, shift);
+    else paged_write_kernel<T, 8><<<grid, 256, 0, st>>>(*a, shift);
 }
 
 // ------------------------------------------------------------------------------------------------ decode
@@ -292,14 +289,13 @@ extern "C" int sisa_paged_write(const sisa_paged_write_args* a, void* stream) {
                  "sisa_paged_write: k, v and b rows must be 16-byte aligned");
     SISA_REQUIRE(a->g.ptr && (a->f.ptr == nullptr) == (a->pool.f.ptr == nullptr),
                  "sisa_paged_write: g must be given, and f where the pool has one");
-    const int64_t groups = sisa::cdiv((int64_t)a->B * a->M * a->pool.heads, 8);
-    SISA_REQUIRE(groups < ((int64_t)1 << 31), "sisa_paged_write: B*M*H too large for one launch");
-    const int shift = sisa::log2_of(a->pool.page_size);
+    const int64_t rows = (int64_t)a->B * a->M * a->pool.heads;
+    SISA_REQUIRE(rows < ((int64_t)1 << 31), "sisa_paged_write: B*M*H must be below 2^31");
     hipStream_t st = (hipStream_t)stream;
     switch (a->pool.dtype) {
-        case SISA_BF16: paged_write_kernel<__bf16><<<(unsigned)groups, 256, 0, st>>>(*a, shift); break;
-        case SISA_F16: paged_write_kernel<_Float16><<<(unsigned)groups, 256, 0, st>>>(*a, shift); break;
-        default: paged_write_kernel<float><<<(unsigned)groups, 256, 0, st>>>(*a, shift);
+        case SISA_BF16: launch_write<__bf16>(a, rows, st); break;
+        case SISA_F16: launch_write<_Float16>(a, rows, st); break;
+        default: launch_write<float>(a, rows, st);
     }
     return sisa::launch_status("sisa_paged_write");
 }

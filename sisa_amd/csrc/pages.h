@@ -12,7 +12,85 @@ SISA_DEV int page_of(const int32_t* row, int W, int shift, int pages, int64_t po
     return p >= 0 && p < pages ? p : -1;
 }
 
+// Up to ROWS rows of a cache moved by a wave: lane r's row, if `ok`, from (s0, h, s2) of the source views to (d0, h, d2) of the
+// destination's; no lane from ROWS on has one. 64, or 8 where there are too few rows to fill the chip with waves of 64. Every load and store instruction covers whole rows (k and v of 16 bits: 8 rows of 128 bytes, 8 lanes a
+// row), and all of a pass's loads are under way before its first store: 32 rows a pass in 16 bits, 16 in fp32 (40 registers
+// either way). A row per half wave instead, with three dependent loads in front of each, left the chip waiting: an eviction
+// of 8 x 12 heads from 16,384 to 4,096 positions took 147 us for its copies.
+struct RowViews {
+    sisa_view k, v, b, g, f;
+};
+
+SISA_DEV int64_t lane_value(int64_t x, int lane) {
+    const int lo = __shfl((int)x, lane), hi = __shfl((int)(x >> 32), lane);
+    return (int64_t)hi << 32 | (unsigned)lo;
+}
+
+template <class T, int ROWS>
+SISA_DEV void move_rows(const RowViews& src, const RowViews& dst, bool ok, int64_t s0, int64_t d0, int64_t h, int64_t s2,
+                        int64_t d2, int lane) {
+    constexpr int E = 16 / (int)sizeof(T);             // elements of a piece
+    constexpr int KP = 64 / E, BP = 32 / E;            // pieces of a k or v row, of a b row
+    constexpr int MOST = sizeof(T) == 2 ? 32 : 16, PASS = ROWS < MOST ? ROWS : MOST;      // rows of a pass
+    constexpr int NK = PASS * KP / 64, NB = (PASS * BP + 63) / 64;
+    static_assert(PASS * KP % 64 == 0, "whole instructions");
+    const uint64_t rows = __ballot(ok);
+    auto at = [&](const sisa_view& x, int64_t i0, int64_t i2) { return i0 * x.sb + h * x.sh + i2 * x.sl; };
+    const int64_t sk = at(src.k, s0, s2), sv = at(src.v, s0, s2), sb = at(src.b, s0, s2);
+    const int64_t dk = at(dst.k, d0, d2), dv = at(dst.v, d0, d2), db = at(dst.b, d0, d2);
+    float g = 0.f, f = 0.f;
+    if (ok) {
+        g = ((const float*)src.g.ptr)[at(src.g, s0, s2)];
+        if (src.f.ptr) f = ((const float*)src.f.ptr)[at(src.f, s0, s2)];
+    }
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROWS; r0 += PASS) {
+        u32x4 xk[NK], xv[NK], xb[NB];
+        const int pk = lane % KP, rk = r0 + lane / KP, pb = lane % BP, rb = r0 + lane / BP;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int r = rk + i * (64 / KP);
+            const int64_t ok_ = lane_value(sk, r), ov = lane_value(sv, r);
+            if (rows >> r & 1) {
+                xk[i] = *reinterpret_cast<const u32x4*>((const T*)src.k.ptr + ok_ + E * pk);
+                xv[i] = *reinterpret_cast<const u32x4*>((const T*)src.v.ptr + ov + E * pk);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int r = rb + i * (64 / BP);
+            const int64_t o = lane_value(sb, r);
+            if (rows >> r & 1) xb[i] = *reinterpret_cast<const u32x4*>((const T*)src.b.ptr + o + E * pb);
+        }
+        __builtin_amdgcn_sched_barrier(0);             // the destinations are worked out while the loads are under way
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+            const int r = rk + i * (64 / KP);
+            const int64_t ok_ = lane_value(dk, r), ov = lane_value(dv, r);
+            if (rows >> r & 1) {
+                *reinterpret_cast<u32x4*>((T*)dst.k.ptr + ok_ + E * pk) = xk[i];
+                *reinterpret_cast<u32x4*>((T*)dst.v.ptr + ov + E * pk) = xv[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int r = rb + i * (64 / BP);
+            const int64_t o = lane_value(db, r);
+            if (rows >> r & 1) *reinterpret_cast<u32x4*>((T*)dst.b.ptr + o + E * pb) = xb[i];
+        }
+    }
+    if (ok) {
+        ((float*)dst.g.ptr)[at(dst.g, d0, d2)] = g;
+        if (dst.f.ptr) ((float*)dst.f.ptr)[at(dst.f, d0, d2)] = f;
+    }
+}
+
+SISA_DEV RowViews rows_of_pool(const sisa_page_pool& p) { return RowViews{p.k, p.v, p.b, p.g, p.f}; }
+
 namespace sisa {
+
+// Rows a wave moves: 64 from two waves of that on every SIMD on.
+inline int rows_per_wave(int64_t rows) { return rows >= 64 * 2048 ? 64 : 8; }
 
 inline int log2_of(int32_t page_size) { return 31 - __builtin_clz((unsigned)page_size); }
 
