@@ -38,10 +38,20 @@ void launch_write(const sisa_paged_write_args* a, int64_t rows, hipStream_t st) 
 }
 
 // ------------------------------------------------------------------------------------------------ decode
-constexpr int DW = 4;                 // waves per workgroup
-constexpr int KCH = 64 * DW;          // positions per chunk (workgroup)
-constexpr int PART = DH + 2;          // chunk partial: max, sum, out[64]
+// A wave takes 64 positions. Eight neighbouring lanes share a position, 8 features of its k and v row and 4 of its b row
+// each, so that every load covers whole rows; lane (kq, fg) has positions kq + 8 i, i < 8. A group of eight lies in one page:
+// the page's number is in a scalar register. The partial dot products are summed over a position's lanes by halving
+// exchanges, which leave position kq + 8 fg with lane (kq, fg): every score, exponential and gate is worked out once.
+//
+// The chain of dependent loads is what a short cache costs: pages are looked up beside the length, not after it (entries
+// behind the last are read within the table and then ignored).
+constexpr int TILE = 64;              // positions of a wave
+constexpr int DW = 4;                 // waves per workgroup where the positions are split
+constexpr int KCH = TILE * DW;        // positions per chunk (workgroup)
 constexpr int PIECE = 1024;           // positions of tracked weights per workgroup of the join
+
+// Waves of a workgroup that takes a whole row: as many as fit.
+template <class T> constexpr int whole_waves() { return sizeof(T) == 2 ? 16 : 8; }
 
 // Positions that query row m of a sequence of n sees, or -1 for a length that the call does not take.
 SISA_DEV int visible(int n, int max_len, int64_t held, int M, int m) {
@@ -50,33 +60,55 @@ SISA_DEV int visible(int n, int max_len, int64_t held, int M, int m) {
     return last > 0 ? last : 0;
 }
 
-// One workgroup per (query row, chunk of 256 positions), a wave per 64 of them; 8 neighbouring lanes share a position (8
-// features each), so that every load covers whole 128-byte rows. A group of 8 positions lies in one page.
-template <class T, bool TRACK>
-__global__ __launch_bounds__(64 * DW) void paged_chunk_kernel(sisa_paged_decode_args a, int shift, int nchunk, float* part,
-                                                             float* scores) {
-    __shared__ float wm[DW], wl[DW], wo[DW][DH];
+template <int CTRL> SISA_DEV float dpp(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, XOR7 = 0x141, XOR8 = 0x128;    // of a lane's number (8: a rotation of 16 lanes by 8)
+
+// x[i] summed over the eight lanes that share lane / 8; lane 8 k + i gets the sum of x[i].
+SISA_DEV float sum_scatter(const float (&x)[8], int fg) {
+    float y[4], z[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (fg & 4 ? x[i + 4] : x[i]) + dpp<XOR7>(fg & 4 ? x[i] : x[i + 4]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) z[i] = (fg & 2 ? y[i + 2] : y[i]) + dpp<XOR2>(fg & 2 ? y[i] : y[i + 2]);
+    return (fg & 1 ? z[1] : z[0]) + dpp<XOR1>(fg & 1 ? z[0] : z[1]);
+}
+
+// 256 MB, the last-level cache: from there on 16-bit rows are loaded with the non-temporal hint, as csrc/decode.hip does (516
+// MB 102 -> 90 us; 77 MB 21.0 -> 22.9). The host does not know the lengths; a call is taken to read the smaller of
+// max_len positions of every sequence and the whole pool.
+constexpr int64_t STREAM_BYTES = (int64_t)256 << 20;
+template <class V, bool STREAM> SISA_DEV V load_as(const void* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    else return *reinterpret_cast<const V*>(p);
+}
+
+// A workgroup of NW waves per (query row, chunk of 64 NW positions). ONE: one chunk, which writes the row's output, and its
+// weights. Otherwise the chunk's largest score and sum go to stat, its unnormalised output to part, and with TRACK the
+// scores to `scores`.
+template <class T, int NW, bool ONE, bool TRACK, bool STREAM>
+__global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_args a, int shift, int nchunk, f32x2* stat,
+                                                              float* part, float* scores) {
+    __shared__ float wm[NW], wl[NW], wo[NW][DH];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fg = lane & 7, kq = lane >> 3;
-    const int chunk = blockIdx.x % nchunk, row = blockIdx.x / nchunk;
+    // chunk by chunk over the rows: the chunks behind the shorter sequences' ends come last and hold nothing up
+    const int rows = a.B * a.pool.heads * a.M, chunk = ONE ? 0 : blockIdx.x / rows, row = ONE ? blockIdx.x : blockIdx.x % rows;
     const int H = a.pool.heads, m = row % a.M, nh = row / a.M, h = nh % H, n = nh / H;
-    const int vis = visible(a.lengths[n], a.max_len, (int64_t)a.W << shift, a.M, m);
-    if (chunk * KCH >= vis) return;                    // nothing here: the join does not read this partial
-    const int jw = chunk * KCH + w * 64;
-    const int32_t* table = a.table + n * a.s_table;
     const sisa_page_pool& P = a.pool;
+    const int jw = (chunk * NW + w) * TILE;
+    // lane i < 8: the page of positions jw + 8 i .. + 7
+    const int group = (jw + 8 * fg) >> shift;
+    int pg = group < a.W ? a.table[n * a.s_table + group] : -1;
+    const int len = a.lengths[n];
+    const int vis = visible(len, a.max_len, (int64_t)a.W << shift, a.M, m);
+    if (!ONE && chunk * KCH >= vis) return;            // nothing here: the join does not read this chunk's partial
+    pg = pg >= 0 && pg < P.pages ? pg : -1;
     const int mask = P.page_size - 1;
-    // lane i < 8: the page of positions jw + 8 i .. + 7, -1 where there are none or no such page
-    int pg = -1;
-    if (lane < 8 && jw + 8 * lane < vis) pg = page_of(table, a.W, shift, P.pages, jw + 8 * lane);
-    const T* Q = (const T*)a.q.ptr + n * a.q.sb + h * a.q.sh + m * a.q.sl;
-    const T* C = (const T*)a.c.ptr + n * a.c.sb + h * a.c.sh + m * a.c.sl;
-    const float gq = ((const float*)a.gq.ptr)[n * a.gq.sb + h * a.gq.sh + m * a.gq.sl];
-    const bool has_f = P.f.ptr != nullptr;
-    const float fq = has_f ? ((const float*)a.fq.ptr)[n * a.fq.sb + h * a.fq.sh + m * a.fq.sl] : 0.f;
-    const float lam = a.lam[h * a.s_lam];
 
-    frag8<T> kr[8], vr[8], br[8];
+    frag8<T> kr[8], vr[8];
+    vec4<T> br[8];
     bool ok[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -85,115 +117,123 @@ __global__ __launch_bounds__(64 * DW) void paged_chunk_kernel(sisa_paged_decode_
         ok[i] = page >= 0 && j < vis;
         if (ok[i]) {
             const int64_t slot = j & mask;
-            kr[i] = load8<T>((const T*)P.k.ptr + page * P.k.sb + h * P.k.sh + slot * P.k.sl + 8 * fg);
-            vr[i] = load8<T>((const T*)P.v.ptr + page * P.v.sb + h * P.v.sh + slot * P.v.sl + 8 * fg);
-            if (fg < DS / 8) br[i] = load8<T>((const T*)P.b.ptr + page * P.b.sb + h * P.b.sh + slot * P.b.sl + 8 * fg);
+            kr[i] = load_as<frag8<T>, STREAM>((const T*)P.k.ptr + (page * P.k.sb + h * P.k.sh) + slot * P.k.sl + 8 * fg);
+            vr[i] = load_as<frag8<T>, STREAM>((const T*)P.v.ptr + (page * P.v.sb + h * P.v.sh) + slot * P.v.sl + 8 * fg);
+            br[i] = load_as<vec4<T>, STREAM>((const T*)P.b.ptr + (page * P.b.sb + h * P.b.sh) + slot * P.b.sl + 4 * fg);
         }
     }
-    // per-position scalars with lane = position: lam exp(g_m - g_j) and F_m - F_j; NaN for a page that is not there
-    const int64_t mine = __shfl(pg, lane >> 3);
-    float dec = 0.f, fd = 0.f;
-    if (jw + lane < vis) {
-        if (mine < 0) {
-            fd = __builtin_nanf("");
-        } else {
-            const int64_t slot = (jw + lane) & mask;
-            dec = lam * expf(gq - ((const float*)P.g.ptr)[mine * P.g.sb + h * P.g.sh + slot * P.g.sl]);
-            if (has_f) fd = fq - ((const float*)P.f.ptr)[mine * P.f.sb + h * P.f.sh + slot * P.f.sl];
-        }
+    const f32x8 qv = load_f32x8<T>((const T*)a.q.ptr + n * a.q.sb + h * a.q.sh + m * a.q.sl + 8 * fg);
+    const f32x4 cv = __builtin_convertvector(load4<T>((const T*)a.c.ptr + n * a.c.sb + h * a.c.sh + m * a.c.sl + 4 * fg), f32x4);
+    const bool has_f = P.f.ptr != nullptr;
+    const float gq = ((const float*)a.gq.ptr)[n * a.gq.sb + h * a.gq.sh + m * a.gq.sl];
+    const float fq = has_f ? ((const float*)a.fq.ptr)[n * a.fq.sb + h * a.fq.sh + m * a.fq.sl] : 0.f;
+    const float lam = a.lam[h * a.s_lam];
+    // the lane's own position kq + 8 fg: lam exp(g_m - g_j) and F_m - F_j, NaN for a page that is not there
+    const int j = jw + 8 * fg + kq;                    // group fg's page is lane fg's, and every lane 8 k + fg's
+    float dec = 0.f, fd = __builtin_nanf("");
+    if (j < vis && pg >= 0) {
+        const int64_t slot = j & mask;
+        dec = lam * expf(gq - ((const float*)P.g.ptr)[pg * P.g.sb + h * P.g.sh + slot * P.g.sl]);
+        fd = has_f ? fq - ((const float*)P.f.ptr)[pg * P.f.sb + h * P.f.sh + slot * P.f.sl] : 0.f;
     }
-    const f32x8 qv = load_f32x8<T>(Q + 8 * fg);
-    f32x8 cv;
-    if (fg < DS / 8) cv = load_f32x8<T>(C + 8 * fg);
+    float old = 0.f;
+    if constexpr (ONE && TRACK)
+        if (j < vis) old = ((const float*)a.w_in.ptr)[n * a.w_in.sb + h * a.w_in.sh + j * a.w_in.sl];
 
-    float s[8], mx = -__builtin_inff();
+    float qk[8], cb[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float di = __shfl(dec, kq + 8 * i), fi = __shfl(fd, kq + 8 * i);
-        float qk = 0.f, cb = 0.f;
+        qk[i] = cb[i] = 0.f;
         if (ok[i]) {
             const f32x8 kv = __builtin_convertvector(kr[i], f32x8);
+            const f32x4 bv = __builtin_convertvector(br[i], f32x4);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qk = fmaf(qv[e], kv[e], qk);
-            if (fg < DS / 8) {
-                const f32x8 bv = __builtin_convertvector(br[i], f32x8);
+            for (int e = 0; e < 8; ++e) qk[i] = fmaf(qv[e], kv[e], qk[i]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) cb = fmaf(cv[e], bv[e], cb);
-            }
+            for (int e = 0; e < 4; ++e) cb[i] = fmaf(cv[e], bv[e], cb[i]);
         }
-        float t = fmaf(qk, 0.125f, di * cb);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) t += __shfl_xor(t, o);
-        s[i] = jw + 8 * i + kq < vis ? t + fi : -__builtin_inff();
-        mx = fmaxf(mx, s[i]);
     }
-    if constexpr (TRACK) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (fg == 0 && jw + 8 * i + kq < vis) scores[(int64_t)row * a.max_len + jw + 8 * i + kq] = s[i];
-    }
-#pragma unroll
-    for (int o = 8; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float tq = sum_scatter(qk, fg), tc = sum_scatter(cb, fg);      // every lane takes part in the exchanges
+    const float s = j < vis ? fmaf(tq, 0.125f, dec * tc) + fd : -__builtin_inff();
+    if constexpr (TRACK && !ONE)
+        if (j < vis) scores[(int64_t)row * a.max_len + j] = s;
+    float mx = fmaxf(s, dpp<XOR1>(s));
+    mx = fmaxf(mx, dpp<XOR2>(mx));
+    mx = fmaxf(mx, dpp<XOR7>(mx));
+    mx = group_max(fmaxf(mx, dpp<XOR8>(mx)));
     const float ref = mx == -__builtin_inff() ? 0.f : mx;      // all -inf: the weights are 0, not NaN
-    float p[8], l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        p[i] = expf(s[i] - ref);                               // 0 for positions that are not visible
-        l += p[i];
-    }
-#pragma unroll
-    for (int o = 8; o < 64; o <<= 1) l += __shfl_xor(l, o);
+    const float p = expf(s - ref);                             // 0 for positions that are not visible
+    float l = p + dpp<XOR1>(p);
+    l += dpp<XOR2>(l);
+    l += dpp<XOR7>(l);
+    l = group_sum(l + dpp<XOR8>(l));
     f32x8 acc;
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (ok[i] && p[i] != 0.f) {
+        const float pi = __shfl(p, (lane & 56) | i);
+        if (ok[i] && pi != 0.f) {
             const f32x8 vv = __builtin_convertvector(vr[i], f32x8);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(p[i], vv[e], acc[e]);
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(pi, vv[e], acc[e]);
         }
     }
 #pragma unroll
-    for (int o = 8; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor(acc[e], o);
+    for (int e = 0; e < 8; ++e) acc[e] = group_sum(acc[e] + dpp<XOR8>(acc[e]));
     if (lane == 0) wm[w] = mx, wl[w] = l;
     if (kq == 0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) wo[w][8 * fg + e] = acc[e];
     }
     __syncthreads();
-    if (w != 0) return;
+    if (!(ONE && TRACK) && w != 0) return;
     float cm = wm[0];
 #pragma unroll
-    for (int k = 1; k < DW; ++k) cm = fmaxf(cm, wm[k]);
+    for (int k = 1; k < NW; ++k) cm = fmaxf(cm, wm[k]);
     float cl = 0.f, co = 0.f;
 #pragma unroll
-    for (int k = 0; k < DW; ++k) {
+    for (int k = 0; k < NW; ++k) {
         const float sc = wm[k] == -__builtin_inff() ? 1.f : expf(wm[k] - cm);      // all -inf: sums of 0, or NaN
         cl = fmaf(wl[k], sc, cl);
         co = fmaf(wo[k][lane], sc, co);
     }
-    float* dst = part + ((int64_t)row * nchunk + chunk) * PART;
-    dst[2 + lane] = co;
-    if (lane == 0) dst[0] = cm, dst[1] = cl;
+    if constexpr (ONE) {
+        if (w == 0) a.out[(int64_t)row * DH + lane] = vis < 0 ? __builtin_nanf("") : vis == 0 ? 0.f : co / cl;
+        if constexpr (TRACK)
+            if (j < vis)
+                ((float*)a.w_out.ptr)[n * a.w_out.sb + h * a.w_out.sh + j * a.w_out.sl] =
+                    old + expf(s - (cm == -__builtin_inff() ? 0.f : cm)) / cl;
+    } else {
+        const int64_t at = (int64_t)row * nchunk + chunk;
+        part[at * DH + lane] = co;
+        if (lane == 0) stat[at] = f32x2{cm, cl};
+    }
 }
 
-// The join: chunk c's factor exp(max_c - max) is formed by thread c mod 256, sums go in chunk order. A workgroup per
-// query row; or, with tracked weights, per (sequence and head, 1,024 positions), whose rows are taken in order and whose
-// first workgroup writes the outputs.
+// The join of a row's chunks, in a fixed order. A workgroup per query row; or, with tracked weights, per (sequence and head,
+// 1,024 positions), whose rows are taken in order and whose first workgroup writes the outputs. What the weights need is
+// loaded before the row's sum is known.
 template <bool TRACK>
-__global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args a, int shift, int nchunk, const float* part,
-                                                         const float* scores) {
+__global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args a, int shift, int nchunk, const f32x2* stat,
+                                                         const float* part, const float* scores) {
     __shared__ float red[2][4], wo[4][DH];
+    constexpr int PER = PIECE / 256;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int pieces = TRACK ? (a.max_len + PIECE - 1) / PIECE : 1;
     const int piece = blockIdx.x % pieces, item = blockIdx.x / pieces;
     const int H = a.pool.heads, nh = TRACK ? item : item / a.M, h = nh % H, n = nh / H;
     const int len = a.lengths[n];
+    if (TRACK && piece > 0 && piece * PIECE >= len) return;
     const bool outs = piece == 0;
-    float add[PIECE / 256] = {0.f, 0.f, 0.f, 0.f};
+    float sum[PER];
+    if constexpr (TRACK) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int64_t j = piece * PIECE + 256 * i + tid;
+            sum[i] = j < len && j < a.max_len ? ((const float*)a.w_in.ptr)[n * a.w_in.sb + h * a.w_in.sh + j * a.w_in.sl] : 0.f;
+        }
+    }
     for (int m = TRACK ? 0 : item % a.M; m < (TRACK ? a.M : item % a.M + 1); ++m) {
         const int64_t row = (int64_t)nh * a.M + m;
         const int vis = visible(len, a.max_len, (int64_t)a.W << shift, a.M, m);
@@ -201,73 +241,103 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
             if (outs && tid < DH) a.out[row * DH + tid] = vis < 0 ? __builtin_nanf("") : 0.f;
             continue;
         }
-        const float* P = part + row * nchunk * PART;
-        const int nc = (vis + KCH - 1) / KCH;
-        float mx = -__builtin_inff();
-        for (int c = tid; c < nc; c += 256) mx = fmaxf(mx, P[(int64_t)c * PART]);
+        float s[PER];
+        if constexpr (TRACK) {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        __syncthreads();
-        if (lane == 0) red[0][w] = mx;
+            for (int i = 0; i < PER; ++i) {
+                const int j = piece * PIECE + 256 * i + tid;
+                s[i] = j < vis ? scores[row * a.max_len + j] : -__builtin_inff();
+            }
+        }
+        const f32x2* S = stat + row * nchunk;
+        const int nc = (vis + KCH - 1) / KCH;
+        float mx = -__builtin_inff(), l = 0.f;
+        for (int c = tid; c < nc; c += 256) {
+            const f32x2 x = S[c];
+            const float to = fmaxf(mx, x[0]), ref = to == -__builtin_inff() ? 0.f : to;
+            l = l * (mx == -__builtin_inff() ? 1.f : expf(mx - ref)) + x[1] * (x[0] == -__builtin_inff() ? 1.f : expf(x[0] - ref));
+            mx = to;
+        }
+        float wmx = mx;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) wmx = fmaxf(wmx, __shfl_xor(wmx, o));
+        l *= mx == -__builtin_inff() ? 1.f : expf(mx - wmx);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+        __syncthreads();                               // the last row's sums have been read
+        if (lane == 0) red[0][w] = wmx, red[1][w] = l;
         __syncthreads();
         mx = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
         const float ref = mx == -__builtin_inff() ? 0.f : mx;
-        float l = 0.f;
-        for (int c = tid; c < nc; c += 256) {
-            const float mc = P[(int64_t)c * PART];
-            l = fmaf(P[(int64_t)c * PART + 1], mc == -__builtin_inff() ? 1.f : expf(mc - ref), l);
-        }
+        l = 0.f;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
-        if (lane == 0) red[1][w] = l;
-        __syncthreads();
-        l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+        for (int k = 0; k < 4; ++k) l = fmaf(red[1][k], red[0][k] == -__builtin_inff() ? 1.f : expf(red[0][k] - ref), l);
         const float inv = 1.f / l;
         if (outs) {
             float o = 0.f;
             for (int c = w; c < nc; c += 4) {
-                const float mc = P[(int64_t)c * PART];
-                o = fmaf(P[(int64_t)c * PART + 2 + lane], mc == -__builtin_inff() ? 1.f : expf(mc - ref), o);
+                const float mc = S[c][0];
+                o = fmaf(part[(row * nchunk + c) * DH + lane], mc == -__builtin_inff() ? 1.f : expf(mc - ref), o);
             }
             wo[w][lane] = o;
             __syncthreads();
-            if (tid < DH) a.out[row * DH + tid] = (wo[0][tid] + wo[1][tid] + wo[2][tid] + wo[3][tid]) * inv;
+            if (tid < DH) a.out[row * DH + tid] = ((wo[0][tid] + wo[1][tid]) + (wo[2][tid] + wo[3][tid])) * inv;
         }
         if constexpr (TRACK) {
 #pragma unroll
-            for (int i = 0; i < PIECE / 256; ++i) {
-                const int j = piece * PIECE + 256 * i + tid;
-                if (j < vis) add[i] += expf(scores[row * a.max_len + j] - ref) * inv;
-            }
+            for (int i = 0; i < PER; ++i) sum[i] += expf(s[i] - ref) * inv;
         }
     }
     if constexpr (TRACK) {
-        if (len < 0 || len > a.max_len || len > ((int64_t)a.W << shift)) return;
+        if (visible(len, a.max_len, (int64_t)a.W << shift, 1, 0) <= 0) return;
 #pragma unroll
-        for (int i = 0; i < PIECE / 256; ++i) {
+        for (int i = 0; i < PER; ++i) {
             const int64_t j = piece * PIECE + 256 * i + tid;
-            if (j < len)
-                ((float*)a.w_out.ptr)[n * a.w_out.sb + h * a.w_out.sh + j * a.w_out.sl] =
-                    ((const float*)a.w_in.ptr)[n * a.w_in.sb + h * a.w_in.sh + j * a.w_in.sl] + add[i];
+            if (j < len) ((float*)a.w_out.ptr)[n * a.w_out.sb + h * a.w_out.sh + j * a.w_out.sl] = sum[i];
         }
     }
 }
 
-int64_t part_bytes(int64_t rows, int64_t max_len) {
-    return (rows * sisa::cdiv(max_len, KCH) * PART * (int64_t)sizeof(float) + 255) / 256 * 256;
+struct DecodeSpace {
+    f32x2* stat;
+    float *part, *scores;
+    int64_t bytes;
+};
+
+int64_t pad256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+DecodeSpace decode_space(char* base, int64_t rows, int64_t max_len, bool tracked) {
+    const int64_t chunks = rows * sisa::cdiv(max_len, KCH);
+    DecodeSpace s{};
+    s.stat = (f32x2*)base;
+    s.part = (float*)(base + pad256(chunks * 8));
+    s.scores = (float*)((char*)s.part + pad256(chunks * DH * 4));
+    s.bytes = (char*)s.scores - base + (tracked ? rows * max_len * 4 : 0);
+    return s;
 }
 
 template <class T, bool TRACK>
 int launch_decode(const sisa_paged_decode_args* a, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size), nchunk = (int)sisa::cdiv(a->max_len, KCH);
     const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
-    float* part = (float*)a->workspace;
-    float* scores = (float*)((char*)a->workspace + part_bytes(rows, a->max_len));
-    paged_chunk_kernel<T, TRACK><<<(unsigned)(rows * nchunk), 64 * DW, 0, st>>>(*a, shift, nchunk, part, scores);
+    const DecodeSpace ws = decode_space((char*)a->workspace, rows, a->max_len, TRACK);
+    // Caches that one workgroup takes whole need no join (tracked weights: with one query row, which is the only one to add
+    // to them).
+    constexpr int NW = whole_waves<T>();
+    if (a->max_len <= TILE * NW && (!TRACK || a->M == 1)) {
+        paged_chunk_kernel<T, NW, true, TRACK, false><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, shift, 1, ws.stat, ws.part, ws.scores);
+        return sisa::launch_status("sisa_paged_decode");
+    }
+    const unsigned grid = (unsigned)(rows * nchunk);
+    const int64_t held = (int64_t)a->pool.pages * a->pool.heads * a->pool.page_size;
+    const int64_t most = rows * a->max_len, bytes = (most < held ? most : held) * ((2 * DH + DS) * (int64_t)sizeof(T) + 8);
+    if (sizeof(T) == 2 && a->M == 1 && bytes >= STREAM_BYTES)
+        paged_chunk_kernel<T, DW, false, TRACK, sizeof(T) == 2><<<grid, KCH, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
+    else paged_chunk_kernel<T, DW, false, TRACK, false><<<grid, KCH, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
     const int rc = sisa::launch_status("sisa_paged_decode");
     if (rc) return rc;
     const int64_t groups = TRACK ? rows / a->M * sisa::cdiv(a->max_len, PIECE) : rows;
-    paged_join_kernel<TRACK><<<(unsigned)groups, 256, 0, st>>>(*a, shift, nchunk, part, scores);
+    paged_join_kernel<TRACK><<<(unsigned)groups, 256, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
     return sisa::launch_status("sisa_paged_decode (join)");
 }
 
@@ -275,7 +345,6 @@ template <class T>
 int launch_decode(const sisa_paged_decode_args* a, hipStream_t st) {
     return a->w_out.ptr ? launch_decode<T, true>(a, st) : launch_decode<T, false>(a, st);
 }
-
 
 }  // namespace
 
@@ -302,8 +371,7 @@ extern "C" int sisa_paged_write(const sisa_paged_write_args* a, void* stream) {
 
 extern "C" int64_t sisa_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t max_len, int32_t tracked) {
     if (B < 1 || H < 1 || M < 1 || max_len < 1) return 0;
-    const int64_t rows = (int64_t)B * H * M;
-    return part_bytes(rows, max_len) + (tracked ? rows * max_len * (int64_t)sizeof(float) : 0);
+    return decode_space(nullptr, (int64_t)B * H * M, max_len, tracked != 0).bytes;
 }
 
 extern "C" int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream) {
