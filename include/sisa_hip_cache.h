@@ -72,6 +72,7 @@ int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream);
  * all of them), summed:  out_j = sum over i >= j, n - window <= i < n, of softmax_j(s_ij), with the score of sisa_attn_fwd
  * and n = lengths[b] (NULL: L; values outside 0 .. L count as the nearer of the two); 0 for j >= n. Workspace:
  * sisa_attn_weights_workspace_bytes(B, H, L, window). */
+#define SISA_ATTN_WEIGHTS_MAX_STRIDE (1 << 24)    /* of the positions of q, k, c and b, in elements */
 typedef struct {
     int32_t B, H, L;
     int32_t window;            /* 0 .. L */
@@ -79,11 +80,11 @@ typedef struct {
     int32_t reserved;
     sisa_view q, k;            /* (B,H,L,64) */
     sisa_view c, b;            /* (B,H,L,32) */
-    sisa_view g, f;            /* (B,H,L) fp32; f.ptr NULL = no forget term */
+    sisa_view g, f;            /* (B,H,L) fp32, position stride 1; f.ptr NULL = no forget term */
     const float* lam; int64_t s_lam;           /* (H) fp32 */
     const int32_t* lengths;    /* (B) or NULL */
     float* out;                /* (B,H,L) contiguous */
-    void* workspace;
+    void* workspace;           /* 16-byte aligned */
 } sisa_attn_weights_args;
 
 int64_t sisa_attn_weights_workspace_bytes(int32_t B, int32_t H, int32_t L, int32_t window);

@@ -5,8 +5,8 @@
 //
 // Two passes over the scores, neither of which keeps them: the queries' log-sum-exp over their keys, then every key's sum
 // over its queries. Scores are 16x16 MFMA blocks with K = 64 (q.k) and 32 (c.b). A wave holds 64 queries (keys) in
-// registers and streams 16 keys (queries) at a time straight from memory, which L2 serves, the next 16 loaded before the
-// present ones are used; four waves share the 64 and take every fourth of the 16s. In the first pass a lane owns one query
+// registers and streams 16 keys (queries) at a time, which L2 serves, the next 16 in LDS and those after them under way
+// while the present ones are used; four waves share the 64 and take every fourth of the 16s. In the first pass a lane owns one query
 // per block (the keys are the block's rows), in the second one key: the running sums need no lane exchange before the end.
 //
 // Bound by the vector unit: the products of a block take 48 cycles of the matrix pipe, its 256 scores' exponentials alone
@@ -37,31 +37,115 @@ SISA_DEV Rows rows_of(const sisa_attn_weights_args& a, int b) {
     return Rows{n, n - count, count};
 }
 
-// The operand of 16 positions, r0 + lane % 16, features 0..31 and 32..63 and the state's 0..31; positions beyond the last
-// of the view as the last one.
-template <class T> struct Frags { frag8<T> x0, x1, s; };
-template <class T>
-SISA_DEV Frags<T> frags(const sisa_view& x, const sisa_view& s, int b, int h, int r0, int L, int lane) {
-    const int row = r0 + (lane & 15) < L ? r0 + (lane & 15) : L - 1, f = 8 * (lane >> 4);
-    const T* p = (const T*)x.ptr + b * x.sb + h * x.sh + row * x.sl;
-    const T* q = (const T*)s.ptr + b * s.sb + h * s.sh + row * s.sl;
-    return Frags<T>{load8<T>(p + f), load8<T>(p + 32 + f), load8<T>(q + f)};
+// 16 positions on their way into a wave's operands. They come from memory in whole rows (a lane takes 16 consecutive bytes,
+// its neighbours the rest of the row) and pass through LDS that the wave has to itself: an operand's lanes next to each other
+// belong to different rows, so that loading operands directly makes a cache access of every lane (287 accesses a tile; the
+// L1 cache was what both passes waited for: 62 us each for 4 x 2,048 positions of 12 heads).
+template <class T> struct Frags { frag8<T> x0, x1, s; };      // features 0..31, 32..63 and the state's 0..31
+template <class T> struct Tile {
+    Frags<T> x;
+    f32x4 g, f, st;                               // of the lane's positions 4 grp .. + 3
+};
+template <class T> struct alignas(16) Buffer {
+    T x[16 * DH], s[16 * DS];
+    float gates[3 * 16];
+};
+template <class T> struct Raw {
+    static constexpr int E = 16 / (int)sizeof(T), CX = DH / E, CS = DS / E, NX = 16 * CX / 64, NS = 16 * CS / 64;
+    u32x4 x[NX], s[NS];
+    float gate;
+};
+
+// Where a lane's pieces are: positions 0 .. 15 of a (batch, head), gates g (lanes 0..15), F (16..31), starts (32..47). Byte
+// offsets within 16 positions are below 2^31 (checked by the host): a load takes a scalar base and one register.
+template <class T> struct Stream {
+    using R = Raw<T>;
+    const char *x, *s;
+    int64_t sx, ss;                               // bytes of a position
+    const float* gate;
+    int lane;
+    bool starts;                                  // the lane reads starts
+
+    SISA_DEV Stream(const sisa_view& vx, const sisa_view& vs, const sisa_attn_weights_args& a, int b, int h, const float* start,
+                    int lane_) {
+        lane = lane_;
+        x = (const char*)((const T*)vx.ptr + b * vx.sb + h * vx.sh);
+        s = (const char*)((const T*)vs.ptr + b * vs.sb + h * vs.sh);
+        sx = vx.sl * (int)sizeof(T);
+        ss = vs.sl * (int)sizeof(T);
+        const float* g = (const float*)a.g.ptr + b * a.g.sb + h * a.g.sh;
+        const float* f = a.f.ptr ? (const float*)a.f.ptr + b * a.f.sb + h * a.f.sh : g;
+        starts = start && lane >= 32 && lane < 48;
+        gate = (starts ? start : lane >= 16 && lane < 32 ? f : g) + (lane & 15);
+    }
+    SISA_DEV void go(int64_t positions) {
+        x += positions * sx;
+        s += positions * ss;
+        gate += positions;
+    }
+    // the 16 positions from here, all of them there
+    SISA_DEV R load() const {
+        R r;
+#pragma unroll
+        for (int i = 0; i < R::NX; ++i) {
+            const int p = lane + 64 * i;
+            r.x[i] = *reinterpret_cast<const u32x4*>(x + (unsigned)((p / R::CX) * (int)sx + 16 * (p % R::CX)));
+        }
+#pragma unroll
+        for (int i = 0; i < R::NS; ++i) {
+            const int p = lane + 64 * i;
+            r.s[i] = *reinterpret_cast<const u32x4*>(s + (unsigned)((p / R::CS) * (int)ss + 16 * (p % R::CS)));
+        }
+        r.gate = *gate;
+        return r;
+    }
+    // the 16 positions from r0 (this stream is at 0), those from L on as the last one; the start of row r, which has its own
+    // numbering and is padded to 16
+    SISA_DEV R load_edge(int r0, int L, int r = 0) const {
+        R o;
+#pragma unroll
+        for (int i = 0; i < R::NX; ++i) {
+            const int p = lane + 64 * i, row = r0 + p / R::CX < L ? r0 + p / R::CX : L - 1;
+            o.x[i] = *reinterpret_cast<const u32x4*>(x + row * sx + 16 * (p % R::CX));
+        }
+#pragma unroll
+        for (int i = 0; i < R::NS; ++i) {
+            const int p = lane + 64 * i, row = r0 + p / R::CS < L ? r0 + p / R::CS : L - 1;
+            o.s[i] = *reinterpret_cast<const u32x4*>(s + row * ss + 16 * (p % R::CS));
+        }
+        const int g = r0 + (lane & 15) < L ? r0 : L - 1 - (lane & 15);
+        o.gate = gate[starts ? r : g];
+        return o;
+    }
+};
+
+// Through the wave's own LDS; a wave's LDS accesses are carried out in their order.
+template <class T, bool FORGET>
+SISA_DEV Tile<T> turn(const Raw<T>& r, Buffer<T>* buf, int lane) {
+    using R = Raw<T>;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < R::NX; ++i) {
+        const int p = lane + 64 * i;
+        *reinterpret_cast<u32x4*>(buf->x + toff<T, DH>(p / R::CX, p % R::CX)) = r.x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < R::NS; ++i) {
+        const int p = lane + 64 * i;
+        *reinterpret_cast<u32x4*>(buf->s + toff<T, DS>(p / R::CS, p % R::CS)) = r.s[i];
+    }
+    if (lane < 48) buf->gates[lane] = r.gate;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int grp = lane >> 4;
+    return Tile<T>{Frags<T>{frag_rows<T, DH>(buf->x, 0, 0, lane), frag_rows<T, DH>(buf->x, 0, 1, lane),
+                            frag_rows<T, DS>(buf->s, 0, 0, lane)},
+                   lds4f(buf->gates + 4 * grp), FORGET ? lds4f(buf->gates + 16 + 4 * grp) : zero4(),
+                   lds4f(buf->gates + 32 + 4 * grp)};
 }
 
 SISA_DEV float gate(const sisa_view& v, int b, int h, int r, int L) {
-    return v.ptr ? ((const float*)v.ptr)[b * v.sb + h * v.sh + (int64_t)(r < L ? r : L - 1) * v.sl] : 0.f;
-}
-
-// Four positions r .. r + 3, one load where they are neighbours in memory (at any alignment); 0 without a forget term.
-struct __attribute__((packed, aligned(4))) Floats4 { f32x4 v; };
-SISA_DEV f32x4 gates4(const sisa_view& v, int b, int h, int r, int L) {
-    if (!v.ptr) return zero4();
-    const float* p = (const float*)v.ptr + b * v.sb + h * v.sh;
-    if (v.sl == 1 && r + 4 <= L) return reinterpret_cast<const Floats4*>(p + r)->v;
-    f32x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = p[(int64_t)(r + e < L ? r + e : L - 1) * v.sl];
-    return x;
+    return v.ptr ? ((const float*)v.ptr)[b * v.sb + h * v.sh + (r < L ? r : L - 1)] : 0.f;
 }
 
 // (m, l) of two parts of a row, log2 units
@@ -71,24 +155,15 @@ SISA_DEV void merge(float& m, float& l, float m2, float l2) {
     m = t;
 }
 
-// 16 streamed positions from r0: operands, g and F of the lane's four
-template <class T> struct Tile {
-    Frags<T> x;
-    f32x4 g, f;
-};
-template <class T>
-SISA_DEV Tile<T> load_tile(const sisa_attn_weights_args& a, bool keys, int b, int h, int r0, int lane) {
-    const int r = r0 + 4 * (lane >> 4);
-    return Tile<T>{keys ? frags<T>(a.k, a.b, b, h, r0, a.L, lane) : frags<T>(a.q, a.c, b, h, r0, a.L, lane),
-                   gates4(a.g, b, h, r, a.L), gates4(a.f, b, h, r, a.L)};
-}
+// What the second pass starts its products from: -lse in units of q.k.
+SISA_DEV float start_of(float m, float l) { return -(m + __log2f(l)) * (1.f / SCALE); }
 
-// First pass. Keys go from the diagonal down, so that the running maximum is right early: a block whose maximum exceeds it
-// by less than 2^GROW leaves it as it is.
+// First pass. A block whose maximum exceeds the running one by less than 2^GROW leaves it as it is.
 constexpr float GROW = 16.f;
-template <class T>
-__global__ __launch_bounds__(64 * WG) void weights_lse_kernel(sisa_attn_weights_args a, int R, int nsplit, float* lse) {
+template <class T, bool FORGET>
+__global__ __launch_bounds__(64 * WG, 2) void weights_lse_kernel(sisa_attn_weights_args a, int R, int nsplit, float* start) {
     __shared__ float sm[WG][OWN], sl[WG][OWN];
+    __shared__ Buffer<T> bufs[WG];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int grp = lane >> 4, col = lane & 15, L = a.L, BH = a.B * a.H;
     // the longest blocks first, the heads side by side (with a multiple of 8 of them each stays on one XCD)
@@ -98,97 +173,127 @@ __global__ __launch_bounds__(64 * WG) void weights_lse_kernel(sisa_attn_weights_
     if (r0 >= rows.count) return;
     const int i0 = rows.first + r0;
     const float lam = a.lam[h * a.s_lam];
+    Buffer<T>* buf = bufs + w;
+    Stream<T> keys(a.k, a.b, a, b, h, nullptr, lane);
     Frags<T> q[4];
+    {
+        const Stream<T> own(a.q, a.c, a, b, h, nullptr, lane);
+        Raw<T> raw[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) raw[u] = own.load_edge(i0 + 16 * u, L);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) q[u] = turn<T, FORGET>(raw[u], buf, lane).x;
+    }
     float gi[4], fi[4], md[4], ld[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        q[u] = frags<T>(a.q, a.c, b, h, i0 + 16 * u, L, lane);
         gi[u] = gate(a.g, b, h, i0 + 16 * u + col, L);
         fi[u] = gate(a.f, b, h, i0 + 16 * u + col, L);
         md[u] = -__builtin_inff();
         ld[u] = 0.f;
     }
-    const float ga = gate(a.g, b, h, i0, L), fa = gate(a.f, b, h, i0, L);
     const int last = i0 + OWN < rows.n ? i0 + OWN : rows.n;          // keys 0 .. last - 1
-    const int tiles = (last + 15) / 16, below = (i0 + 1) / 16;       // tiles 0 .. below - 1 lie at or before i0
-    // tiles from the last down; split s takes a contiguous range of them, wave w every fourth
+    const int tiles = (last + 15) / 16;
+    // split s takes a contiguous range of the tiles, wave w every fourth; tiles up to `below` lie at or before i0
     const int per = (tiles + nsplit - 1) / nsplit;
-    const int t0 = tiles - 1 - split * per, t1 = t0 - per > -1 ? t0 - per : -1;
-    int t = t0 - w;
-    if (t > t1) {
-        Tile<T> now = load_tile<T>(a, true, b, h, 16 * t, lane);
-        for (; t > t1 && t >= below; t -= WG) {                      // meeting the diagonal
-            const int tn = t - WG > 0 ? t - WG : 0;
-            const Tile<T> next = load_tile<T>(a, true, b, h, 16 * tn, lane);
+    const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+    const int below = (i0 + 1) / 16 < t1 ? (i0 + 1) / 16 : t1;
+    for (int t = (below > t0 ? below : t0) + w; t < t1; t += WG) {   // meeting the diagonal
+        const Tile<T> k = turn<T, FORGET>(keys.load_edge(16 * t, L), buf, lane);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (16 * t > i0 + 16 * u + 15) continue;                 // all keys after all queries
+            const f32x4 qk = mma(k.x.x1, q[u].x1, mma(k.x.x0, q[u].x0, zero4())), cb = mma(k.x.s, q[u].s, zero4());
+            float x[4], mx = md[u];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float dec = lam * fast_exp2((gi[u] - k.g[e]) * LOG2E);
+                x[e] = (fmaf(qk[e], 0.125f, dec * cb[e]) + (fi[u] - k.f[e])) * LOG2E;
+                if (16 * t + 4 * grp + e > i0 + 16 * u + col) x[e] = -__builtin_inff();
+                mx = fmaxf(mx, x[e]);
+            }
+            const float ref = mx == -__builtin_inff() ? 0.f : mx;
+            ld[u] *= md[u] == -__builtin_inff() ? 1.f : fast_exp2(md[u] - ref);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ld[u] += fast_exp2(x[e] - ref);
+            md[u] = mx;
+        }
+    }
+    int left = (below - 1 - t0 - w) / WG + 1;                        // whole tiles of this wave, from the diagonal down
+    if (below - 1 - w >= t0) {
+        const float ga = gate(a.g, b, h, i0, L), fa = gate(a.f, b, h, i0, L);
+        // y = 8 score - 8 (F_i - F_a); sums of 2^(y SCALE - ref), the maximum so far in mo
+        float qg[4], mo[4], ref[4], lo[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            qg[u] = 8.f * lam * fast_exp2((gi[u] - ga) * LOG2E);
+            mo[u] = -__builtin_inff();
+            ref[u] = lo[u] = 0.f;
+        }
+        bool fresh = true;                                           // a maximum is still missing
+        keys.go(16 * (int64_t)(below - 1 - w));
+        auto add = [&](const Tile<T>& k) {
+            f32x4 kg, kf;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                kg[e] = fast_exp2((ga - k.g[e]) * LOG2E);
+                kf[e] = FORGET ? 8.f * (fa - k.f[e]) : 0.f;
+            }
+            f32x4 y[4];
+            float mx = -__builtin_inff();
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if (16 * t > i0 + 16 * u + 15) continue;             // all keys after all queries
-                const f32x4 qk = mma(now.x.x1, q[u].x1, mma(now.x.x0, q[u].x0, zero4())), cb = mma(now.x.s, q[u].s, zero4());
-                float x[4], mx = md[u];
+                const f32x4 cb = mma(k.x.s, q[u].s, zero4());
+                y[u] = mma(k.x.x1, q[u].x1, mma(k.x.x0, q[u].x0, kf));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float dec = lam * fast_exp2((gi[u] - now.g[e]) * LOG2E);
-                    x[e] = (fmaf(qk[e], 0.125f, dec * cb[e]) + (fi[u] - now.f[e])) * LOG2E;
-                    if (16 * t + 4 * grp + e > i0 + 16 * u + col) x[e] = -__builtin_inff();
-                    mx = fmaxf(mx, x[e]);
+                    y[u][e] = fmaf(fmaf(cb[e] * kg[e], qg[u], y[u][e]), SCALE, -ref[u]);
+                    mx = fmaxf(mx, y[u][e]);
                 }
-                const float ref = mx == -__builtin_inff() ? 0.f : mx;
-                ld[u] *= md[u] == -__builtin_inff() ? 1.f : fast_exp2(md[u] - ref);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ld[u] += fast_exp2(x[e] - ref);
-                md[u] = mx;
             }
-            now = next;
-        }
-        if (t > t1) {
-            // y = 8 score - 8 (F_i - F_a), the reference mo in log2 units
-            float qg[4], mo[4], lo[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                qg[u] = 8.f * lam * fast_exp2((gi[u] - ga) * LOG2E);
-                mo[u] = -__builtin_inff();
-                lo[u] = 0.f;
-            }
-            for (; t > t1; t -= WG) {
-                const int tn = t - WG > 0 ? t - WG : 0;
-                const Tile<T> next = load_tile<T>(a, true, b, h, 16 * tn, lane);
-                f32x4 kg, kf;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    kg[e] = fast_exp2((ga - now.g[e]) * LOG2E);
-                    kf[e] = 8.f * (fa - now.f[e]);
-                }
-                f32x4 y[4];
-                bool grow = false;
+            if (__any(fresh || mx > GROW)) {
+                asm volatile("");                                    // rarely: not to be worked out beforehand
+                fresh = false;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const f32x4 cb = mma(now.x.s, q[u].s, zero4());
-                    y[u] = mma(now.x.x1, q[u].x1, mma(now.x.x0, q[u].x0, kf));
+                    const float to = fmaxf(mo[u], fmaxf(fmaxf(y[u][0], y[u][1]), fmaxf(y[u][2], y[u][3])) + ref[u]);
+                    const float by = ref[u] - (to == -__builtin_inff() ? 0.f : to);
+                    if (lo[u] != 0.f) lo[u] *= fast_exp2(by);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) y[u][e] = fmaf(cb[e] * kg[e], qg[u], y[u][e]);
-                    const float mx = fmaxf(fmaxf(y[u][0], y[u][1]), fmaxf(y[u][2], y[u][3]));
-                    grow |= mx * SCALE > mo[u] + GROW;
+                    for (int e = 0; e < 4; ++e) y[u][e] += by;
+                    mo[u] = to;
+                    ref[u] -= by;
+                    fresh |= to == -__builtin_inff();
                 }
-                if (__any(grow)) {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const float mx = SCALE * fmaxf(fmaxf(y[u][0], y[u][1]), fmaxf(y[u][2], y[u][3]));
-                        const float to = fmaxf(mo[u], mx);
-                        lo[u] *= mo[u] == -__builtin_inff() ? 1.f : fast_exp2(mo[u] - to);
-                        mo[u] = to;
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float ref = mo[u] == -__builtin_inff() ? 0.f : mo[u];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) lo[u] += fast_exp2(fmaf(y[u][e], SCALE, -ref));
-                }
-                now = next;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) merge(md[u], ld[u], mo[u] + (fi[u] - fa) * LOG2E, lo[u]);
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) lo[u] += fast_exp2(y[u][e]);
+        };
+        // Two tiles ahead in memory, one in LDS; the last one's loads are its own again.
+        auto next = [&]() {
+            if (--left > 0) keys.go(-16 * WG);
+            return keys.load();
+        };
+        Raw<T> raw = keys.load();
+        Tile<T> even = turn<T, FORGET>(raw, buf, lane);
+        raw = next();
+        while (true) {
+            const bool more = left > 0;
+            const Tile<T> odd = turn<T, FORGET>(raw, buf, lane);
+            raw = next();
+            add(even);
+            if (!more) break;
+            const bool yet = left > 0;
+            even = turn<T, FORGET>(raw, buf, lane);
+            raw = next();
+            add(odd);
+            if (!yet) break;
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            merge(md[u], ld[u], (mo[u] == -__builtin_inff() ? mo[u] : ref[u]) + (fi[u] - fa) * LOG2E, lo[u]);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -204,91 +309,127 @@ __global__ __launch_bounds__(64 * WG) void weights_lse_kernel(sisa_attn_weights_
     for (int k = 1; k < WG; ++k) merge(mt, lt, sm[k][lane], sl[k][lane]);
     const int Rp = (R + 15) / 16 * 16;
     if (nsplit == 1) {
-        lse[(int64_t)bh * Rp + r] = mt + __log2f(lt);
+        start[(int64_t)bh * Rp + r] = start_of(mt, lt);
     } else {
-        float* part = lse + (int64_t)BH * Rp + 2 * (((int64_t)bh * Rp + r) * nsplit + split);
+        float* part = start + (int64_t)BH * Rp + 2 * (((int64_t)bh * Rp + r) * nsplit + split);
         part[0] = mt;
         part[1] = lt;
     }
 }
 
-// lse of rows whose keys were split: a wave per row, split k with lane k mod 64, the lanes in a fixed tree
-__global__ __launch_bounds__(256) void weights_merge_kernel(int64_t rows, int nsplit, float* lse) {
+// The starts of rows whose keys were split: a wave per row, split k with lane k mod 64, the lanes in a fixed tree.
+__global__ __launch_bounds__(256) void weights_merge_kernel(int64_t rows, int nsplit, float* start) {
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     if (r >= rows) return;
-    const float* part = lse + rows + 2 * r * nsplit;
+    const float* part = start + rows + 2 * r * nsplit;
     float m = -__builtin_inff(), l = 0.f;
     for (int k = lane; k < nsplit; k += 64) merge(m, l, part[2 * k], part[2 * k + 1]);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) merge(m, l, __shfl_xor(m, o), __shfl_xor(l, o));
-    if (lane == 0) lse[r] = m + __log2f(l);
+    if (lane == 0) start[r] = start_of(m, l);
 }
 
 // Second pass. SHARE waves of a workgroup have the same 64 keys and take every SHARE-th query tile; four, or one where so
 // few queries are counted that the keys' loads weigh more.
-template <class T, int SHARE>
-__global__ __launch_bounds__(64 * WG) void weights_sum_kernel(sisa_attn_weights_args a, int R, const float* lse) {
+template <class T, bool FORGET, int SHARE>
+__global__ __launch_bounds__(64 * WG, 2) void weights_sum_kernel(sisa_attn_weights_args a, int R, const float* start) {
     __shared__ float part[WG][OWN];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ Buffer<T> bufs[WG];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ws = w % SHARE;
     const int grp = lane >> 4, col = lane & 15, L = a.L, BH = a.B * a.H;
     const int bh = blockIdx.x % BH, h = bh % a.H, b = bh / a.H;
     const int j0 = (blockIdx.x / BH * (WG / SHARE) + w / SHARE) * OWN;
     const Rows rows = rows_of(a, b);
     const float lam = a.lam[h * a.s_lam];
-    const float* le0 = lse + (int64_t)bh * ((R + 15) / 16 * 16) + 4 * grp;
+    Buffer<T>* buf = bufs + w;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    // 16-query tiles of the window from the first that reaches j0: those that meet the diagonal, whole ones, the last one
     const int from = j0 > rows.first ? (j0 - rows.first) / 16 : 0, tiles = (rows.count + 15) / 16;
-    int t = from + w % SHARE;
-    if (j0 < rows.n && t < tiles) {
-        Tile<T> now = load_tile<T>(a, false, b, h, rows.first + 16 * t, lane);
-        f32x4 le = *reinterpret_cast<const f32x4*>(le0 + 16 * t);
+    if (j0 < rows.n && from < tiles) {
+        Stream<T> queries(a.q, a.c, a, b, h, start + (int64_t)bh * ((R + 15) / 16 * 16), lane);
         Frags<T> k[4];
-        float gj[4], fj[4], kg[4], kf[4];
-        const float ga = gate(a.g, b, h, j0 + OWN - 1, L), fa = gate(a.f, b, h, j0 + OWN - 1, L);
+        {
+            const Stream<T> own(a.k, a.b, a, b, h, nullptr, lane);
+            Raw<T> raw[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) raw[u] = own.load_edge(j0 + 16 * u, L);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) k[u] = turn<T, FORGET>(raw[u], buf, lane).x;
+        }
+        float gj[4], fj[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            k[u] = frags<T>(a.k, a.b, b, h, j0 + 16 * u, L, lane);
             gj[u] = gate(a.g, b, h, j0 + 16 * u + col, L);
             fj[u] = gate(a.f, b, h, j0 + 16 * u + col, L);
-            kg[u] = lam * LOG2E * fast_exp2((ga - gj[u]) * LOG2E);
-            kf[u] = (fa - fj[u]) * LOG2E;
         }
-        for (; t < tiles; t += SHARE) {
-            const int i0 = rows.first + 16 * t, tn = t + SHARE < tiles ? t + SHARE : t;
-            const Tile<T> next = load_tile<T>(a, false, b, h, rows.first + 16 * tn, lane);
-            const f32x4 le_next = *reinterpret_cast<const f32x4*>(le0 + 16 * tn);
-            if (i0 >= j0 + OWN - 1 && i0 + 16 <= rows.n) {
+        const int clear = j0 + OWN - 1 - rows.first;                 // the first row that sees every key of the block
+        int w0 = clear > 0 ? (clear + 15) / 16 : 0, w1 = rows.count / 16;
+        w0 = w0 < from ? from : w0 < tiles ? w0 : tiles;
+        w1 = w1 < w0 ? w0 : w1;
+        const int edges = w0 - from + tiles - w1;
+        for (int e0 = ws; e0 < edges; e0 += SHARE) {
+            const int t = e0 < w0 - from ? from + e0 : w1 + e0 - (w0 - from), i0 = rows.first + 16 * t;
+            const Tile<T> q = turn<T, FORGET>(queries.load_edge(i0, L, 16 * t), buf, lane);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (j0 + 16 * u > i0 + 15) continue;                 // all keys after all queries
+                const f32x4 qk = mma(q.x.x1, k[u].x1, mma(q.x.x0, k[u].x0, zero4())), cb = mma(q.x.s, k[u].s, zero4());
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = i0 + 4 * grp + e;
+                    const float dec = lam * fast_exp2((q.g[e] - gj[u]) * LOG2E);
+                    const float x = fmaf(qk[e], 0.125f, dec * cb[e]) + (q.f[e] - fj[u]);
+                    const float p = fast_exp2(fmaf(x, LOG2E, q.st[e] * SCALE));
+                    sum[u] += i >= j0 + 16 * u + col && i < rows.n ? p : 0.f;
+                }
+            }
+        }
+        int left = w0 + ws < w1 ? (w1 - 1 - w0 - ws) / SHARE + 1 : 0;
+        if (left > 0) {
+            const float ga = gate(a.g, b, h, j0 + OWN - 1, L), fa = gate(a.f, b, h, j0 + OWN - 1, L);
+            float kg[4], kf[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                kg[u] = lam * LOG2E * fast_exp2((ga - gj[u]) * LOG2E);
+                kf[u] = (fa - fj[u]) * LOG2E;
+            }
+            queries.go(rows.first + 16 * (int64_t)(w0 + ws));
+            if (queries.starts) queries.gate -= rows.first;
+            auto add = [&](const Tile<T>& q) {
                 f32x4 rg, rc;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    rg[e] = fast_exp2((now.g[e] - ga) * LOG2E);
-                    rc[e] = fmaf(now.f[e] - fa, LOG2E, -le[e]);
+                    rg[e] = fast_exp2((q.g[e] - ga) * LOG2E);
+                    rc[e] = FORGET ? fmaf(q.f[e] - fa, 8.f, q.st[e]) : q.st[e];
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const f32x4 qk = mma(now.x.x1, k[u].x1, mma(now.x.x0, k[u].x0, zero4())), cb = mma(now.x.s, k[u].s, zero4());
+                    const f32x4 qk = mma(q.x.x1, k[u].x1, mma(q.x.x0, k[u].x0, rc)), cb = mma(q.x.s, k[u].s, zero4());
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        sum[u] += fast_exp2(fmaf(cb[e] * kg[u], rg[e], fmaf(qk[e], SCALE, kf[u])) + rc[e]);
+                    for (int e = 0; e < 4; ++e) sum[u] += fast_exp2(fmaf(cb[e] * kg[u], rg[e], fmaf(qk[e], SCALE, kf[u])));
                 }
-            } else {
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    if (j0 + 16 * u > i0 + 15) continue;             // all keys after all queries
-                    const f32x4 qk = mma(now.x.x1, k[u].x1, mma(now.x.x0, k[u].x0, zero4())), cb = mma(now.x.s, k[u].s, zero4());
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int i = i0 + 4 * grp + e;
-                        const float dec = lam * fast_exp2((now.g[e] - gj[u]) * LOG2E);
-                        const float x = fmaf(qk[e], 0.125f, dec * cb[e]) + (now.f[e] - fj[u]);
-                        const float p = fast_exp2(fmaf(x, LOG2E, -le[e]));
-                        sum[u] += i >= j0 + 16 * u + col && i < rows.n ? p : 0.f;
-                    }
-                }
+            };
+            // two tiles ahead in memory, one in LDS; the last one's loads are its own again
+            auto next = [&]() {
+                if (--left > 0) queries.go(16 * SHARE);
+                return queries.load();
+            };
+            Raw<T> raw = queries.load();
+            Tile<T> even = turn<T, FORGET>(raw, buf, lane);
+            raw = next();
+            while (true) {
+                const bool more = left > 0;
+                const Tile<T> odd = turn<T, FORGET>(raw, buf, lane);
+                raw = next();
+                add(even);
+                if (!more) break;
+                const bool yet = left > 0;
+                even = turn<T, FORGET>(raw, buf, lane);
+                raw = next();
+                add(odd);
+                if (!yet) break;
             }
-            now = next;
-            le = le_next;
         }
     }
 #pragma unroll
@@ -299,7 +440,7 @@ __global__ __launch_bounds__(64 * WG) void weights_sum_kernel(sisa_attn_weights_
     }
     __syncthreads();
     const int j = j0 + lane;
-    if (w % SHARE || j >= L) return;
+    if (ws || j >= L) return;
     float s = part[w][lane];
 #pragma unroll
     for (int k = 1; k < SHARE; ++k) s += part[w + k][lane];
@@ -320,23 +461,31 @@ int splits_of(int64_t BH, int32_t L, int32_t R) {
 // Up to this many query tiles each wave of the second pass has keys of its own.
 constexpr int FEW_TILES = 16;
 
-template <class T>
+template <class T, bool FORGET>
 int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
     const int R = window_of(a->L, a->window);
     const int64_t BH = (int64_t)a->B * a->H;
     const int nsplit = splits_of(BH, a->L, R);
-    float* lse = (float*)a->workspace;
-    weights_lse_kernel<T><<<(unsigned)(BH * sisa::cdiv(R, OWN) * nsplit), 64 * WG, 0, st>>>(*a, R, nsplit, lse);
+    float* start = (float*)a->workspace;
+    const unsigned grid = (unsigned)(BH * sisa::cdiv(R, OWN) * nsplit);
+    weights_lse_kernel<T, FORGET><<<grid, 64 * WG, 0, st>>>(*a, R, nsplit, start);
     int rc = sisa::launch_status("sisa_attn_weights (rows)");
     if (rc) return rc;
     if (nsplit > 1) {
-        weights_merge_kernel<<<(unsigned)sisa::cdiv(BH * pad16(R), 4), 256, 0, st>>>(BH * pad16(R), nsplit, lse);
+        const int64_t rows = BH * pad16(R);
+        weights_merge_kernel<<<(unsigned)sisa::cdiv(rows, 4), 256, 0, st>>>(rows, nsplit, start);
         rc = sisa::launch_status("sisa_attn_weights (merge)");
         if (rc) return rc;
     }
-    if (R <= 16 * FEW_TILES) weights_sum_kernel<T, 1><<<(unsigned)(BH * sisa::cdiv(a->L, OWN * WG)), 64 * WG, 0, st>>>(*a, R, lse);
-    else weights_sum_kernel<T, WG><<<(unsigned)(BH * sisa::cdiv(a->L, OWN)), 64 * WG, 0, st>>>(*a, R, lse);
+    if (R <= 16 * FEW_TILES)
+        weights_sum_kernel<T, FORGET, 1><<<(unsigned)(BH * sisa::cdiv(a->L, OWN * WG)), 64 * WG, 0, st>>>(*a, R, start);
+    else weights_sum_kernel<T, FORGET, WG><<<(unsigned)(BH * sisa::cdiv(a->L, OWN)), 64 * WG, 0, st>>>(*a, R, start);
     return sisa::launch_status("sisa_attn_weights");
+}
+
+template <class T>
+int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
+    return a->f.ptr ? launch_weights<T, true>(a, st) : launch_weights<T, false>(a, st);
 }
 
 }  // namespace
@@ -357,7 +506,13 @@ extern "C" int sisa_attn_weights(const sisa_attn_weights_args* a, void* stream) 
     SISA_REQUIRE(sisa::view_ok(a->q, a->dtype) && sisa::view_ok(a->k, a->dtype) && sisa::view_ok(a->c, a->dtype) &&
                      sisa::view_ok(a->b, a->dtype),
                  "sisa_attn_weights: q, k, c and b rows must be 16-byte aligned");
-    SISA_REQUIRE(a->g.ptr && a->lam && a->out && a->workspace, "sisa_attn_weights: null pointer");
+    const sisa_view* rows[] = {&a->q, &a->k, &a->c, &a->b};
+    for (const sisa_view* v : rows)
+        SISA_REQUIRE(v->sl >= 0 && v->sl < SISA_ATTN_WEIGHTS_MAX_STRIDE,
+                     "sisa_attn_weights: position strides must be in 0 .. %d elements", SISA_ATTN_WEIGHTS_MAX_STRIDE - 1);
+    SISA_REQUIRE(a->g.ptr && a->lam && a->out && a->workspace && ((uintptr_t)a->workspace & 15) == 0,
+                 "sisa_attn_weights: null pointer, or workspace not 16-byte aligned");
+    SISA_REQUIRE(a->g.sl == 1 && (!a->f.ptr || a->f.sl == 1), "sisa_attn_weights: g and f must be contiguous along positions");
     const int64_t BH = (int64_t)a->B * a->H;
     SISA_REQUIRE(BH * sisa::cdiv(a->L, 64) < ((int64_t)1 << 26), "sisa_attn_weights: B*H*L too large for one launch");
     hipStream_t st = (hipStream_t)stream;

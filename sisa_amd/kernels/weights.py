@@ -12,6 +12,8 @@ from .paged import _DTYPES, _int32, no_grad_wanted, readable
 
 __all__ = ["sisa_attention_weights_hip"]
 
+MAX_STRIDE = 1 << 24           # SISA_ATTN_WEIGHTS_MAX_STRIDE
+
 
 def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor,
                                fgate: Tensor | None = None, *, lengths: Tensor | None = None,
@@ -48,7 +50,9 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     out = torch.empty((B, H, L), device=q.device, dtype=torch.float32)
     if not out.numel():
         return out
-    q, k, c, b = (readable(t) for t in (q, k, c, b))
+    q, k, c, b = (readable(t) if 0 <= t.stride(2) < MAX_STRIDE else t.clone(memory_format=torch.contiguous_format)
+                  for t in (q, k, c, b))
+    g, fgate = (t if t is None or t.stride(2) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (g, fgate))
     window = 0 if window is None or window >= L else window
     ws = torch.empty(_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window), device=q.device, dtype=torch.uint8)
     _lib.call("sisa_attn_weights", _lib.AttnWeightsArgs(
