@@ -22,7 +22,7 @@
 namespace {
 
 constexpr int DH = 64, DS = 32;
-constexpr int WG = 4;                 // waves per workgroup
+constexpr int FEW_ROWS = 256;         // query rows up to which, against four times as many keys, each wave has its own keys
 constexpr int OWN = 64;               // queries (keys) that a wave holds: four blocks of 16
 constexpr float SCALE = LOG2E / 8;    // of q.k into log2 units
 
@@ -160,10 +160,12 @@ SISA_DEV float start_of(float m, float l) { return -(m + __log2f(l)) * (1.f / SC
 
 // First pass. A block whose maximum exceeds the running one by less than 2^GROW leaves it as it is.
 constexpr float GROW = 16.f;
-template <class T, bool FORGET>
-__global__ __launch_bounds__(64 * WG, 2) void weights_lse_kernel(sisa_attn_weights_args a, int R, int nsplit, float* start) {
-    __shared__ float sm[WG][OWN], sl[WG][OWN];
-    __shared__ Buffer<T> bufs[WG];
+// With `parts`, a row's maximum and sum over the split's keys are left for the second pass to join.
+template <class T, bool FORGET, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_kernel(sisa_attn_weights_args a, int R, int nsplit,
+                                                                                     float* start, f32x2* parts) {
+    __shared__ float sm[NW][OWN], sl[NW][OWN];
+    __shared__ Buffer<T> bufs[NW];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int grp = lane >> 4, col = lane & 15, L = a.L, BH = a.B * a.H;
     // the longest blocks first, the heads side by side (with a multiple of 8 of them each stays on one XCD)
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_lse_kernel(sisa_attn_weigh
     const int per = (tiles + nsplit - 1) / nsplit;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
     const int below = (i0 + 1) / 16 < t1 ? (i0 + 1) / 16 : t1;
-    for (int t = (below > t0 ? below : t0) + w; t < t1; t += WG) {   // meeting the diagonal
+    for (int t = (below > t0 ? below : t0) + w; t < t1; t += NW) {   // meeting the diagonal
         const Tile<T> k = turn<T, FORGET>(keys.load_edge(16 * t, L), buf, lane);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_lse_kernel(sisa_attn_weigh
             md[u] = mx;
         }
     }
-    int left = (below - 1 - t0 - w) / WG + 1;                        // whole tiles of this wave, from the diagonal down
+    int left = (below - 1 - t0 - w) / NW + 1;                        // whole tiles of this wave, from the diagonal down
     if (below - 1 - w >= t0) {
         const float ga = gate(a.g, b, h, i0, L), fa = gate(a.f, b, h, i0, L);
         // y = 8 score - 8 (F_i - F_a); sums of 2^(y SCALE - ref), the maximum so far in mo
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_lse_kernel(sisa_attn_weigh
         };
         // Two tiles ahead in memory, one in LDS; the last one's loads are its own again.
         auto next = [&]() {
-            if (--left > 0) keys.go(-16 * WG);
+            if (--left > 0) keys.go(-16 * NW);
             return keys.load();
         };
         Raw<T> raw = keys.load();
@@ -306,48 +308,45 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_lse_kernel(sisa_attn_weigh
     if (w != 0 || r >= rows.count) return;
     float mt = sm[0][lane], lt = sl[0][lane];
 #pragma unroll
-    for (int k = 1; k < WG; ++k) merge(mt, lt, sm[k][lane], sl[k][lane]);
-    const int Rp = (R + 15) / 16 * 16;
-    if (nsplit == 1) {
-        start[(int64_t)bh * Rp + r] = start_of(mt, lt);
-    } else {
-        float* part = start + (int64_t)BH * Rp + 2 * (((int64_t)bh * Rp + r) * nsplit + split);
-        part[0] = mt;
-        part[1] = lt;
-    }
+    for (int k = 1; k < NW; ++k) merge(mt, lt, sm[k][lane], sl[k][lane]);
+    const int64_t at = (int64_t)bh * ((R + 15) / 16 * 16) + r;
+    if (parts) parts[at * nsplit + split] = f32x2{mt, lt};
+    else start[at] = start_of(mt, lt);
 }
 
-// The starts of rows whose keys were split: a wave per row, split k with lane k mod 64, the lanes in a fixed tree.
-__global__ __launch_bounds__(256) void weights_merge_kernel(int64_t rows, int nsplit, float* start) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (r >= rows) return;
-    const float* part = start + rows + 2 * r * nsplit;
-    float m = -__builtin_inff(), l = 0.f;
-    for (int k = lane; k < nsplit; k += 64) merge(m, l, part[2 * k], part[2 * k + 1]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) merge(m, l, __shfl_xor(m, o), __shfl_xor(l, o));
-    if (lane == 0) start[r] = start_of(m, l);
-}
-
-// Second pass. SHARE waves of a workgroup have the same 64 keys and take every SHARE-th query tile; four, or one where so
-// few queries are counted that the keys' loads weigh more.
-template <class T, bool FORGET, int SHARE>
-__global__ __launch_bounds__(64 * WG, 2) void weights_sum_kernel(sisa_attn_weights_args a, int R, const float* start) {
-    __shared__ float part[WG][OWN];
-    __shared__ Buffer<T> bufs[WG];
+// Second pass. SHARE of a workgroup's NW waves have the same 64 keys and take every SHARE-th query tile: all of them, or one
+// where so few queries are counted that the keys' loads weigh more (then the rows' parts from the first pass are joined here,
+// in the order of the splits, by every workgroup: at most 256 rows of 32 parts).
+template <class T, bool FORGET, int NW, int SHARE>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_kernel(sisa_attn_weights_args a, int R, int nsplit,
+                                                                                     const float* start, const f32x2* parts) {
+    constexpr bool FEW = SHARE == 1;
+    __shared__ float part[NW][OWN];
+    __shared__ float starts[FEW ? FEW_ROWS : 4];
+    __shared__ Buffer<T> bufs[NW];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ws = w % SHARE;
     const int grp = lane >> 4, col = lane & 15, L = a.L, BH = a.B * a.H;
     const int bh = blockIdx.x % BH, h = bh % a.H, b = bh / a.H;
-    const int j0 = (blockIdx.x / BH * (WG / SHARE) + w / SHARE) * OWN;
+    const int j0 = (blockIdx.x / BH * (NW / SHARE) + w / SHARE) * OWN;
     const Rows rows = rows_of(a, b);
     const float lam = a.lam[h * a.s_lam];
     Buffer<T>* buf = bufs + w;
+    const int Rp = (R + 15) / 16 * 16;
+    if constexpr (FEW) {
+        for (int r = threadIdx.x; r < rows.count; r += 64 * NW) {
+            const f32x2* p = parts + ((int64_t)bh * Rp + r) * nsplit;
+            float m = p[0][0], l = p[0][1];
+#pragma unroll 4
+            for (int k = 1; k < nsplit; ++k) merge(m, l, p[k][0], p[k][1]);
+            starts[r] = start_of(m, l);
+        }
+        __syncthreads();
+    }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     // 16-query tiles of the window from the first that reaches j0: those that meet the diagonal, whole ones, the last one
     const int from = j0 > rows.first ? (j0 - rows.first) / 16 : 0, tiles = (rows.count + 15) / 16;
     if (j0 < rows.n && from < tiles) {
-        Stream<T> queries(a.q, a.c, a, b, h, start + (int64_t)bh * ((R + 15) / 16 * 16), lane);
+        Stream<T> queries(a.q, a.c, a, b, h, FEW ? nullptr : start + (int64_t)bh * Rp, lane);
         Frags<T> k[4];
         {
             const Stream<T> own(a.k, a.b, a, b, h, nullptr, lane);
@@ -370,7 +369,8 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_sum_kernel(sisa_attn_weigh
         const int edges = w0 - from + tiles - w1;
         for (int e0 = ws; e0 < edges; e0 += SHARE) {
             const int t = e0 < w0 - from ? from + e0 : w1 + e0 - (w0 - from), i0 = rows.first + 16 * t;
-            const Tile<T> q = turn<T, FORGET>(queries.load_edge(i0, L, 16 * t), buf, lane);
+            Tile<T> q = turn<T, FORGET>(queries.load_edge(i0, L, 16 * t), buf, lane);
+            if constexpr (FEW) q.st = lds4f(starts + 16 * t + 4 * grp);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 if (j0 + 16 * u > i0 + 15) continue;                 // all keys after all queries
@@ -396,7 +396,9 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_sum_kernel(sisa_attn_weigh
             }
             queries.go(rows.first + 16 * (int64_t)(w0 + ws));
             if (queries.starts) queries.gate -= rows.first;
-            auto add = [&](const Tile<T>& q) {
+            const float* st = starts + 16 * (w0 + ws) + 4 * grp;      // of the tile that is used next
+            auto add = [&](Tile<T> q) {
+                if constexpr (FEW) q.st = lds4f(st), st += 16 * SHARE;
                 f32x4 rg, rc;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -447,53 +449,59 @@ __global__ __launch_bounds__(64 * WG, 2) void weights_sum_kernel(sisa_attn_weigh
     a.out[(int64_t)bh * L + j] = j < rows.n ? s : 0.f;
 }
 
-int window_of(int32_t L, int32_t window) { return window && window < L ? window : L; }
+// How a call is laid out. A chip of 256 CUs that the 64-row blocks of the queries do not fill gets the keys of the first pass
+// in splits (where few rows are counted: the second pass joins them; of 256 keys at least, 32 at most), or workgroups of
+// twice the waves.
+struct Plan {
+    int R, nsplit, waves;
+    bool few;
+    int64_t Rp, bytes;
+};
 
-int64_t pad16(int64_t R) { return (R + 15) / 16 * 16; }
-
-// Splits of the keys in the first pass: enough workgroups for the chip where few queries are counted, of 256 keys at least.
-int splits_of(int64_t BH, int32_t L, int32_t R) {
-    const int64_t groups = BH * sisa::cdiv(R, OWN), most = sisa::cdiv(L, 256);
-    const int64_t want = groups >= 1024 ? 1 : sisa::cdiv(1024, groups);
-    return (int)(want < most ? want : most);
+Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
+    Plan p{};
+    p.R = window && window < L ? window : L;
+    p.Rp = (p.R + 15) / 16 * 16;
+    p.few = p.R <= FEW_ROWS && L / 4 >= p.R;
+    const int64_t BH = (int64_t)B * H, groups = BH * sisa::cdiv(p.R, OWN);
+    p.waves = groups < 256 ? 8 : 4;
+    p.nsplit = 1;
+    if (p.few && groups < 256) {
+        const int64_t want = 256 / groups, most = sisa::cdiv(L, 256);
+        p.nsplit = (int)(want < most ? want : most);
+        p.nsplit = p.nsplit < 32 ? p.nsplit : 32;
+    }
+    p.bytes = BH * p.Rp * (p.few ? 8 * (int64_t)p.nsplit : 4);
+    return p;
 }
 
-// Up to this many query tiles each wave of the second pass has keys of its own.
-constexpr int FEW_TILES = 16;
-
-template <class T, bool FORGET>
-int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
-    const int R = window_of(a->L, a->window);
+template <class T, bool FORGET, int NW>
+int launch_weights(const sisa_attn_weights_args* a, const Plan& p, hipStream_t st) {
     const int64_t BH = (int64_t)a->B * a->H;
-    const int nsplit = splits_of(BH, a->L, R);
-    float* start = (float*)a->workspace;
-    const unsigned grid = (unsigned)(BH * sisa::cdiv(R, OWN) * nsplit);
-    weights_lse_kernel<T, FORGET><<<grid, 64 * WG, 0, st>>>(*a, R, nsplit, start);
-    int rc = sisa::launch_status("sisa_attn_weights (rows)");
+    float* start = p.few ? nullptr : (float*)a->workspace;
+    f32x2* parts = p.few ? (f32x2*)a->workspace : nullptr;
+    const unsigned grid = (unsigned)(BH * sisa::cdiv(p.R, OWN) * p.nsplit);
+    weights_lse_kernel<T, FORGET, NW><<<grid, 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    const int rc = sisa::launch_status("sisa_attn_weights (rows)");
     if (rc) return rc;
-    if (nsplit > 1) {
-        const int64_t rows = BH * pad16(R);
-        weights_merge_kernel<<<(unsigned)sisa::cdiv(rows, 4), 256, 0, st>>>(rows, nsplit, start);
-        rc = sisa::launch_status("sisa_attn_weights (merge)");
-        if (rc) return rc;
-    }
-    if (R <= 16 * FEW_TILES)
-        weights_sum_kernel<T, FORGET, 1><<<(unsigned)(BH * sisa::cdiv(a->L, OWN * WG)), 64 * WG, 0, st>>>(*a, R, start);
-    else weights_sum_kernel<T, FORGET, WG><<<(unsigned)(BH * sisa::cdiv(a->L, OWN)), 64 * WG, 0, st>>>(*a, R, start);
+    if (p.few)
+        weights_sum_kernel<T, FORGET, 4, 1><<<(unsigned)(BH * sisa::cdiv(a->L, OWN * 4)), 256, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    else weights_sum_kernel<T, FORGET, NW, NW><<<(unsigned)(BH * sisa::cdiv(a->L, OWN)), 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     return sisa::launch_status("sisa_attn_weights");
 }
 
 template <class T>
 int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
-    return a->f.ptr ? launch_weights<T, true>(a, st) : launch_weights<T, false>(a, st);
+    const Plan p = plan_of(a->B, a->H, a->L, a->window);
+    if (p.waves == 8) return a->f.ptr ? launch_weights<T, true, 8>(a, p, st) : launch_weights<T, false, 8>(a, p, st);
+    return a->f.ptr ? launch_weights<T, true, 4>(a, p, st) : launch_weights<T, false, 4>(a, p, st);
 }
 
 }  // namespace
 
 extern "C" int64_t sisa_attn_weights_workspace_bytes(int32_t B, int32_t H, int32_t L, int32_t window) {
     if (B < 1 || H < 1 || L < 1 || window < 0) return 0;
-    const int R = window_of(L, window), nsplit = splits_of((int64_t)B * H, L, R);
-    return (int64_t)B * H * pad16(R) * (nsplit > 1 ? 1 + 2 * nsplit : 1) * (int64_t)sizeof(float);
+    return plan_of(B, H, L, window).bytes;
 }
 
 extern "C" int sisa_attn_weights(const sisa_attn_weights_args* a, void* stream) {
