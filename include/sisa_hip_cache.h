@@ -51,7 +51,7 @@ int sisa_paged_write(const sisa_paged_write_args* a, void* stream);
  * A row without a position (a sequence of no positions, or of fewer than M) is 0. The rows of a sequence whose length is
  * negative or above max_len or W pages, or one of whose pages is not in the pool, are NaN (its w_out is left as it is for
  * such a length, and NaN for such a page). max_len bounds the lengths for the launch: at most W * page_size. Workspace:
- * sisa_paged_decode_workspace_bytes(B, H, M, max_len, whether w_out is given). */
+ * sisa_paged_decode_workspace_bytes(B, H, M, max_len, dtype, whether w_out is given), which may be none. */
 typedef struct {
     int32_t B, M, W, max_len;
     sisa_page_pool pool;
@@ -62,10 +62,10 @@ typedef struct {
     const float* lam; int64_t s_lam;           /* (H) fp32 */
     sisa_view w_in, w_out;     /* (B,H,max_len) fp32, or both NULL */
     float* out;                /* (B,H,M,64) contiguous */
-    void* workspace;
+    void* workspace;           /* 16-byte aligned; NULL where none is needed */
 } sisa_paged_decode_args;
 
-int64_t sisa_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t max_len, int32_t tracked);
+int64_t sisa_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t max_len, int32_t dtype, int32_t tracked);
 int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream);
 
 /* The softmax weights that each position j of a prompt receives from the last `window` queries of its sequence (0: from

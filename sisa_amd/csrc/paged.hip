@@ -298,6 +298,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
     }
 }
 
+// Caches that one workgroup takes whole need no join (tracked weights: with one query row, the only one to add to them).
+bool takes_whole(int M, int64_t max_len, int elem, bool tracked) {
+    return max_len <= TILE * (elem == 2 ? whole_waves<__bf16>() : whole_waves<float>()) && (!tracked || M == 1);
+}
+
 struct DecodeSpace {
     f32x2* stat;
     float *part, *scores;
@@ -321,10 +326,8 @@ int launch_decode(const sisa_paged_decode_args* a, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size), nchunk = (int)sisa::cdiv(a->max_len, KCH);
     const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
     const DecodeSpace ws = decode_space((char*)a->workspace, rows, a->max_len, TRACK);
-    // Caches that one workgroup takes whole need no join (tracked weights: with one query row, which is the only one to add
-    // to them).
     constexpr int NW = whole_waves<T>();
-    if (a->max_len <= TILE * NW && (!TRACK || a->M == 1)) {
+    if (takes_whole(a->M, a->max_len, (int)sizeof(T), TRACK)) {
         paged_chunk_kernel<T, NW, true, TRACK, false><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, shift, 1, ws.stat, ws.part, ws.scores);
         return sisa::launch_status("sisa_paged_decode");
     }
@@ -369,8 +372,9 @@ extern "C" int sisa_paged_write(const sisa_paged_write_args* a, void* stream) {
     return sisa::launch_status("sisa_paged_write");
 }
 
-extern "C" int64_t sisa_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t max_len, int32_t tracked) {
-    if (B < 1 || H < 1 || M < 1 || max_len < 1) return 0;
+extern "C" int64_t sisa_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t max_len, int32_t dtype,
+                                                     int32_t tracked) {
+    if (B < 1 || H < 1 || M < 1 || max_len < 1 || takes_whole(M, max_len, sisa::elem_size(dtype), tracked != 0)) return 0;
     return decode_space(nullptr, (int64_t)B * H * M, max_len, tracked != 0).bytes;
 }
 
@@ -382,7 +386,10 @@ extern "C" int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream) 
                  "sisa_paged_decode: bad shape B=%d M=%d W=%d max_len=%d (at most W pages of %d, and 2^30)", a->B, a->M, a->W,
                  a->max_len, a->pool.page_size);
     if (a->B == 0) return SISA_OK;
-    SISA_REQUIRE(a->table && a->lengths && a->lam && a->out && a->workspace, "sisa_paged_decode: null pointer");
+    SISA_REQUIRE(a->table && a->lengths && a->lam && a->out, "sisa_paged_decode: null pointer");
+    SISA_REQUIRE(takes_whole(a->M, a->max_len, sisa::elem_size(a->pool.dtype), a->w_out.ptr != nullptr) ||
+                     (a->workspace && sisa::aligned16(a->workspace)),
+                 "sisa_paged_decode: null workspace, or not 16-byte aligned");
     SISA_REQUIRE(sisa::view_ok(a->q, a->pool.dtype) && sisa::view_ok(a->c, a->pool.dtype),
                  "sisa_paged_decode: q and c rows must be 16-byte aligned");
     SISA_REQUIRE(a->gq.ptr && (a->fq.ptr == nullptr) == (a->pool.f.ptr == nullptr),

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
@@ -238,7 +239,7 @@ CE_SIGNATURES = {
 # caches in pages (include/sisa_hip_cache.h)
 CACHE_SIGNATURES = {
     "sisa_paged_write": ([POINTER(PagedWriteArgs), c_void_p], c_int),
-    "sisa_paged_decode_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32, c_int32], c_int64),
+    "sisa_paged_decode_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32, c_int32, c_int32], c_int64),
     "sisa_paged_decode": ([POINTER(PagedDecodeArgs), c_void_p], c_int),
     "sisa_attn_weights_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32], c_int64),
     "sisa_attn_weights": ([POINTER(AttnWeightsArgs), c_void_p], c_int),
@@ -322,6 +323,35 @@ def call_values(name: str, dev_tensor: torch.Tensor, *values) -> None:
     if rc != 0:
         msg = lib.sisa_last_error().decode(errors="replace")
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
+
+
+_CODES = {c_int32: "i", c_int64: "q", c_void_p: "P"}
+
+
+def _codes(cls) -> str:
+    return "".join(_CODES.get(t) or (f"{ctypes.sizeof(t)}s" if t is PagePoolArgs else _codes(t)) for _, t in cls._fields_)
+
+
+class Packed:
+    """An entry point whose argument structure is packed from flat values: the fields in order, a view as its address (0:
+    null) and three strides, a pool as its bytes. One call that packs them all costs a few microseconds less than the
+    structure and its views as objects."""
+
+    def __init__(self, name: str, cls) -> None:
+        self.name, layout = name, struct.Struct("@" + _codes(cls))
+        if layout.size != ctypes.sizeof(cls):
+            raise TypeError(f"{cls.__name__} does not pack to its C size")
+        self.pack, self.fn = layout.pack, None
+
+    def __call__(self, dev_tensor: torch.Tensor, *values) -> None:
+        if self.fn is None:
+            fn = load()[self.name]            # a function object of its own: bytes in place of the structure
+            fn.argtypes, fn.restype = [c_char_p, c_void_p], c_int
+            self.fn = fn
+        rc = launch(self.fn, dev_tensor, self.pack(*values))
+        if rc != 0:
+            msg = load().sisa_last_error().decode(errors="replace")
+            raise RuntimeError(f"{self.name} failed (code {rc}): {msg}")
 
 
 def workspace_bytes(name: str, *dims: int) -> int:

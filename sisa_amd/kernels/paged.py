@@ -28,31 +28,32 @@ __all__ = ["PagePool", "Evicted", "sisa_paged_write_hip", "sisa_paged_decode_hip
 
 MIN_PAGE_SIZE = 16             # SISA_MIN_PAGE_SIZE
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
-_NO_VIEW = _lib.View(None, 0, 0, 0)
+_NO_VIEW = (0, 0, 0, 0)
+
+_write = _lib.Packed("sisa_paged_write", _lib.PagedWriteArgs)
+_decode = _lib.Packed("sisa_paged_decode", _lib.PagedDecodeArgs)
+_evict = _lib.Packed("sisa_cache_evict", _lib.CacheEvictArgs)
 
 
-def vector_rows(t: Tensor) -> bool:
-    """Rows of ``t`` can be read with 16-byte loads: unit last stride, 16-byte aligned base and outer strides."""
-    es = t.element_size()
-    *outer, last = t.stride()
-    return last == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in outer)
+def row_view(t: Tensor) -> tuple[Tensor, int, int, int, int]:
+    """``t`` ``(B, H, L, .)``, its address and its three outer strides; of a copy where 16-byte loads cannot read its rows.
+    (A copy in any case then: ``contiguous()`` hands back a tensor of one row wherever it begins.)"""
+    s0, s1, s2, s3 = t.stride()
+    address = t.data_ptr()
+    if s3 != 1 or (address | (s0 | s1 | s2) * t.element_size()) & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, s2, _ = t.stride()
+        address = t.data_ptr()
+    return t, address, s0, s1, s2
 
 
-def readable(t: Tensor) -> Tensor:
-    """``t``, or a copy of it where 16-byte loads cannot read its rows. A copy in any case then: ``contiguous()`` hands back a
-    tensor of one row wherever it begins."""
-    return t if vector_rows(t) else t.clone(memory_format=torch.contiguous_format)
+def inference_only(name: str) -> None:
+    raise RuntimeError(f"{name} is for inference: call it under torch.no_grad() or on detached tensors")
 
 
-def no_grad_wanted(name: str, *tensors: Tensor | None) -> None:
-    """Inference only: refuse inputs whose gradient the call would lose."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} is for inference: call it under torch.no_grad() or on detached tensors")
-
-
-def _int32(name: str, what: str, t: Tensor, shape: tuple, device: int) -> None:
+def check_ints(name: str, what: str, t: Tensor, shape: tuple, device: int) -> None:
     if t.dtype is not torch.int32 or t.shape != shape or t.get_device() != device:
-        raise ValueError(f"{name}: {what} must be an int32 tensor of shape {shape} on the pool's GPU, got "
+        raise ValueError(f"{name}: {what} must be an int32 tensor of shape {shape} on the GPU of the others, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: {what} must be contiguous along its last axis")
@@ -64,7 +65,7 @@ class PagePool:
     power of two of at least 16. Rows must be readable with 16-byte loads; the tensors may be views of a larger one. The
     handle keeps the tensors and checks them once."""
 
-    __slots__ = ("k", "v", "b", "g", "fgate", "pages", "heads", "page_size", "dtype", "device_index", "args")
+    __slots__ = ("k", "v", "b", "g", "fgate", "pages", "heads", "page_size", "dtype", "device_index", "packed")
 
     def __init__(self, k: Tensor, v: Tensor, b: Tensor, g: Tensor, fgate: Tensor | None = None):
         if k.dim() != 4 or k.shape[-1] != HIP_D_HEAD or v.shape != k.shape:
@@ -85,11 +86,11 @@ class PagePool:
         device = _lib.device_index(k)
         if any(t is not None and t.get_device() != device for t in (v, b, g, fgate)):
             raise ValueError("PagePool: the tensors are on different devices")
-        if not (vector_rows(k) and vector_rows(v) and vector_rows(b)):
+        if any(row_view(t)[0] is not t for t in (k, v, b)):
             raise ValueError("PagePool: k, v, b need rows that 16-byte loads can read (unit last stride, 16-byte aligned)")
         self.k, self.v, self.b, self.g, self.fgate = k, v, b, g, fgate
         self.pages, self.heads, self.page_size, self.dtype, self.device_index = P, H, S, k.dtype, device
-        self.args = _lib.PagePoolArgs(P, H, S, _lib.dtype_code(k.dtype), *(_lib.view(t) for t in (k, v, b, g, fgate)))
+        self.packed = bytes(_lib.PagePoolArgs(P, H, S, _lib.dtype_code(k.dtype), *(_lib.view(t) for t in (k, v, b, g, fgate))))
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int, dtype: torch.dtype, device) -> "PagePool":
@@ -99,19 +100,22 @@ class PagePool:
         return cls(new(HIP_D_HEAD), new(HIP_D_HEAD), new(HIP_D_STATE), new(dt=torch.float32), new(dt=torch.float32))
 
 
-def _rows(name: str, what: str, t: Tensor, shape: tuple, pool: PagePool) -> Tensor:
-    """``t`` checked against the pool, copied where 16-byte loads cannot read its rows."""
-    if t.shape != shape or t.dtype != pool.dtype or t.get_device() != pool.device_index:
+def _rows(name: str, what: str, t: Tensor, shape: tuple, pool: PagePool) -> tuple:
+    """:func:`row_view` of ``t`` checked against the pool."""
+    if t.shape != shape or t.dtype is not pool.dtype or t.get_device() != pool.device_index:
         raise ValueError(f"{name}: {what} must be {shape} in {pool.dtype} on the pool's GPU, got {tuple(t.shape)} {t.dtype} "
                          f"on {t.device}")
-    return readable(t)
+    return row_view(t)
 
 
-def _gates(name: str, what: str, t: Tensor | None, shape: tuple, pool: PagePool) -> Tensor | None:
-    if t is not None and (t.shape != shape or t.dtype is not torch.float32 or t.get_device() != pool.device_index):
+def _gates(name: str, what: str, t: Tensor | None, shape: tuple, pool: PagePool) -> tuple:
+    """Address and strides of a float32 ``(B, H, .)`` tensor checked against the pool."""
+    if t is None:
+        return _NO_VIEW
+    if t.shape != shape or t.dtype is not torch.float32 or t.get_device() != pool.device_index:
         raise ValueError(f"{name}: {what} must be {shape} float32 on the pool's GPU, got {tuple(t.shape)} {t.dtype} on "
                          f"{t.device}")
-    return t
+    return t.data_ptr(), *t.stride()
 
 
 def _forget(name: str, f: Tensor | None, pool: PagePool) -> None:
@@ -126,35 +130,36 @@ def sisa_paged_write_hip(pool: PagePool, table: Tensor, start: Tensor, k: Tensor
     ``(B,)`` int32. A row whose position has no page of the pool is left out. The written pages of two sequences must
     differ."""
     name = "sisa_paged_write_hip"
-    no_grad_wanted(name, k, v, b, g, fgate)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or b.requires_grad or g.requires_grad
+                                    or (fgate is not None and fgate.requires_grad)):
+        inference_only(name)
     if k.dim() != 4 or table.dim() != 2:
         raise ValueError(f"{name}: k must be (B, H, M, {HIP_D_HEAD}) and table (B, W), got {tuple(k.shape)} and "
                          f"{tuple(table.shape)}")
     (B, _, M, _), W, H, device = k.shape, table.shape[1], pool.heads, pool.device_index
     _forget(name, fgate, pool)
-    k = _rows(name, "k", k, (B, H, M, HIP_D_HEAD), pool)
-    v = _rows(name, "v", v, (B, H, M, HIP_D_HEAD), pool)
-    b = _rows(name, "b", b, (B, H, M, HIP_D_STATE), pool)
-    g, fgate = (_gates(name, "g and fgate", t, (B, H, M), pool) for t in (g, fgate))
-    _int32(name, "table", table, (B, W), device)
-    _int32(name, "start", start, (B,), device)
+    k, *vk = _rows(name, "k", k, (B, H, M, HIP_D_HEAD), pool)
+    v, *vv = _rows(name, "v", v, (B, H, M, HIP_D_HEAD), pool)
+    b, *vb = _rows(name, "b", b, (B, H, M, HIP_D_STATE), pool)
+    vg, vf = _gates(name, "g", g, (B, H, M), pool), _gates(name, "fgate", fgate, (B, H, M), pool)
+    check_ints(name, "table", table, (B, W), device)
+    check_ints(name, "start", start, (B,), device)
     if count is not None:
-        _int32(name, "count", count, (B,), device)
-    if not W and B and M:
-        raise ValueError(f"{name}: the table has no entries")
+        check_ints(name, "count", count, (B,), device)
     if not B or not M:
         return
-    _lib.call("sisa_paged_write", _lib.PagedWriteArgs(
-        B, M, W, 0, pool.args, table.data_ptr(), table.stride(0), start.data_ptr(), _lib.ptr(count), _lib.view(k),
-        _lib.view(v), _lib.view(b), _lib.view(g), _lib.view(fgate)), pool.k)
+    if not W:
+        raise ValueError(f"{name}: the table has no entries")
+    _write(k, B, M, W, 0, pool.packed, table.data_ptr(), table.stride(0), start.data_ptr(),
+           0 if count is None else count.data_ptr(), *vk, *vv, *vb, *vg, *vf)
 
 
-def _weights_view(name: str, what: str, t: Tensor, B: int, H: int, max_len: int, pool: PagePool) -> _lib.View:
-    if t.dim() != 3 or t.shape[:2] != (B, H) or t.shape[2] < max_len or t.dtype is not torch.float32 \
+def _weights_view(name: str, what: str, t: Tensor, B: int, H: int, max_len: int, pool: PagePool) -> tuple:
+    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != H or t.shape[2] < max_len or t.dtype is not torch.float32 \
             or t.get_device() != pool.device_index:
         raise ValueError(f"{name}: {what} must be ({B}, {H}, at least {max_len}) float32 on the pool's GPU, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
-    return _lib.view(t)
+    return t.data_ptr(), *t.stride()
 
 
 def _max_len(name: str, max_len: int | None, W: int, pool: PagePool) -> int:
@@ -181,20 +186,23 @@ def sisa_paged_decode_hip(q: Tensor, c: Tensor, g_q: Tensor, f_q: Tensor | None,
     A row that sees no position (an empty sequence) is 0. Every row of a sequence whose length is negative or above
     ``max_len``, or one of whose pages is not in the pool, is NaN."""
     name = "sisa_paged_decode_hip"
-    no_grad_wanted(name, q, c, g_q, f_q, lam, weights)
+    if torch.is_grad_enabled() and (q.requires_grad or c.requires_grad or g_q.requires_grad or lam.requires_grad
+                                    or (f_q is not None and f_q.requires_grad)
+                                    or (weights is not None and weights.requires_grad)):
+        inference_only(name)
     if q.dim() != 4 or table.dim() != 2:
         raise ValueError(f"{name}: q must be (B, H, M, {HIP_D_HEAD}) and table (B, W), got {tuple(q.shape)} and "
                          f"{tuple(table.shape)}")
     (B, _, M, _), W, H, device = q.shape, table.shape[1], pool.heads, pool.device_index
     _forget(name, f_q, pool)
-    q = _rows(name, "q", q, (B, H, M, HIP_D_HEAD), pool)
-    c = _rows(name, "c", c, (B, H, M, HIP_D_STATE), pool)
-    g_q, f_q = (_gates(name, "g_q and f_q", t, (B, H, M), pool) for t in (g_q, f_q))
+    q, *vq = _rows(name, "q", q, (B, H, M, HIP_D_HEAD), pool)
+    c, *vc = _rows(name, "c", c, (B, H, M, HIP_D_STATE), pool)
+    vg, vf = _gates(name, "g_q", g_q, (B, H, M), pool), _gates(name, "f_q", f_q, (B, H, M), pool)
     if lam.shape != (H,) or lam.dtype is not torch.float32 or lam.get_device() != device:
         raise ValueError(f"{name}: lam must be ({H},) float32 on the pool's GPU, got {tuple(lam.shape)} {lam.dtype}")
-    _int32(name, "table", table, (B, W), device)
-    _int32(name, "lengths", lengths, (B,), device)
-    out = torch.empty((B, H, M, HIP_D_HEAD), device=q.device, dtype=torch.float32)
+    check_ints(name, "table", table, (B, W), device)
+    check_ints(name, "lengths", lengths, (B,), device)
+    out = lam.new_empty((B, H, M, HIP_D_HEAD))
     if not B or not M:
         return out
     if not W:
@@ -207,11 +215,12 @@ def sisa_paged_decode_hip(q: Tensor, c: Tensor, g_q: Tensor, f_q: Tensor | None,
     else:
         w_in = _weights_view(name, "weights", weights, B, H, max_len, pool)
         w_out = w_in if weights_out is None else _weights_view(name, "weights_out", weights_out, B, H, max_len, pool)
-    ws = torch.empty(_lib.load().sisa_paged_decode_workspace_bytes(B, H, M, max_len, weights is not None),
-                     device=q.device, dtype=torch.uint8)
-    _lib.call("sisa_paged_decode", _lib.PagedDecodeArgs(
-        B, M, W, max_len, pool.args, table.data_ptr(), table.stride(0), lengths.data_ptr(), _lib.view(q), _lib.view(c),
-        _lib.view(g_q), _lib.view(f_q), lam.data_ptr(), lam.stride(0), w_in, w_out, out.data_ptr(), ws.data_ptr()), q)
+        if 0 in w_out[1:]:
+            raise ValueError(f"{name}: the weights that are written must not be an expanded tensor")
+    size = _lib.load().sisa_paged_decode_workspace_bytes(B, H, M, max_len, _lib.dtype_code(pool.dtype), weights is not None)
+    ws = lam.new_empty((size // 4,)) if size else None
+    _decode(q, B, M, W, max_len, pool.packed, table.data_ptr(), table.stride(0), lengths.data_ptr(), *vq, *vc, *vg, *vf,
+            lam.data_ptr(), lam.stride(0), *w_in, *w_out, out.data_ptr(), 0 if ws is None else ws.data_ptr())
     return out
 
 
@@ -234,29 +243,28 @@ def sisa_cache_evict_hip(pool: PagePool, table: Tensor, lengths: Tensor, weights
     exactly as a softmax over the kept keys. Lengths that are negative or above ``max_len``, too few new pages, and pages
     outside their pool answer with a new length of -1, which :func:`sisa_paged_decode_hip` turns into NaN."""
     name = "sisa_cache_evict_hip"
-    no_grad_wanted(name, weights)
+    if weights.requires_grad and torch.is_grad_enabled():
+        inference_only(name)
     if table.dim() != 2 or new_table.dim() != 2:
         raise ValueError(f"{name}: tables must be (B, W), got {tuple(table.shape)} and {tuple(new_table.shape)}")
-    (B, W), H, device = table.shape, pool.heads, pool.device_index
+    (B, W), H, W_new, device = table.shape, pool.heads, new_table.shape[1], pool.device_index
     if new_pool is not pool and (new_pool.heads != H or new_pool.dtype != pool.dtype or new_pool.device_index != device
                                  or (new_pool.fgate is None) != (pool.fgate is None)):
         raise ValueError(f"{name}: the pools must agree in heads, dtype, GPU and the forget term")
     if not 1 <= recent <= keep:
         raise ValueError(f"{name}: recent = {recent} must be in 1 .. keep = {keep}")
-    _int32(name, "table", table, (B, W), device)
-    _int32(name, "new_table", new_table, (B, new_table.shape[1]), device)
-    _int32(name, "lengths", lengths, (B,), device)
-    dev = pool.k.device
-    new_lengths = torch.empty((B,), device=dev, dtype=torch.int32)
-    new_weights = torch.empty((B, H, keep), device=dev, dtype=torch.float32)
-    positions = torch.empty((B, H, keep), device=dev, dtype=torch.int32)
+    check_ints(name, "table", table, (B, W), device)
+    check_ints(name, "new_table", new_table, (B, W_new), device)
+    check_ints(name, "lengths", lengths, (B,), device)
     if B:
-        if not W or not new_table.shape[1]:
+        if not W or not W_new:
             raise ValueError(f"{name}: a table has no entries")
         max_len = _max_len(name, max_len, W, pool)
-        _lib.call("sisa_cache_evict", _lib.CacheEvictArgs(
-            B, W, new_table.shape[1], max_len, keep, recent, pool.args, new_pool.args, table.data_ptr(), table.stride(0),
-            new_table.data_ptr(), new_table.stride(0), lengths.data_ptr(),
-            _weights_view(name, "weights", weights, B, H, max_len, pool), new_lengths.data_ptr(), new_weights.data_ptr(),
-            positions.data_ptr()), pool.k)
+    w_in = _weights_view(name, "weights", weights, B, H, max_len if B else 0, pool)
+    new_lengths = torch.empty_like(lengths, memory_format=torch.contiguous_format)
+    new_weights, positions = weights.new_empty((B, H, keep)), table.new_empty((B, H, keep))
+    if B:
+        _evict(pool.k, B, W, W_new, max_len, keep, recent, pool.packed, new_pool.packed, table.data_ptr(), table.stride(0),
+               new_table.data_ptr(), new_table.stride(0), lengths.data_ptr(), *w_in, new_lengths.data_ptr(),
+               new_weights.data_ptr(), positions.data_ptr())
     return Evicted(new_lengths, new_weights, positions)

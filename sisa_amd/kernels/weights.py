@@ -8,11 +8,18 @@ from torch import Tensor
 
 from ..config import HIP_D_HEAD, HIP_D_STATE
 from . import _lib
-from .paged import _DTYPES, _int32, no_grad_wanted, readable
+from .paged import _DTYPES, _NO_VIEW, check_ints, inference_only, row_view
 
 __all__ = ["sisa_attention_weights_hip"]
 
 MAX_STRIDE = 1 << 24           # SISA_ATTN_WEIGHTS_MAX_STRIDE
+
+_weights = _lib.Packed("sisa_attn_weights", _lib.AttnWeightsArgs)
+
+
+def _near(t: Tensor, stride: int) -> Tensor:
+    """``t``, or a copy where its positions (axis 2) are ``stride`` elements or more apart."""
+    return t if t.stride(2) < stride else t.clone(memory_format=torch.contiguous_format)
 
 
 def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor,
@@ -27,7 +34,8 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     two); what lies behind is not looked at and receives 0. Returns ``(B, H, L)`` float32. The scores are formed twice and
     never stored."""
     name = "sisa_attention_weights_hip"
-    no_grad_wanted(name, q, k, c, b, g, lam, fgate)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, c, b, g, lam, fgate)):
+        inference_only(name)
     if q.dim() != 4 or q.shape[-1] != HIP_D_HEAD or k.shape != q.shape:
         raise ValueError(f"{name}: q and k must be (B, H, L, {HIP_D_HEAD}), got {tuple(q.shape)} and {tuple(k.shape)}")
     B, H, L, _ = q.shape
@@ -46,16 +54,15 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     if window is not None and window < 1:
         raise ValueError(f"{name}: window = {window} must be positive or None")
     if lengths is not None:
-        _int32(name, "lengths", lengths, (B,), device)
-    out = torch.empty((B, H, L), device=q.device, dtype=torch.float32)
+        check_ints(name, "lengths", lengths, (B,), device)
+    out = lam.new_empty((B, H, L))
     if not out.numel():
         return out
-    q, k, c, b = (readable(t) if 0 <= t.stride(2) < MAX_STRIDE else t.clone(memory_format=torch.contiguous_format)
-                  for t in (q, k, c, b))
-    g, fgate = (t if t is None or t.stride(2) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (g, fgate))
+    (q, *vq), (k, *vk), (c, *vc), (b, *vb) = (row_view(_near(t, MAX_STRIDE)) for t in (q, k, c, b))
+    g, fgate = _near(g, 2), None if fgate is None else _near(fgate, 2)
     window = 0 if window is None or window >= L else window
-    ws = torch.empty(_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window), device=q.device, dtype=torch.uint8)
-    _lib.call("sisa_attn_weights", _lib.AttnWeightsArgs(
-        B, H, L, window, _lib.dtype_code(q.dtype), 0, _lib.view(q), _lib.view(k), _lib.view(c), _lib.view(b), _lib.view(g),
-        _lib.view(fgate), lam.data_ptr(), lam.stride(0), _lib.ptr(lengths), out.data_ptr(), ws.data_ptr()), q)
+    ws = lam.new_empty((_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window) // 4,))
+    _weights(q, B, H, L, window, _lib.dtype_code(q.dtype), 0, *vq, *vk, *vc, *vb, g.data_ptr(), *g.stride(),
+             *(_NO_VIEW if fgate is None else (fgate.data_ptr(), *fgate.stride())), lam.data_ptr(), lam.stride(0),
+             0 if lengths is None else lengths.data_ptr(), out.data_ptr(), ws.data_ptr())
     return out

@@ -84,7 +84,8 @@ def test_entry_points_refuse_bad_arguments(lib):
         return _lib.PagedDecodeArgs(B, M, W, max_len, _pool(lib), 4096, W, 4096, q, row, gate, fq, 4096, 1, w_in, w_out, out, ws)
     for args, word in ((decode(max_len=17), "max_len"), (decode(max_len=0), "max_len"), (decode(M=0), "M=0"),
                        (decode(q=crooked), "aligned"), (decode(fq=none), "fq"), (decode(w_in=gate), "together"),
-                       (decode(out=None), "null"), (decode(ws=None), "null")):
+                       (decode(out=None), "null"), (decode(W=100, max_len=1600, ws=None), "null workspace"),
+                       (decode(W=100, max_len=1600, ws=4104), "aligned")):
         _refused(lib, "sisa_paged_decode", args, word)
     assert lib.sisa_paged_decode(ctypes.byref(decode(B=0)), None) == 0
 
@@ -106,9 +107,14 @@ def test_entry_points_refuse_bad_arguments(lib):
 
 
 def test_workspaces(lib):
-    assert lib.sisa_paged_decode_workspace_bytes(0, 1, 1, 1, 0) == 0
-    one = lib.sisa_paged_decode_workspace_bytes(2, 3, 1, 1000, 0)
-    assert one > 0 and lib.sisa_paged_decode_workspace_bytes(2, 3, 1, 1000, 1) == one + 2 * 3 * 1000 * 4
+    from sisa_amd.kernels import _lib
+    size = lib.sisa_paged_decode_workspace_bytes
+    assert size(0, 1, 1, 1, _lib.BF16, 0) == 0
+    one = size(2, 3, 1, 5000, _lib.BF16, 0)
+    assert one > 0 and size(2, 3, 1, 5000, _lib.BF16, 1) == one + 2 * 3 * 5000 * 4
+    # a cache that one workgroup takes whole needs none, but for the tracked weights of several rows
+    assert size(2, 3, 1, 1024, _lib.BF16, 1) == size(2, 3, 4, 512, _lib.F32, 0) == 0
+    assert size(2, 3, 2, 1024, _lib.BF16, 1) > 0 and size(2, 3, 1, 513, _lib.F32, 0) > 0
     assert lib.sisa_attn_weights_workspace_bytes(2, 3, 100, 0) >= 2 * 3 * 100 * 4
     assert lib.sisa_attn_weights_workspace_bytes(2, 3, 0, 0) == 0
 
