@@ -7,6 +7,8 @@ Main entry points (same names as the reference):
 * :class:`SISAAttention` - the attention sublayer (``attn_impl="auto" | "torch" | "hip" | "hip_fused"``).
 * :class:`SISAForCausalLM` - the language model (blocks of SISA attention and SwiGLU, tied LM head, fused CE,
   ``generate``, ``save_pretrained`` / ``from_pretrained``); :func:`load_paper_checkpoint`.
+* :class:`SISACache`, :class:`SISAPagedCache` - decode caches: one length for all sequences, or pages, lengths of their
+  own and eviction by accumulated attention weight.
 * :mod:`sisa_amd.kernels` - ``sisa_attention_hip``, ``sisa_fused``, ``fused_layout``, ``concat_fused_weights``,
   ``linear_cross_entropy``.
 * :mod:`sisa_amd.backends` - HIP availability, backend selection and the runtime check mode.
@@ -20,11 +22,12 @@ from .config import ATTN_IMPLS, PRESETS, SISAConfig
 from .functional import rotate_pairs, sisa_attention, sisa_attention_torch
 from .generation import SISACache, generate
 from .modeling import RMSNorm, SISAAttention, SISABlock, SISAForCausalLM, SISAModel, SISAOutput, SwiGLU
+from .paged import SISAPagedCache
 
 __version__ = "0.1.0"
 
 __all__ = ["SISAConfig", "PRESETS", "ATTN_IMPLS", "SISAAttention", "SISABlock", "SISAModel", "SISAForCausalLM",
-           "SISAOutput", "RMSNorm", "SwiGLU", "SISACache", "generate", "sisa_attention", "sisa_attention_torch",
+           "SISAOutput", "RMSNorm", "SwiGLU", "SISACache", "SISAPagedCache", "generate", "sisa_attention", "sisa_attention_torch",
            "rotate_pairs", "set_check_mode", "load_paper_checkpoint", "__version__"]
 
 

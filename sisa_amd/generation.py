@@ -10,8 +10,9 @@ The cache is a set of preallocated slabs per layer, ``(B, H, capacity, .)``, fil
 writes its rows in place and the layer state handed to the attention is a view of the filled prefix, so a step costs
 the new rows' bytes, not a copy of the whole cache. ``generate`` sizes the slabs for the prompt plus every new token
 up front; a cache made without a capacity grows by doubling. When the appended rows carry autograd history the slab
-is rebuilt out of place instead, so gradients still flow. Batched decoding assumes equal-length prompts (there is no
-padding mask).
+is rebuilt out of place instead, so gradients still flow. Batched decoding with this cache assumes equal-length prompts
+(there is no padding mask); prompts of unequal lengths, and a bound on the positions that are kept, go through
+:class:`sisa_amd.paged.SISAPagedCache`.
 """
 from __future__ import annotations
 
@@ -21,6 +22,8 @@ from typing import TYPE_CHECKING, Iterable
 
 import torch
 from torch import Tensor
+
+from .paged import SISAPagedCache
 
 if TYPE_CHECKING:  # pragma: no cover
     from .modeling import SISAForCausalLM
@@ -173,16 +176,59 @@ def _pick(logits: Tensor, do_sample: bool, temperature: float, top_k: int | None
     return torch.multinomial(scores.softmax(-1), 1, generator=generator).squeeze(-1)
 
 
+def _prompt_lengths(prompt_lengths, rows: Tensor) -> list[int] | None:
+    """The prompts' lengths as a list, or None where every row is full."""
+    if prompt_lengths is None:
+        return None
+    lengths = prompt_lengths.tolist() if torch.is_tensor(prompt_lengths) else list(prompt_lengths)
+    if len(lengths) != rows.shape[0] or not all(isinstance(n, numbers.Integral) and 1 <= n <= rows.shape[1] for n in lengths):
+        raise ValueError(f"prompt_lengths = {lengths}: expected an integer in 1 .. {rows.shape[1]} for each of the "
+                         f"{rows.shape[0]} rows")
+    lengths = [int(n) for n in lengths]
+    return None if min(lengths) == rows.shape[1] else lengths
+
+
+class _Budget:
+    """When a cache is cut, and to what: to ``keep`` positions, of them the last ``recent``, once it has grown ``slack`` over
+    them."""
+
+    def __init__(self, keep: int, recent: int | None) -> None:
+        if keep < 1:
+            raise ValueError(f"cache_budget = {keep} must be positive")
+        self.keep, self.recent = keep, max(1, keep // 4) if recent is None else recent
+        if not 1 <= self.recent <= keep:
+            raise ValueError(f"cache_recent = {recent} must be in 1 .. cache_budget = {keep}")
+        self.slack = max(16, keep // 8)
+
+
+def _paged_cache(rows: int, longest: int, new: int, budget: _Budget | None) -> SISAPagedCache:
+    """A cache for prompts of up to ``longest`` positions and ``new`` more, or for what a budget lets them grow to."""
+    if budget is None:
+        return SISAPagedCache(rows, longest + new)
+    top = max(longest + 1, min(longest + new, budget.keep + budget.slack) + 1)
+    size, each = 64, lambda n: -(-n // 64)  # noqa: E731
+    return SISAPagedCache(rows, top, pages=rows * (each(top) + each(budget.keep)), page_size=size, track=True)
+
+
 @torch.no_grad()
 def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, temperature: float = 1.0,
              top_k: int | None = None, eos_token_id: int | Iterable[int] | Tensor | None = None,
-             do_sample: bool = False, *, generator: torch.Generator | None = None) -> Tensor:
+             do_sample: bool = False, *, generator: torch.Generator | None = None,
+             prompt_lengths: Iterable[int] | Tensor | None = None, cache_budget: int | None = None,
+             cache_recent: int | None = None) -> Tensor:
     """Continue the prompts ``input_ids`` (``(B, L)`` of equal-length rows, or ``(L,)``) by up to ``max_new_tokens``
     tokens: greedy, or sampled at ``temperature`` from the ``top_k`` most likely tokens with ``do_sample``.
 
     A row that emits an ``eos_token_id`` is finished and padded with the first such id from then on; generation
     ends when every row is finished. Returns ``(B, L + n)`` ids, ``n <= max_new_tokens``, with the rank of
     ``input_ids``.
+
+    ``prompt_lengths``: the prompts are right-padded rows of these lengths. A row's tokens follow its prompt, and what is
+    left of the row behind them is the first ``eos_token_id``, or 0 without one.
+
+    ``cache_budget``: how many positions each layer and head keeps: the last ``cache_recent`` (default: a quarter) and those
+    that have received the largest softmax weight. The cache is cut after the prompt, and whenever it has grown by an eighth
+    (at least 16) over its budget; until a cut nothing is left out.
     """
     if max_new_tokens < 0:
         raise ValueError(f"max_new_tokens = {max_new_tokens} is negative")
@@ -194,6 +240,10 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     if rows.dim() != 2 or rows.shape[1] == 0:
         raise ValueError(f"generate needs at least one prompt token per row in a (B, L) or (L,) tensor, got shape "
                          f"{tuple(input_ids.shape)}")
+    if cache_recent is not None and cache_budget is None:
+        raise ValueError("cache_recent goes with cache_budget")
+    lengths = _prompt_lengths(prompt_lengths, rows)
+    budget = None if cache_budget is None else _Budget(cache_budget, cache_recent)
     stops = _eos_ids(eos_token_id)
     stop_ids = torch.tensor(stops, device=rows.device, dtype=rows.dtype) if stops else None
     prompt = rows.shape[1]
@@ -201,18 +251,35 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     out[:, :prompt] = rows
     length = prompt
     if max_new_tokens:
-        cache = SISACache(capacity=prompt + max_new_tokens)
+        if lengths is None and budget is None:
+            cache = SISACache(capacity=prompt + max_new_tokens)
+        else:
+            cache = _paged_cache(rows.shape[0], max(lengths or [prompt]), max_new_tokens, budget)
         finished = torch.zeros(rows.shape[0], dtype=torch.bool, device=rows.device)
-        logits = model(rows, cache=cache, logits_to_keep=1).logits[:, -1]
+        ends = None
+        if lengths is None:
+            logits = model(rows, cache=cache, logits_to_keep=1).logits[:, -1]
+        else:
+            cache.expect(lengths)
+            logits = model(rows, cache=cache, logits_at=[n - 1 for n in lengths]).logits[:, -1]
+            # rows are laid out from their own ends
+            n = torch.tensor(lengths, device=rows.device)
+            out[torch.arange(out.shape[1], device=rows.device) >= n[:, None]] = stops[0] if stops else 0
+            ends = n[:, None]
         while True:
             token = _pick(logits, do_sample, temperature, top_k, generator).to(rows.dtype)
             if stop_ids is not None:
                 token = torch.where(finished, stop_ids[0], token)
                 finished |= torch.isin(token, stop_ids)
-            out[:, length] = token
+            if ends is None:
+                out[:, length] = token
+            else:
+                out.scatter_(1, ends + (length - prompt), token[:, None])
             length += 1
             if length == out.shape[1] or (stop_ids is not None and bool(finished.all())):
                 break
+            if budget is not None and (length == prompt + 1 or cache.seq_len >= budget.keep + budget.slack):
+                cache.evict(budget.keep, budget.recent)
             logits = model(token[:, None], cache=cache, logits_to_keep=1).logits[:, -1]
     result = out[:, :length].contiguous()
     return result if input_ids.dim() == 2 else result.squeeze(0)

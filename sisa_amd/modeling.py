@@ -19,7 +19,7 @@ Module tree, parameter names and shapes, initial values and loss conventions are
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import TYPE_CHECKING, Any, Iterable, NamedTuple
+from typing import TYPE_CHECKING, Any, Iterable, NamedTuple, Sequence
 
 import torch
 import torch.nn as nn
@@ -30,6 +30,7 @@ from torch.utils.checkpoint import checkpoint
 from . import backends
 from .config import SISAConfig
 from .functional import attend_block, autocast_disabled, rotate_pairs, sisa_attention, working_dtype
+from .paged import SISAPagedCache, takes_kernels
 
 if TYPE_CHECKING:  # pragma: no cover
     from .generation import SISACache
@@ -251,6 +252,8 @@ class SISAAttention(nn.Module):
         """Generation. An empty layer entry means prefill: the unfused route (the fused one keeps no k, v, b, g, F to
         cache) with "hip" standing in for "hip_fused". Otherwise a step: the new rows attend to the whole cache, on
         the HIP decode kernel on the GPU, else exactly in float32 torch."""
+        if isinstance(cache, SISAPagedCache):
+            return self._forward_paged(x, cache, requested)
         state = cache.get(self.layer_idx)
         p = self._unfused_inputs(x, state)
         if state is None:
@@ -271,9 +274,26 @@ class SISAAttention(nn.Module):
         keys = (state.k.to(wd), state.v.to(wd), state.b.to(wd), state.g.to(wd), state.fgate.to(wd))
         return self._output(attend_block(rows, keys, self.lam().to(wd), first).to(p.q.dtype))
 
-    def forward(self, x: Tensor, *, cache: "SISACache | None" = None, impl: str | None = None) -> Tensor:
+    def _forward_paged(self, x: Tensor, cache: SISAPagedCache, requested: str) -> Tensor:
+        """Generation with a cache in pages, on the HIP kernels of :mod:`sisa_amd.kernels.paged` where they serve ``x``. A
+        first pass attends as a prefill does; its positions' received weights are taken afterwards, if tracked."""
+        last = cache.last(self.layer_idx)
+        p, lam = self._unfused_inputs(x, last), self.lam()
+        hip = _kernels_on(x, self.config) and takes_kernels(p.k, p.b)
+        if last is None:
+            impl = backends.select_impl("hip" if requested == "hip_fused" else requested, x, self.config)
+            y = self._attention(p, "hip" if impl == "hip_fused" else impl)
+            cache.extend(self.layer_idx, p, hip)
+            if cache.tracked:
+                cache.receive(self.layer_idx, p, lam, hip)
+            return self._output(y)
+        cache.extend(self.layer_idx, p, hip)
+        return self._output(cache.attend(self.layer_idx, p, lam, hip).to(p.q.dtype))
+
+    def forward(self, x: Tensor, *, cache: "SISACache | SISAPagedCache | None" = None, impl: str | None = None) -> Tensor:
         """The sublayer on the normalised input ``x`` ``(B, L, d_model)``, returning ``(B, L, d_model)``. ``cache``:
-        a :class:`sisa_amd.generation.SISACache` to fill (prefill) or extend (decode step); ``impl`` overrides
+        a :class:`sisa_amd.generation.SISACache` or :class:`sisa_amd.paged.SISAPagedCache` to fill (prefill) or extend
+        (decode step); ``impl`` overrides
         ``config.attn_impl`` for this call."""
         requested = impl or self.config.attn_impl
         if cache is not None:
@@ -555,25 +575,32 @@ class SISAForCausalLM(SISAModel):
         super().__init__(config)
         self._loss_fn = _lm_head_loss
 
-    def forward(self, input_ids: Tensor, labels: Tensor | None = None, *, cache: "SISACache | None" = None,
-                fused_ce: bool = False, return_logits: bool = True, logits_to_keep: int = 0) -> SISAOutput:
+    def forward(self, input_ids: Tensor, labels: Tensor | None = None, *,
+                cache: "SISACache | SISAPagedCache | None" = None, fused_ce: bool = False, return_logits: bool = True,
+                logits_to_keep: int = 0, logits_at: Sequence[int] | None = None) -> SISAOutput:
         """Loss and/or logits of ``input_ids`` ``(B, L)``.
 
         ``fused_ce=True`` (with labels): the loss from the HIP linear cross-entropy on the GPU, no logits returned.
         ``return_logits=False``: the loss alone. ``logits_to_keep > 0``: logits of the last that many positions only
-        (without labels). ``cache``: generation state (:func:`sisa_amd.generation.generate`).
+        (without labels). ``logits_at``: logits ``(B, 1, V)`` of one position of each row (without labels). ``cache``:
+        generation state (:func:`sisa_amd.generation.generate`).
         """
         if labels is not None:
             if labels.shape != input_ids.shape:
                 raise ValueError(f"labels {tuple(labels.shape)} and input_ids {tuple(input_ids.shape)} differ in "
                                  f"shape")
-            if logits_to_keep:
-                raise ValueError("logits_to_keep is for generation; it cannot be combined with labels")
+            if logits_to_keep or logits_at is not None:
+                raise ValueError("logits_to_keep and logits_at are for generation; they cannot be combined with labels")
+        if logits_at is not None and (logits_to_keep or len(logits_at) != input_ids.shape[0]):
+            raise ValueError("logits_at is one position for each row, in place of logits_to_keep")
         hidden = SISAModel.forward(self, input_ids, cache=cache)
         head = self.embed.weight
         if labels is None:
             if not return_logits:
                 return SISAOutput()
+            if logits_at is not None:
+                hidden = hidden[torch.arange(len(logits_at), device=hidden.device),
+                                torch.tensor(logits_at, device=hidden.device)][:, None]
             return SISAOutput(logits=F.linear(hidden[:, -logits_to_keep:] if logits_to_keep else hidden, head))
         inputs, targets = hidden[:, :-1], labels[:, 1:]          # position t predicts token t + 1
         if fused_ce:

@@ -1,0 +1,320 @@
+"""SISAPagedCache and what generate() does with it: on the CPU in float64 against the contiguous cache and against dense
+formulas, on the GPU (bf16, fp32) against the same model in float64."""
+import math
+
+import pytest
+import torch
+
+from model_utils import rel_err, tiny_model, token_ids
+from sisa_amd import SISACache, SISAPagedCache, generate
+from sisa_amd.paged import attention_weights
+
+DEV = "cuda:0"
+
+
+# The gates are float32 in a float64 model, and torch rounds their functions differently in a vector's body and its tail, so
+# in passes of other shapes. Here their sums are below 64 in magnitude and of at most 50 steps, each rounded by at most 2^-19
+# (half a step below 64) on either side: scores differ by at most 2 * 2 * 50 * 2^-19 = 3.9e-4 in g and F together, weights by
+# 7.8e-4 of themselves, logits after two layers by no more than a few of that.
+GATES = 2e-3
+
+
+def _model64(**kw):
+    return tiny_model(seed=3, theta_scale=0.25, **kw).double().eval()
+
+
+def _logits(model, ids, cache, first, counts=None, at=None):
+    """Logits of every later position, by a first pass and then one by one."""
+    with torch.no_grad():
+        if counts is not None:
+            cache.expect(counts)
+        out = [model(ids[:, :first], cache=cache).logits]
+        out += [model(ids[:, t:t + 1], cache=cache).logits for t in range(first, ids.shape[1])]
+    return torch.cat(out, 1)
+
+
+def test_equal_lengths_continue_as_the_contiguous_cache():
+    model = _model64()
+    ids = token_ids(3, 70, seed=1)
+    want = _logits(model, ids, SISACache(), 40)
+    for page_size, kw in ((16, {}), (64, dict(track=True))):
+        cache = SISAPagedCache(3, 70, page_size=page_size, **kw)
+        got = _logits(model, ids, cache, 40)
+        assert rel_err(got, want) <= 1e-12 and cache.lengths == [70] * 3 and cache.seq_len == 70
+    # several positions at once behind a filled cache
+    # (the float32 sums of the gates depend on where a pass ends: the same passes on both sides)
+    cache, other = SISAPagedCache(3, 70, track=True), SISACache()
+    with torch.no_grad():
+        got, want = (torch.cat([model(ids[:, a:b], cache=c).logits for a, b in ((0, 33), (33, 50), (50, 70))], 1)
+                     for c in (cache, other))
+    assert rel_err(got, want) <= 1e-12
+    # every query's weights sum to one, however they came in
+    for layer in range(2):
+        w = cache.weights(layer)
+        assert (w.double().sum(-1) - 70).abs().max() <= 70 * 70 * 2 ** -24 and w.shape == (3, 2, 70)
+
+
+def test_unequal_lengths_are_what_each_gives_alone():
+    model = _model64()
+    ids, counts = token_ids(4, 60, seed=2), [37, 1, 16, 40]
+    cache = SISAPagedCache(4, 61, page_size=16, track=True)
+    with torch.no_grad():
+        cache.expect(counts)
+        first = model(ids[:, :40], cache=cache, logits_at=[n - 1 for n in counts]).logits
+        later = [model(ids[:, t:t + 1], cache=cache).logits for t in range(40, 45)]
+    assert cache.lengths == [n + 5 for n in counts]
+    for i, n in enumerate(counts):
+        row = torch.cat([ids[i:i + 1, :n], ids[i:i + 1, 40:45]], 1)
+        alone = SISACache()
+        want = _logits(model, row, alone, n)
+        got = torch.cat([first[i:i + 1], *(x[i:i + 1] for x in later)], 1)
+        assert rel_err(got, want[:, n - 1:]) <= GATES
+        one = SISAPagedCache(1, 50, track=True)
+        _logits(model, row, one, n)
+        for layer in range(2):
+            held, single = cache.weights(layer)[i], one.weights(layer)[0]
+            assert rel_err(held[:, :n + 5], single[:, :n + 5]) <= GATES
+            assert held[:, n + 5:].eq(0).all()
+
+
+def test_parts_release_and_reuse():
+    model = _model64()
+    ids = token_ids(3, 50, seed=4)
+    cache = SISAPagedCache(3, 50, pages=8, page_size=16)
+    want = [_logits(model, ids[i:i + 1], SISACache(), 20) for i in range(3)]
+    with torch.no_grad():
+        for i in (2, 0):                                    # one after the other, not in order
+            assert rel_err(model(ids[i:i + 1, :20], cache=cache[i]).logits, want[i][:, :20]) <= GATES
+        assert cache.lengths == [20, 0, 20] and cache.free_pages == 4
+        with pytest.raises(ValueError, match="some of these sequences are empty"):
+            model(ids[:, 20:21], cache=cache)
+        assert rel_err(model(ids[1:2, :20], cache=cache[1]).logits, want[1][:, :20]) <= GATES
+        step = model(ids[:, 20:21], cache=cache).logits
+        assert rel_err(step, torch.cat(want)[:, 20:21]) <= GATES
+        cache[0:2].release()
+        assert cache.lengths == [0, 0, 21] and cache.free_pages == 6
+        # the pages go to another sequence; the third is not touched
+        assert rel_err(model(ids[1:2, :20], cache=cache[0]).logits, want[1][:, :20]) <= GATES
+        assert rel_err(model(ids[2:, 21:22], cache=cache[-1]).logits, want[2][:, 21:22]) <= GATES
+        cache[1].reserve(40)                                # before its first pass
+        assert cache.free_pages == 1
+        with pytest.raises(RuntimeError, match="more pages"):
+            model(ids[:1, 20:49], cache=cache[0:1])         # 49 positions: two pages more
+        assert cache.lengths == [20, 0, 22]
+    assert len(cache) == 3 and len(cache[1:]) == 2
+    for bad in (slice(2, 1), slice(0, 3, 2)):
+        with pytest.raises(ValueError):
+            cache[bad]
+    with pytest.raises(IndexError):
+        cache[3]
+
+
+def _dense(model, x, layer, kept):
+    """Attention of the last row of ``x`` (1, n, d), the layer's normalised input, over the rows ``kept[h]``."""
+    at = model.layers[layer].attn
+    p, lam, n = at._unfused_inputs(x), at.lam().double(), x.shape[1]
+    heads = []
+    for h, rows in enumerate(kept):
+        j = torch.tensor(rows)
+        s = p.k[0, h, j] @ p.q[0, h, -1] / 8 + lam[h] * (p.g[0, h, -1] - p.g[0, h, j]).exp() * (p.b[0, h, j] @ p.c[0, h, -1])
+        w = (s + p.fgate[0, h, -1] - p.fgate[0, h, j]).softmax(0)
+        heads.append((w @ p.v[0, h, j], w))
+    return torch.cat([o for o, _ in heads]), [w for _, w in heads]
+
+
+@pytest.mark.parametrize("keep,recent", [(12, 4), (12, 12), (20, 1), (1, 1)])
+def test_evict_leaves_a_softmax_over_what_is_kept(keep, recent):
+    """One layer, whose inputs do not depend on what it keeps: positions chosen by sorting, attention over them alone."""
+    model = _model64(n_layer=1)
+    block, at = model.layers[0], model.layers[0].attn
+    ids = token_ids(1, 60, seed=5)
+    cache = SISAPagedCache(1, 60, page_size=16, track=True, pages=8)
+    with torch.no_grad():
+        x = block.attn_norm(model.embed(ids))
+        p = at._unfused_inputs(x[:, :40])
+        w = attention_weights(p.q, p.k, p.c, p.b, p.g, at.lam(), p.fgate, torch.tensor([40]))[0]
+        at(x[:, :40], cache=cache)
+        kept = [list(range(40)) for _ in range(2)]
+        w = [row for row in w.double()]
+        for t in range(40, 60):
+            if t in (40, 47, 48):
+                before = cache.free_pages
+                cache.evict(keep, recent)
+                for h in range(2):
+                    n = len(kept[h])
+                    if n > keep:
+                        old = sorted(range(n - recent), key=lambda i: (-float(w[h][i]), i))[:keep - recent]
+                        stay = sorted(old) + list(range(n - recent, n))
+                        kept[h], w[h] = [kept[h][i] for i in stay], w[h][stay]
+                assert cache.lengths == [min(keep, t)] and cache.free_pages >= before
+            for h in range(2):
+                kept[h].append(t)
+            y = at(x[:, t:t + 1], cache=cache)
+            want, new = _dense(model, x[:, :t + 1], 0, kept)
+            assert rel_err(y[0, 0], at.W_O(want)) <= GATES
+            w = [torch.cat([a, a.new_zeros(1)]) + b for a, b in zip(w, new)]
+        for h in range(2):
+            assert rel_err(cache.weights(0)[0, h, :len(kept[h])], w[h]) <= GATES
+            assert cache.weights(0)[0, h, len(kept[h]):].eq(0).all()
+
+
+def test_evict_with_few_free_pages_goes_sequence_by_sequence():
+    model = _model64()
+    ids = token_ids(3, 64, seed=6)
+    with torch.no_grad():
+        roomy, tight = SISAPagedCache(3, 64, page_size=16, pages=30, track=True), SISAPagedCache(
+            3, 64, page_size=16, pages=13, track=True)
+        for c in (roomy, tight):
+            model(ids[:, :63], cache=c)
+            c.evict(10, 3)
+        assert roomy.lengths == tight.lengths == [10] * 3 and tight.free_pages == 10
+        for layer in range(2):
+            assert torch.equal(roomy.weights(layer), tight.weights(layer))
+        a, b = (model(ids[:, 63:], cache=c).logits for c in (roomy, tight))
+        assert torch.equal(a, b)
+        none = SISAPagedCache(1, 64, page_size=16, pages=4, track=True)
+        model(ids[:1, :63], cache=none)
+        with pytest.raises(RuntimeError, match="free pages"):
+            none.evict(10, 3)
+        assert none.lengths == [63] and rel_err(model(ids[:1, 63:], cache=none).logits,
+                                                _logits(model, ids[:1], SISACache(), 63)[:, 63:]) <= GATES
+
+
+def test_refusals():
+    model = _model64()
+    ids = token_ids(2, 20, seed=7)
+    for kw in (dict(sequences=0), dict(max_length=0), dict(page_size=8), dict(page_size=48), dict(pages=0)):
+        with pytest.raises(ValueError):
+            SISAPagedCache(**(dict(sequences=1, max_length=4) | kw))
+    cache = SISAPagedCache(2, 20)
+    with pytest.raises(RuntimeError, match="inference"):
+        model(ids, cache=cache)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="2 sequences"):
+            model(ids[:1], cache=cache)
+        with pytest.raises(ValueError, match="track=True"):
+            cache.evict(4, 1)
+        with pytest.raises(ValueError, match="track=True"):
+            cache.weights(0)
+        for counts in ([3], [0, 3], [3, 3, 3]):
+            with pytest.raises(ValueError, match="expect"):
+                cache.expect(counts)
+        cache.expect([3, 21])
+        with pytest.raises(ValueError, match="were expected"):
+            model(ids, cache=cache)
+        cache.expect([20, 3])
+        model(ids, cache=cache)
+        with pytest.raises(ValueError, match="first pass"):
+            cache.expect([1, 1])
+        with pytest.raises(ValueError, match="max_length"):
+            model(ids[:, :1], cache=cache)
+        tracked = SISAPagedCache(2, 20, track=True)
+        model(ids, cache=tracked)
+        for keep, recent in ((4, 0), (4, 5), (0, 0)):
+            with pytest.raises(ValueError, match="recent"):
+                tracked.evict(keep, recent)
+        with pytest.raises(ValueError, match="logits_at"):
+            model(ids, logits_at=[1])
+        with pytest.raises(ValueError, match="labels"):
+            model(ids, labels=ids, logits_at=[1, 1])
+
+
+# ------------------------------------------------------------------------------------------------ generate
+def test_generate_from_unequal_prompts():
+    model = _model64()
+    ids, lengths = token_ids(3, 24, seed=8), [24, 3, 11]
+    got = generate(model, ids, 9, prompt_lengths=lengths)
+    assert got.shape == (3, 33)
+    for i, n in enumerate(lengths):
+        want = generate(model, ids[i:i + 1, :n], 9)
+        assert torch.equal(got[i, :n + 9], want[0]) and got[i, n + 9:].eq(0).all()
+    assert torch.equal(generate(model, ids, 9, prompt_lengths=torch.tensor([24, 24, 24])), generate(model, ids, 9))
+    # an end: the row's rest is the first stop id
+    stop = int(got[1, 5])
+    ended = generate(model, ids, 9, prompt_lengths=lengths, eos_token_id=[stop, 300])
+    first = got[1, 3:12].tolist().index(stop)
+    assert ended[1, 3 + first:].eq(stop).all() and torch.equal(ended[1, :3 + first], got[1, :3 + first])
+    one = generate(model, ids[1], 4, prompt_lengths=[3])
+    assert one.dim() == 1 and torch.equal(one[:7], got[1, :7])
+    for bad in ([24, 3], [24, 0, 3], [25, 3, 3], [24.0, 3, 3]):
+        with pytest.raises(ValueError, match="prompt_lengths"):
+            generate(model, ids, 2, prompt_lengths=bad)
+
+
+def test_generate_within_a_budget():
+    model = _model64()
+    ids = token_ids(2, 50, seed=9)
+    free = generate(model, ids, 40)
+    assert torch.equal(generate(model, ids, 40, cache_budget=90), free)            # a budget that is never reached
+    cut = generate(model, ids, 40, cache_budget=16, cache_recent=8)
+    assert cut.shape == (2, 90) and torch.equal(cut[:, :51], free[:, :51])         # the prompt itself is seen whole
+    # by hand: cut after the prompt, and when 16 more have come
+    cache = SISAPagedCache(2, 90, track=True)
+    with torch.no_grad():
+        token, out = model(ids, cache=cache).logits[:, -1].argmax(-1), [ids]
+        cache.evict(16, 8)
+        for _ in range(39):
+            out.append(token[:, None])
+            if cache.seq_len >= 32:
+                cache.evict(16, 8)
+            token = model(token[:, None], cache=cache).logits[:, -1].argmax(-1)
+    assert torch.equal(cut, torch.cat([*out, token[:, None]], 1))
+    assert generate(model, ids, 30, cache_budget=1, prompt_lengths=[50, 2]).shape == (2, 80)
+    for kw in (dict(cache_budget=0), dict(cache_recent=3), dict(cache_budget=4, cache_recent=5), dict(cache_budget=4, cache_recent=0)):
+        with pytest.raises(ValueError, match="cache_"):
+            generate(model, ids, 2, **kw)
+
+
+# ------------------------------------------------------------------------------------------------ on the GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bound", [(torch.float32, 2e-5), (torch.bfloat16, 5e-2), (torch.float16, 1e-2)])
+def test_unequal_lengths_on_the_gpu(dtype, bound, monkeypatch):
+    """Ragged prompts, steps, an eviction, steps, against the model's float64 copy on the CPU with the same positions kept.
+    Bounds: the contiguous cache's logits of these models are off float64 by up to half of them."""
+    from sisa_amd.kernels import paged as K
+    model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).to(dtype).eval()
+    ref = tiny_model(seed=3, theta_scale=0.25).eval()
+    ref.load_state_dict({n: t.cpu() for n, t in model.state_dict().items()})
+    ref = ref.double()
+    used, real = [], (K.sisa_paged_decode_hip, K.sisa_cache_evict_hip)
+    monkeypatch.setattr(K, "sisa_paged_decode_hip", lambda *a, **kw: used.append("decode") or real[0](*a, **kw))
+    ids, counts = token_ids(3, 120, seed=10), [90, 17, 64]
+    monkeypatch.setattr(K, "sisa_cache_evict_hip", lambda *a, **kw: used.append("evict") or real[1](*a, **kw))
+    caches = [SISAPagedCache(3, 128, page_size=32, pages=20, track=True) for _ in range(2)]
+    outs = []
+    for m, cache, dev in ((model, caches[0], DEV), (ref, caches[1], "cpu")):
+        x = ids.to(dev)
+        with torch.no_grad():
+            cache.expect(counts)
+            got = [m(x[:, :90], cache=cache, logits_at=[n - 1 for n in counts]).logits]
+            got += [m(x[:, t:t + 1], cache=cache).logits for t in range(90, 95)]
+            if m is model:
+                weights = [cache.weights(layer).clone() for layer in range(2)]
+            else:
+                for layer in range(2):
+                    assert rel_err(weights[layer].cpu(), cache.weights(layer).double()) <= bound
+                    # choose by the GPU's weights: near ties may fall differently
+                    cache.weights(layer).copy_(weights[layer])
+            cache.evict(40, 10)
+            got += [m(x[:, t:t + 1], cache=cache).logits for t in range(95, 100)]
+        outs.append(torch.cat(got, 1).cpu())
+        assert cache.lengths == [45, 27, 45]
+    assert used.count("decode") == 20 and used.count("evict") >= 2
+    assert rel_err(outs[0], outs[1]) <= bound
+    for i in range(3):
+        assert rel_err(outs[0][i], outs[1][i]) <= 1.5 * bound
+
+
+@pytest.mark.gpu
+def test_generate_on_the_gpu_with_lengths_and_budget():
+    model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).eval()
+    ids, lengths = token_ids(3, 40, seed=11).to(DEV), [40, 9, 25]
+    got = generate(model, ids, 12, prompt_lengths=lengths)
+    for i, n in enumerate(lengths):
+        assert torch.equal(got[i, :n + 12], generate(model, ids[i:i + 1, :n], 12)[0])
+    assert torch.equal(generate(model, ids, 12, cache_budget=64), generate(model, ids, 12))
+    cut = generate(model, ids, 30, cache_budget=16, prompt_lengths=lengths)
+    again = generate(model, ids, 30, cache_budget=16, prompt_lengths=lengths)
+    assert cut.shape == (3, 70) and torch.equal(cut, again)
+    half = model.to(torch.bfloat16)
+    assert generate(half, ids, 20, cache_budget=32, cache_recent=8).shape == (3, 60)
