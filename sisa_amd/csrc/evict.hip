@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
 }
 
 // A wave moves ROWS kept rows. A row without a page marks its sequence.
-template <class T, int ROWS>
+template <class T, int ROWS, bool STREAM>
 __global__ __launch_bounds__(256) void evict_copy_kernel(sisa_cache_evict_args a, int shift, int new_shift) {
     const int lane = threadIdx.x & 63;
     const unsigned id = (blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS + lane, keep = a.keep, H = a.from.heads;
@@ -170,8 +170,8 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(sisa_cache_evict_args a
         dst = page_of(a.new_table + n * a.s_new, a.W_new, new_shift, a.to.pages, i);
         if (src < 0 || dst < 0) a.new_lengths[n] = -1;
     }
-    move_rows<T, ROWS>(rows_of_pool(a.from), rows_of_pool(a.to), src >= 0 && dst >= 0, src, dst, h,
-                       j & (a.from.page_size - 1), i & (a.to.page_size - 1), lane);
+    move_rows<T, ROWS, STREAM>(rows_of_pool(a.from), rows_of_pool(a.to), src >= 0 && dst >= 0, src, dst, h,
+                               j & (a.from.page_size - 1), i & (a.to.page_size - 1), lane);
 }
 
 template <class T>
@@ -179,8 +179,10 @@ void launch_copy(const sisa_cache_evict_args* a, int64_t rows, hipStream_t st) {
     const int shift = sisa::log2_of(a->from.page_size), new_shift = sisa::log2_of(a->to.page_size);
     const int per = 4 * sisa::rows_per_wave(rows);
     const unsigned grid = (unsigned)sisa::cdiv(rows, per);
-    if (per == 256) evict_copy_kernel<T, 64><<<grid, 256, 0, st>>>(*a, shift, new_shift);
-    else evict_copy_kernel<T, 8><<<grid, 256, 0, st>>>(*a, shift, new_shift);
+    if (per != 256) evict_copy_kernel<T, 8, false><<<grid, 256, 0, st>>>(*a, shift, new_shift);
+    else if (sisa::cache_bytes(a->from, a->B, a->max_len) < STREAM_BYTES)
+        evict_copy_kernel<T, 64, false><<<grid, 256, 0, st>>>(*a, shift, new_shift);
+    else evict_copy_kernel<T, 64, true><<<grid, 256, 0, st>>>(*a, shift, new_shift);
 }
 
 }  // namespace

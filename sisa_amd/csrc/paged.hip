@@ -13,7 +13,7 @@ constexpr int DH = 64, DS = 32;
 // ------------------------------------------------------------------------------------------------ write
 // A wave moves ROWS rows, numbered with the positions of a head as neighbours: a prompt's rows of a head become neighbours
 // in a page.
-template <class T, int ROWS>
+template <class T, int ROWS, bool STREAM>
 __global__ __launch_bounds__(256) void paged_write_kernel(sisa_paged_write_args a, int shift) {
     const int lane = threadIdx.x & 63;
     const unsigned id = (blockIdx.x * 4 + (threadIdx.x >> 6)) * ROWS + lane, M = a.M, H = a.pool.heads;
@@ -25,16 +25,17 @@ __global__ __launch_bounds__(256) void paged_write_kernel(sisa_paged_write_args 
         pos = (int64_t)a.start[n] + m;
         page = page_of(a.table + n * a.s_table, a.W, shift, a.pool.pages, pos);
     }
-    move_rows<T, ROWS>(RowViews{a.k, a.v, a.b, a.g, a.f}, rows_of_pool(a.pool), page >= 0, n, page, h, m,
-                       pos & (a.pool.page_size - 1), lane);
+    move_rows<T, ROWS, STREAM>(RowViews{a.k, a.v, a.b, a.g, a.f}, rows_of_pool(a.pool), page >= 0, n, page, h, m,
+                               pos & (a.pool.page_size - 1), lane);
 }
 
 template <class T>
 void launch_write(const sisa_paged_write_args* a, int64_t rows, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size), per = 4 * sisa::rows_per_wave(rows);
     const unsigned grid = (unsigned)sisa::cdiv(rows, per);
-    if (per == 256) paged_write_kernel<T, 64><<<grid, 256, 0, st>>>(*a, shift);
-    else paged_write_kernel<T, 8><<<grid, 256, 0, st>>>(*a, shift);
+    if (per != 256) paged_write_kernel<T, 8, false><<<grid, 256, 0, st>>>(*a, shift);
+    else if (2 * rows * sisa::row_bytes(a->pool.dtype) < STREAM_BYTES) paged_write_kernel<T, 64, false><<<grid, 256, 0, st>>>(*a, shift);
+    else paged_write_kernel<T, 64, true><<<grid, 256, 0, st>>>(*a, shift);
 }
 
 // ------------------------------------------------------------------------------------------------ decode
@@ -75,15 +76,9 @@ SISA_DEV float sum_scatter(const float (&x)[8], int fg) {
     return (fg & 1 ? z[1] : z[0]) + dpp<XOR1>(fg & 1 ? z[0] : z[1]);
 }
 
-// 256 MB, the last-level cache: from there on 16-bit rows are loaded with the non-temporal hint, as csrc/decode.hip does (516
-// MB 102 -> 90 us; 77 MB 21.0 -> 22.9). The host does not know the lengths; a call is taken to read the smaller of
-// max_len positions of every sequence and the whole pool.
-constexpr int64_t STREAM_BYTES = (int64_t)256 << 20;
-template <class V, bool STREAM> SISA_DEV V load_as(const void* p) {
-    if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
-    else return *reinterpret_cast<const V*>(p);
-}
-
+// STREAM: 16-bit rows of a cache of 256 MB or more, loaded with the non-temporal hint as csrc/decode.hip does (516 MB 102 ->
+// 90 us; 77 MB 21.0 -> 22.9).
+//
 // A workgroup of NW waves per (query row, chunk of 64 NW positions). ONE: one chunk, which writes the row's output, and its
 // weights. Otherwise the chunk's largest score and sum go to stat, its unnormalised output to part, and with TRACK the
 // scores to `scores`.
@@ -117,9 +112,9 @@ __global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_
         ok[i] = page >= 0 && j < vis;
         if (ok[i]) {
             const int64_t slot = j & mask;
-            kr[i] = load_as<frag8<T>, STREAM>((const T*)P.k.ptr + (page * P.k.sb + h * P.k.sh) + slot * P.k.sl + 8 * fg);
-            vr[i] = load_as<frag8<T>, STREAM>((const T*)P.v.ptr + (page * P.v.sb + h * P.v.sh) + slot * P.v.sl + 8 * fg);
-            br[i] = load_as<vec4<T>, STREAM>((const T*)P.b.ptr + (page * P.b.sb + h * P.b.sh) + slot * P.b.sl + 4 * fg);
+            kr[i] = load_hint<frag8<T>, STREAM>((const T*)P.k.ptr + (page * P.k.sb + h * P.k.sh) + slot * P.k.sl + 8 * fg);
+            vr[i] = load_hint<frag8<T>, STREAM>((const T*)P.v.ptr + (page * P.v.sb + h * P.v.sh) + slot * P.v.sl + 8 * fg);
+            br[i] = load_hint<vec4<T>, STREAM>((const T*)P.b.ptr + (page * P.b.sb + h * P.b.sh) + slot * P.b.sl + 4 * fg);
         }
     }
     const f32x8 qv = load_f32x8<T>((const T*)a.q.ptr + n * a.q.sb + h * a.q.sh + m * a.q.sl + 8 * fg);
@@ -332,9 +327,7 @@ int launch_decode(const sisa_paged_decode_args* a, hipStream_t st) {
         return sisa::launch_status("sisa_paged_decode");
     }
     const unsigned grid = (unsigned)(rows * nchunk);
-    const int64_t held = (int64_t)a->pool.pages * a->pool.heads * a->pool.page_size;
-    const int64_t most = rows * a->max_len, bytes = (most < held ? most : held) * ((2 * DH + DS) * (int64_t)sizeof(T) + 8);
-    if (sizeof(T) == 2 && a->M == 1 && bytes >= STREAM_BYTES)
+    if (sizeof(T) == 2 && a->M == 1 && sisa::cache_bytes(a->pool, a->B, a->max_len) >= STREAM_BYTES)
         paged_chunk_kernel<T, DW, false, TRACK, sizeof(T) == 2><<<grid, KCH, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
     else paged_chunk_kernel<T, DW, false, TRACK, false><<<grid, KCH, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
     const int rc = sisa::launch_status("sisa_paged_decode");
