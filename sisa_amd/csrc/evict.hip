@@ -24,49 +24,63 @@ SISA_DEV unsigned order_of(float x) {
 SISA_DEV int count_of(uint64_t lanes) { return __builtin_popcountll(lanes); }
 SISA_DEV int below(uint64_t lanes, int lane) { return __builtin_popcountll(lanes & ((1ull << lane) - 1)); }
 
+// x summed over the wave's lanes up to this one.
+template <int CTRL, int ROWS> SISA_DEV unsigned from_lane(unsigned x) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+SISA_DEV unsigned wave_scan(unsigned x) {
+    x += from_lane<0x111, 0xf>(x);                     // 1, 2, 4, 8 lanes below within the rows of 16
+    x += from_lane<0x112, 0xf>(x);
+    x += from_lane<0x114, 0xf>(x);
+    x += from_lane<0x118, 0xf>(x);
+    x += from_lane<0x142, 0xa>(x);                     // the last lane of rows 0 and 2 to rows 1 and 3
+    return x + from_lane<0x143, 0xc>(x);               // lane 31 to rows 2 and 3
+}
+
 constexpr int COPIES = 8, COPY = 257;  // counters' copies, and from one to the next (a digit's copies on banks of their own)
 
 // NK keys a thread in registers, or 0: read from memory each time they are needed.
 template <int NK>
 __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_args a, int shift, int new_shift) {
-    __shared__ unsigned hist[COPIES * COPY];
+    __shared__ unsigned hists[4][COPIES * COPY];       // of the four digits
     __shared__ unsigned found, left;                   // the digit with the last one to keep, and how many to keep in it
     __shared__ int gt[SW], eq[SW];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int H = a.from.heads, nh = blockIdx.x, h = nh % H, n = nh / H;
     const int len = a.lengths[n], keep = a.keep, recent = a.recent;
     int32_t* pos = a.positions + (int64_t)nh * keep;
-    float* neww = a.new_weights + (int64_t)nh * keep;
     const float* W = (const float*)a.weights.ptr + n * a.weights.sb + h * a.weights.sh;
     const int64_t sl = a.weights.sl;
     const int out = len < keep ? len : keep;
     const bool bad = len < 0 || len > a.max_len || len > ((int64_t)a.W << shift) || out > ((int64_t)a.W_new << new_shift);
     if (h == 0 && tid == 0) a.new_lengths[n] = bad ? -1 : out;
-    for (int i = (bad ? 0 : out) + tid; i < keep; i += 64 * SW) pos[i] = -1, neww[i] = 0.f;
+    for (int i = (bad ? 0 : out) + tid; i < keep; i += 64 * SW) pos[i] = -1;
     if (bad) return;
     if (len <= keep) {
-        for (int i = tid; i < len; i += 64 * SW) pos[i] = i, neww[i] = W[i * sl];
+        for (int i = tid; i < len; i += 64 * SW) pos[i] = i;
         return;
     }
     const int old = len - recent, pick = keep - recent;        // pick of the first `old`, then the recent ones
     // the wave's range of positions, 64 at a time
     const int steps = ((old + SW - 1) / SW + 63) / 64, i0 = w * steps * 64;
-    float x[NK ? NK : 1];
+    unsigned key[NK ? NK : 1];
     if constexpr (NK > 0) {
+        float x[NK];
 #pragma unroll
-        for (int s = 0; s < NK; ++s)
-            if (s < steps && i0 + 64 * s + lane < old) x[s] = W[(i0 + 64 * s + lane) * sl];
+        for (int s = 0; s < NK; ++s) x[s] = s < steps && i0 + 64 * s + lane < old ? W[(i0 + 64 * s + lane) * sl] : 0.f;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) key[s] = order_of(x[s]);
     }
-    for (int i = tid; i < recent; i += 64 * SW) pos[pick + i] = old + i, neww[pick + i] = W[(old + i) * sl];
+    for (int i = tid; i < recent; i += 64 * SW) pos[pick + i] = old + i;
     if (pick == 0) return;
-    // f(position, weight) for each of the wave's positions in order, all lanes together; position -1 where there is none
+    // f(position, key) for each of the wave's positions in order, all lanes together; position -1 where there is none
     auto each = [&](auto&& f) {
         if constexpr (NK > 0) {
 #pragma unroll
             for (int s = 0; s < NK; ++s)
                 if (s < steps) {
                     const int i = i0 + 64 * s + lane;
-                    f(i < old ? i : -1, x[s]);
+                    f(i < old ? i : -1, key[s]);
                 }
         } else {
             for (int s0 = 0; s0 < steps; s0 += 8) {            // eight loads under way
@@ -80,7 +94,7 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
                 for (int e = 0; e < 8; ++e)
                     if (s0 + e < steps) {
                         const int i = i0 + 64 * (s0 + e) + lane;
-                        f(i < old ? i : -1, y[e]);
+                        f(i < old ? i : -1, order_of(y[e]));
                     }
             }
         }
@@ -88,12 +102,12 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
 
     // The smallest key that stays, digit by digit; `want` of the keys with the digits so far are still to be picked.
     unsigned prefix = 0, want = pick;
+    for (int i = tid; i < 4 * COPIES * COPY; i += 64 * SW) (&hists[0][0])[i] = 0;
+    __syncthreads();
     for (int d = 24; d >= 0; d -= 8) {
-        for (int i = tid; i < COPIES * COPY; i += 64 * SW) hist[i] = 0;
-        __syncthreads();
+        unsigned* hist = hists[d >> 3];
         const unsigned high = d == 24 ? 0u : prefix >> (d + 8);
-        each([&](int i, float v) {
-            const unsigned k = order_of(v);
+        each([&](int i, unsigned k) {
             if (i >= 0 && (d == 24 || k >> (d + 8) == high)) atomicAdd(&hist[(lane & (COPIES - 1)) * COPY + (k >> d & 255)], 1u);
         });
         __syncthreads();
@@ -107,13 +121,7 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
                 for (int k = 0; k < COPIES; ++k) c[e] += hist[k * COPY + 255 - 4 * lane - e];
                 mine += c[e];
             }
-            unsigned incl = mine;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const unsigned t = __shfl_up(incl, o);
-                if (lane >= o) incl += t;
-            }
-            unsigned above = incl - mine;
+            unsigned above = wave_scan(mine) - mine;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (above < want && want <= above + c[e]) found = 255 - 4 * lane - e, left = want - above;
@@ -127,8 +135,7 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
 
     // Those above the smallest key, and its equals from the lowest position on.
     int ng = 0, ne = 0;
-    each([&](int i, float v) {
-        const unsigned k = order_of(v);
+    each([&](int i, unsigned k) {
         ng += count_of(__ballot(i >= 0 && k > prefix));
         ne += count_of(__ballot(i >= 0 && k == prefix));
     });
@@ -140,22 +147,17 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
         at += gt[k] + (take < 0 ? 0 : take < eq[k] ? take : eq[k]);
         equals += eq[k];
     }
-    each([&](int i, float v) {
-        const unsigned k = order_of(v);
+    each([&](int i, unsigned k) {
         const uint64_t same = __ballot(i >= 0 && k == prefix);
         const bool stay = i >= 0 && (k > prefix || (k == prefix && equals + below(same, lane) < (int)want));
         const uint64_t stays = __ballot(stay);
-        if (stay) {
-            const int to = at + below(stays, lane);
-            pos[to] = i;
-            neww[to] = v;
-        }
+        if (stay) pos[at + below(stays, lane)] = i;
         at += count_of(stays);
         equals += count_of(same);
     });
 }
 
-// A wave moves ROWS kept rows. A row without a page marks its sequence.
+// A wave moves ROWS kept rows and their weights. A row without a page marks its sequence.
 template <class T, int ROWS, bool STREAM>
 __global__ __launch_bounds__(256) void evict_copy_kernel(sisa_cache_evict_args a, int shift, int new_shift) {
     const int lane = threadIdx.x & 63;
@@ -163,13 +165,17 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(sisa_cache_evict_args a
     const unsigned nh = id / keep, h = nh % H;
     const int i = id % keep;
     const int64_t n = nh / H;
-    const int j = lane < ROWS && n < a.B ? a.positions[id] : -1;
+    const bool mine = lane < ROWS && n < a.B;
+    const int j = mine ? a.positions[id] : -1;
     int src = -1, dst = -1;
+    float weight = 0.f;
     if (j >= 0) {
+        weight = ((const float*)a.weights.ptr)[n * a.weights.sb + h * a.weights.sh + j * a.weights.sl];
         src = page_of(a.table + n * a.s_table, a.W, shift, a.from.pages, j);
         dst = page_of(a.new_table + n * a.s_new, a.W_new, new_shift, a.to.pages, i);
         if (src < 0 || dst < 0) a.new_lengths[n] = -1;
     }
+    if (mine) a.new_weights[id] = weight;
     move_rows<T, ROWS, STREAM>(rows_of_pool(a.from), rows_of_pool(a.to), src >= 0 && dst >= 0, src, dst, h,
                                j & (a.from.page_size - 1), i & (a.to.page_size - 1), lane);
 }

@@ -23,11 +23,6 @@ template <class V, bool HINT> SISA_DEV void store_hint(void* p, V x) {
     else *reinterpret_cast<V*>(p) = x;
 }
 
-// Up to ROWS rows of a cache moved by a wave: lane r's row, if `ok`, from (s0, h, s2) of the source views to (d0, h, d2) of the
-// destination's; no lane from ROWS on has one. 64, or 8 where there are too few rows to fill the chip with waves of 64. Every load and store instruction covers whole rows (k and v of 16 bits: 8 rows of 128 bytes, 8 lanes a
-// row), and all of a pass's loads are under way before its first store: 32 rows a pass in 16 bits, 16 in fp32 (40 registers
-// either way). A row per half wave instead, with three dependent loads in front of each, left the chip waiting: an eviction
-// of 8 x 12 heads from 16,384 to 4,096 positions took 147 us for its copies.
 struct RowViews {
     sisa_view k, v, b, g, f;
 };
@@ -37,11 +32,18 @@ SISA_DEV int64_t lane_value(int64_t x, int lane) {
     return (int64_t)hi << 32 | (unsigned)lo;
 }
 
+// Up to ROWS rows of a cache moved by a wave: lane r's row, if `ok`, from (s0, h, s2) of the source views to (d0, h, d2) of the
+// destination's; no lane from ROWS on has one. 64, or 8 where there are too few rows to fill the chip with waves of 64.
 //
-// Many rows (ROWS = 64) are stored with the non-temporal hint: nothing reads them before the launch ends. Out of a cache
-// larger than the last-level cache those of k and v are loaded with it, too (STREAM; b rows share their lines: with the
-// hint 59.7 us in place of 54.1). Copies of evictions, plain / stores / both: 92 MB
-// out of caches of 130 MB 21.4 / 17.7 / 21.4 us, 258 MB out of 516 MB 64.1 / 62.1 / 54.1.
+// Every load and store instruction covers whole rows (k and v of 16 bits: 8 rows of 128 bytes, 8 lanes a row), and all of a
+// pass's loads are under way before its first store: 32 rows a pass in 16 bits, 16 in fp32 (40 registers either way). A row
+// per half wave instead, with three dependent loads in front of each, left the chip waiting: an eviction of 8 x 12 heads from
+// 16,384 to 4,096 positions took 147 us for its copies.
+//
+// Many rows (ROWS = 64) are stored with the non-temporal hint: nothing reads them before the launch ends. Out of a cache larger
+// than the last-level cache those of k and v are loaded with it, too (STREAM; b rows share their lines: with the hint 59.7 us
+// in place of 54.1). Copies of evictions, plain / stores / both: 92 MB out of caches of 130 MB 21.4 / 17.7 / 21.4 us, 258 MB out
+// of 516 MB 64.1 / 62.1 / 54.1 (4.8 TB/s).
 template <class T, int ROWS, bool STREAM>
 SISA_DEV void move_rows(const RowViews& src, const RowViews& dst, bool ok, int64_t s0, int64_t d0, int64_t h, int64_t s2,
                         int64_t d2, int lane) {
