@@ -111,6 +111,33 @@ typedef struct {
 
 int sisa_cache_evict(const sisa_cache_evict_args* a, void* stream);
 
+/* sisa_step (sisa_hip_step.h) with its cache in pages: one new token of each of B rows through a decoder layer, sequence n's
+ * at position start[n], lengths[n] = start[n] + 1. The recurrences continue from g_last, f_last and phi, which are advanced in
+ * place. weights: accumulated weights as sisa_paged_decode's, in place, or NULL. A sequence whose position has no page of the
+ * pool, or whose length sisa_paged_decode does not take, gives NaN. */
+typedef struct {
+    int32_t B, H, D, FF;       /* rows 1..SISA_STEP_MAX_ROWS, heads, width (64 H), hidden width of the FFN */
+    int32_t dtype;             /* SISA_BF16 or SISA_F16, of the pool, too */
+    int32_t W, max_len, reserved;
+    float eps_attn, eps_ffn;
+    const void* x; int64_t sx;         /* (B, D), row stride sx */
+    const void* res;                   /* (B, D) contiguous, added to x first, or NULL */
+    const void *attn_norm, *w_q, *w_k, *w_v, *w_b, *w_c, *w_theta, *w_alpha, *b_alpha, *w_forget, *b_forget, *w_o;
+    const void *ffn_norm, *w_gate, *w_up, *w_down;     /* all contiguous, (outputs, inputs) */
+    const float* lambda_raw;           /* (H) */
+    sisa_page_pool pool;               /* with f */
+    const int32_t* table; int64_t s_table;             /* (B, W) */
+    const int32_t *start, *lengths;    /* (B) */
+    float *g_last, *f_last, *phi;      /* (B,H), (B,H), (B,H,16) contiguous */
+    sisa_view weights;                 /* (B,H,max_len) fp32 or NULL */
+    void *h, *ffn;                     /* (B, D) contiguous outputs */
+    void* workspace;                   /* sisa_step_paged_workspace_bytes(B,H,D,FF,max_len,dtype,tracked), 256-byte aligned */
+} sisa_step_paged_args;
+
+int64_t sisa_step_paged_workspace_bytes(int32_t B, int32_t H, int32_t D, int32_t FF, int32_t max_len, int32_t dtype,
+                                        int32_t tracked);
+int sisa_step_paged(const sisa_step_paged_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

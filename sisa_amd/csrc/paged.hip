@@ -79,12 +79,13 @@ SISA_DEV float sum_scatter(const float (&x)[8], int fg) {
 // STREAM: 16-bit rows of a cache of 256 MB or more, loaded with the non-temporal hint as csrc/decode.hip does (516 MB 102 ->
 // 90 us; 77 MB 21.0 -> 22.9).
 //
-// A workgroup of NW waves per (query row, chunk of 64 NW positions). ONE: one chunk, which writes the row's output, and its
+// A workgroup of NW waves per (query row, chunk of 64 NW positions). Outputs are TO: float, or the pool's dtype for a layer
+// step, whose next product reads them. ONE: one chunk, which writes the row's output, and its
 // weights. Otherwise the chunk's largest score and sum go to stat, its unnormalised output to part, and with TRACK the
 // scores to `scores`.
-template <class T, int NW, bool ONE, bool TRACK, bool STREAM>
-__global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_args a, int shift, int nchunk, f32x2* stat,
-                                                              float* part, float* scores) {
+template <class T, class TO, int NW, bool ONE, bool TRACK, bool STREAM>
+__global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_args a, TO* out, int shift, int nchunk,
+                                                              f32x2* stat, float* part, float* scores) {
     __shared__ float wm[NW], wl[NW], wo[NW][DH];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int fg = lane & 7, kq = lane >> 3;
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_
         co = fmaf(wo[k][lane], sc, co);
     }
     if constexpr (ONE) {
-        if (w == 0) a.out[(int64_t)row * DH + lane] = vis < 0 ? __builtin_nanf("") : vis == 0 ? 0.f : co / cl;
+        if (w == 0) out[(int64_t)row * DH + lane] = cvt<TO>(vis < 0 ? __builtin_nanf("") : vis == 0 ? 0.f : co / cl);
         if constexpr (TRACK)
             if (j < vis)
                 ((float*)a.w_out.ptr)[n * a.w_out.sb + h * a.w_out.sh + j * a.w_out.sl] =
@@ -209,9 +210,9 @@ __global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_
 // The join of a row's chunks, in a fixed order. A workgroup per query row; or, with tracked weights, per (sequence and head,
 // 1,024 positions), whose rows are taken in order and whose first workgroup writes the outputs. What the weights need is
 // loaded before the row's sum is known.
-template <bool TRACK>
-__global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args a, int shift, int nchunk, const f32x2* stat,
-                                                         const float* part, const float* scores) {
+template <class TO, bool TRACK>
+__global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args a, TO* out, int shift, int nchunk,
+                                                         const f32x2* stat, const float* part, const float* scores) {
     __shared__ float red[2][4], wo[4][DH];
     constexpr int PER = PIECE / 256;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
         const int64_t row = (int64_t)nh * a.M + m;
         const int vis = visible(len, a.max_len, (int64_t)a.W << shift, a.M, m);
         if (vis <= 0) {
-            if (outs && tid < DH) a.out[row * DH + tid] = vis < 0 ? __builtin_nanf("") : 0.f;
+            if (outs && tid < DH) out[row * DH + tid] = cvt<TO>(vis < 0 ? __builtin_nanf("") : 0.f);
             continue;
         }
         float s[PER];
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
             }
             wo[w][lane] = o;
             __syncthreads();
-            if (tid < DH) a.out[row * DH + tid] = ((wo[0][tid] + wo[1][tid]) + (wo[2][tid] + wo[3][tid])) * inv;
+            if (tid < DH) out[row * DH + tid] = cvt<TO>(((wo[0][tid] + wo[1][tid]) + (wo[2][tid] + wo[3][tid])) * inv);
         }
         if constexpr (TRACK) {
 #pragma unroll
@@ -316,33 +317,45 @@ DecodeSpace decode_space(char* base, int64_t rows, int64_t max_len, bool tracked
     return s;
 }
 
-template <class T, bool TRACK>
-int launch_decode(const sisa_paged_decode_args* a, hipStream_t st) {
+template <class T, class TO, bool TRACK>
+int launch_decode(const sisa_paged_decode_args* a, TO* out, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size), nchunk = (int)sisa::cdiv(a->max_len, KCH);
     const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
     const DecodeSpace ws = decode_space((char*)a->workspace, rows, a->max_len, TRACK);
     constexpr int NW = whole_waves<T>();
     if (takes_whole(a->M, a->max_len, (int)sizeof(T), TRACK)) {
-        paged_chunk_kernel<T, NW, true, TRACK, false><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, shift, 1, ws.stat, ws.part, ws.scores);
+        paged_chunk_kernel<T, TO, NW, true, TRACK, false><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, out, shift, 1, nullptr, nullptr,
+                                                                                             nullptr);
         return sisa::launch_status("sisa_paged_decode");
     }
     const unsigned grid = (unsigned)(rows * nchunk);
     if (sizeof(T) == 2 && a->M == 1 && sisa::cache_bytes(a->pool, a->B, a->max_len) >= STREAM_BYTES)
-        paged_chunk_kernel<T, DW, false, TRACK, sizeof(T) == 2><<<grid, KCH, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
-    else paged_chunk_kernel<T, DW, false, TRACK, false><<<grid, KCH, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
+        paged_chunk_kernel<T, TO, DW, false, TRACK, sizeof(T) == 2><<<grid, KCH, 0, st>>>(*a, out, shift, nchunk, ws.stat, ws.part,
+                                                                                         ws.scores);
+    else paged_chunk_kernel<T, TO, DW, false, TRACK, false><<<grid, KCH, 0, st>>>(*a, out, shift, nchunk, ws.stat, ws.part, ws.scores);
     const int rc = sisa::launch_status("sisa_paged_decode");
     if (rc) return rc;
     const int64_t groups = TRACK ? rows / a->M * sisa::cdiv(a->max_len, PIECE) : rows;
-    paged_join_kernel<TRACK><<<(unsigned)groups, 256, 0, st>>>(*a, shift, nchunk, ws.stat, ws.part, ws.scores);
+    paged_join_kernel<TO, TRACK><<<(unsigned)groups, 256, 0, st>>>(*a, out, shift, nchunk, ws.stat, ws.part, ws.scores);
     return sisa::launch_status("sisa_paged_decode (join)");
 }
 
-template <class T>
-int launch_decode(const sisa_paged_decode_args* a, hipStream_t st) {
-    return a->w_out.ptr ? launch_decode<T, true>(a, st) : launch_decode<T, false>(a, st);
+template <class T, class TO>
+int launch_decode(const sisa_paged_decode_args* a, TO* out, hipStream_t st) {
+    return a->w_out.ptr ? launch_decode<T, TO, true>(a, out, st) : launch_decode<T, TO, false>(a, out, st);
 }
 
 }  // namespace
+
+namespace sisa {
+namespace detail {
+// The attention of 16-bit operands with the result rounded to their dtype, (B,H,M,64) contiguous (checked by the caller:
+// sisa_step_paged).
+__attribute__((visibility("hidden"))) int paged_attn_out16(const sisa_paged_decode_args* a, void* out, hipStream_t st) {
+    return a->pool.dtype == SISA_BF16 ? launch_decode<__bf16>(a, (__bf16*)out, st) : launch_decode<_Float16>(a, (_Float16*)out, st);
+}
+}  // namespace detail
+}  // namespace sisa
 
 extern "C" int sisa_paged_write(const sisa_paged_write_args* a, void* stream) {
     SISA_REQUIRE(a != nullptr, "sisa_paged_write: null args");
@@ -393,8 +406,8 @@ extern "C" int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream) 
     SISA_REQUIRE(rows * sisa::cdiv(a->max_len, KCH) < ((int64_t)1 << 31), "sisa_paged_decode: too many rows for one launch");
     hipStream_t st = (hipStream_t)stream;
     switch (a->pool.dtype) {
-        case SISA_BF16: return launch_decode<__bf16>(a, st);
-        case SISA_F16: return launch_decode<_Float16>(a, st);
-        default: return launch_decode<float>(a, st);
+        case SISA_BF16: return launch_decode<__bf16>(a, a->out, st);
+        case SISA_F16: return launch_decode<_Float16>(a, a->out, st);
+        default: return launch_decode<float>(a, a->out, st);
     }
 }

@@ -16,13 +16,13 @@
 // That gives (rows / 16) workgroups, 206 for the projections of a 768-wide layer. The norm in front of a product is
 // recomputed by every workgroup (B short rows, served by L2) while its first weights are on their way: one launch and
 // one dependent round trip less than a norm of its own.
-#include "common.h"
-#include "host.h"
+#include "pages.h"
 #include "sisa_hip_step.h"
 
 namespace sisa {
 namespace detail {
 __attribute__((visibility("hidden"))) int decode_attn_out16(const sisa_decode_args* a, void* out, hipStream_t st);   // decode.hip
+__attribute__((visibility("hidden"))) int paged_attn_out16(const sisa_paged_decode_args* a, void* out, hipStream_t st);  // paged.hip
 }
 }  // namespace sisa
 
@@ -215,15 +215,47 @@ struct AppendArgs {
     int H, pos;
 };
 
+// Where the new position of (b, h) goes, and what g and F continue from.
+struct Place {
+    int64_t b, slot;                   // first and last index of the cache views
+    const float *g, *f;
+    bool there;
+};
+SISA_DEV Place place_of(const AppendArgs& a, int b, int h) {
+    const float* g = (const float*)a.g.ptr + b * a.g.sb + h * a.g.sh + (int64_t)(a.pos - 1) * a.g.sl;
+    const float* f = (const float*)a.f.ptr + b * a.f.sb + h * a.f.sh + (int64_t)(a.pos - 1) * a.f.sl;
+    return Place{b, a.pos, g, f, true};
+}
+
+struct PagedAppendArgs : AppendArgs {  // phi_in, phi_out: the same memory
+    const int32_t *table, *start;
+    int64_t s_table;
+    int W, shift, pages;
+    float *g_last, *f_last;            // (B, H), advanced
+};
+SISA_DEV Place place_of(const PagedAppendArgs& a, int b, int h) {
+    const int64_t pos = a.start[b];
+    const int page = page_of(a.table + b * a.s_table, a.W, a.shift, a.pages, pos);
+    return Place{page, pos & ((1 << a.shift) - 1), a.g_last + b * a.H + h, a.f_last + b * a.H + h, page >= 0};
+}
+SISA_DEV void keep_last(const AppendArgs&, int, float*, float) {}
+SISA_DEV void keep_last(const PagedAppendArgs&, int bh, float* last, float v) { last[bh] = v; }
+SISA_DEV float* g_last(const AppendArgs&) { return nullptr; }
+SISA_DEV float* f_last(const AppendArgs&) { return nullptr; }
+SISA_DEV float* g_last(const PagedAppendArgs& a) { return a.g_last; }
+SISA_DEV float* f_last(const PagedAppendArgs& a) { return a.f_last; }
+
 // One wave per (batch row, head): the recurrences advanced by the new position, c and b rotated by the new phase, the
 // position's k, v, b~, g and F written to the cache.
-template <class T>
-__global__ __launch_bounds__(64) void step_append_kernel(AppendArgs a) {
+template <class T, class Args>
+__global__ __launch_bounds__(64) void step_append_kernel(Args a) {
     const int lane = threadIdx.x, H = a.H, bh = blockIdx.x, b = bh / H, h = bh % H;
     const T* P = (const T*)a.proj + (int64_t)b * 272 * H;
-    const int64_t pos = a.pos;
-    ((T*)a.k.ptr)[b * a.k.sb + h * a.k.sh + pos * a.k.sl + lane] = P[(H + h) * DH + lane];
-    ((T*)a.v.ptr)[b * a.v.sb + h * a.v.sh + pos * a.v.sl + lane] = P[(2 * H + h) * DH + lane];
+    const Place at = place_of(a, b, h);
+    if (at.there) {
+        ((T*)a.k.ptr)[at.b * a.k.sb + h * a.k.sh + at.slot * a.k.sl + lane] = P[(H + h) * DH + lane];
+        ((T*)a.v.ptr)[at.b * a.v.sb + h * a.v.sh + at.slot * a.v.sl + lane] = P[(2 * H + h) * DH + lane];
+    }
     if (lane < DS / 2) {
         const int64_t p = (int64_t)bh * (DS / 2) + lane;
         const float phi = a.phi_in[p] + (float)P[256 * H + h * (DS / 2) + lane];
@@ -232,24 +264,28 @@ __global__ __launch_bounds__(64) void step_append_kernel(AppendArgs a) {
         const T* bp = P + 192 * H + h * DS + 2 * lane;
         const T* cp = P + 224 * H + h * DS + 2 * lane;
         const float b0 = (float)bp[0], b1 = (float)bp[1], c0 = (float)cp[0], c1 = (float)cp[1];
-        T* bo = (T*)a.b.ptr + b * a.b.sb + h * a.b.sh + pos * a.b.sl + 2 * lane;
+        T* bo = (T*)a.b.ptr + at.b * a.b.sb + h * a.b.sh + at.slot * a.b.sl + 2 * lane;
         T* co = (T*)a.c + (int64_t)bh * DS + 2 * lane;
-        bo[0] = cvt<T>(b0 * cs - b1 * sn);
-        bo[1] = cvt<T>(b1 * cs + b0 * sn);
+        if (at.there) {
+            bo[0] = cvt<T>(b0 * cs - b1 * sn);
+            bo[1] = cvt<T>(b1 * cs + b0 * sn);
+        }
         co[0] = cvt<T>(c0 * cs - c1 * sn);
         co[1] = cvt<T>(c1 * cs + c0 * sn);
     } else if (lane == 32) {           // g = g_prev - softplus(alpha), as torch's softplus (threshold 20)
-        float* g = (float*)a.g.ptr + b * a.g.sb + h * a.g.sh + pos * a.g.sl;
+        float* g = (float*)a.g.ptr + at.b * a.g.sb + h * a.g.sh + at.slot * a.g.sl;
         const float al = a.alpha[bh];
-        const float v = g[-a.g.sl] - (al > 20.f ? al : log1pf(expf(al)));
-        g[0] = v;
+        const float v = *at.g - (al > 20.f ? al : log1pf(expf(al)));
+        if (at.there) g[0] = v;
         a.gq[bh] = v;
+        keep_last(a, bh, g_last(a), v);
     } else if (lane == 33) {           // F = F_prev + logsigmoid(z)
-        float* f = (float*)a.f.ptr + b * a.f.sb + h * a.f.sh + pos * a.f.sl;
+        float* f = (float*)a.f.ptr + at.b * a.f.sb + h * a.f.sh + at.slot * a.f.sl;
         const float z = a.z[bh];
-        const float v = f[-a.f.sl] + ((z < 0.f ? z : (z != z ? z : 0.f)) - log1pf(expf(-fabsf(z))));
-        f[0] = v;
+        const float v = *at.f + ((z < 0.f ? z : (z != z ? z : 0.f)) - log1pf(expf(-fabsf(z))));
+        if (at.there) f[0] = v;
         a.fq[bh] = v;
+        keep_last(a, bh, f_last(a), v);
     } else if (lane == 34 && b == 0) {
         const float r = a.lambda_raw[h];
         a.lam[h] = r > 20.f ? r : log1pf(expf(r));
@@ -342,7 +378,7 @@ struct Ws {
 
 int64_t pad256(int64_t b) { return (b + 255) / 256 * 256; }
 
-Ws workspace(char* base, int64_t B, int64_t H, int64_t D, int64_t FF, int64_t N) {
+Ws workspace(char* base, int64_t B, int64_t H, int64_t D, int64_t FF, int64_t attn_bytes) {
     Ws w{};
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -360,7 +396,7 @@ Ws workspace(char* base, int64_t B, int64_t H, int64_t D, int64_t FF, int64_t N)
     w.gq = (float*)take(B * H * 4);
     w.fq = (float*)take(B * H * 4);
     w.lam = (float*)take(H * 4);
-    w.attn = (float*)take(sisa_decode_workspace_bytes((int32_t)B, (int32_t)H, 1, (int32_t)N));
+    w.attn = (float*)take(attn_bytes);
     w.bytes = at;
     return w;
 }
@@ -371,10 +407,10 @@ int64_t norm_lds(int JB, int D, int NS) {
     return rows > part ? rows : part;
 }
 
-template <class T, int JB>
-int launch_step(const sisa_step_args* a, hipStream_t st) {
+// A layer's step; `attend` appends the position and attends, from the projections in the workspace to ws.y.
+template <class T, int JB, class Attend>
+int launch_layer(const sisa_step_args* a, const Ws& ws, Attend&& attend, hipStream_t st) {
     const int B = a->B, H = a->H, D = a->D, FF = a->FF, FP = (FF + 31) / 32 * 32;
-    const Ws ws = workspace((char*)a->workspace, B, H, D, FF, a->pos + 1);
     ProjArgs p{};
     p.nr = NormRows{a->x, a->sx, a->res, a->attn_norm, ws.h0, a->eps_attn, B, D};
     const void* w[8] = {a->w_q, a->w_k, a->w_v, a->w_b, a->w_c, a->w_theta, a->w_alpha, a->w_forget};
@@ -389,31 +425,7 @@ int launch_step(const sisa_step_args* a, hipStream_t st) {
     step_proj_kernel<T, JB><<<groups, 64 * NORM_NWV, norm_lds(JB, D, 1), st>>>(p);
     int rc = sisa::launch_status("sisa_step (projections)");
     if (rc) return rc;
-    step_append_kernel<T><<<(unsigned)(B * H), 64, 0, st>>>(AppendArgs{ws.proj, ws.alpha, ws.z, a->phi_in, a->lambda_raw,
-                                                                       a->k, a->v, a->b, a->g, a->f, a->phi_out, ws.gq,
-                                                                       ws.fq, ws.lam, ws.c, H, a->pos});
-    rc = sisa::launch_status("sisa_step (append)");
-    if (rc) return rc;
-    sisa_decode_args d{};
-    d.B = B;
-    d.H = H;
-    d.M = 1;
-    d.N = a->pos + 1;
-    d.dtype = a->dtype;
-    d.q_start = a->pos;
-    d.q = sisa_view{ws.proj, (int64_t)272 * H, DH, DH};
-    d.c = sisa_view{ws.c, (int64_t)H * DS, DS, DS};
-    d.gq = sisa_view{ws.gq, H, 1, 1};
-    d.fq = sisa_view{ws.fq, H, 1, 1};
-    d.k = a->k;
-    d.v = a->v;
-    d.b = a->b;
-    d.gk = a->g;
-    d.fk = a->f;
-    d.lam = ws.lam;
-    d.s_lam = 1;
-    d.workspace = ws.attn;
-    rc = sisa::detail::decode_attn_out16(&d, ws.y, st);
+    rc = attend();
     if (rc) return rc;
     // h = (x + res) + W_O y, then the FFN of its norm
     step_linear_kernel<T, NORM_NWV, JB, true><<<(unsigned)(D / 16), 64 * NORM_NWV, 0, st>>>(
@@ -436,11 +448,139 @@ int launch_step(const sisa_step_args* a, hipStream_t st) {
     return sisa::launch_status("sisa_step (down)");
 }
 
+template <class T, class Attend>
+int launch_rows(const sisa_step_args* a, const Ws& ws, Attend&& attend, hipStream_t st) {
+    if (a->B <= 16) return launch_layer<T, 1>(a, ws, attend, st);
+    if (a->B <= 32) return launch_layer<T, 2>(a, ws, attend, st);
+    return launch_layer<T, 4>(a, ws, attend, st);
+}
+
 template <class T>
-int launch_step_rows(const sisa_step_args* a, hipStream_t st) {
-    if (a->B <= 16) return launch_step<T, 1>(a, st);
-    if (a->B <= 32) return launch_step<T, 2>(a, st);
-    return launch_step<T, 4>(a, st);
+int launch_step(const sisa_step_args* a, hipStream_t st) {
+    const int B = a->B, H = a->H;
+    const Ws ws = workspace((char*)a->workspace, B, H, a->D, a->FF, sisa_decode_workspace_bytes(B, H, 1, a->pos + 1));
+    return launch_rows<T>(a, ws, [&]() -> int {
+        step_append_kernel<T><<<(unsigned)(B * H), 64, 0, st>>>(AppendArgs{ws.proj, ws.alpha, ws.z, a->phi_in, a->lambda_raw,
+                                                                           a->k, a->v, a->b, a->g, a->f, a->phi_out, ws.gq,
+                                                                           ws.fq, ws.lam, ws.c, H, a->pos});
+        const int rc = sisa::launch_status("sisa_step (append)");
+        if (rc) return rc;
+        sisa_decode_args d{};
+        d.B = B;
+        d.H = H;
+        d.M = 1;
+        d.N = a->pos + 1;
+        d.dtype = a->dtype;
+        d.q_start = a->pos;
+        d.q = sisa_view{ws.proj, (int64_t)272 * H, DH, DH};
+        d.c = sisa_view{ws.c, (int64_t)H * DS, DS, DS};
+        d.gq = sisa_view{ws.gq, H, 1, 1};
+        d.fq = sisa_view{ws.fq, H, 1, 1};
+        d.k = a->k;
+        d.v = a->v;
+        d.b = a->b;
+        d.gk = a->g;
+        d.fk = a->f;
+        d.lam = ws.lam;
+        d.s_lam = 1;
+        d.workspace = ws.attn;
+        return sisa::detail::decode_attn_out16(&d, ws.y, st);
+    }, st);
+}
+
+// The fields that a step with the cache in pages shares with sisa_step.
+sisa_step_args common_of(const sisa_step_paged_args* a) {
+    sisa_step_args c{};
+    c.B = a->B;
+    c.H = a->H;
+    c.D = a->D;
+    c.FF = a->FF;
+    c.dtype = a->dtype;
+    c.eps_attn = a->eps_attn;
+    c.eps_ffn = a->eps_ffn;
+    c.x = a->x;
+    c.sx = a->sx;
+    c.res = a->res;
+    c.attn_norm = a->attn_norm;
+    c.w_q = a->w_q;
+    c.w_k = a->w_k;
+    c.w_v = a->w_v;
+    c.w_b = a->w_b;
+    c.w_c = a->w_c;
+    c.w_theta = a->w_theta;
+    c.w_alpha = a->w_alpha;
+    c.b_alpha = a->b_alpha;
+    c.w_forget = a->w_forget;
+    c.b_forget = a->b_forget;
+    c.w_o = a->w_o;
+    c.ffn_norm = a->ffn_norm;
+    c.w_gate = a->w_gate;
+    c.w_up = a->w_up;
+    c.w_down = a->w_down;
+    c.lambda_raw = a->lambda_raw;
+    c.h = a->h;
+    c.ffn = a->ffn;
+    c.workspace = a->workspace;
+    return c;
+}
+
+template <class T>
+int launch_step_paged(const sisa_step_paged_args* a, hipStream_t st) {
+    const int B = a->B, H = a->H;
+    const sisa_page_pool& p = a->pool;
+    const sisa_step_args c = common_of(a);
+    const Ws ws = workspace((char*)a->workspace, B, H, a->D, a->FF,
+                            sisa_paged_decode_workspace_bytes(B, H, 1, a->max_len, a->dtype, a->weights.ptr != nullptr));
+    return launch_rows<T>(&c, ws, [&]() -> int {
+        PagedAppendArgs ap{};
+        static_cast<AppendArgs&>(ap) = AppendArgs{ws.proj, ws.alpha, ws.z, a->phi, a->lambda_raw, p.k, p.v, p.b, p.g, p.f, a->phi,
+                                                  ws.gq, ws.fq, ws.lam, ws.c, H, 0};
+        ap.table = a->table;
+        ap.start = a->start;
+        ap.s_table = a->s_table;
+        ap.W = a->W;
+        ap.shift = sisa::log2_of(p.page_size);
+        ap.pages = p.pages;
+        ap.g_last = a->g_last;
+        ap.f_last = a->f_last;
+        step_append_kernel<T><<<(unsigned)(B * H), 64, 0, st>>>(ap);
+        const int rc = sisa::launch_status("sisa_step_paged (append)");
+        if (rc) return rc;
+        sisa_paged_decode_args d{};
+        d.B = B;
+        d.M = 1;
+        d.W = a->W;
+        d.max_len = a->max_len;
+        d.pool = p;
+        d.table = a->table;
+        d.s_table = a->s_table;
+        d.lengths = a->lengths;
+        d.q = sisa_view{ws.proj, (int64_t)272 * H, DH, DH};
+        d.c = sisa_view{ws.c, (int64_t)H * DS, DS, DS};
+        d.gq = sisa_view{ws.gq, H, 1, 1};
+        d.fq = sisa_view{ws.fq, H, 1, 1};
+        d.lam = ws.lam;
+        d.s_lam = 1;
+        d.w_in = d.w_out = a->weights;
+        d.workspace = ws.attn;
+        return sisa::detail::paged_attn_out16(&d, ws.y, st);
+    }, st);
+}
+
+// Null where a step's arguments can be used, else what is wrong with them.
+const char* step_fault(const sisa_step_args* a) {
+    if (a->B < 1 || a->B > SISA_STEP_MAX_ROWS || a->H < 1 || a->D != DH * a->H || a->D > SISA_STEP_MAX_D || a->FF < 1)
+        return "B must be in 1 .. 64, D = 64 H at most 1024, FF positive";
+    if (a->dtype != SISA_BF16 && a->dtype != SISA_F16) return "dtype must be bf16 or fp16";
+    const void* given[] = {a->x, a->attn_norm, a->w_q, a->w_k, a->w_v, a->w_b, a->w_c, a->w_theta, a->w_alpha, a->w_forget,
+                           a->w_o, a->ffn_norm, a->w_gate, a->w_up, a->h, a->ffn};
+    for (const void* p : given)
+        if (!p || !sisa::aligned16(p)) return "tensors must be given and 16-byte aligned";
+    if (!a->w_down || (a->FF % 8 == 0 && !sisa::aligned16(a->w_down))) return "w_down not aligned";
+    if ((a->res && !sisa::aligned16(a->res)) || a->sx < a->D || a->sx % 8) return "x rows and res must be 16-byte aligned";
+    if (!a->b_alpha || !a->b_forget || !a->lambda_raw || !a->workspace || ((uintptr_t)a->workspace & 255))
+        return "null pointer, or workspace not 256-byte aligned";
+    return nullptr;
 }
 
 // ------------------------------------------------------------------------------------------------ cache fill
@@ -478,7 +618,7 @@ bool slab_ok(const sisa_view& v, int dtype) { return sisa::view_ok(v, dtype); }
 
 extern "C" int64_t sisa_step_workspace_bytes(int32_t B, int32_t H, int32_t D, int32_t FF, int32_t N) {
     if (B < 1 || H < 1 || D < 1 || FF < 1 || N < 1) return 0;
-    return workspace(nullptr, B, H, D, FF, N).bytes;
+    return workspace(nullptr, B, H, D, FF, sisa_decode_workspace_bytes(B, H, 1, N)).bytes;
 }
 
 extern "C" int sisa_step(const sisa_step_args* a, void* stream) {
@@ -502,7 +642,28 @@ extern "C" int sisa_step(const sisa_step_args* a, void* stream) {
     SISA_REQUIRE(slab_ok(a->k, a->dtype) && slab_ok(a->v, a->dtype) && slab_ok(a->b, a->dtype),
                  "sisa_step: cache rows must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
-    return a->dtype == SISA_BF16 ? launch_step_rows<__bf16>(a, st) : launch_step_rows<_Float16>(a, st);
+    return a->dtype == SISA_BF16 ? launch_step<__bf16>(a, st) : launch_step<_Float16>(a, st);
+}
+
+extern "C" int64_t sisa_step_paged_workspace_bytes(int32_t B, int32_t H, int32_t D, int32_t FF, int32_t max_len,
+                                                   int32_t dtype, int32_t tracked) {
+    if (B < 1 || H < 1 || D < 1 || FF < 1 || max_len < 1) return 0;
+    return workspace(nullptr, B, H, D, FF, sisa_paged_decode_workspace_bytes(B, H, 1, max_len, dtype, tracked)).bytes;
+}
+
+extern "C" int sisa_step_paged(const sisa_step_paged_args* a, void* stream) {
+    SISA_REQUIRE(a != nullptr, "sisa_step_paged: null args");
+    const sisa_step_args c = common_of(a);
+    const char* fault = step_fault(&c);
+    SISA_REQUIRE(fault == nullptr, "sisa_step_paged: %s (B=%d H=%d D=%d FF=%d dtype=%d)", fault, a->B, a->H, a->D, a->FF, a->dtype);
+    SISA_REQUIRE_POOL("sisa_step_paged", a->pool);
+    SISA_REQUIRE(a->pool.heads == a->H && a->pool.dtype == a->dtype && a->pool.f.ptr,
+                 "sisa_step_paged: the pool must have the layer's heads and dtype, and f");
+    SISA_REQUIRE(a->W >= 1 && a->max_len >= 1 && a->max_len <= (int64_t)a->W * a->pool.page_size && a->max_len <= (1 << 30),
+                 "sisa_step_paged: max_len=%d (at most W=%d pages of %d, and 2^30)", a->max_len, a->W, a->pool.page_size);
+    SISA_REQUIRE(a->table && a->start && a->lengths && a->g_last && a->f_last && a->phi, "sisa_step_paged: null pointer");
+    hipStream_t st = (hipStream_t)stream;
+    return a->dtype == SISA_BF16 ? launch_step_paged<__bf16>(a, st) : launch_step_paged<_Float16>(a, st);
 }
 
 extern "C" int sisa_cache_fill(const sisa_cache_fill_args* a, void* stream) {

@@ -180,6 +180,18 @@ class CacheEvictArgs(Structure):
                 ("weights", View), ("new_lengths", c_void_p), ("new_weights", c_void_p), ("positions", c_void_p)]
 
 
+class StepPagedArgs(Structure):
+    _fields_ = [("B", c_int32), ("H", c_int32), ("D", c_int32), ("FF", c_int32), ("dtype", c_int32), ("W", c_int32),
+                ("max_len", c_int32), ("reserved", c_int32), ("eps_attn", c_float), ("eps_ffn", c_float),
+                ("x", c_void_p), ("sx", c_int64), ("res", c_void_p),
+                *((n, c_void_p) for n in ("attn_norm", "w_q", "w_k", "w_v", "w_b", "w_c", "w_theta", "w_alpha",
+                                          "b_alpha", "w_forget", "b_forget", "w_o", "ffn_norm", "w_gate", "w_up",
+                                          "w_down", "lambda_raw")),
+                ("pool", PagePoolArgs), ("table", c_void_p), ("s_table", c_int64), ("start", c_void_p),
+                ("lengths", c_void_p), ("g_last", c_void_p), ("f_last", c_void_p), ("phi", c_void_p),
+                ("weights", View), ("h", c_void_p), ("ffn", c_void_p), ("workspace", c_void_p)]
+
+
 class Round16Args(Structure):
     _fields_ = [("n", c_int64), ("dtype", c_int32), ("x", c_void_p), ("y", c_void_p), ("back", c_void_p)]
 
@@ -244,6 +256,8 @@ CACHE_SIGNATURES = {
     "sisa_attn_weights_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32], c_int64),
     "sisa_attn_weights": ([POINTER(AttnWeightsArgs), c_void_p], c_int),
     "sisa_cache_evict": ([POINTER(CacheEvictArgs), c_void_p], c_int),
+    "sisa_step_paged_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32], c_int64),
+    "sisa_step_paged": ([POINTER(StepPagedArgs), c_void_p], c_int),
 }
 
 _LOCK = threading.Lock()
@@ -325,7 +339,7 @@ def call_values(name: str, dev_tensor: torch.Tensor, *values) -> None:
         raise RuntimeError(f"{name} failed (code {rc}): {msg}")
 
 
-_CODES = {c_int32: "i", c_int64: "q", c_void_p: "P"}
+_CODES = {c_int32: "i", c_int64: "q", c_void_p: "P", c_float: "f"}
 
 
 def _codes(cls) -> str:

@@ -1,5 +1,6 @@
 """Generation on the HIP kernels of csrc/step.hip and csrc/prefill.hip: one new token of every row through a whole
-decoder layer with a filled cache (``sisa_step``, seven launches behind one C call), a prompt through a layer with an empty
+decoder layer with a filled cache (``sisa_step``, and ``sisa_step_paged`` for a cache in pages, seven launches behind one C
+call), a prompt through a layer with an empty
 one (``sisa_prefill``, thirteen), and the filling of a layer's cache after a prefill on the fused route
 (``sisa_cache_fill``). The module path these stand in for is src/sisa/modeling.py:171-199, 224-238,
 288-291; there a layer's step is about seventy torch kernels, whose launches cost four times what they compute.
@@ -20,7 +21,7 @@ from . import attention as A
 from . import fused_prep as P
 
 __all__ = ["unobserved", "plain", "plain_linears", "rows_ok", "whole", "prefill_takes", "step_weights",
-           "layer_step", "layer_prefill", "prefill", "MAX_ROWS", "MAX_WIDTH", "PREFILL_ROWS", "PREFILL_WORK"]
+           "layer_step", "layer_step_paged", "layer_prefill", "prefill", "MAX_ROWS", "MAX_WIDTH", "PREFILL_ROWS", "PREFILL_WORK"]
 
 MAX_ROWS, MAX_WIDTH = 64, 1024          # SISA_STEP_MAX_ROWS, SISA_STEP_MAX_D
 #: Prompts of at most this many tokens (all rows together) take ``sisa_prefill``, and at most PREFILL_WORK / width of them
@@ -126,6 +127,29 @@ def layer_step(x: Tensor, res: Tensor | None, weights: list[int], d_ff: int, lam
                          phi_out.data_ptr(), h.data_ptr(), ffn.data_ptr(), ws.data_ptr())
     _lib.call("sisa_step", args, x)
     return h, ffn, phi_out
+
+
+_step_paged = _lib.Packed("sisa_step_paged", _lib.StepPagedArgs)
+
+
+def layer_step_paged(x: Tensor, res: Tensor | None, weights: list[int], d_ff: int, lambda_raw: Tensor,
+                     eps: tuple[float, float], cache, layer_idx: int) -> tuple[Tensor, Tensor]:
+    """:func:`layer_step` with a :class:`sisa_amd.paged.SISAPagedCache` whose sequences all hold positions in this layer's
+    HIP pool: ``(h, ffn)``, the cache extended by a position of every sequence."""
+    B, _, D = x.shape
+    H = D // HIP_D_HEAD
+    at = cache.begin_step(layer_idx)
+    h, ffn = torch.empty((2, B, 1, D), device=x.device, dtype=x.dtype).unbind(0)
+    tracked, dtype = at.weights is not None, _lib.dtype_code(x.dtype)
+    size = _lib.load().sisa_step_paged_workspace_bytes(B, H, D, d_ff, at.max_len, dtype, tracked)
+    ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
+    w = (at.weights.data_ptr(), *at.weights.stride()) if tracked else (0, 0, 0, 0)
+    _step_paged(x, B, H, D, d_ff, dtype, at.table.shape[1], at.max_len, 0, *eps, x.data_ptr(), x.stride(0),
+                0 if res is None else res.data_ptr(), *weights, lambda_raw.data_ptr(), at.pool.packed, at.table.data_ptr(),
+                at.table.stride(0), at.start.data_ptr(), at.end.data_ptr(), *(t.data_ptr() for t in at.last), *w,
+                h.data_ptr(), ffn.data_ptr(), ws.data_ptr())
+    cache.end_step(layer_idx)
+    return h, ffn
 
 
 def _fill(cache, layer_idx: int, name: str, args, x: Tensor) -> None:

@@ -345,7 +345,8 @@ class SISABlock(nn.Module):
     def _forward_cached_hip(self, x: Tensor, res: Tensor | None, cache: "SISACache"):
         """Generation on HIP kernels, or None where it does not apply. A prompt (empty cache entry) takes
         ``sisa_prefill`` in a 16-bit model while it is short, else :meth:`_forward_hip` with the cache filled from the
-        fused projections; one new position of at most 64 rows of a 16-bit model takes ``sisa_step``. All return
+        fused projections; one new position of at most 64 rows of a 16-bit model takes ``sisa_step``, or with a cache in
+        pages, whose prompts take the module path, ``sisa_step_paged``. All return
         ``(h, f)`` as :meth:`_forward_hip` with ``defer``. Only for inference with nothing watching the modules in
         between: other calls take the module path."""
         from .generation import SISACache
@@ -354,7 +355,9 @@ class SISABlock(nn.Module):
         # Cheap conditions first: a call that keeps the module path pays for them in every layer. A forced implementation
         # that x does not meet raises in the module path, or not at all: a cached fp32 call runs the unfused kernels in
         # place of "hip_fused", and a decode step selects nothing.
-        if type(cache) is not SISACache or not self._norm_rows_ok(x) or self.config.attn_impl not in ("auto", "hip_fused"):
+        paged = type(cache) is SISAPagedCache
+        if not (paged or type(cache) is SISACache) or not self._norm_rows_ok(x) \
+                or self.config.attn_impl not in ("auto", "hip_fused"):
             return None
         autocast = torch.is_autocast_enabled("cuda")
         if (torch.get_autocast_dtype("cuda") if autocast else x.dtype) not in _LOW_PRECISION:
@@ -363,8 +366,10 @@ class SISABlock(nn.Module):
         at, ffn, n1, n2 = mods["attn"], mods["ffn"], mods["attn_norm"], mods["ffn_norm"]
         if not step.plain(at, SISAAttention):
             return None
-        slab, mode = cache._slabs.get(at.layer_idx), backends.get_check_mode()
         (B, L, D), H = x.shape, self.config.n_head
+        if paged and not cache.kernel_layer(at.layer_idx, x, H):
+            return None
+        slab, mode = cache if paged else cache._slabs.get(at.layer_idx), backends.get_check_mode()
         if slab is not None and (autocast or L != 1 or B > step.MAX_ROWS or D > step.MAX_WIDTH):
             return None
         if not (step.unobserved(x) and step.plain(self, SISABlock) and step.plain(ffn, SwiGLU) and step.plain(n1, RMSNorm)
@@ -373,7 +378,10 @@ class SISABlock(nn.Module):
         lam = at.lambda_raw
         native = (not autocast and lam.dtype == torch.float32 and lam.shape == (H,)
                   and lam.get_device() == x.get_device() and lam.is_contiguous())
-        if slab is not None:
+        if paged:
+            if not native or not step.rows_ok(x) or not step.whole(res):
+                return None
+        elif slab is not None:
             buf = slab.buffers
             if not native or slab.filled < 1 or not step.rows_ok(x) or not step.whole(res) or buf["k"].dtype != x.dtype \
                     or buf["k"].shape[:2] != (B, H) or buf["k"].get_device() != x.get_device():
@@ -392,6 +400,8 @@ class SISABlock(nn.Module):
         weights = step.step_weights(linears, n1._parameters.get("weight"), n2._parameters.get("weight"), H, x)
         if weights is None:
             return None
+        if paged:
+            return step.layer_step_paged(x, res, *weights, lam, (n1.eps, n2.eps), cache, at.layer_idx)
         slab = cache.room(at.layer_idx, 1, buf, slab.phi)
         h, f, phi = step.layer_step(x, res, *weights, lam, (n1.eps, n2.eps), slab, slab.phi.contiguous())
         slab.filled, slab.phi = slab.filled + 1, phi

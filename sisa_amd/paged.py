@@ -134,6 +134,18 @@ class _Last(NamedTuple):
     phi: Tensor
 
 
+class _Step(NamedTuple):
+    """What a layer's step is given: the pool, the sequences' table rows, their lengths before and after, what the recurrences
+    continue from (advanced in place), the accumulated weights, and a bound on the lengths."""
+    pool: object
+    table: Tensor
+    start: Tensor
+    end: Tensor
+    last: _Last
+    weights: Tensor | None
+    max_len: int
+
+
 class _Layer:
     """One layer: its pages, the last position's recurrences, how many positions each sequence holds, and the accumulated
     weights ``(sequences, H, max_length)`` of a tracked cache."""
@@ -267,7 +279,7 @@ class SISAPagedCache:
                              "their own (cache[n])")
         return _Last(*(t[self._lo:self._hi] for t in layer.last))
 
-    def _begin(self, layer: _Layer, M: int, device: torch.device) -> None:
+    def _begin(self, layer: _Layer, M: int) -> None:
         """The positions of a pass of ``M``, at its first layer; the later ones find them there."""
         st, lo, hi = self._store, self._lo, self._hi
         if layer.filled[lo:hi] != st.lengths[lo:hi]:
@@ -326,7 +338,7 @@ class SISAPagedCache:
         if (layer.pool.k.dtype, layer.pool.k.shape[1]) != (p.k.dtype, p.k.shape[1]):
             raise ValueError(f"SISAPagedCache: filled in {layer.pool.k.dtype} with {layer.pool.k.shape[1]} heads, got "
                              f"{p.k.dtype} and {p.k.shape[1]}")
-        self._begin(layer, M, p.k.device)
+        self._begin(layer, M)
         padded = [n - m for n, m in zip(self.lengths, layer.filled[lo:hi])] != [M] * B
         count = st.end[lo:hi] - st.start[lo:hi] if padded or not hip else None
         rows = (p.k, p.v, p.b, p.g.float(), p.fgate.float())
@@ -371,6 +383,26 @@ class SISAPagedCache:
             w = attention_weights(p.q, p.k, p.c, p.b, p.g, lam, p.fgate, st.end[lo:hi])
         N = min(L, st.max_length)                          # a padded batch may be wider than the cache
         st.layers[layer_idx].weights[lo:hi, :, :N] = w[:, :, :N]
+
+    def kernel_layer(self, layer_idx: int, like: Tensor, heads: int) -> bool:
+        """Whether every sequence holds positions in this layer, in a pool of the HIP kernels for rows of ``like``'s dtype and
+        device with ``heads`` heads."""
+        layer = self._store.layers.get(layer_idx)
+        return (layer is not None and not isinstance(layer.pool, _Pages) and all(layer.filled[self._lo:self._hi])
+                and (layer.pool.dtype, layer.pool.heads, layer.pool.device_index) == (like.dtype, heads, like.get_device())
+                and len(self) == like.shape[0])
+
+    def begin_step(self, layer_idx: int) -> "_Step":
+        """One more position of every sequence of a :meth:`kernel_layer`: what a kernel that writes it, advances the
+        recurrences and attends needs; :meth:`end_step` follows."""
+        st, lo, hi = self._store, self._lo, self._hi
+        layer = st.layers[layer_idx]
+        self._begin(layer, 1)
+        return _Step(layer.pool, st.table[lo:hi], st.start[lo:hi], st.end[lo:hi], _Last(*(t[lo:hi] for t in layer.last)),
+                     None if layer.weights is None else layer.weights[lo:hi], self.seq_len)
+
+    def end_step(self, layer_idx: int) -> None:
+        self._store.layers[layer_idx].filled[self._lo:self._hi] = self.lengths
 
     # -------------------------------------------------------------------------------------------- memory
     def reserve(self, positions: int) -> None:

@@ -24,7 +24,7 @@ def lib():
 def test_header_functions_are_exported(lib):
     from sisa_amd.kernels import _lib
     declared = set(re.findall(r"^(?:int|int64_t)\s+(sisa_\w+)\(", open(HEADER).read(), re.M))
-    assert declared == set(_lib.CACHE_SIGNATURES) and len(declared) == 6
+    assert declared == set(_lib.CACHE_SIGNATURES) and len(declared) == 8
     assert all(hasattr(lib, name) for name in declared)
 
 
@@ -32,7 +32,7 @@ def test_struct_layout_matches_c(tmp_path):
     from sisa_amd.kernels import _lib
     pairs = {"PagePoolArgs": "sisa_page_pool", "PagedWriteArgs": "sisa_paged_write_args",
              "PagedDecodeArgs": "sisa_paged_decode_args", "AttnWeightsArgs": "sisa_attn_weights_args",
-             "CacheEvictArgs": "sisa_cache_evict_args"}
+             "CacheEvictArgs": "sisa_cache_evict_args", "StepPagedArgs": "sisa_step_paged_args"}
     lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "sisa_hip_cache.h"', "int main(void) {"]
     expect = []
     for py, c in pairs.items():
@@ -104,6 +104,27 @@ def test_entry_points_refuse_bad_arguments(lib):
                        (evict(to=_pool(lib, f=none)), "agree"), (evict(w=none), "null"), (evict(positions=None), "null")):
         _refused(lib, "sisa_cache_evict", args, word)
     assert lib.sisa_cache_evict(ctypes.byref(evict(B=0)), None) == 0
+
+
+def test_step_refuses_bad_arguments(lib):
+    from sisa_amd.kernels import _lib
+    assert lib.sisa_step_paged(None, None) == 1 and lib.sisa_last_error().decode().startswith("sisa_step_paged")
+
+    def step(B=1, H=2, D=128, dtype=_lib.BF16, W=1, max_len=16, w_q=4096, pool=None, g_last=4096, ws=4096):
+        return _lib.StepPagedArgs(B, H, D, 256, dtype, W, max_len, 0, 1e-6, 1e-6, 4096, D, None, 4096, w_q, *[4096] * 15,
+                                  pool or _pool(lib), 4096, W, 4096, 4096, g_last, 4096, 4096, _lib.View(None, 0, 0, 0), 4096,
+                                  4096, ws)
+    none = _lib.View(None, 0, 0, 0)
+    for args, word in ((step(B=0), "B must be"), (step(B=65), "B must be"), (step(D=192), "B must be"),
+                       (step(dtype=_lib.F32), "bf16 or fp16"), (step(w_q=None), "given"), (step(w_q=4098), "aligned"),
+                       (step(ws=4112), "256-byte"), (step(pool=_pool(lib, dtype=_lib.F16)), "heads and dtype"),
+                       (step(pool=_pool(lib, heads=3)), "heads and dtype"), (step(pool=_pool(lib, f=none)), "and f"),
+                       (step(pool=_pool(lib, page_size=20)), "power of two"), (step(max_len=17), "max_len"),
+                       (step(g_last=None), "null")):
+        _refused(lib, "sisa_step_paged", args, word)
+    assert lib.sisa_step_paged_workspace_bytes(0, 2, 128, 256, 16, _lib.BF16, 0) == 0
+    assert lib.sisa_step_paged_workspace_bytes(1, 2, 128, 256, 9000, _lib.BF16, 1) > \
+        lib.sisa_step_paged_workspace_bytes(1, 2, 128, 256, 9000, _lib.BF16, 0) > 0
 
 
 def test_workspaces(lib):

@@ -272,12 +272,15 @@ def test_unequal_lengths_on_the_gpu(dtype, bound, monkeypatch):
     """Ragged prompts, steps, an eviction, steps, against the model's float64 copy on the CPU with the same positions kept.
     Bounds: the contiguous cache's logits of these models are off float64 by up to half of them."""
     from sisa_amd.kernels import paged as K
+    from sisa_amd.kernels import step
     model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).to(dtype).eval()
     ref = tiny_model(seed=3, theta_scale=0.25).eval()
     ref.load_state_dict({n: t.cpu() for n, t in model.state_dict().items()})
     ref = ref.double()
     used, real = [], (K.sisa_paged_decode_hip, K.sisa_cache_evict_hip)
     monkeypatch.setattr(K, "sisa_paged_decode_hip", lambda *a, **kw: used.append("decode") or real[0](*a, **kw))
+    whole = step.layer_step_paged
+    monkeypatch.setattr(step, "layer_step_paged", lambda *a: used.append("step") or whole(*a))
     ids, counts = token_ids(3, 120, seed=10), [90, 17, 64]
     monkeypatch.setattr(K, "sisa_cache_evict_hip", lambda *a, **kw: used.append("evict") or real[1](*a, **kw))
     caches = [SISAPagedCache(3, 128, page_size=32, pages=20, track=True) for _ in range(2)]
@@ -299,7 +302,7 @@ def test_unequal_lengths_on_the_gpu(dtype, bound, monkeypatch):
             got += [m(x[:, t:t + 1], cache=cache).logits for t in range(95, 100)]
         outs.append(torch.cat(got, 1).cpu())
         assert cache.lengths == [45, 27, 45]
-    assert used.count("decode") == 20 and used.count("evict") >= 2
+    assert used.count("decode" if dtype == torch.float32 else "step") == 20 and used.count("evict") >= 2
     assert rel_err(outs[0], outs[1]) <= bound
     for i in range(3):
         assert rel_err(outs[0][i], outs[1][i]) <= 1.5 * bound
@@ -318,3 +321,87 @@ def test_generate_on_the_gpu_with_lengths_and_budget():
     assert cut.shape == (3, 70) and torch.equal(cut, again)
     half = model.to(torch.bfloat16)
     assert generate(half, ids, 20, cache_budget=32, cache_recent=8).shape == (3, 60)
+
+
+# rows: one and two column groups of the products; a hidden width that is no multiple of 8; few and many heads; with and without
+# tracking; a cache that one workgroup takes whole, and longer ones
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,d_ff,longest,track", [(1, 2, 256, 40, False), (3, 12, 2744, 300, True), (17, 5, 329, 65, True),
+                                                    (64, 16, 1000, 20, False), (2, 2, 256, 1500, True)])
+def test_step_matches_modules(B, H, d_ff, longest, track, dtype, monkeypatch):
+    """A layer's step behind one C call against the module path: near prompts' lengths of their own, steps, an eviction in
+    between. Both round the same quantities: neither is further from the float64 model than the other by more than the spread
+    of such errors (the bound of the contiguous cache's step test)."""
+    from sisa_amd.kernels import step as K
+    steps = 6
+    model = tiny_model(seed=B, theta_scale=0.25, attn_impl="auto", n_head=H, d_model=64 * H, d_ff=d_ff).to(DEV).to(dtype).eval()
+    ids, counts = token_ids(B, longest + steps, seed=H).to(DEV), [max(1, longest * (i + 1) // B) for i in range(B)]
+    calls, real = [], K.layer_step_paged
+    monkeypatch.setattr(K, "layer_step_paged", lambda *a: calls.append(1) or real(*a))
+    outs, held = [], []
+    for watched in (False, True):
+        hooks = [blk.attn.W_Q.register_forward_hook(lambda *a: None) for blk in model.layers] if watched else []
+        cache = SISAPagedCache(B, longest + steps, page_size=32, track=track, pages=2 * B * -(-(longest + steps) // 32))
+        calls.clear()
+        with torch.no_grad():
+            cache.expect(counts)
+            model(ids[:, :longest], cache=cache)
+            if not watched:
+                first = cache
+            got = []
+            for t in range(longest, longest + steps):
+                if track and t == longest + 3:
+                    cache.evict(max(1, longest // 2), max(1, longest // 4))
+                got.append(model(ids[:, t:t + 1], cache=cache).logits)
+        assert len(calls) == (0 if watched else 2 * steps)
+        outs.append(torch.cat(got, 1).float())
+        held.append(cache)
+        for h in hooks:
+            h.remove()
+    assert held[0].lengths == held[1].lengths
+    # Without an eviction against float64: each row's own prompt and the steps' tokens. With one, rows that keep other
+    # positions after a near tie cannot be compared: the first three steps.
+    n = 3 if track else steps
+    rows = [torch.cat([ids[i:i + 1, :c], ids[i:i + 1, longest:longest + n]], 1) for i, c in enumerate(counts)][:4]
+    from oracle import model64 as M64
+    p64 = M64.params64(model, requires_grad=False)
+    ref = torch.cat([M64.logits64(model, p64, r)[:, c:] for r, c in zip(rows, counts)])
+    a, b = (rel_err(o[:4, :n], ref) for o in outs)
+    assert a <= 1.25 * b + 1e-3
+    eps = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    if track:
+        assert all(torch.isfinite(o).all() for o in outs)
+        for layer in range(2):
+            w = [c.weights(layer) for c in held]
+            assert all(x.isfinite().all() and (x >= 0).all() for x in w)
+    else:
+        for layer in range(2):
+            x, y = (c.last(layer) for c in held)
+            for u, v in zip(x, y):
+                assert rel_err(u, v) <= 2 * eps + 1e-6
+
+
+@pytest.mark.gpu
+def test_calls_that_keep_the_module_path_with_pages(monkeypatch):
+    from sisa_amd.kernels import step as K
+    calls, real = [], K.layer_step_paged
+    monkeypatch.setattr(K, "layer_step_paged", lambda *a: calls.append(1) or real(*a))
+    model = tiny_model(seed=1, attn_impl="auto").to(DEV).to(torch.bfloat16).eval()
+
+    def steps_of(model, rows=3, n=1, ctx=torch.no_grad, part=None):
+        ids = token_ids(rows, 12, seed=1).to(DEV)
+        cache = SISAPagedCache(rows, 20)
+        calls.clear()
+        with torch.no_grad():
+            model(ids[:, :8], cache=cache)
+            with ctx():
+                model(ids[:1, 8:8 + n] if part else ids[:, 8:8 + n], cache=cache[0] if part else cache)
+        return len(calls)
+
+    assert steps_of(model) == 2 and steps_of(model, part=True) == 2
+    assert steps_of(model, n=2) == 0 and steps_of(model, rows=65) == 0
+    assert steps_of(model, ctx=lambda: torch.autocast("cuda", dtype=torch.bfloat16)) == 0
+    model.set_attn_impl("hip")
+    assert steps_of(model) == 0
+    assert steps_of(tiny_model(seed=1, attn_impl="auto").to(DEV).eval()) == 0
