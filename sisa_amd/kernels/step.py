@@ -21,7 +21,7 @@ from . import attention as A
 from . import fused_prep as P
 
 __all__ = ["unobserved", "plain", "plain_linears", "rows_ok", "whole", "prefill_takes", "step_weights",
-           "layer_step", "layer_step_paged", "layer_prefill", "prefill", "MAX_ROWS", "MAX_WIDTH", "PREFILL_ROWS", "PREFILL_WORK"]
+           "layer_step", "layer_step_paged", "prefill_paged", "layer_prefill", "prefill", "MAX_ROWS", "MAX_WIDTH", "PREFILL_ROWS", "PREFILL_WORK"]
 
 MAX_ROWS, MAX_WIDTH = 64, 1024          # SISA_STEP_MAX_ROWS, SISA_STEP_MAX_D
 #: Prompts of at most this many tokens (all rows together) take ``sisa_prefill``, and at most PREFILL_WORK / width of them
@@ -209,4 +209,25 @@ def prefill(proj: Tensor, z: Tensor, lam: Tensor, n_head: int, cache, layer_idx:
         pp.br.data_ptr(), pp.g.data_ptr(), pp.f.data_ptr(), pp.totals.data_ptr(),
         *(_lib.view(buf[n]) for n in ("k", "v", "b", "g", "fgate")), phi.data_ptr()), proj)
     slab.filled = L
+    return fw.o.transpose(1, 2).flatten(2)
+
+
+def prefill_paged(proj: Tensor, z: Tensor, lam: Tensor, n_head: int, cache, layer_idx: int) -> Tensor:
+    """:func:`prefill` with a :class:`sisa_amd.paged.SISAPagedCache` that is empty in this layer: the real positions of a
+    right-padded batch go to its pages, their received weights are tracked where the cache does."""
+    B, L, _ = proj.shape
+    lay = P.fused_layout(n_head)
+    pp = P.prep_forward(proj, z, n_head)
+    q, k, v = (P._heads(proj, lay[n], n_head) for n in ("Q", "K", "V"))
+    c, b = pp.state_views()
+    fw = A.attn_forward(q, k, v, c, b, pp.g, lam, pp.f)
+    count = cache.begin(layer_idx, k, b, True)
+    rates = proj[..., lay["TH"]:lay["TH"] + n_head * HIP_D_STATE // 2]
+    if count is not None:
+        real = torch.arange(L, device=proj.device) < count[:, None]
+        rates = torch.where(real[..., None], rates, 0.0)
+    phi = rates.sum(1, dtype=torch.float32).view(B, n_head, HIP_D_STATE // 2)
+    cache.put(layer_idx, (k, v, b, pp.g, pp.f), phi, count, True)
+    if cache.tracked:
+        cache.receive(layer_idx, q, k, c, b, pp.g, lam, pp.f, True)
     return fw.o.transpose(1, 2).flatten(2)

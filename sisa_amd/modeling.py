@@ -228,7 +228,7 @@ class SISAAttention(nn.Module):
                                     self.W_C.weight, self.theta_proj.weight, self.alpha_proj.weight,
                                     self.alpha_proj.bias)
 
-    def _forward_fused(self, x: Tensor, z: Tensor | None = None, cache: "SISACache | None" = None) -> Tensor:
+    def _forward_fused(self, x: Tensor, z: Tensor | None = None, cache: "SISACache | SISAPagedCache | None" = None) -> Tensor:
         """The fused route. ``z``: forget-gate logits already produced by the decoder block's norm kernel; with it
         the projections use the HIP weight-gradient GEMM path of the block, without it (the sublayer called on its
         own) plain ``F.linear``. ``cache`` (with ``z``, inference): also fill this layer's empty entry."""
@@ -240,9 +240,10 @@ class SISAAttention(nn.Module):
             y = sisa_fused(F.linear(x, weight, bias), self._forget_logits(x), self.lam(), n_head)
             return self.W_O(y)                         # y: (B, L, d), heads side by side
         if cache is not None:
-            from .kernels.step import prefill
+            from .kernels.step import prefill, prefill_paged
 
-            return F.linear(prefill(F.linear(x, weight, bias), z, self.lam(), n_head, cache, self.layer_idx),
+            fill = prefill_paged if isinstance(cache, SISAPagedCache) else prefill
+            return F.linear(fill(F.linear(x, weight, bias), z, self.lam(), n_head, cache, self.layer_idx),
                             self.W_O.weight)
         a0 = fused_layout(n_head)["A"]                 # the bias is a parameter on the alpha columns only
         y = sisa_fused(_linear(x, weight, bias, (a0, a0 + n_head)), z, self.lam(), n_head)
@@ -285,7 +286,7 @@ class SISAAttention(nn.Module):
             y = self._attention(p, "hip" if impl == "hip_fused" else impl)
             cache.extend(self.layer_idx, p, hip)
             if cache.tracked:
-                cache.receive(self.layer_idx, p, lam, hip)
+                cache.receive(self.layer_idx, p.q, p.k, p.c, p.b, p.g, lam, p.fgate, hip)
             return self._output(y)
         cache.extend(self.layer_idx, p, hip)
         return self._output(cache.attend(self.layer_idx, p, lam, hip).to(p.q.dtype))
@@ -346,7 +347,7 @@ class SISABlock(nn.Module):
         """Generation on HIP kernels, or None where it does not apply. A prompt (empty cache entry) takes
         ``sisa_prefill`` in a 16-bit model while it is short, else :meth:`_forward_hip` with the cache filled from the
         fused projections; one new position of at most 64 rows of a 16-bit model takes ``sisa_step``, or with a cache in
-        pages, whose prompts take the module path, ``sisa_step_paged``. All return
+        pages, whose prompts all go by :meth:`_forward_hip`, ``sisa_step_paged``. All return
         ``(h, f)`` as :meth:`_forward_hip` with ``defer``. Only for inference with nothing watching the modules in
         between: other calls take the module path."""
         from .generation import SISACache
@@ -367,9 +368,15 @@ class SISABlock(nn.Module):
         if not step.plain(at, SISAAttention):
             return None
         (B, L, D), H = x.shape, self.config.n_head
-        if paged and not cache.kernel_layer(at.layer_idx, x, H):
+        mode = backends.get_check_mode()
+        if not paged:
+            slab = cache._slabs.get(at.layer_idx)
+        elif cache.empty(at.layer_idx):
+            slab = None
+        elif cache.kernel_layer(at.layer_idx, x, H):
+            slab = cache
+        else:
             return None
-        slab, mode = cache if paged else cache._slabs.get(at.layer_idx), backends.get_check_mode()
         if slab is not None and (autocast or L != 1 or B > step.MAX_ROWS or D > step.MAX_WIDTH):
             return None
         if not (step.unobserved(x) and step.plain(self, SISABlock) and step.plain(ffn, SwiGLU) and step.plain(n1, RMSNorm)
@@ -378,7 +385,7 @@ class SISABlock(nn.Module):
         lam = at.lambda_raw
         native = (not autocast and lam.dtype == torch.float32 and lam.shape == (H,)
                   and lam.get_device() == x.get_device() and lam.is_contiguous())
-        if paged:
+        if paged and slab is not None:
             if not native or not step.rows_ok(x) or not step.whole(res):
                 return None
         elif slab is not None:
@@ -390,7 +397,7 @@ class SISABlock(nn.Module):
         if linears is None or not backends.meets("hip_fused", x, self.config):
             return None
         if slab is None:
-            native = (native and step.prefill_takes(B * L, D, ffn.w_gate.out_features) and mode != "sync"
+            native = (native and not paged and step.prefill_takes(B * L, D, ffn.w_gate.out_features) and mode != "sync"
                       and step.whole(x) and step.whole(res))
             weights = native and step.step_weights(linears, n1._parameters.get("weight"), n2._parameters.get("weight"), H, x)
             if not weights:

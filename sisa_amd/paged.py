@@ -126,6 +126,14 @@ def _evict(pool: _Pages, table: Tensor, lengths: Tensor, weights: Tensor, keep: 
 
 
 # ------------------------------------------------------------------------------------------------ the cache
+def at_last(x: Tensor, count: Tensor | None) -> Tensor:
+    """The last real position of ``x`` ``(B, H, M, ...)``, kept as an axis of one."""
+    if count is None:
+        return x[:, :, -1:]
+    at = (count.long() - 1).view(-1, 1, 1, *[1] * (x.dim() - 3))
+    return x.gather(2, at.expand(x.shape[0], x.shape[1], 1, *x.shape[3:]))
+
+
 class _Last(NamedTuple):
     """What a layer's recurrences continue from: ``g, fgate`` ``(B, H, 1)`` and ``phi`` ``(B, H, d_state // 2)`` at the last
     position of every sequence."""
@@ -271,9 +279,9 @@ class SISAPagedCache:
 
     def last(self, layer_idx: int) -> _Last | None:
         """What the layer's recurrences continue from, or None before its first pass."""
-        layer = self._store.layers.get(layer_idx)
-        if layer is None or not any(layer.filled[self._lo:self._hi]):
+        if self.empty(layer_idx):
             return None
+        layer = self._store.layers[layer_idx]
         if not all(layer.filled[self._lo:self._hi]):
             raise ValueError("SISAPagedCache: some of these sequences are empty and some are not; fill the empty ones on "
                              "their own (cache[n])")
@@ -325,38 +333,44 @@ class SISAPagedCache:
         layer = st.layers[layer_idx] = _Layer(pool, last, weights, st.sequences)
         return layer
 
-    def extend(self, layer_idx: int, p, hip: bool) -> None:
-        """Write a pass's rows (``p``: :class:`sisa_amd.modeling.Prepared`) of one layer behind what its sequences hold."""
+    def begin(self, layer_idx: int, k: Tensor, b: Tensor, hip: bool) -> Tensor | None:
+        """Room in a layer for a pass of ``k.shape[2]`` positions of every sequence. Returns how many of them are real, a
+        tensor, or None where all are."""
         st, lo, hi = self._store, self._lo, self._hi
-        B, _, M, _ = p.k.shape
+        B, _, M, _ = k.shape
         if B != len(self):
             raise ValueError(f"SISAPagedCache: {B} rows for {len(self)} sequences")
-        if torch.is_grad_enabled() and (p.k.requires_grad or p.g.requires_grad):
-            raise RuntimeError("SISAPagedCache is for inference: run the model under torch.no_grad()")
-        st.device_state(p.k.device)
-        layer = self._layer(layer_idx, p.k, p.b, hip)
-        if (layer.pool.k.dtype, layer.pool.k.shape[1]) != (p.k.dtype, p.k.shape[1]):
+        st.device_state(k.device)
+        layer = self._layer(layer_idx, k, b, hip)
+        if (layer.pool.k.dtype, layer.pool.k.shape[1]) != (k.dtype, k.shape[1]):
             raise ValueError(f"SISAPagedCache: filled in {layer.pool.k.dtype} with {layer.pool.k.shape[1]} heads, got "
-                             f"{p.k.dtype} and {p.k.shape[1]}")
+                             f"{k.dtype} and {k.shape[1]}")
         self._begin(layer, M)
         padded = [n - m for n, m in zip(self.lengths, layer.filled[lo:hi])] != [M] * B
-        count = st.end[lo:hi] - st.start[lo:hi] if padded or not hip else None
-        rows = (p.k, p.v, p.b, p.g.float(), p.fgate.float())
+        return st.end[lo:hi] - st.start[lo:hi] if padded else None
+
+    def put(self, layer_idx: int, rows: Sequence[Tensor], phi: Tensor, count: Tensor | None, hip: bool) -> None:
+        """The rows ``k, v, b, g, fgate`` of a pass that :meth:`begin` made room for, and the phase ``(B, H, d_state // 2)``
+        at each sequence's last one."""
+        st, lo, hi = self._store, self._lo, self._hi
+        layer = st.layers[layer_idx]
         if hip:
             from .kernels.paged import sisa_paged_write_hip
 
             sisa_paged_write_hip(layer.pool, st.table[lo:hi], st.start[lo:hi], *rows, count)
         else:
-            _write(layer.pool, st.table[lo:hi], st.start[lo:hi], count, rows)
-        # what the next position continues from
-        for t, x in zip(layer.last, (rows[3], rows[4], p.phi)):
-            if padded:
-                at = (count.long() - 1).view(B, 1, 1, *[1] * (x.dim() - 3))
-                x = x.gather(2, at.expand(B, x.shape[1], 1, *x.shape[3:]))
-            else:
-                x = x[:, :, -1:]
-            t[lo:hi].copy_(x if x.dim() == 3 else x[:, :, 0])
+            _write(layer.pool, st.table[lo:hi], st.start[lo:hi], st.end[lo:hi] - st.start[lo:hi], rows)
+        for t, x in zip(layer.last, (rows[3], rows[4])):
+            t[lo:hi].copy_(at_last(x, count))
+        layer.last.phi[lo:hi].copy_(phi)
         layer.filled[lo:hi] = self.lengths
+
+    def extend(self, layer_idx: int, p, hip: bool) -> None:
+        """Write a pass's rows (``p``: :class:`sisa_amd.modeling.Prepared`) of one layer behind what its sequences hold."""
+        if torch.is_grad_enabled() and (p.k.requires_grad or p.g.requires_grad):
+            raise RuntimeError("SISAPagedCache is for inference: run the model under torch.no_grad()")
+        count = self.begin(layer_idx, p.k, p.b, hip)
+        self.put(layer_idx, (p.k, p.v, p.b, p.g.float(), p.fgate.float()), at_last(p.phi, count)[:, :, 0], count, hip)
 
     def attend(self, layer_idx: int, p, lam: Tensor, hip: bool) -> Tensor:
         """The attention of the rows that :meth:`extend` has just written, ``(B, H, M, d_head)`` float32 (float64 rows:
@@ -371,18 +385,23 @@ class SISAPagedCache:
                                          max_len=self.seq_len, weights=weights)
         return paged_attention(p.q, p.c, p.g, p.fgate, lam, layer.pool, st.table[lo:hi], st.end[lo:hi], self.seq_len, weights)
 
-    def receive(self, layer_idx: int, p, lam: Tensor, hip: bool) -> None:
+    def receive(self, layer_idx: int, q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor, fgate: Tensor,
+                hip: bool) -> None:
         """Track the weights of a first pass, in which the rows attended to each other."""
         st, lo, hi = self._store, self._lo, self._hi
-        L = p.k.shape[2]
         if hip:
             from .kernels.weights import sisa_attention_weights_hip
 
-            w = sisa_attention_weights_hip(p.q, p.k, p.c, p.b, p.g.float(), lam, p.fgate.float(), lengths=st.end[lo:hi])
+            w = sisa_attention_weights_hip(q, k, c, b, g.float(), lam, fgate.float(), lengths=st.end[lo:hi])
         else:
-            w = attention_weights(p.q, p.k, p.c, p.b, p.g, lam, p.fgate, st.end[lo:hi])
-        N = min(L, st.max_length)                          # a padded batch may be wider than the cache
+            w = attention_weights(q, k, c, b, g, lam, fgate, st.end[lo:hi])
+        N = min(k.shape[2], st.max_length)                 # a padded batch may be wider than the cache
         st.layers[layer_idx].weights[lo:hi, :, :N] = w[:, :, :N]
+
+    def empty(self, layer_idx: int) -> bool:
+        """Whether no sequence holds a position in this layer."""
+        layer = self._store.layers.get(layer_idx)
+        return layer is None or not any(layer.filled[self._lo:self._hi])
 
     def kernel_layer(self, layer_idx: int, like: Tensor, heads: int) -> bool:
         """Whether every sequence holds positions in this layer, in a pool of the HIP kernels for rows of ``like``'s dtype and
