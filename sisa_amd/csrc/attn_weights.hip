@@ -23,7 +23,6 @@ namespace {
 
 constexpr int DH = 64, DS = 32;
 constexpr int FEW_ROWS = 256;         // query rows up to which, against four times as many keys, each wave has its own keys
-constexpr int OWN = 64;               // queries (keys) that a wave holds: four blocks of 16
 constexpr float SCALE = LOG2E / 8;    // of q.k into log2 units
 
 struct Rows {                         // queries of a sequence: first .. first + count - 1
@@ -161,9 +160,10 @@ SISA_DEV float start_of(float m, float l) { return -(m + __log2f(l)) * (1.f / SC
 // First pass. A block whose maximum exceeds the running one by less than 2^GROW leaves it as it is.
 constexpr float GROW = 16.f;
 // With `parts`, a row's maximum and sum over the split's keys are left for the second pass to join.
-template <class T, bool FORGET, int NW>
+template <class T, bool FORGET, int U, int NW>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_kernel(sisa_attn_weights_args a, int R, int nsplit,
                                                                                      float* start, f32x2* parts) {
+    constexpr int OWN = 16 * U;
     __shared__ float sm[NW][OWN], sl[NW][OWN];
     __shared__ Buffer<T> bufs[NW];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -177,18 +177,18 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
     const float lam = a.lam[h * a.s_lam];
     Buffer<T>* buf = bufs + w;
     Stream<T> keys(a.k, a.b, a, b, h, nullptr, lane);
-    Frags<T> q[4];
+    Frags<T> q[U];
     {
         const Stream<T> own(a.q, a.c, a, b, h, nullptr, lane);
-        Raw<T> raw[4];
+        Raw<T> raw[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) raw[u] = own.load_edge(i0 + 16 * u, L);
+        for (int u = 0; u < U; ++u) raw[u] = own.load_edge(i0 + 16 * u, L);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) q[u] = turn<T, FORGET>(raw[u], buf, lane).x;
+        for (int u = 0; u < U; ++u) q[u] = turn<T, FORGET>(raw[u], buf, lane).x;
     }
-    float gi[4], fi[4], md[4], ld[4];
+    float gi[U], fi[U], md[U], ld[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
         gi[u] = gate(a.g, b, h, i0 + 16 * u + col, L);
         fi[u] = gate(a.f, b, h, i0 + 16 * u + col, L);
         md[u] = -__builtin_inff();
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
     for (int t = (below > t0 ? below : t0) + w; t < t1; t += NW) {   // meeting the diagonal
         const Tile<T> k = turn<T, FORGET>(keys.load_edge(16 * t, L), buf, lane);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < U; ++u) {
             if (16 * t > i0 + 16 * u + 15) continue;                 // all keys after all queries
             const f32x4 qk = mma(k.x.x1, q[u].x1, mma(k.x.x0, q[u].x0, zero4())), cb = mma(k.x.s, q[u].s, zero4());
             float x[4], mx = md[u];
@@ -225,9 +225,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
     if (below - 1 - w >= t0) {
         const float ga = gate(a.g, b, h, i0, L), fa = gate(a.f, b, h, i0, L);
         // y = 8 score - 8 (F_i - F_a); sums of 2^(y SCALE - ref), the maximum so far in mo
-        float qg[4], mo[4], ref[4], lo[4];
+        float qg[U], mo[U], ref[U], lo[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < U; ++u) {
             qg[u] = 8.f * lam * fast_exp2((gi[u] - ga) * LOG2E);
             mo[u] = -__builtin_inff();
             ref[u] = lo[u] = 0.f;
@@ -241,10 +241,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
                 kg[e] = fast_exp2((ga - k.g[e]) * LOG2E);
                 kf[e] = FORGET ? 8.f * (fa - k.f[e]) : 0.f;
             }
-            f32x4 y[4];
+            f32x4 y[U];
             float mx = -__builtin_inff();
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const f32x4 cb = mma(k.x.s, q[u].s, zero4());
                 y[u] = mma(k.x.x1, q[u].x1, mma(k.x.x0, q[u].x0, kf));
 #pragma unroll
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
                 asm volatile("");                                    // rarely: not to be worked out beforehand
                 fresh = false;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < U; ++u) {
                     const float to = fmaxf(mo[u], fmaxf(fmaxf(y[u][0], y[u][1]), fmaxf(y[u][2], y[u][3])) + ref[u]);
                     const float by = ref[u] - (to == -__builtin_inff() ? 0.f : to);
                     if (lo[u] != 0.f) lo[u] *= fast_exp2(by);
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
                 }
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) lo[u] += fast_exp2(y[u][e]);
         };
@@ -294,18 +294,18 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
             if (!yet) break;
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
             merge(md[u], ld[u], (mo[u] == -__builtin_inff() ? mo[u] : ref[u]) + (fi[u] - fa) * LOG2E, lo[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int o = 16; o < 64; o <<= 1) merge(md[u], ld[u], __shfl_xor(md[u], o), __shfl_xor(ld[u], o));
         if (grp == 0) sm[w][16 * u + col] = md[u], sl[w][16 * u + col] = ld[u];
     }
     __syncthreads();
     const int r = r0 + lane;
-    if (w != 0 || r >= rows.count) return;
+    if (w != 0 || lane >= OWN || r >= rows.count) return;
     float mt = sm[0][lane], lt = sl[0][lane];
 #pragma unroll
     for (int k = 1; k < NW; ++k) merge(mt, lt, sm[k][lane], sl[k][lane]);
@@ -317,10 +317,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
 // Second pass. SHARE of a workgroup's NW waves have the same 64 keys and take every SHARE-th query tile: all of them, or one
 // where so few queries are counted that the keys' loads weigh more (then the rows' parts from the first pass are joined here,
 // in the order of the splits, by every workgroup: at most 256 rows of 32 parts).
-template <class T, bool FORGET, int NW, int SHARE>
+template <class T, bool FORGET, int U, int NW, int SHARE>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_kernel(sisa_attn_weights_args a, int R, int nsplit,
                                                                                      const float* start, const f32x2* parts) {
     constexpr bool FEW = SHARE == 1;
+    constexpr int OWN = 16 * U;
     __shared__ float part[NW][OWN];
     __shared__ float starts[FEW ? FEW_ROWS : 4];
     __shared__ Buffer<T> bufs[NW];
@@ -332,6 +333,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
     const float lam = a.lam[h * a.s_lam];
     Buffer<T>* buf = bufs + w;
     const int Rp = (R + 15) / 16 * 16;
+    Raw<T> raw[U];                                                   // the keys, under way while the rows' parts are joined
+    {
+        const Stream<T> own(a.k, a.b, a, b, h, nullptr, lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = own.load_edge(j0 + 16 * u, L);
+    }
     if constexpr (FEW) {
         for (int r = threadIdx.x; r < rows.count; r += 64 * NW) {
             const f32x2* p = parts + ((int64_t)bh * Rp + r) * nsplit;
@@ -342,23 +349,17 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
         }
         __syncthreads();
     }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float sum[U] = {};
     // 16-query tiles of the window from the first that reaches j0: those that meet the diagonal, whole ones, the last one
     const int from = j0 > rows.first ? (j0 - rows.first) / 16 : 0, tiles = (rows.count + 15) / 16;
     if (j0 < rows.n && from < tiles) {
         Stream<T> queries(a.q, a.c, a, b, h, FEW ? nullptr : start + (int64_t)bh * Rp, lane);
-        Frags<T> k[4];
-        {
-            const Stream<T> own(a.k, a.b, a, b, h, nullptr, lane);
-            Raw<T> raw[4];
+        Frags<T> k[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) raw[u] = own.load_edge(j0 + 16 * u, L);
+        for (int u = 0; u < U; ++u) k[u] = turn<T, FORGET>(raw[u], buf, lane).x;
+        float gj[U], fj[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) k[u] = turn<T, FORGET>(raw[u], buf, lane).x;
-        }
-        float gj[4], fj[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < U; ++u) {
             gj[u] = gate(a.g, b, h, j0 + 16 * u + col, L);
             fj[u] = gate(a.f, b, h, j0 + 16 * u + col, L);
         }
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
             Tile<T> q = turn<T, FORGET>(queries.load_edge(i0, L, 16 * t), buf, lane);
             if constexpr (FEW) q.st = lds4f(starts + 16 * t + 4 * grp);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 if (j0 + 16 * u > i0 + 15) continue;                 // all keys after all queries
                 const f32x4 qk = mma(q.x.x1, k[u].x1, mma(q.x.x0, k[u].x0, zero4())), cb = mma(q.x.s, k[u].s, zero4());
 #pragma unroll
@@ -388,9 +389,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
         int left = w0 + ws < w1 ? (w1 - 1 - w0 - ws) / SHARE + 1 : 0;
         if (left > 0) {
             const float ga = gate(a.g, b, h, j0 + OWN - 1, L), fa = gate(a.f, b, h, j0 + OWN - 1, L);
-            float kg[4], kf[4];
+            float kg[U], kf[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < U; ++u) {
                 kg[u] = lam * LOG2E * fast_exp2((ga - gj[u]) * LOG2E);
                 kf[u] = (fa - fj[u]) * LOG2E;
             }
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
                     rc[e] = FORGET ? fmaf(q.f[e] - fa, 8.f, q.st[e]) : q.st[e];
                 }
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < U; ++u) {
                     const f32x4 qk = mma(q.x.x1, k[u].x1, mma(q.x.x0, k[u].x0, rc)), cb = mma(q.x.s, k[u].s, zero4());
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[u] += fast_exp2(fmaf(cb[e] * kg[u], rg[e], fmaf(qk[e], SCALE, kf[u])));
@@ -435,26 +436,26 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
         }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int o = 16; o < 64; o <<= 1) sum[u] += __shfl_xor(sum[u], o);
         if (grp == 0) part[w][16 * u + col] = sum[u];
     }
     __syncthreads();
     const int j = j0 + lane;
-    if (ws || j >= L) return;
+    if (ws || lane >= OWN || j >= L) return;
     float s = part[w][lane];
 #pragma unroll
     for (int k = 1; k < SHARE; ++k) s += part[w + k][lane];
     a.out[(int64_t)bh * L + j] = j < rows.n ? s : 0.f;
 }
 
-// How a call is laid out. A chip of 256 CUs that the 64-row blocks of the queries do not fill gets the keys of the first pass
-// in splits (where few rows are counted: the second pass joins them; of 256 keys at least, 32 at most), or workgroups of
-// twice the waves.
+// How a call is laid out. Waves hold 64 queries (keys), four share them. Where the 64-row blocks of the queries are fewer than
+// the chip's 256 CUs: 16 of them, eight waves to share; or, where few rows are counted against many keys, the keys of the first
+// pass in splits (of 256 keys at least, 32 at most), which the second joins, and there each wave its own keys.
 struct Plan {
-    int R, nsplit, waves;
-    bool few;
+    int R, nsplit;
+    bool few, small;
     int64_t Rp, bytes;
 };
 
@@ -463,8 +464,8 @@ Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
     p.R = window && window < L ? window : L;
     p.Rp = (p.R + 15) / 16 * 16;
     p.few = p.R <= FEW_ROWS && L / 4 >= p.R;
-    const int64_t BH = (int64_t)B * H, groups = BH * sisa::cdiv(p.R, OWN);
-    p.waves = groups < 256 ? 8 : 4;
+    const int64_t BH = (int64_t)B * H, groups = BH * sisa::cdiv(p.R, 64);
+    p.small = !p.few && groups < 256;
     p.nsplit = 1;
     if (p.few && groups < 256) {
         const int64_t want = 256 / groups, most = sisa::cdiv(L, 256);
@@ -475,26 +476,32 @@ Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
     return p;
 }
 
-template <class T, bool FORGET, int NW>
+// U blocks of 16 queries, NW waves in the first pass; keys likewise in the second, NW2 waves of which SHARE have the same.
+template <class T, bool FORGET, int U, int NW, int NW2, int SHARE>
 int launch_weights(const sisa_attn_weights_args* a, const Plan& p, hipStream_t st) {
     const int64_t BH = (int64_t)a->B * a->H;
     float* start = p.few ? nullptr : (float*)a->workspace;
     f32x2* parts = p.few ? (f32x2*)a->workspace : nullptr;
-    const unsigned grid = (unsigned)(BH * sisa::cdiv(p.R, OWN) * p.nsplit);
-    weights_lse_kernel<T, FORGET, NW><<<grid, 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    const unsigned rows = (unsigned)(BH * sisa::cdiv(p.R, 16 * U) * p.nsplit);
+    weights_lse_kernel<T, FORGET, U, NW><<<rows, 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     const int rc = sisa::launch_status("sisa_attn_weights (rows)");
     if (rc) return rc;
-    if (p.few)
-        weights_sum_kernel<T, FORGET, 4, 1><<<(unsigned)(BH * sisa::cdiv(a->L, OWN * 4)), 256, 0, st>>>(*a, p.R, p.nsplit, start, parts);
-    else weights_sum_kernel<T, FORGET, NW, NW><<<(unsigned)(BH * sisa::cdiv(a->L, OWN)), 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    const unsigned keys = (unsigned)(BH * sisa::cdiv(a->L, 16 * U * (NW2 / SHARE)));
+    weights_sum_kernel<T, FORGET, U, NW2, SHARE><<<keys, 64 * NW2, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     return sisa::launch_status("sisa_attn_weights");
+}
+
+template <class T, bool FORGET>
+int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
+    const Plan p = plan_of(a->B, a->H, a->L, a->window);
+    if (p.few) return launch_weights<T, FORGET, 4, 8, 4, 1>(a, p, st);
+    if (p.small) return launch_weights<T, FORGET, 1, 8, 8, 8>(a, p, st);
+    return launch_weights<T, FORGET, 4, 4, 4, 4>(a, p, st);
 }
 
 template <class T>
 int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
-    const Plan p = plan_of(a->B, a->H, a->L, a->window);
-    if (p.waves == 8) return a->f.ptr ? launch_weights<T, true, 8>(a, p, st) : launch_weights<T, false, 8>(a, p, st);
-    return a->f.ptr ? launch_weights<T, true, 4>(a, p, st) : launch_weights<T, false, 4>(a, p, st);
+    return a->f.ptr ? launch_weights<T, true>(a, st) : launch_weights<T, false>(a, st);
 }
 
 }  // namespace
