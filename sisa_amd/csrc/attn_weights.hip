@@ -476,8 +476,8 @@ Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
     return p;
 }
 
-// U blocks of 16 queries, NW waves in the first pass; keys likewise in the second, NW2 waves of which SHARE have the same.
-template <class T, bool FORGET, int U, int NW, int NW2, int SHARE>
+// U blocks of 16 queries, NW waves in the first pass; U2 of keys, NW2 waves of which SHARE have the same in the second.
+template <class T, bool FORGET, int U, int NW, int U2, int NW2, int SHARE>
 int launch_weights(const sisa_attn_weights_args* a, const Plan& p, hipStream_t st) {
     const int64_t BH = (int64_t)a->B * a->H;
     float* start = p.few ? nullptr : (float*)a->workspace;
@@ -486,17 +486,17 @@ int launch_weights(const sisa_attn_weights_args* a, const Plan& p, hipStream_t s
     weights_lse_kernel<T, FORGET, U, NW><<<rows, 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     const int rc = sisa::launch_status("sisa_attn_weights (rows)");
     if (rc) return rc;
-    const unsigned keys = (unsigned)(BH * sisa::cdiv(a->L, 16 * U * (NW2 / SHARE)));
-    weights_sum_kernel<T, FORGET, U, NW2, SHARE><<<keys, 64 * NW2, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    const unsigned keys = (unsigned)(BH * sisa::cdiv(a->L, 16 * U2 * (NW2 / SHARE)));
+    weights_sum_kernel<T, FORGET, U2, NW2, SHARE><<<keys, 64 * NW2, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     return sisa::launch_status("sisa_attn_weights");
 }
 
 template <class T, bool FORGET>
 int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
     const Plan p = plan_of(a->B, a->H, a->L, a->window);
-    if (p.few) return launch_weights<T, FORGET, 4, 8, 4, 1>(a, p, st);
-    if (p.small) return launch_weights<T, FORGET, 1, 8, 8, 8>(a, p, st);
-    return launch_weights<T, FORGET, 4, 4, 4, 4>(a, p, st);
+    if (p.few) return launch_weights<T, FORGET, 4, 8, 4, 4, 1>(a, p, st);
+    if (p.small) return launch_weights<T, FORGET, 1, 8, 1, 8, 8>(a, p, st);
+    return launch_weights<T, FORGET, 4, 4, 4, 4, 4>(a, p, st);
 }
 
 template <class T>

@@ -215,7 +215,7 @@ def sisa_paged_decode_hip(q: Tensor, c: Tensor, g_q: Tensor, f_q: Tensor | None,
     else:
         w_in = _weights_view(name, "weights", weights, B, H, max_len, pool)
         w_out = w_in if weights_out is None else _weights_view(name, "weights_out", weights_out, B, H, max_len, pool)
-        if 0 in w_out[1:]:
+        if any(step == 0 and size > 1 for step, size in zip(w_out[1:], (B, H, max_len))):
             raise ValueError(f"{name}: the weights that are written must not be an expanded tensor")
     size = _lib.load().sisa_paged_decode_workspace_bytes(B, H, M, max_len, _lib.dtype_code(pool.dtype), weights is not None)
     ws = lam.new_empty((size // 4,)) if size else None

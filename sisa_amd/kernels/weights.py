@@ -59,7 +59,7 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     if not out.numel():
         return out
     (q, *vq), (k, *vk), (c, *vc), (b, *vb) = (row_view(_near(t, MAX_STRIDE)) for t in (q, k, c, b))
-    g, fgate = _near(g, 2), None if fgate is None else _near(fgate, 2)
+    g, fgate = (t if t is None or t.stride(2) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (g, fgate))
     window = 0 if window is None or window >= L else window
     ws = lam.new_empty((_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window) // 4,))
     _weights(q, B, H, L, window, _lib.dtype_code(q.dtype), 0, *vq, *vk, *vc, *vb, g.data_ptr(), *g.stride(),

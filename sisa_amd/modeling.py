@@ -608,8 +608,10 @@ class SISAForCausalLM(SISAModel):
                                  f"shape")
             if logits_to_keep or logits_at is not None:
                 raise ValueError("logits_to_keep and logits_at are for generation; they cannot be combined with labels")
-        if logits_at is not None and (logits_to_keep or len(logits_at) != input_ids.shape[0]):
-            raise ValueError("logits_at is one position for each row, in place of logits_to_keep")
+        if logits_at is not None and (logits_to_keep or len(logits_at) != input_ids.shape[0]
+                                      or not all(0 <= i < input_ids.shape[1] for i in logits_at)):
+            raise ValueError(f"logits_at is one of the positions 0 .. {input_ids.shape[1] - 1} for each row, in place of "
+                             f"logits_to_keep; got {list(logits_at)}")
         hidden = SISAModel.forward(self, input_ids, cache=cache)
         head = self.embed.weight
         if labels is None:

@@ -179,6 +179,8 @@ class _Store:
             width = -(-self.max_length // self.page_size)
             self.table = torch.full((self.sequences, width), -1, dtype=torch.int32, device=device)
             self.start, self.end = (torch.zeros(self.sequences, dtype=torch.int32, device=device) for _ in range(2))
+            if any(self.held):                             # reserved before the first pass
+                self.show(range(self.sequences))
         elif self.table.device != device:
             raise ValueError(f"SISAPagedCache: filled on {self.table.device}, used on {device}")
 
@@ -345,6 +347,9 @@ class SISAPagedCache:
         if (layer.pool.k.dtype, layer.pool.k.shape[1]) != (k.dtype, k.shape[1]):
             raise ValueError(f"SISAPagedCache: filled in {layer.pool.k.dtype} with {layer.pool.k.shape[1]} heads, got "
                              f"{k.dtype} and {k.shape[1]}")
+        if isinstance(layer.pool, _Pages) == hip:
+            raise ValueError(f"SISAPagedCache: filled by the {'torch' if hip else 'HIP'} implementation, which cannot be changed "
+                             f"while sequences are held; make a new cache")
         self._begin(layer, M)
         padded = [n - m for n, m in zip(self.lengths, layer.filled[lo:hi])] != [M] * B
         return st.end[lo:hi] - st.start[lo:hi] if padded else None

@@ -210,6 +210,51 @@ def test_decode_marks_lengths_and_pages_outside_the_pool():
     assert out[1:].isnan().all() and w[1:3, :, :300].isnan().all() and w[3:].eq(0).all() and w[1:3, :, 300:].eq(0).all()
 
 
+def test_refusals_on_the_gpu():
+    """What the calls can see from the host: shapes, dtypes, devices, gradients, expanded outputs."""
+    from sisa_amd.kernels.paged import PagePool, sisa_cache_evict_hip, sisa_paged_decode_hip, sisa_paged_write_hip
+    cache = Cache([20, 30], 2, 16, torch.float16, seed=1)
+    q, c, g, f = cache.queries()
+    n, lam, pool, table = _ints(20, 30), cache.lam, cache.pool, cache.table
+    wide = torch.zeros(2, 2, 32, device=DEV)
+    for bad, kind in ((dict(q=q.float()), ValueError), (dict(q=q[:, :1]), ValueError), (dict(q=q[..., :32]), ValueError),
+                      (dict(f=None), ValueError), (dict(lam=lam[:1]), ValueError), (dict(lam=lam.double()), ValueError),
+                      (dict(g=g.double()), ValueError), (dict(table=table.long()), ValueError), (dict(table=table[0]), ValueError),
+                      (dict(n=n[:1]), ValueError), (dict(n=n.cpu()), ValueError), (dict(max_len=0), ValueError),
+                      (dict(max_len=33), ValueError), (dict(weights=wide[:, :, :20]), ValueError),
+                      (dict(weights=wide.double()), ValueError), (dict(weights_out=wide), ValueError),
+                      (dict(weights=wide, weights_out=wide[:, :1].expand(2, 2, 32)), ValueError),
+                      (dict(table=table[:, :0]), ValueError), (dict(q=q.clone().requires_grad_(True)), RuntimeError)):
+        a = dict(q=q, c=c, g=g, f=f, lam=lam, pool=pool, table=table, n=n) | bad
+        args = [a.pop(x) for x in ("q", "c", "g", "f", "lam", "pool", "table", "n")]
+        with pytest.raises(kind):
+            sisa_paged_decode_hip(*args, **a)
+    one = wide[:1, :1].expand(1, 1, 32)                         # expanded along axes of one: written like any other
+    single = Cache([20], 1, 16, torch.float16, seed=2)
+    sisa_paged_decode_hip(*single.queries(), single.lam, single.pool, single.table, _ints(20), max_len=32, weights=one)
+    row = cache.rows
+    for bad in (dict(k=row["k"].float()), dict(v=row["v"][:, :1]), dict(b=row["k"]), dict(g=row["g"][:, :, :3]), dict(f=None),
+                dict(start=n.long()), dict(count=n[:1]), dict(table=table[:1])):
+        a = dict(pool=pool, table=table, start=_ints(0, 0), k=row["k"], v=row["v"], b=row["b"], g=row["g"], f=row["f"],
+                 count=None) | bad
+        with pytest.raises(ValueError):
+            sisa_paged_write_hip(*a.values())
+    other = PagePool.empty(4, 3, 16, torch.float16, DEV)
+    for bad in (dict(recent=0), dict(recent=9), dict(new=other), dict(w=wide[:, :, :31]), dict(max_len=33),
+                dict(new_table=table[:1]), dict(new_table=table[:, :0]), dict(w=wide.clone().requires_grad_(True))):
+        a = dict(pool=pool, table=table, n=n, w=wide, keep=8, recent=2, new=pool, new_table=table) | bad
+        args = [a.pop(x) for x in ("pool", "table", "n", "w", "keep", "recent", "new", "new_table")]
+        with pytest.raises((ValueError, RuntimeError)):
+            sisa_cache_evict_hip(*args, **a)
+    # nothing to do
+    none = sisa_paged_decode_hip(q[:0], c[:0], g[:0], f[:0], lam, pool, table[:0], n[:0])
+    assert none.shape == (0, 2, 1, 64)
+    assert sisa_paged_decode_hip(q[:, :, :0], c[:, :, :0], g[:, :, :0], f[:, :, :0], lam, pool, table, n).shape == (2, 2, 0, 64)
+    sisa_paged_write_hip(pool, table[:0], n[:0], *(row[x][:0] for x in ("k", "v", "b", "g", "f")))
+    got = sisa_cache_evict_hip(pool, table[:0], n[:0], wide[:0], 8, 2, pool, table[:0])
+    assert got.lengths.shape == (0,) and got.weights.shape == got.positions.shape == (0, 2, 8)
+
+
 def test_decode_beyond_32_bit_offsets():
     """Pages whose rows start past 2^31 elements, and 2^32 bytes, of their tensor."""
     from sisa_amd.kernels.paged import PagePool, sisa_cache_evict_hip, sisa_paged_decode_hip, sisa_paged_write_hip
@@ -444,6 +489,22 @@ def test_received_weights_with_steep_gates():
         got = sisa_attention_weights_hip(*x, g, lam, f)
         # |F| reaches 16,000 here: a difference of two is exact to 2^-24 of the larger in both, the inputs being the same
         assert _rel(got, _weights64(*x, g, lam, f, [L], None)) <= TOL
+
+
+def test_received_weights_of_other_layouts():
+    """Positions far apart in memory, gates that are not neighbours, expanded ones, rows that begin off 16 bytes: copied."""
+    from sisa_amd.kernels.weights import sisa_attention_weights_hip
+    gen, B, H, L = _gen(17), 2, 3, 70
+    x = [torch.randn(B, H, L, w, generator=gen, device=DEV).to(torch.float16) for w in (64, 64, 32, 32)]
+    g, f = _gates(gen, B, H, L), _gates(gen, B, L, H).transpose(1, 2)
+    lam = torch.rand(1, device=DEV).expand(H)
+    off = torch.zeros(B, H, L, 65, device=DEV, dtype=torch.float16)
+    off[..., 1:] = x[1]
+    got = sisa_attention_weights_hip(x[0].transpose(0, 2).contiguous().transpose(0, 2), off[..., 1:], x[2], x[3], g, lam, f)
+    assert torch.equal(got, sisa_attention_weights_hip(*x, g, lam.contiguous(), f.contiguous()))
+    flat = torch.zeros(B, H, 1, device=DEV)                     # no decay, no forgetting: one value for every position
+    got = sisa_attention_weights_hip(*x, flat.expand(B, H, L), lam, flat.expand(B, H, L))
+    assert _rel(got, _weights64(*x, flat.expand(B, H, L), lam, None, [L] * B, None)) <= TOL
 
 
 def test_received_weights_of_values_that_are_not_finite():

@@ -101,6 +101,10 @@ def test_parts_release_and_reuse():
         with pytest.raises(RuntimeError, match="more pages"):
             model(ids[:1, 20:49], cache=cache[0:1])         # 49 positions: two pages more
         assert cache.lengths == [20, 0, 22]
+    early = SISAPagedCache(2, 50, page_size=16)             # reserved before there is a device to show the table on
+    early.reserve(50)
+    assert early.free_pages == 0
+    assert rel_err(_logits(model, ids[:2], early, 20), torch.cat(want[:2])) <= GATES
     assert len(cache) == 3 and len(cache[1:]) == 2
     for bad in (slice(2, 1), slice(0, 3, 2)):
         with pytest.raises(ValueError):
@@ -213,8 +217,9 @@ def test_refusals():
         for keep, recent in ((4, 0), (4, 5), (0, 0)):
             with pytest.raises(ValueError, match="recent"):
                 tracked.evict(keep, recent)
-        with pytest.raises(ValueError, match="logits_at"):
-            model(ids, logits_at=[1])
+        for at in ([1], [1, 20], [-1, 0]):
+            with pytest.raises(ValueError, match="logits_at"):
+                model(ids, logits_at=at)
         with pytest.raises(ValueError, match="labels"):
             model(ids, labels=ids, logits_at=[1, 1])
 
@@ -404,4 +409,10 @@ def test_calls_that_keep_the_module_path_with_pages(monkeypatch):
     assert steps_of(model, ctx=lambda: torch.autocast("cuda", dtype=torch.bfloat16)) == 0
     model.set_attn_impl("hip")
     assert steps_of(model) == 0
+    ids, cache = token_ids(2, 9).to(DEV), SISAPagedCache(2, 20)
+    with torch.no_grad():
+        model(ids[:, :8], cache=cache)
+        model.set_attn_impl("torch")
+        with pytest.raises(ValueError, match="HIP implementation"):
+            model(ids[:, 8:], cache=cache)
     assert steps_of(tiny_model(seed=1, attn_impl="auto").to(DEV).eval()) == 0
