@@ -17,9 +17,16 @@ MAX_STRIDE = 1 << 24           # SISA_ATTN_WEIGHTS_MAX_STRIDE
 _weights = _lib.Packed("sisa_attn_weights", _lib.AttnWeightsArgs)
 
 
-def _near(t: Tensor, stride: int) -> Tensor:
-    """``t``, or a copy where its positions (axis 2) are ``stride`` elements or more apart."""
-    return t if t.stride(2) < stride else t.clone(memory_format=torch.contiguous_format)
+def _rows(t: Tensor) -> tuple:
+    """:func:`row_view`, of a copy also where positions are MAX_STRIDE elements or more apart."""
+    return row_view(t if t.stride(2) < MAX_STRIDE else t.clone(memory_format=torch.contiguous_format))
+
+
+def _gates(t: Tensor) -> tuple:
+    """``t`` ``(B, H, L)``, its address and strides; of a copy where its positions are not neighbours."""
+    if t.stride(2) != 1:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), *t.stride()
 
 
 def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor,
@@ -34,7 +41,8 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     two); what lies behind is not looked at and receives 0. Returns ``(B, H, L)`` float32. The scores are formed twice and
     never stored."""
     name = "sisa_attention_weights_hip"
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, c, b, g, lam, fgate)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or c.requires_grad or b.requires_grad or g.requires_grad
+                                    or lam.requires_grad or (fgate is not None and fgate.requires_grad)):
         inference_only(name)
     if q.dim() != 4 or q.shape[-1] != HIP_D_HEAD or k.shape != q.shape:
         raise ValueError(f"{name}: q and k must be (B, H, L, {HIP_D_HEAD}), got {tuple(q.shape)} and {tuple(k.shape)}")
@@ -49,7 +57,8 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
                                                                          and fgate.dtype is not torch.float32):
         raise TypeError(f"{name}: g, fgate and lam must be float32")
     device = _lib.device_index(q)
-    if any(t is not None and t.get_device() != device for t in (k, c, b, g, lam, fgate)):
+    if k.get_device() != device or c.get_device() != device or b.get_device() != device or g.get_device() != device \
+            or lam.get_device() != device or (fgate is not None and fgate.get_device() != device):
         raise ValueError(f"{name}: the tensors are on different devices")
     if window is not None and window < 1:
         raise ValueError(f"{name}: window = {window} must be positive or None")
@@ -58,11 +67,14 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     out = lam.new_empty((B, H, L))
     if not out.numel():
         return out
-    (q, *vq), (k, *vk), (c, *vc), (b, *vb) = (row_view(_near(t, MAX_STRIDE)) for t in (q, k, c, b))
-    g, fgate = (t if t is None or t.stride(2) == 1 else t.clone(memory_format=torch.contiguous_format) for t in (g, fgate))
+    q, *vq = _rows(q)
+    k, *vk = _rows(k)
+    c, *vc = _rows(c)
+    b, *vb = _rows(b)
+    g, *vg = _gates(g)
+    fgate, *vf = (None, *_NO_VIEW) if fgate is None else _gates(fgate)
     window = 0 if window is None or window >= L else window
     ws = lam.new_empty((_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window) // 4,))
-    _weights(q, B, H, L, window, _lib.dtype_code(q.dtype), 0, *vq, *vk, *vc, *vb, g.data_ptr(), *g.stride(),
-             *(_NO_VIEW if fgate is None else (fgate.data_ptr(), *fgate.stride())), lam.data_ptr(), lam.stride(0),
+    _weights(q, B, H, L, window, _lib.dtype_code(q.dtype), 0, *vq, *vk, *vc, *vb, *vg, *vf, lam.data_ptr(), lam.stride(0),
              0 if lengths is None else lengths.data_ptr(), out.data_ptr(), ws.data_ptr())
     return out
