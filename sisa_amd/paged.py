@@ -184,16 +184,17 @@ class _Store:
         elif self.table.device != device:
             raise ValueError(f"SISAPagedCache: filled on {self.table.device}, used on {device}")
 
-    def take(self, sequence: int, positions: int) -> list[int]:
-        """Pages so that ``sequence`` has room for ``positions``; the new ones."""
-        need = -(-positions // self.page_size) - len(self.held[sequence])
-        if need > len(self.free):
-            raise RuntimeError(f"SISAPagedCache: {need} more pages of {self.page_size} positions are needed, "
+    def take(self, lo: int, ends: Sequence[int]) -> list[int]:
+        """Pages so that the sequences from ``lo`` on have room for ``ends`` positions, all of them or, where there are too few
+        pages, none; the sequences that got any."""
+        need = [max(0, -(-end // self.page_size) - len(held)) for end, held in zip(ends, self.held[lo:])]
+        if sum(need) > len(self.free):
+            raise RuntimeError(f"SISAPagedCache: {sum(need)} more pages of {self.page_size} positions are needed, "
                                f"{len(self.free)} of {self.pages} are free (evict, release a sequence, or make the pool "
                                f"larger)")
-        new = [self.free.pop() for _ in range(max(0, need))]
-        self.held[sequence] += new
-        return new
+        for n, pages in enumerate(need, lo):
+            self.held[n] += [self.free.pop() for _ in range(pages)]
+        return [n for n, pages in enumerate(need, lo) if pages]
 
     def show(self, sequences: Sequence[int]) -> None:
         """The device's table of these sequences, from the host's."""
@@ -302,7 +303,7 @@ class SISAPagedCache:
         ends = [n + c for n, c in zip(self.lengths, counts)]
         if max(ends) > st.max_length:
             raise ValueError(f"SISAPagedCache: {max(ends)} positions exceed max_length = {st.max_length}")
-        fresh = [n for n, end in zip(range(lo, hi), ends) if st.take(n, end)]
+        fresh = st.take(lo, ends)
         if fresh:
             st.show(fresh if len(fresh) == 1 else range(lo, hi))
         st.start[lo:hi].copy_(st.end[lo:hi])
@@ -433,8 +434,7 @@ class SISAPagedCache:
         """Take the pages that ``positions`` more positions of every sequence need now, not as they come."""
         st = self._store
         ends = [min(n + positions, st.max_length) for n in self.lengths]
-        taken = [n for n, end in zip(range(self._lo, self._hi), ends) if st.take(n, end)]
-        if taken and st.table is not None:
+        if st.take(self._lo, ends) and st.table is not None:
             st.show(range(self._lo, self._hi))
 
     def release(self) -> None:

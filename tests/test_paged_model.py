@@ -113,6 +113,22 @@ def test_parts_release_and_reuse():
         cache[3]
 
 
+def test_a_pass_without_enough_pages_takes_none():
+    model = _model64()
+    ids = token_ids(2, 17, seed=4)
+    want = _logits(model, ids, SISACache(), 16)
+    cache = SISAPagedCache(2, 40, pages=3, page_size=16)
+    with torch.no_grad():
+        model(ids[:, :16], cache=cache)
+        for more in (lambda: model(ids[:, 16:], cache=cache), lambda: cache.reserve(1)):
+            with pytest.raises(RuntimeError, match="2 more pages"):
+                more()
+            assert cache.free_pages == 1 and cache.lengths == [16, 16]
+        cache[1].release()
+        assert rel_err(model(ids[:1, 16:], cache=cache[0]).logits, want[:1, 16:]) <= GATES
+        assert cache.lengths == [17, 0] and cache.free_pages == 1
+
+
 def _dense(model, x, layer, kept):
     """Attention of the last row of ``x`` (1, n, d), the layer's normalised input, over the rows ``kept[h]``."""
     at = model.layers[layer].attn
