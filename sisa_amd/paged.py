@@ -171,6 +171,7 @@ class _Store:
         self.free = list(range(pages - 1, -1, -1))
         self.held: list[list[int]] = [[] for _ in range(sequences)]
         self.starts, self.lengths = [0] * sequences, [0] * sequences   # before and after the last forward pass
+        self.expected: list[int | None] = [None] * sequences           # real positions of the next pass, if not all
         self.layers: dict[int, _Layer] = {}
         self.table = self.start = self.end = None          # on the model's device, made by the first pass
 
@@ -223,7 +224,6 @@ class SISAPagedCache:
             raise ValueError(f"SISAPagedCache: pages = {pages} must be positive")
         self._store = _Store(sequences, max_length, sequences * each if pages is None else pages, page_size, track)
         self._lo, self._hi = 0, sequences
-        self._expected: list[int] | None = None
 
     # -------------------------------------------------------------------------------------------- parts
     def __getitem__(self, which: int | slice) -> "SISAPagedCache":
@@ -238,7 +238,7 @@ class SISAPagedCache:
             lo = which % n
             hi = lo + 1
         part = object.__new__(SISAPagedCache)
-        part._store, part._lo, part._hi, part._expected = self._store, self._lo + lo, self._lo + hi, None
+        part._store, part._lo, part._hi = self._store, self._lo + lo, self._lo + hi
         return part
 
     def __len__(self) -> int:
@@ -278,7 +278,7 @@ class SISAPagedCache:
             raise ValueError(f"SISAPagedCache.expect: {counts}: a positive count for each of the {len(self)} sequences")
         if any(self.lengths):
             raise ValueError("SISAPagedCache.expect: only the first pass of a sequence may be padded")
-        self._expected = counts
+        self._store.expected[self._lo:self._hi] = counts
 
     def last(self, layer_idx: int) -> _Last | None:
         """What the layer's recurrences continue from, or None before its first pass."""
@@ -297,7 +297,7 @@ class SISAPagedCache:
             if layer.filled[lo:hi] != st.starts[lo:hi]:
                 raise RuntimeError("SISAPagedCache: an earlier forward pass did not reach every layer; release() the sequences")
             return
-        counts = self._expected or [M] * len(self)
+        counts = [M if c is None else c for c in st.expected[lo:hi]]
         if max(counts) > M:
             raise ValueError(f"SISAPagedCache: {max(counts)} positions were expected, the pass has {M}")
         ends = [n + c for n, c in zip(self.lengths, counts)]
@@ -307,12 +307,12 @@ class SISAPagedCache:
         if fresh:
             st.show(fresh if len(fresh) == 1 else range(lo, hi))
         st.start[lo:hi].copy_(st.end[lo:hi])
-        if self._expected is None:
+        if counts == [M] * len(self):
             st.end[lo:hi].add_(M)
         else:
             st.end[lo:hi].copy_(torch.tensor(ends, dtype=torch.int32))
         st.starts[lo:hi], st.lengths[lo:hi] = self.lengths, ends
-        self._expected = None
+        st.expected[lo:hi] = [None] * len(self)
 
     def _layer(self, layer_idx: int, k: Tensor, b: Tensor, hip: bool) -> _Layer:
         st = self._store
@@ -451,7 +451,7 @@ class SISAPagedCache:
         if st.table is not None:
             st.table[lo:hi].fill_(-1)
             st.end[lo:hi].zero_()
-        self._expected = None
+        st.expected[lo:hi] = [None] * len(self)
 
     def evict(self, keep: int, recent: int) -> None:
         """Cut every sequence down to ``keep`` positions per layer and head: its last ``recent`` ones and, of the others,

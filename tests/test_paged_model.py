@@ -129,6 +129,24 @@ def test_a_pass_without_enough_pages_takes_none():
         assert cache.lengths == [17, 0] and cache.free_pages == 1
 
 
+def test_what_is_expected_belongs_to_the_sequences():
+    model = _model64()
+    ids = token_ids(3, 20, seed=5)
+    want = [_logits(model, ids[i:i + 1, :n], SISACache(), n) for i, n in enumerate((7, 20, 12))]
+    cache = SISAPagedCache(3, 40, page_size=16)
+    with torch.no_grad():
+        cache[0].expect([7])                                # another handle of the sequence than the pass is given
+        assert rel_err(model(ids[:1], cache=cache[0]).logits[:, :7], want[0]) <= GATES and cache.lengths == [7, 0, 0]
+        cache[1:].expect([20, 12])
+        got = [model(ids[i:i + 1], cache=cache[i]).logits for i in (1, 2)]
+        assert all(rel_err(y[:, :w.shape[1]], w) <= GATES for y, w in zip(got, want[1:])) and cache.lengths == [7, 20, 12]
+        cache[2].release()
+        cache[2].expect([5])
+        cache.release()
+        model(ids, cache=cache)
+        assert cache.lengths == [20] * 3
+
+
 def _dense(model, x, layer, kept):
     """Attention of the last row of ``x`` (1, n, d), the layer's normalised input, over the rows ``kept[h]``."""
     at = model.layers[layer].attn
