@@ -4,10 +4,10 @@
  * by them. Conventions (views, status codes, streams, caller-owned buffers) are those of sisa_hip.h.
  *
  * A pool holds `pages` pages of `page_size` positions for every head. Position j of sequence n lives in slot
- * j % page_size of page table[n * s_table + j / page_size]; each sequence has W entries, and those behind its last
- * position are not read. Lengths, tables and counts are device memory that the host does not see: where one of them names
- * a place outside the pool, no memory outside it is touched, and the call answers as its declaration says. The tables of
- * two sequences may name the same page for reading (a shared prefix), not for writing.
+ * j % page_size of page table[n * s_table + j / page_size]; each sequence has W entries, and what those behind its last
+ * position hold does not matter. Lengths, tables and counts are device memory that the host does not see: where one of them
+ * names a place outside the pool, no memory outside it is touched, and the call answers as its declaration says. The tables
+ * of two sequences may name the same page for reading (a shared prefix), not for writing.
  *
  * No counterpart in the reference, whose cache is one tensor per layer that grows (src/sisa/generation.py:34-100).
  */

@@ -482,12 +482,13 @@ int launch_weights(const sisa_attn_weights_args* a, const Plan& p, hipStream_t s
     const int64_t BH = (int64_t)a->B * a->H;
     float* start = p.few ? nullptr : (float*)a->workspace;
     f32x2* parts = p.few ? (f32x2*)a->workspace : nullptr;
-    const unsigned rows = (unsigned)(BH * sisa::cdiv(p.R, 16 * U) * p.nsplit);
-    weights_lse_kernel<T, FORGET, U, NW><<<rows, 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    const int64_t rows = BH * sisa::cdiv(p.R, 16 * U) * p.nsplit, keys = BH * sisa::cdiv(a->L, 16 * U2 * (NW2 / SHARE));
+    SISA_REQUIRE(rows <= sisa::MAX_THREADS / (64 * NW) && keys <= sisa::MAX_THREADS / (64 * NW2),
+                 "sisa_attn_weights: B*H*L too large for one launch");
+    weights_lse_kernel<T, FORGET, U, NW><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     const int rc = sisa::launch_status("sisa_attn_weights (rows)");
     if (rc) return rc;
-    const unsigned keys = (unsigned)(BH * sisa::cdiv(a->L, 16 * U2 * (NW2 / SHARE)));
-    weights_sum_kernel<T, FORGET, U2, NW2, SHARE><<<keys, 64 * NW2, 0, st>>>(*a, p.R, p.nsplit, start, parts);
+    weights_sum_kernel<T, FORGET, U2, NW2, SHARE><<<(unsigned)keys, 64 * NW2, 0, st>>>(*a, p.R, p.nsplit, start, parts);
     return sisa::launch_status("sisa_attn_weights");
 }
 
@@ -528,8 +529,6 @@ extern "C" int sisa_attn_weights(const sisa_attn_weights_args* a, void* stream) 
     SISA_REQUIRE(a->g.ptr && a->lam && a->out && a->workspace && ((uintptr_t)a->workspace & 15) == 0,
                  "sisa_attn_weights: null pointer, or workspace not 16-byte aligned");
     SISA_REQUIRE(a->g.sl == 1 && (!a->f.ptr || a->f.sl == 1), "sisa_attn_weights: g and f must be contiguous along positions");
-    const int64_t BH = (int64_t)a->B * a->H;
-    SISA_REQUIRE(BH * sisa::cdiv(a->L, 64) < ((int64_t)1 << 26), "sisa_attn_weights: B*H*L too large for one launch");
     hipStream_t st = (hipStream_t)stream;
     switch (a->dtype) {
         case SISA_BF16: return launch_weights<__bf16>(a, st);

@@ -210,7 +210,8 @@ extern "C" int sisa_cache_evict(const sisa_cache_evict_args* a, void* stream) {
     SISA_REQUIRE(a->table && a->new_table && a->lengths && a->weights.ptr && a->new_lengths && a->new_weights && a->positions,
                  "sisa_cache_evict: null pointer");
     const int64_t heads = (int64_t)a->B * a->from.heads, rows = heads * a->keep;
-    SISA_REQUIRE(rows < ((int64_t)1 << 31), "sisa_cache_evict: B*H*keep must be below 2^31");
+    SISA_REQUIRE(rows < ((int64_t)1 << 31) && heads <= sisa::MAX_THREADS / (64 * SW),
+                 "sisa_cache_evict: B*H*keep must be below 2^31, B*H below 2^22");
     const int shift = sisa::log2_of(a->from.page_size), new_shift = sisa::log2_of(a->to.page_size);
     hipStream_t st = (hipStream_t)stream;
     const int64_t per = sisa::cdiv(a->max_len, 64 * SW);       // keys a thread

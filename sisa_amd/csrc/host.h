@@ -40,6 +40,9 @@ inline int launch_status(const char* what) {
     return SISA_OK;
 }
 
+// Threads of a launch: the dispatcher counts them in 32 bits.
+constexpr int64_t MAX_THREADS = ((int64_t)1 << 32) - 1;
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace sisa

@@ -299,6 +299,12 @@ bool takes_whole(int M, int64_t max_len, int elem, bool tracked) {
     return max_len <= TILE * (elem == 2 ? whole_waves<__bf16>() : whole_waves<float>()) && (!tracked || M == 1);
 }
 
+bool fits(int64_t rows, int M, int64_t max_len, int elem, bool tracked) {
+    const int64_t threads = takes_whole(M, max_len, elem, tracked) ? 64 * (elem == 2 ? whole_waves<__bf16>() : whole_waves<float>())
+                                                                   : sisa::cdiv(max_len, KCH) * KCH;
+    return rows <= sisa::MAX_THREADS / threads;
+}
+
 struct DecodeSpace {
     f32x2* stat;
     float *part, *scores;
@@ -403,7 +409,8 @@ extern "C" int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream) 
     SISA_REQUIRE((a->w_in.ptr == nullptr) == (a->w_out.ptr == nullptr),
                  "sisa_paged_decode: w_in and w_out must be given together");
     const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
-    SISA_REQUIRE(rows * sisa::cdiv(a->max_len, KCH) < ((int64_t)1 << 31), "sisa_paged_decode: too many rows for one launch");
+    SISA_REQUIRE(fits(rows, a->M, a->max_len, sisa::elem_size(a->pool.dtype), a->w_out.ptr != nullptr),
+                 "sisa_paged_decode: B*H*M*max_len too large for one launch");
     hipStream_t st = (hipStream_t)stream;
     switch (a->pool.dtype) {
         case SISA_BF16: return launch_decode<__bf16>(a, a->out, st);

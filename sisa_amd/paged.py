@@ -27,6 +27,10 @@ from .functional import autocast_disabled, working_dtype
 __all__ = ["SISAPagedCache", "attention_weights", "paged_attention"]
 
 
+#: Scores of a call of the attention kernel over pages that several new positions take: about 5 bytes of workspace each.
+MAX_SCORES = 1 << 26
+
+
 # ------------------------------------------------------------------------------------------------ plain forms
 class _Pages(NamedTuple):
     """The tensors of a pool, as :class:`sisa_amd.kernels.paged.PagePool` has them, on any device and of any head size."""
@@ -385,11 +389,21 @@ class SISAPagedCache:
         layer = st.layers[layer_idx]
         weights = None if layer.weights is None else layer.weights[lo:hi]
         if hip:
-            from .kernels.paged import sisa_paged_decode_hip
-
-            return sisa_paged_decode_hip(p.q, p.c, p.g, p.fgate, lam, layer.pool, st.table[lo:hi], st.end[lo:hi],
-                                         max_len=self.seq_len, weights=weights)
+            return self._attend_hip(p, lam, layer.pool, weights)
         return paged_attention(p.q, p.c, p.g, p.fgate, lam, layer.pool, st.table[lo:hi], st.end[lo:hi], self.seq_len, weights)
+
+    def _attend_hip(self, p, lam: Tensor, pool, weights: Tensor | None) -> Tensor:
+        from .kernels.paged import sisa_paged_decode_hip
+
+        st, lo, hi = self._store, self._lo, self._hi
+        table, lengths, longest, (B, H, M, _) = st.table[lo:hi], st.end[lo:hi], self.seq_len, p.q.shape
+        rows = max(1, MAX_SCORES // (B * H * longest))
+        if rows >= M:
+            return sisa_paged_decode_hip(p.q, p.c, p.g, p.fgate, lam, pool, table, lengths, max_len=longest, weights=weights)
+        # the workspace grows with the rows' scores: some rows at a time, for which the sequences end with the last of them
+        return torch.cat([sisa_paged_decode_hip(*(t[:, :, m:m + rows] for t in (p.q, p.c, p.g, p.fgate)), lam, pool, table,
+                                                lengths - max(0, M - m - rows), max_len=longest, weights=weights)
+                          for m in range(0, M, rows)], 2)
 
     def receive(self, layer_idx: int, q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor, fgate: Tensor,
                 hip: bool) -> None:

@@ -450,3 +450,31 @@ def test_calls_that_keep_the_module_path_with_pages(monkeypatch):
         with pytest.raises(ValueError, match="HIP implementation"):
             model(ids[:, 8:], cache=cache)
     assert steps_of(tiny_model(seed=1, attn_impl="auto").to(DEV).eval()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("track", [False, True])
+def test_many_new_positions_in_parts(track, monkeypatch):
+    """Twenty positions behind ragged prompts, three at a time, against the model's float64 copy; the bound as above."""
+    from sisa_amd import paged
+    from sisa_amd.kernels import paged as K
+    model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).eval()
+    ref = tiny_model(seed=3, theta_scale=0.25).eval()
+    ref.load_state_dict({n: t.cpu() for n, t in model.state_dict().items()})
+    ref = ref.double()
+    ids, counts = token_ids(3, 60, seed=11), [40, 1, 17]
+    monkeypatch.setattr(paged, "MAX_SCORES", 3 * 3 * model.config.n_head * 60 + 1)
+    calls, real = [], K.sisa_paged_decode_hip
+    monkeypatch.setattr(K, "sisa_paged_decode_hip", lambda q, *a, **kw: calls.append(q.shape[2]) or real(q, *a, **kw))
+    caches = [SISAPagedCache(3, 64, page_size=16, track=track) for _ in range(2)]
+    outs = []
+    for m, cache, dev in ((model, caches[0], DEV), (ref, caches[1], "cpu")):
+        with torch.no_grad():
+            cache.expect(counts)
+            m(ids[:, :40].to(dev), cache=cache)
+            outs.append(m(ids[:, 40:].to(dev), cache=cache).logits.cpu())
+    assert calls == [3, 3, 3, 3, 3, 3, 2] * 2 and caches[0].lengths == [60, 21, 37]
+    assert rel_err(outs[0], outs[1]) <= 2e-5
+    if track:
+        for layer in range(2):
+            assert rel_err(caches[0].weights(layer).cpu(), caches[1].weights(layer).double()) <= 2e-5
