@@ -3,11 +3,15 @@
 //
 // The selection is a radix select on the weights' bit patterns, mapped so that they order as unsigned integers: one
 // workgroup per (sequence, head) counts the digits of eight bits from the top in LDS (integer counts: their order does not
-// matter), narrows to the digit that holds the last position to keep, and after four digits knows the smallest weight that
-// stays and how many of its equals do. Waves own contiguous ranges of positions, so positions come out in order. The keys
-// stay in registers (up to 24 a thread: 24,576 positions; longer caches are read again for every digit). Accumulated
-// weights share their leading bits, so that the lanes of a wave count the same few digits: eight copies of the counters,
-// one per lane modulo 8, keep a count from waiting for 63 others.
+// matter), narrows to the digit that holds the last position to keep, and after four digits, or once all that have the digit
+// stay, knows the smallest weight that stays and how many of its equals do. Waves own contiguous ranges of positions, so
+// positions come out in order. The keys stay in registers (up to 24 a thread: 24,576 positions; longer caches are read again
+// for every digit), loaded beside the length. Accumulated weights share their leading bits, so that the lanes of a wave count
+// the same few digits: eight copies of the counters, one per lane modulo 8, keep a count from waiting for 63 others.
+//
+// Bound by latency: 96 workgroups of 16,384 positions take 11.8 us, of it 3 before the first count (length, weights, cleared
+// counters), 2.5 for the first digit, whose counts meet most often, 1.2 for each other one (two barriers and wave 0's scan
+// between them) and 2.5 for the positions; 256 of up to 5,003 positions 7.5 us (with 16 keys a thread in place of 8: 9.8).
 #include "pages.h"
 
 namespace {
@@ -22,7 +26,9 @@ SISA_DEV unsigned order_of(float x) {
 }
 
 SISA_DEV int count_of(uint64_t lanes) { return __builtin_popcountll(lanes); }
-SISA_DEV int below(uint64_t lanes, int lane) { return __builtin_popcountll(lanes & ((1ull << lane) - 1)); }
+SISA_DEV int below(uint64_t lanes) {                   // of them before this lane
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)lanes, 0u));
+}
 
 // x summed over the wave's lanes up to this one.
 template <int CTRL, int ROWS> SISA_DEV unsigned from_lane(unsigned x) {
@@ -37,20 +43,30 @@ SISA_DEV unsigned wave_scan(unsigned x) {
     return x + from_lane<0x143, 0xc>(x);               // lane 31 to rows 2 and 3
 }
 
-constexpr int COPIES = 8, COPY = 257;  // counters' copies, and from one to the next (a digit's copies on banks of their own)
+constexpr int COPIES = 8, COPY = 260;  // counters' copies, and from one to the next (a digit's copies on banks of their own)
 
 // NK keys a thread in registers, or 0: read from memory each time they are needed.
 template <int NK>
 __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_args a, int shift, int new_shift) {
-    __shared__ unsigned hists[4][COPIES * COPY];       // of the four digits
+    __shared__ __attribute__((aligned(16))) unsigned hists[4][COPIES * COPY];       // of the four digits
     __shared__ unsigned found, left;                   // the digit with the last one to keep, and how many to keep in it
+    __shared__ bool whole;                             // which are all that have it
     __shared__ int gt[SW], eq[SW];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int H = a.from.heads, nh = blockIdx.x, h = nh % H, n = nh / H;
+    // The wave's range of positions, 64 at a time. Its weights are under way beside the length, not after it.
+    const int steps = ((a.max_len + SW - 1) / SW + 63) / 64, i0 = w * steps * 64;
+    const int64_t step = 64 * a.weights.sl;
+    const float* W = (const float*)a.weights.ptr + (n * a.weights.sb + h * a.weights.sh) + (int64_t)(i0 + lane) * a.weights.sl;
+    float x[NK ? NK : 1];
+    if constexpr (NK > 0) {
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+            x[s] = s < steps && i0 + 64 * s + lane < a.max_len ? W[s * step] : 0.f;
+        }
+    }
     const int len = a.lengths[n], keep = a.keep, recent = a.recent;
     int32_t* pos = a.positions + (int64_t)nh * keep;
-    const float* W = (const float*)a.weights.ptr + n * a.weights.sb + h * a.weights.sh;
-    const int64_t sl = a.weights.sl;
     const int out = len < keep ? len : keep;
     const bool bad = len < 0 || len > a.max_len || len > ((int64_t)a.W << shift) || out > ((int64_t)a.W_new << new_shift);
     if (h == 0 && tid == 0) a.new_lengths[n] = bad ? -1 : out;
@@ -61,40 +77,33 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
         return;
     }
     const int old = len - recent, pick = keep - recent;        // pick of the first `old`, then the recent ones
-    // the wave's range of positions, 64 at a time
-    const int steps = ((old + SW - 1) / SW + 63) / 64, i0 = w * steps * 64;
-    unsigned key[NK ? NK : 1];
+    unsigned key[NK ? NK : 1];                         // 0, below every weight's, where there is no position
     if constexpr (NK > 0) {
-        float x[NK];
 #pragma unroll
-        for (int s = 0; s < NK; ++s) x[s] = s < steps && i0 + 64 * s + lane < old ? W[(i0 + 64 * s + lane) * sl] : 0.f;
-#pragma unroll
-        for (int s = 0; s < NK; ++s) key[s] = order_of(x[s]);
+        for (int s = 0; s < NK; ++s) key[s] = i0 + 64 * s + lane < old ? order_of(x[s]) : 0u;
     }
     for (int i = tid; i < recent; i += 64 * SW) pos[pick + i] = old + i;
     if (pick == 0) return;
-    // f(position, key) for each of the wave's positions in order, all lanes together; position -1 where there is none
+    // f(position, key) for each of the wave's positions in order, all lanes together; key 0 where there is none
+    const int mine = i0 >= old ? 0 : (old - i0 + 63) / 64 < steps ? (old - i0 + 63) / 64 : steps;
     auto each = [&](auto&& f) {
         if constexpr (NK > 0) {
 #pragma unroll
             for (int s = 0; s < NK; ++s)
-                if (s < steps) {
-                    const int i = i0 + 64 * s + lane;
-                    f(i < old ? i : -1, key[s]);
-                }
+                if (s < mine) f(i0 + 64 * s + lane, key[s]);
         } else {
-            for (int s0 = 0; s0 < steps; s0 += 8) {            // eight loads under way
+            for (int s0 = 0; s0 < mine; s0 += 8) {             // eight loads under way
                 float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int i = i0 + 64 * (s0 + e) + lane;
-                    y[e] = s0 + e < steps && i < old ? W[i * sl] : 0.f;
+                    y[e] = s0 + e < mine && i < old ? W[(s0 + e) * step] : 0.f;
                 }
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (s0 + e < steps) {
+                    if (s0 + e < mine) {
                         const int i = i0 + 64 * (s0 + e) + lane;
-                        f(i < old ? i : -1, order_of(y[e]));
+                        f(i, i < old ? order_of(y[e]) : 0u);
                     }
             }
         }
@@ -107,39 +116,42 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
     for (int d = 24; d >= 0; d -= 8) {
         unsigned* hist = hists[d >> 3];
         const unsigned high = d == 24 ? 0u : prefix >> (d + 8);
-        each([&](int i, unsigned k) {
-            if (i >= 0 && (d == 24 || k >> (d + 8) == high)) atomicAdd(&hist[(lane & (COPIES - 1)) * COPY + (k >> d & 255)], 1u);
+        each([&](int, unsigned k) {
+            if (k && (d == 24 || k >> (d + 8) == high)) atomicAdd(&hist[(lane & (COPIES - 1)) * COPY + (k >> d & 255)], 1u);
         });
         __syncthreads();
         if (w == 0) {
             // lane l: digits 255 - 4 l down to 252 - 4 l; above: how many keys have a larger digit
-            unsigned c[4], mine = 0;
+            u32x4 c = {0, 0, 0, 0};                        // of digits 252 - 4 l up
+#pragma unroll
+            for (int k = 0; k < COPIES; ++k) c += *reinterpret_cast<const u32x4*>(hist + k * COPY + 252 - 4 * lane);
+            const unsigned four = (c[0] + c[1]) + (c[2] + c[3]);
+            unsigned above = wave_scan(four) - four;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                c[e] = 0;
-#pragma unroll
-                for (int k = 0; k < COPIES; ++k) c[e] += hist[k * COPY + 255 - 4 * lane - e];
-                mine += c[e];
-            }
-            unsigned above = wave_scan(mine) - mine;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (above < want && want <= above + c[e]) found = 255 - 4 * lane - e, left = want - above;
-                above += c[e];
+                if (above < want && want <= above + c[3 - e])
+                    found = 255 - 4 * lane - e, left = want - above, whole = want == above + c[3 - e];
+                above += c[3 - e];
             }
         }
         __syncthreads();
         prefix |= found << d;
         want = left;
+        if (whole && prefix) {                         // all with this digit stay: nothing is left to tell apart
+            --prefix, want = 0;
+            break;
+        }
     }
 
     // Those above the smallest key, and its equals from the lowest position on.
-    int ng = 0, ne = 0;
-    each([&](int i, unsigned k) {
-        ng += count_of(__ballot(i >= 0 && k > prefix));
-        ne += count_of(__ballot(i >= 0 && k == prefix));
+    unsigned ng = 0, ne = 0;
+    each([&](int, unsigned k) {
+        ng += k > prefix;
+        ne += k == prefix;
     });
-    if (lane == 0) gt[w] = ng, eq[w] = ne;
+    ng = wave_scan(ng);
+    ne = wave_scan(ne);
+    if (lane == 63) gt[w] = ng, eq[w] = ne;
     __syncthreads();
     int at = 0, equals = 0;
     for (int k = 0; k < w; ++k) {
@@ -147,11 +159,19 @@ __global__ __launch_bounds__(64 * SW) void evict_select_kernel(sisa_cache_evict_
         at += gt[k] + (take < 0 ? 0 : take < eq[k] ? take : eq[k]);
         equals += eq[k];
     }
+    if (equals >= (int)want) {                         // no equals of this wave
+        each([&](int i, unsigned k) {
+            const uint64_t stays = __ballot(k > prefix);
+            if (k > prefix) pos[at + below(stays)] = i;
+            at += count_of(stays);
+        });
+        return;
+    }
     each([&](int i, unsigned k) {
-        const uint64_t same = __ballot(i >= 0 && k == prefix);
-        const bool stay = i >= 0 && (k > prefix || (k == prefix && equals + below(same, lane) < (int)want));
+        const uint64_t same = __ballot(k == prefix);
+        const bool stay = k > prefix || (k == prefix && equals + below(same) < (int)want);
         const uint64_t stays = __ballot(stay);
-        if (stay) pos[at + below(stays, lane)] = i;
+        if (stay) pos[at + below(stays)] = i;
         at += count_of(stays);
         equals += count_of(same);
     });
@@ -216,6 +236,7 @@ extern "C" int sisa_cache_evict(const sisa_cache_evict_args* a, void* stream) {
     hipStream_t st = (hipStream_t)stream;
     const int64_t per = sisa::cdiv(a->max_len, 64 * SW);       // keys a thread
     if (per <= 4) evict_select_kernel<4><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
+    else if (per <= 8) evict_select_kernel<8><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
     else if (per <= 16) evict_select_kernel<16><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
     else if (per <= 24) evict_select_kernel<24><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
     else evict_select_kernel<0><<<(unsigned)heads, 64 * SW, 0, st>>>(*a, shift, new_shift);
