@@ -213,9 +213,9 @@ __global__ __launch_bounds__(64 * NW) void paged_chunk_kernel(sisa_paged_decode_
 template <class TO, bool TRACK>
 __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args a, TO* out, int shift, int nchunk,
                                                          const f32x2* stat, const float* part, const float* scores) {
-    __shared__ float red[2][4], wo[4][DH];
-    constexpr int PER = PIECE / 256;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ float red[2][4], wo[4][DH], ms[256];    // ms: up to 256 chunks' factors
+    constexpr int PER = PIECE / 256, AHEAD = 8;        // partial outputs of a wave under way
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int pieces = TRACK ? (a.max_len + PIECE - 1) / PIECE : 1;
     const int piece = blockIdx.x % pieces, item = blockIdx.x / pieces;
     const int H = a.pool.heads, nh = TRACK ? item : item / a.M, h = nh % H, n = nh / H;
@@ -247,9 +247,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
         }
         const f32x2* S = stat + row * nchunk;
         const int nc = (vis + KCH - 1) / KCH;
-        float mx = -__builtin_inff(), l = 0.f;
+        float mx = -__builtin_inff(), l = 0.f, m0 = 0.f;
         for (int c = tid; c < nc; c += 256) {
             const f32x2 x = S[c];
+            if (c == tid) m0 = x[0];
             const float to = fmaxf(mx, x[0]), ref = to == -__builtin_inff() ? 0.f : to;
             l = l * (mx == -__builtin_inff() ? 1.f : expf(mx - ref)) + x[1] * (x[0] == -__builtin_inff() ? 1.f : expf(x[0] - ref));
             mx = to;
@@ -271,10 +272,26 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
         const float inv = 1.f / l;
         if (outs) {
             float o = 0.f;
-            for (int c = w; c < nc; c += 4) {
-                const float mc = S[c][0];
-                o = fmaf(part[(row * nchunk + c) * DH + lane], mc == -__builtin_inff() ? 1.f : expf(mc - ref), o);
-            }
+            auto factor = [&](float mc) { return mc == -__builtin_inff() ? 1.f : expf(mc - ref); };
+            ms[tid] = factor(m0);
+            __syncthreads();
+            // every fourth chunk; behind the last the last again, which is left out
+            const float* O = part + row * nchunk * DH + lane;
+            auto add = [&](auto&& scale) {
+                for (int c0 = w; c0 < nc; c0 += 4 * AHEAD) {
+                    float x[AHEAD], by[AHEAD];
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k) {
+                        const int c = c0 + 4 * k < nc ? c0 + 4 * k : nc - 1;
+                        x[k] = O[c * DH];
+                        by[k] = scale(c);
+                    }
+#pragma unroll
+                    for (int k = 0; k < AHEAD; ++k) o = c0 + 4 * k < nc ? fmaf(x[k], by[k], o) : o;
+                }
+            };
+            if (nc <= 256) add([&](int c) { return ms[c]; });
+            else add([&](int c) { return factor(S[c][0]); });
             wo[w][lane] = o;
             __syncthreads();
             if (tid < DH) out[row * DH + tid] = cvt<TO>(((wo[0][tid] + wo[1][tid]) + (wo[2][tid] + wo[3][tid])) * inv);
