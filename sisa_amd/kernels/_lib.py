@@ -8,6 +8,7 @@ the HIP device on ROCm builds).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 import threading
@@ -366,6 +367,13 @@ class Packed:
         if rc != 0:
             msg = load().sisa_last_error().decode(errors="replace")
             raise RuntimeError(f"{self.name} failed (code {rc}): {msg}")
+
+
+@functools.lru_cache(maxsize=1024)
+def floats(name: str, *dims: int) -> int:
+    """The float32 elements of the workspace that an entry point's ``name`` asks for; dimensions are remembered, for calls whose
+    host time counts."""
+    return -(-workspace_bytes(name, *dims) // 4)
 
 
 def workspace_bytes(name: str, *dims: int) -> int:

@@ -65,7 +65,8 @@ class PagePool:
     power of two of at least 16. Rows must be readable with 16-byte loads; the tensors may be views of a larger one. The
     handle keeps the tensors and checks them once."""
 
-    __slots__ = ("k", "v", "b", "g", "fgate", "pages", "heads", "page_size", "dtype", "device_index", "packed")
+    __slots__ = ("k", "v", "b", "g", "fgate", "pages", "heads", "page_size", "dtype", "dtype_code", "device_index",
+                 "packed")
 
     def __init__(self, k: Tensor, v: Tensor, b: Tensor, g: Tensor, fgate: Tensor | None = None):
         if k.dim() != 4 or k.shape[-1] != HIP_D_HEAD or v.shape != k.shape:
@@ -90,7 +91,8 @@ class PagePool:
             raise ValueError("PagePool: k, v, b need rows that 16-byte loads can read (unit last stride, 16-byte aligned)")
         self.k, self.v, self.b, self.g, self.fgate = k, v, b, g, fgate
         self.pages, self.heads, self.page_size, self.dtype, self.device_index = P, H, S, k.dtype, device
-        self.packed = bytes(_lib.PagePoolArgs(P, H, S, _lib.dtype_code(k.dtype), *(_lib.view(t) for t in (k, v, b, g, fgate))))
+        self.dtype_code = _lib.dtype_code(k.dtype)
+        self.packed = bytes(_lib.PagePoolArgs(P, H, S, self.dtype_code, *(_lib.view(t) for t in (k, v, b, g, fgate))))
 
     @classmethod
     def empty(cls, pages: int, heads: int, page_size: int, dtype: torch.dtype, device) -> "PagePool":
@@ -217,8 +219,8 @@ def sisa_paged_decode_hip(q: Tensor, c: Tensor, g_q: Tensor, f_q: Tensor | None,
         w_out = w_in if weights_out is None else _weights_view(name, "weights_out", weights_out, B, H, max_len, pool)
         if any(step == 0 and size > 1 for step, size in zip(w_out[1:], (B, H, max_len))):
             raise ValueError(f"{name}: the weights that are written must not be an expanded tensor")
-    size = _lib.load().sisa_paged_decode_workspace_bytes(B, H, M, max_len, _lib.dtype_code(pool.dtype), weights is not None)
-    ws = lam.new_empty((size // 4,)) if size else None
+    size = _lib.floats("sisa_paged_decode_workspace_bytes", B, H, M, max_len, pool.dtype_code, weights is not None)
+    ws = lam.new_empty((size,)) if size else None
     _decode(q, B, M, W, max_len, pool.packed, table.data_ptr(), table.stride(0), lengths.data_ptr(), *vq, *vc, *vg, *vf,
             lam.data_ptr(), lam.stride(0), *w_in, *w_out, out.data_ptr(), 0 if ws is None else ws.data_ptr())
     return out

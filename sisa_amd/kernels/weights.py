@@ -74,7 +74,7 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     g, *vg = _gates(g)
     fgate, *vf = (None, *_NO_VIEW) if fgate is None else _gates(fgate)
     window = 0 if window is None or window >= L else window
-    ws = lam.new_empty((_lib.load().sisa_attn_weights_workspace_bytes(B, H, L, window) // 4,))
+    ws = lam.new_empty((_lib.floats("sisa_attn_weights_workspace_bytes", B, H, L, window),))
     _weights(q, B, H, L, window, _lib.dtype_code(q.dtype), 0, *vq, *vk, *vc, *vb, *vg, *vf, lam.data_ptr(), lam.stride(0),
              0 if lengths is None else lengths.data_ptr(), out.data_ptr(), ws.data_ptr())
     return out
