@@ -23,6 +23,7 @@ namespace {
 
 constexpr int DH = 64, DS = 32;
 constexpr int FEW_ROWS = 256;         // query rows up to which, against four times as many keys, each wave has its own keys
+constexpr int MAX_SPLITS = 32;        // of the keys in the first pass
 constexpr float SCALE = LOG2E / 8;    // of q.k into log2 units
 
 struct Rows {                         // queries of a sequence: first .. first + count - 1
@@ -152,6 +153,11 @@ SISA_DEV void merge(float& m, float& l, float m2, float l2) {
     const float t = fmaxf(m, m2), ref = t == -__builtin_inff() ? 0.f : t;
     l = l * (m == -__builtin_inff() ? 1.f : fast_exp2(m - ref)) + l2 * (m2 == -__builtin_inff() ? 1.f : fast_exp2(m2 - ref));
     m = t;
+}
+
+// x of the lane whose number differs in bit 0 (0xB1) or bit 1 (0x4E).
+template <int CTRL> SISA_DEV float in_quad(float x) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
 }
 
 // What the second pass starts its products from: -lse in units of q.k.
@@ -340,12 +346,30 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
         for (int u = 0; u < U; ++u) raw[u] = own.load_edge(j0 + 16 * u, L);
     }
     if constexpr (FEW) {
-        for (int r = threadIdx.x; r < rows.count; r += 64 * NW) {
-            const f32x2* p = parts + ((int64_t)bh * Rp + r) * nsplit;
-            float m = p[0][0], l = p[0][1];
-#pragma unroll 4
-            for (int k = 1; k < nsplit; ++k) merge(m, l, p[k][0], p[k][1]);
-            starts[r] = start_of(m, l);
+        // four lanes a row, all of their parts under way at once
+        const int sub = threadIdx.x & 3;
+        for (int r0 = 0; r0 < rows.count; r0 += 16 * NW) {
+            const int r = r0 + threadIdx.x / 4;
+            const f32x2* p = parts + ((int64_t)bh * Rp + (r < rows.count ? r : 0)) * nsplit;
+            f32x2 x[MAX_SPLITS / 4];
+            float m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+            for (int k = 0; k < MAX_SPLITS / 4; ++k)
+                x[k] = 4 * k < nsplit ? p[4 * k + sub < nsplit ? 4 * k + sub : 0] : f32x2{-__builtin_inff(), 0.f};
+#pragma unroll
+            for (int k = 0; k < MAX_SPLITS / 4; ++k) {
+                if (4 * k + sub >= nsplit) x[k] = f32x2{-__builtin_inff(), 0.f};
+                m = fmaxf(m, x[k][0]);
+            }
+            m = fmaxf(m, in_quad<0xB1>(m));
+            m = fmaxf(m, in_quad<0x4E>(m));
+            const float ref = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+            for (int k = 0; k < MAX_SPLITS / 4; ++k)
+                if (4 * k < nsplit) l += x[k][1] * (x[k][0] == -__builtin_inff() ? 1.f : fast_exp2(x[k][0] - ref));
+            l += in_quad<0xB1>(l);
+            l += in_quad<0x4E>(l);
+            if (sub == 0 && r < rows.count) starts[r] = start_of(m, l);
         }
         __syncthreads();
     }
@@ -470,7 +494,7 @@ Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
     if (p.few && groups < 256) {
         const int64_t want = 256 / groups, most = sisa::cdiv(L, 256);
         p.nsplit = (int)(want < most ? want : most);
-        p.nsplit = p.nsplit < 32 ? p.nsplit : 32;
+        p.nsplit = p.nsplit < MAX_SPLITS ? p.nsplit : MAX_SPLITS;
     }
     p.bytes = BH * p.Rp * (p.few ? 8 * (int64_t)p.nsplit : 4);
     return p;
