@@ -475,8 +475,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
 }
 
 // How a call is laid out. Waves hold 64 queries (keys), four share them. Where the 64-row blocks of the queries are fewer than
-// the chip's 256 CUs: 16 of them, eight waves to share; or, where few rows are counted against many keys, the keys of the first
-// pass in splits (of 256 keys at least, 32 at most), which the second joins, and there each wave its own keys.
+// the chip's 256 CUs: 16 of them, eight waves to share (2 x 333 positions of 4 heads, fp32: both passes 36 -> 16 us); or, where
+// few rows are counted against many keys, the keys of the first pass in splits (of 256 keys at least, 32 at most), which the
+// second joins, and there each wave its own keys (the last 64 of 16,384 positions of 16 heads: 43 -> 35.5 us, 35 with four lanes
+// to a row's join; 512 to 2,048 workgroups of splits in place of 256: first pass 15.6 -> 17 to 20.9).
 struct Plan {
     int R, nsplit;
     bool few, small;

@@ -9,9 +9,9 @@
 // for every digit), loaded beside the length. Accumulated weights share their leading bits, so that the lanes of a wave count
 // the same few digits: eight copies of the counters, one per lane modulo 8, keep a count from waiting for 63 others.
 //
-// Bound by latency: 96 workgroups of 16,384 positions take 11.8 us, of it 3 before the first count (length, weights, cleared
-// counters), 2.5 for the first digit, whose counts meet most often, 1.2 for each other one (two barriers and wave 0's scan
-// between them) and 2.5 for the positions; 256 of up to 5,003 positions 7.5 us (with 16 keys a thread in place of 8: 9.8).
+// Bound by latency: 96 workgroups of 16,384 positions take 11.8 us, of it 3.5 before the first count (the weights, from HBM),
+// 1.7 for the first digit, whose counts meet most often, 1.2 for each other one (two barriers, wave 0's scan between them) and
+// 1.5 for the positions; 256 of up to 5,003 positions 7.5 us (room for 16 keys a thread in place of 8: 9.8).
 #include "pages.h"
 
 namespace {
