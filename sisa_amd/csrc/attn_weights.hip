@@ -4,15 +4,16 @@
 //   s_ij = q_i.k_j / 8 + lam exp(g_i - g_j) (c_i.b_j) + (F_i - F_j)
 //
 // Two passes over the scores, neither of which keeps them: the queries' log-sum-exp over their keys, then every key's sum
-// over its queries. Scores are 16x16 MFMA blocks with K = 64 (q.k) and 32 (c.b). A wave holds 64 queries (keys) in
+// over its queries. Scores are 16x16 MFMA blocks with K = 64 (q.k) and 32 (c.b). A wave holds up to 64 queries (keys) in
 // registers and streams 16 keys (queries) at a time, which L2 serves, the next 16 in LDS and those after them under way
-// while the present ones are used; four waves share the 64 and take every fourth of the 16s. In the first pass a lane owns one query
-// per block (the keys are the block's rows), in the second one key: the running sums need no lane exchange before the end.
+// while the present ones are used; four or eight waves share the 64 and take every fourth or eighth of the 16s. In the first
+// pass a lane owns one query per block (the keys are the block's rows), in the second one key: the running sums need no lane
+// exchange before the end.
 //
 // Bound by the vector unit: the products of a block take 48 cycles of the matrix pipe, its 256 scores' exponentials alone
 // 32 of issue. So blocks away from the diagonal factor the decay, exp(g_i - g_j) = exp(g_i - g_a) exp(g_a - g_j), and split
-// the forget term, (F_i - F_a) + (F_a - F_j), at an anchor a between the two: the first query of the 64 in the first pass,
-// the last key in the second. Both factors are at most 1 and both terms at most 0 there, so nothing overflows and rounding
+// the forget term, (F_i - F_a) + (F_a - F_j), at an anchor a between the two: the wave's first query in the first pass,
+// its last key in the second. Both factors are at most 1 and both terms at most 0 there, so nothing overflows and rounding
 // grows with the differences of F, not with F. That leaves a product, two FMAs and one exponential for a score. Blocks
 // that meet the diagonal or the end of the sequence take the formula as it stands.
 #include "common.h"
@@ -474,15 +475,21 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
     a.out[(int64_t)bh * L + j] = j < rows.n ? s : 0.f;
 }
 
-// How a call is laid out. Waves hold 64 queries (keys), four share them. Where the 64-row blocks of the queries are fewer than
-// the chip's 256 CUs: 16 of them, eight waves to share (2 x 333 positions of 4 heads, fp32: both passes 36 -> 16 us); or, where
-// few rows are counted against many keys, the keys of the first pass in splits (of 256 keys at least, 32 at most), which the
-// second joins, and there each wave its own keys (the last 64 of 16,384 positions of 16 heads: 43 -> 35.5 us, 35 with four lanes
-// to a row's join; 512 to 2,048 workgroups of splits in place of 256: first pass 15.6 -> 17 to 20.9).
+// How a call is laid out. Waves hold 64 queries (keys), four share them, where such blocks of all the queries are many. Where
+// they are fewer, less: `groups` counts them, and both passes together took (us)
+//                              16 rows, 8 waves   32 rows, 8   32 rows, 4   64 rows, 4
+//   1 x 512 x 12 heads,  96          13.7            13.8         14.9         17.6
+//   1 x 1,024 x 12,     192          22.5            18.5         21.0         25.1
+//   2 x 920 x 12,       360          32.1            26.4         21.5         25.8
+//   1 x 2,048 x 16,     512          65              44.8         41.2         44.8
+//   4 x 1,024 x 12,     768          64              45.7         37.3         33.1
+// Where few rows are counted against many keys, the keys of the first pass are split (256 keys at least, 32 splits at most),
+// the second joins the parts, and there each wave has its own keys (the last 64 of 16,384 positions of 16 heads: 43 -> 35.5 us,
+// 35 with four lanes to a row's join; 512 to 2,048 workgroups of splits in place of 256: first pass 15.6 -> 17 to 20.9).
 struct Plan {
     int R, nsplit;
-    bool few, small;
-    int64_t Rp, bytes;
+    bool few;
+    int64_t groups, Rp, bytes;
 };
 
 Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
@@ -490,11 +497,11 @@ Plan plan_of(int32_t B, int32_t H, int32_t L, int32_t window) {
     p.R = window && window < L ? window : L;
     p.Rp = (p.R + 15) / 16 * 16;
     p.few = p.R <= FEW_ROWS && L / 4 >= p.R;
-    const int64_t BH = (int64_t)B * H, groups = BH * sisa::cdiv(p.R, 64);
-    p.small = !p.few && groups < 256;
+    const int64_t BH = (int64_t)B * H;
+    p.groups = BH * sisa::cdiv(p.R, 64);
     p.nsplit = 1;
-    if (p.few && groups < 256) {
-        const int64_t want = 256 / groups, most = sisa::cdiv(L, 256);
+    if (p.few && p.groups < 256) {
+        const int64_t want = 256 / p.groups, most = sisa::cdiv(L, 256);
         p.nsplit = (int)(want < most ? want : most);
         p.nsplit = p.nsplit < MAX_SPLITS ? p.nsplit : MAX_SPLITS;
     }
@@ -522,7 +529,9 @@ template <class T, bool FORGET>
 int launch_weights(const sisa_attn_weights_args* a, hipStream_t st) {
     const Plan p = plan_of(a->B, a->H, a->L, a->window);
     if (p.few) return launch_weights<T, FORGET, 4, 8, 4, 4, 1>(a, p, st);
-    if (p.small) return launch_weights<T, FORGET, 1, 8, 1, 8, 8>(a, p, st);
+    if (p.groups < 128) return launch_weights<T, FORGET, 1, 8, 1, 8, 8>(a, p, st);
+    if (p.groups < 256) return launch_weights<T, FORGET, 2, 8, 2, 8, 8>(a, p, st);
+    if (p.groups < 640) return launch_weights<T, FORGET, 2, 4, 2, 4, 4>(a, p, st);
     return launch_weights<T, FORGET, 4, 4, 4, 4, 4>(a, p, st);
 }
 

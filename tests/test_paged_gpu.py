@@ -476,6 +476,16 @@ def test_received_weights(lengths, L, H, window, dtype):
         assert sisa_attention_weights_hip(*x, lam, f, lengths=_ints(-4), window=window).eq(0).all()
 
 
+# heads and sequences enough for every width of the blocks: 135 to 720 blocks of 64 rows; whole tiles, an anchor
+# within a block, ends at the edges of 16 and 32
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,L,H,window", [([130, 0, 64, 95], 130, 12, None), ([530, 300, 33], 530, 9, 280),
+                                                ([129, 97, 128, 32, 1, 79], 129, 20, None), ([400, 127], 400, 24, None),
+                                                ([130, 33, 31, 130, 7, 96, 64, 65], 130, 30, None)])
+def test_received_weights_of_many_heads(lengths, L, H, window, dtype):
+    test_received_weights(lengths, L, H, window, dtype)
+
+
 def test_received_weights_with_steep_gates():
     """Gates that fall by tens per position, and by hundreds over the sequence: the weights gather on the diagonal, and
     what underflows is 0."""
