@@ -51,9 +51,6 @@ constexpr int DW = 4;                 // waves per workgroup where the positions
 constexpr int KCH = TILE * DW;        // positions per chunk (workgroup)
 constexpr int PIECE = 1024;           // positions of tracked weights per workgroup of the join
 
-// Waves of a workgroup that takes a whole row: as many as fit.
-template <class T> constexpr int whole_waves() { return sizeof(T) == 2 ? 16 : 8; }
-
 // Positions that query row m of a sequence of n sees, or -1 for a length that the call does not take.
 SISA_DEV int visible(int n, int max_len, int64_t held, int M, int m) {
     if (n < 0 || n > max_len || n > held) return -1;
@@ -311,15 +308,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(sisa_paged_decode_args 
     }
 }
 
-// Caches that one workgroup takes whole need no join (tracked weights: with one query row, the only one to add to them).
-bool takes_whole(int M, int64_t max_len, int elem, bool tracked) {
-    return max_len <= TILE * (elem == 2 ? whole_waves<__bf16>() : whole_waves<float>()) && (!tracked || M == 1);
+// The waves of a workgroup that takes a query row whole, so that no join is needed; 0: the row is split. With tracked weights
+// it must be the only row to add to them. 16 waves fill a CU alone: more rows than CUs are split (whole / split, us: 192 rows of
+// 1,000 positions, tracked, 16.7 / 20.4, 576 of 1,000 49.8 / 43.9; with 8 waves 544 rows of 452 20.7 / 23.5, with 4 768 of 100
+// 9.4 / 13.6; with 16 waves the last two 27.1 and 17.9).
+int whole_waves(int64_t rows, int M, int64_t max_len, int elem, bool tracked) {
+    if (tracked && M > 1) return 0;
+    return max_len <= KCH ? DW : max_len <= 2 * KCH ? 8 : max_len <= 4 * KCH && elem == 2 && rows <= 256 ? 16 : 0;
 }
 
 bool fits(int64_t rows, int M, int64_t max_len, int elem, bool tracked) {
-    const int64_t threads = takes_whole(M, max_len, elem, tracked) ? 64 * (elem == 2 ? whole_waves<__bf16>() : whole_waves<float>())
-                                                                   : sisa::cdiv(max_len, KCH) * KCH;
-    return rows <= sisa::MAX_THREADS / threads;
+    const int waves = whole_waves(rows, M, max_len, elem, tracked);
+    return rows <= sisa::MAX_THREADS / (waves ? 64 * waves : sisa::cdiv(max_len, KCH) * KCH);
 }
 
 struct DecodeSpace {
@@ -340,16 +340,23 @@ DecodeSpace decode_space(char* base, int64_t rows, int64_t max_len, bool tracked
     return s;
 }
 
+template <class T, class TO, int NW, bool TRACK>
+int launch_whole(const sisa_paged_decode_args* a, TO* out, int64_t rows, hipStream_t st) {
+    paged_chunk_kernel<T, TO, NW, true, TRACK, false><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, out, sisa::log2_of(a->pool.page_size),
+                                                                                         1, nullptr, nullptr, nullptr);
+    return sisa::launch_status("sisa_paged_decode");
+}
+
 template <class T, class TO, bool TRACK>
 int launch_decode(const sisa_paged_decode_args* a, TO* out, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size), nchunk = (int)sisa::cdiv(a->max_len, KCH);
     const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
     const DecodeSpace ws = decode_space((char*)a->workspace, rows, a->max_len, TRACK);
-    constexpr int NW = whole_waves<T>();
-    if (takes_whole(a->M, a->max_len, (int)sizeof(T), TRACK)) {
-        paged_chunk_kernel<T, TO, NW, true, TRACK, false><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, out, shift, 1, nullptr, nullptr,
-                                                                                             nullptr);
-        return sisa::launch_status("sisa_paged_decode");
+    switch (whole_waves(rows, a->M, a->max_len, (int)sizeof(T), TRACK)) {
+        case 4: return launch_whole<T, TO, 4, TRACK>(a, out, rows, st);
+        case 8: return launch_whole<T, TO, 8, TRACK>(a, out, rows, st);
+        case 16:
+            if constexpr (sizeof(T) == 2) return launch_whole<T, TO, 16, TRACK>(a, out, rows, st);
     }
     const unsigned grid = (unsigned)(rows * nchunk);
     if (sizeof(T) == 2 && a->M == 1 && sisa::cache_bytes(a->pool, a->B, a->max_len) >= STREAM_BYTES)
@@ -403,7 +410,8 @@ extern "C" int sisa_paged_write(const sisa_paged_write_args* a, void* stream) {
 
 extern "C" int64_t sisa_paged_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t max_len, int32_t dtype,
                                                      int32_t tracked) {
-    if (B < 1 || H < 1 || M < 1 || max_len < 1 || takes_whole(M, max_len, sisa::elem_size(dtype), tracked != 0)) return 0;
+    if (B < 1 || H < 1 || M < 1 || max_len < 1 || whole_waves((int64_t)B * H * M, M, max_len, sisa::elem_size(dtype), tracked != 0))
+        return 0;
     return decode_space(nullptr, (int64_t)B * H * M, max_len, tracked != 0).bytes;
 }
 
@@ -416,7 +424,8 @@ extern "C" int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream) 
                  a->max_len, a->pool.page_size);
     if (a->B == 0) return SISA_OK;
     SISA_REQUIRE(a->table && a->lengths && a->lam && a->out, "sisa_paged_decode: null pointer");
-    SISA_REQUIRE(takes_whole(a->M, a->max_len, sisa::elem_size(a->pool.dtype), a->w_out.ptr != nullptr) ||
+    const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
+    SISA_REQUIRE(whole_waves(rows, a->M, a->max_len, sisa::elem_size(a->pool.dtype), a->w_out.ptr != nullptr) ||
                      (a->workspace && sisa::aligned16(a->workspace)),
                  "sisa_paged_decode: null workspace, or not 16-byte aligned");
     SISA_REQUIRE(sisa::view_ok(a->q, a->pool.dtype) && sisa::view_ok(a->c, a->pool.dtype),
@@ -425,7 +434,6 @@ extern "C" int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream) 
                  "sisa_paged_decode: gq must be given, and fq where the pool has f");
     SISA_REQUIRE((a->w_in.ptr == nullptr) == (a->w_out.ptr == nullptr),
                  "sisa_paged_decode: w_in and w_out must be given together");
-    const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
     SISA_REQUIRE(fits(rows, a->M, a->max_len, sisa::elem_size(a->pool.dtype), a->w_out.ptr != nullptr),
                  "sisa_paged_decode: B*H*M*max_len too large for one launch");
     hipStream_t st = (hipStream_t)stream;

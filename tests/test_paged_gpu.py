@@ -136,6 +136,14 @@ def test_decode(lengths, H, S, M, dtype):
                    for i, n in enumerate(lengths))
 
 
+# rows that a workgroup of 4, 8 or 16 waves takes whole, or that are too many for it
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,H,S,M", [([256, 0, 31], 3, 16, 1), ([512, 300, 257, 1], 3, 64, 1), ([1000, 513, 0, 1024], 2, 128, 1),
+                                           ([600, 513, 64, 1, 0, 257, 570, 599, 80], 30, 32, 1), ([500, 40], 3, 16, 2)])
+def test_decode_of_rows_taken_whole(lengths, H, S, M, dtype):
+    test_decode(lengths, H, S, M, dtype)
+
+
 def test_decode_continues_the_contiguous_cache():
     """The same rows through sisa_decode_hip, whose cache is one tensor."""
     from sisa_amd.kernels.decode import sisa_decode_hip

@@ -166,7 +166,7 @@ def test_entry_points_refuse_more_than_a_launch_takes(lib):
     """The threads of a launch are counted in 32 bits."""
     from sisa_amd.kernels import _lib
     none, row, gate = _lib.View(None, 0, 0, 0), _lib.View(4096, 1024, 64, 64), _lib.View(4096, 32, 16, 1)
-    for B, M, W, w in ((1 << 14, 128, 100, none), (1 << 21, 1, 1, none), (1 << 21, 1, 1, gate)):
+    for B, M, W, w in ((1 << 14, 128, 100, none), (1 << 23, 1, 1, none), (1 << 22, 1, 32, gate)):
         args = _lib.PagedDecodeArgs(B, M, W, 16 * W, _pool(lib), 4096, W, 4096, row, row, gate, gate, 4096, 1, w, w, 4096, 4096)
         _refused(lib, "sisa_paged_decode", args, "too large")
     for B, H, L, window in ((1 << 14, 1 << 6, 2048, 0), (1, 1, 1 << 30, 300), (1 << 10, 1 << 10, 4096, 1)):
