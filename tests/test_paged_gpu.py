@@ -402,6 +402,25 @@ def test_evict_to_another_page_size(dtype):
     _evict_case([333, 90], 3, 16, 100, 20, dtype, _heavy, seed=5, S_new=128)
 
 
+# as many positions as a thread holds 8, 16 and 24 of, and the edges between
+@pytest.mark.parametrize("values", [_heavy, _tied, _odd])
+@pytest.mark.parametrize("lengths,keep,recent", [([4097, 8192, 30], 700, 20), ([8193, 16384], 3000, 1000),
+                                                 ([24576, 16385, 0, 12000], 9000, 1)])
+def test_evict_of_more_positions_a_thread(lengths, keep, recent, values):
+    _evict_case(lengths, 1, 1024, keep, recent, torch.float16, values, seed=keep)
+
+
+@pytest.mark.parametrize("high,low", [(1e6, 1e-6), (0.0, -math.inf), (math.nan, math.inf), (-1.0, -2.0), (1.5, 1.4999999)])
+@pytest.mark.parametrize("more", [0, 1, -1])
+def test_evict_where_a_digit_settles_it(high, low, more):
+    """As many positions of one weight as are picked, one more, or one fewer; all others of another."""
+    def values(gen, B, H, n):
+        w = torch.full((B, H, n), low, device=DEV)
+        w[..., 3:3 + 40 + more] = high
+        return w
+    _evict_case([300, 53, 51], 2, 16, 50, 10, torch.bfloat16, values)
+
+
 def test_evict_of_a_long_cache():
     """More positions than a workgroup keeps at once; equal weights, of which the lowest stay, among them."""
     from sisa_amd.kernels.paged import PagePool, sisa_cache_evict_hip
