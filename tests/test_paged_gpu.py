@@ -144,6 +144,13 @@ def test_decode_of_rows_taken_whole(lengths, H, S, M, dtype):
     test_decode(lengths, H, S, M, dtype)
 
 
+# more than 256 chunks a row. The positions whose F lies more than 40 away have weights below exp(-30) of the nearest ones'.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 2])
+def test_decode_of_many_chunks(M, dtype):
+    test_decode([70_000, 200, 65_537], 1, 1024, M, dtype)
+
+
 def test_decode_continues_the_contiguous_cache():
     """The same rows through sisa_decode_hip, whose cache is one tensor."""
     from sisa_amd.kernels.decode import sisa_decode_hip
