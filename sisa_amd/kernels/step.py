@@ -139,16 +139,17 @@ def layer_step_paged(x: Tensor, res: Tensor | None, weights: list[int], d_ff: in
     B, _, D = x.shape
     H = D // HIP_D_HEAD
     at = cache.begin_step(layer_idx)
-    h, ffn = torch.empty((2, B, 1, D), device=x.device, dtype=x.dtype).unbind(0)
-    tracked, dtype = at.weights is not None, _lib.dtype_code(x.dtype)
-    size = _lib.load().sisa_step_paged_workspace_bytes(B, H, D, d_ff, at.max_len, dtype, tracked)
-    ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
-    w = (at.weights.data_ptr(), *at.weights.stride()) if tracked else (0, 0, 0, 0)
-    _step_paged(x, B, H, D, d_ff, dtype, at.table.shape[1], at.max_len, 0, *eps, x.data_ptr(), x.stride(0),
-                0 if res is None else res.data_ptr(), *weights, lambda_raw.data_ptr(), at.pool.packed, at.table.data_ptr(),
-                at.table.stride(0), at.start.data_ptr(), at.end.data_ptr(), *(t.data_ptr() for t in at.last), *w,
-                h.data_ptr(), ffn.data_ptr(), ws.data_ptr())
-    cache.end_step(layer_idx)
+    with cache.writing(layer_idx):
+        h, ffn = torch.empty((2, B, 1, D), device=x.device, dtype=x.dtype).unbind(0)
+        tracked, dtype = at.weights is not None, _lib.dtype_code(x.dtype)
+        size = _lib.load().sisa_step_paged_workspace_bytes(B, H, D, d_ff, at.max_len, dtype, tracked)
+        ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
+        w = (at.weights.data_ptr(), *at.weights.stride()) if tracked else (0, 0, 0, 0)
+        _step_paged(x, B, H, D, d_ff, dtype, at.table.shape[1], at.max_len, 0, *eps, x.data_ptr(), x.stride(0),
+                    0 if res is None else res.data_ptr(), *weights, lambda_raw.data_ptr(), at.pool.packed, at.table.data_ptr(),
+                    at.table.stride(0), at.start.data_ptr(), at.end.data_ptr(), *(t.data_ptr() for t in at.last), *w,
+                    h.data_ptr(), ffn.data_ptr(), ws.data_ptr())
+        cache.end_step(layer_idx)
     return h, ffn
 
 
@@ -222,12 +223,13 @@ def prefill_paged(proj: Tensor, z: Tensor, lam: Tensor, n_head: int, cache, laye
     c, b = pp.state_views()
     fw = A.attn_forward(q, k, v, c, b, pp.g, lam, pp.f)
     count = cache.begin(layer_idx, k, b, True)
-    rates = proj[..., lay["TH"]:lay["TH"] + n_head * HIP_D_STATE // 2]
-    if count is not None:
-        real = torch.arange(L, device=proj.device) < count[:, None]
-        rates = torch.where(real[..., None], rates, 0.0)
-    phi = rates.sum(1, dtype=torch.float32).view(B, n_head, HIP_D_STATE // 2)
-    cache.put(layer_idx, (k, v, b, pp.g, pp.f), phi, count, True)
+    with cache.writing(layer_idx):
+        rates = proj[..., lay["TH"]:lay["TH"] + n_head * HIP_D_STATE // 2]
+        if count is not None:
+            real = torch.arange(L, device=proj.device) < count[:, None]
+            rates = torch.where(real[..., None], rates, 0.0)
+        phi = rates.sum(1, dtype=torch.float32).view(B, n_head, HIP_D_STATE // 2)
+        cache.put(layer_idx, (k, v, b, pp.g, pp.f), phi, count, True)
     if cache.tracked:
         cache.receive(layer_idx, q, k, c, b, pp.g, lam, pp.f, True)
     return fw.o.transpose(1, 2).flatten(2)

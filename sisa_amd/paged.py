@@ -158,6 +158,16 @@ class _Step(NamedTuple):
     max_len: int
 
 
+class _Begun(NamedTuple):
+    """A pass whose first layer is not written yet: its sequences, and what the store held for them before."""
+    lo: int
+    hi: int
+    pages: list[int]
+    starts: list[int]
+    lengths: list[int]
+    expected: list
+
+
 class _Layer:
     """One layer: its pages, the last position's recurrences, how many positions each sequence holds, and the accumulated
     weights ``(sequences, H, max_length)`` of a tracked cache."""
@@ -175,7 +185,9 @@ class _Store:
         self.free = list(range(pages - 1, -1, -1))
         self.held: list[list[int]] = [[] for _ in range(sequences)]
         self.starts, self.lengths = [0] * sequences, [0] * sequences   # before and after the last forward pass
+        self.widths = [0] * sequences                                  # that pass's positions, padding included
         self.expected: list[int | None] = [None] * sequences           # real positions of the next pass, if not all
+        self.begun: _Begun | None = None
         self.layers: dict[int, _Layer] = {}
         self.table = self.start = self.end = None          # on the model's device, made by the first pass
 
@@ -201,11 +213,40 @@ class _Store:
             self.held[n] += [self.free.pop() for _ in range(pages)]
         return [n for n, pages in enumerate(need, lo) if pages]
 
+    def undo(self) -> None:
+        """Take back the pass that has begun and written nothing: the cache is as it was before."""
+        was, self.begun = self.begun, None
+        if was is None:
+            return
+        lo, hi = was.lo, was.hi
+        for n in reversed(range(lo, hi)):
+            pages = was.pages[n - lo]
+            self.free += reversed(self.held[n][pages:])
+            del self.held[n][pages:]
+        self.starts[lo:hi], self.lengths[lo:hi], self.expected[lo:hi] = was.starts, was.lengths, was.expected
+        self.end[lo:hi].copy_(torch.tensor(was.lengths, dtype=torch.int32))
+        self.show(range(lo, hi))
+
     def show(self, sequences: Sequence[int]) -> None:
         """The device's table of these sequences, from the host's."""
         rows = [self.held[n] + [-1] * (self.table.shape[1] - len(self.held[n])) for n in sequences]
         lo, hi = sequences[0], sequences[-1] + 1
         self.table[lo:hi].copy_(torch.tensor(rows, dtype=torch.int32))
+
+
+class _Writing:
+    """Around what a layer does for a pass that has begun: an error in it takes the pass back, or marks the layer."""
+    __slots__ = ("cache", "layer_idx")
+
+    def __init__(self, cache: "SISAPagedCache", layer_idx: int) -> None:
+        self.cache, self.layer_idx = cache, layer_idx
+
+    def __enter__(self) -> None:
+        pass
+
+    def __exit__(self, kind, *_) -> None:
+        if kind is not None:
+            self.cache._failed(self.layer_idx)
 
 
 class SISAPagedCache:
@@ -215,7 +256,10 @@ class SISAPagedCache:
 
     The first pass of a sequence may be right-padded: ``cache.expect([5, 9])`` before it says how many of its positions are
     there. Later passes add the same number of positions to every sequence. ``cache[n]`` and ``cache[a:b]`` are the caches of
-    some of the sequences, sharing everything with the whole."""
+    some of the sequences, sharing everything with the whole.
+
+    A pass that is refused, or fails before its first layer is written, leaves the cache as it was. One that fails later has
+    reached some layers and not others: its sequences refuse further passes until they are released."""
 
     def __init__(self, sequences: int, max_length: int, *, pages: int | None = None, page_size: int = 64,
                  track: bool = False) -> None:
@@ -294,12 +338,29 @@ class SISAPagedCache:
                              "their own (cache[n])")
         return _Last(*(t[self._lo:self._hi] for t in layer.last))
 
+    def writing(self, layer_idx: int) -> _Writing:
+        """For a with statement around what a layer does between :meth:`begin` or :meth:`begin_step` and its end."""
+        return _Writing(self, layer_idx)
+
+    def _failed(self, layer_idx: int) -> None:
+        st = self._store
+        if st.begun is not None:
+            st.undo()
+        else:                                              # some layers have this pass's positions, this one may have
+            st.layers[layer_idx].filled[self._lo:self._hi] = [-1] * len(self)
+
     def _begin(self, layer: _Layer, M: int) -> None:
         """The positions of a pass of ``M``, at its first layer; the later ones find them there."""
         st, lo, hi = self._store, self._lo, self._hi
-        if layer.filled[lo:hi] != st.lengths[lo:hi]:
-            if layer.filled[lo:hi] != st.starts[lo:hi]:
-                raise RuntimeError("SISAPagedCache: an earlier forward pass did not reach every layer; release() the sequences")
+        st.undo()                                          # of a pass that was given up between two calls
+        first = layer.filled[lo:hi] == st.lengths[lo:hi]
+        if first:
+            whole = all(x.filled[lo:hi] == st.lengths[lo:hi] for x in st.layers.values())
+        else:
+            whole = layer.filled[lo:hi] == st.starts[lo:hi] and st.widths[lo:hi] == [M] * len(self)
+        if not whole:
+            raise RuntimeError("SISAPagedCache: an earlier forward pass did not reach every layer; release() the sequences")
+        if not first:
             return
         counts = [M if c is None else c for c in st.expected[lo:hi]]
         if max(counts) > M:
@@ -307,15 +368,21 @@ class SISAPagedCache:
         ends = [n + c for n, c in zip(self.lengths, counts)]
         if max(ends) > st.max_length:
             raise ValueError(f"SISAPagedCache: {max(ends)} positions exceed max_length = {st.max_length}")
-        fresh = st.take(lo, ends)
-        if fresh:
-            st.show(fresh if len(fresh) == 1 else range(lo, hi))
-        st.start[lo:hi].copy_(st.end[lo:hi])
-        if counts == [M] * len(self):
-            st.end[lo:hi].add_(M)
-        else:
-            st.end[lo:hi].copy_(torch.tensor(ends, dtype=torch.int32))
-        st.starts[lo:hi], st.lengths[lo:hi] = self.lengths, ends
+        st.begun = _Begun(lo, hi, [len(pages) for pages in st.held[lo:hi]], st.starts[lo:hi], st.lengths[lo:hi],
+                          st.expected[lo:hi])
+        try:
+            fresh = st.take(lo, ends)
+            if fresh:
+                st.show(fresh if len(fresh) == 1 else range(lo, hi))
+            st.start[lo:hi].copy_(st.end[lo:hi])
+            if counts == [M] * len(self):
+                st.end[lo:hi].add_(M)
+            else:
+                st.end[lo:hi].copy_(torch.tensor(ends, dtype=torch.int32))
+        except BaseException:
+            st.undo()
+            raise
+        st.starts[lo:hi], st.lengths[lo:hi], st.widths[lo:hi] = self.lengths, ends, [M] * len(self)
         st.expected[lo:hi] = [None] * len(self)
 
     def _layer(self, layer_idx: int, k: Tensor, b: Tensor, hip: bool) -> _Layer:
@@ -356,8 +423,9 @@ class SISAPagedCache:
             raise ValueError(f"SISAPagedCache: filled by the {'torch' if hip else 'HIP'} implementation, which cannot be changed "
                              f"while sequences are held; make a new cache")
         self._begin(layer, M)
-        padded = [n - m for n, m in zip(self.lengths, layer.filled[lo:hi])] != [M] * B
-        return st.end[lo:hi] - st.start[lo:hi] if padded else None
+        with self.writing(layer_idx):
+            padded = [n - m for n, m in zip(self.lengths, layer.filled[lo:hi])] != [M] * B
+            return st.end[lo:hi] - st.start[lo:hi] if padded else None
 
     def put(self, layer_idx: int, rows: Sequence[Tensor], phi: Tensor, count: Tensor | None, hip: bool) -> None:
         """The rows ``k, v, b, g, fgate`` of a pass that :meth:`begin` made room for, and the phase ``(B, H, d_state // 2)``
@@ -370,17 +438,21 @@ class SISAPagedCache:
             sisa_paged_write_hip(layer.pool, st.table[lo:hi], st.start[lo:hi], *rows, count)
         else:
             _write(layer.pool, st.table[lo:hi], st.start[lo:hi], st.end[lo:hi] - st.start[lo:hi], rows)
-        for t, x in zip(layer.last, (rows[3], rows[4])):
-            t[lo:hi].copy_(at_last(x, count))
-        layer.last.phi[lo:hi].copy_(phi)
-        layer.filled[lo:hi] = self.lengths
+        for t, x in zip(layer.last, (*(at_last(x, count) for x in (rows[3], rows[4])), phi)):
+            t[lo:hi].copy_(x)
+        self._written(layer)
+
+    def _written(self, layer: _Layer) -> None:
+        layer.filled[self._lo:self._hi] = self.lengths
+        self._store.begun = None
 
     def extend(self, layer_idx: int, p, hip: bool) -> None:
         """Write a pass's rows (``p``: :class:`sisa_amd.modeling.Prepared`) of one layer behind what its sequences hold."""
         if torch.is_grad_enabled() and (p.k.requires_grad or p.g.requires_grad):
             raise RuntimeError("SISAPagedCache is for inference: run the model under torch.no_grad()")
         count = self.begin(layer_idx, p.k, p.b, hip)
-        self.put(layer_idx, (p.k, p.v, p.b, p.g.float(), p.fgate.float()), at_last(p.phi, count)[:, :, 0], count, hip)
+        with self.writing(layer_idx):
+            self.put(layer_idx, (p.k, p.v, p.b, p.g.float(), p.fgate.float()), at_last(p.phi, count)[:, :, 0], count, hip)
 
     def attend(self, layer_idx: int, p, lam: Tensor, hip: bool) -> Tensor:
         """The attention of the rows that :meth:`extend` has just written, ``(B, H, M, d_head)`` float32 (float64 rows:
@@ -388,9 +460,11 @@ class SISAPagedCache:
         st, lo, hi = self._store, self._lo, self._hi
         layer = st.layers[layer_idx]
         weights = None if layer.weights is None else layer.weights[lo:hi]
-        if hip:
-            return self._attend_hip(p, lam, layer.pool, weights)
-        return paged_attention(p.q, p.c, p.g, p.fgate, lam, layer.pool, st.table[lo:hi], st.end[lo:hi], self.seq_len, weights)
+        with self.writing(layer_idx):
+            if hip:
+                return self._attend_hip(p, lam, layer.pool, weights)
+            return paged_attention(p.q, p.c, p.g, p.fgate, lam, layer.pool, st.table[lo:hi], st.end[lo:hi], self.seq_len,
+                                   weights)
 
     def _attend_hip(self, p, lam: Tensor, pool, weights: Tensor | None) -> Tensor:
         from .kernels.paged import sisa_paged_decode_hip
@@ -409,14 +483,15 @@ class SISAPagedCache:
                 hip: bool) -> None:
         """Track the weights of a first pass, in which the rows attended to each other."""
         st, lo, hi = self._store, self._lo, self._hi
-        if hip:
-            from .kernels.weights import sisa_attention_weights_hip
+        with self.writing(layer_idx):
+            if hip:
+                from .kernels.weights import sisa_attention_weights_hip
 
-            w = sisa_attention_weights_hip(q, k, c, b, g.float(), lam, fgate.float(), lengths=st.end[lo:hi])
-        else:
-            w = attention_weights(q, k, c, b, g, lam, fgate, st.end[lo:hi])
-        N = min(k.shape[2], st.max_length)                 # a padded batch may be wider than the cache
-        st.layers[layer_idx].weights[lo:hi, :, :N] = w[:, :, :N]
+                w = sisa_attention_weights_hip(q, k, c, b, g.float(), lam, fgate.float(), lengths=st.end[lo:hi])
+            else:
+                w = attention_weights(q, k, c, b, g, lam, fgate, st.end[lo:hi])
+            N = min(k.shape[2], st.max_length)             # a padded batch may be wider than the cache
+            st.layers[layer_idx].weights[lo:hi, :, :N] = w[:, :, :N]
 
     def empty(self, layer_idx: int) -> bool:
         """Whether no sequence holds a position in this layer."""
@@ -441,7 +516,7 @@ class SISAPagedCache:
                      None if layer.weights is None else layer.weights[lo:hi], self.seq_len)
 
     def end_step(self, layer_idx: int) -> None:
-        self._store.layers[layer_idx].filled[self._lo:self._hi] = self.lengths
+        self._written(self._store.layers[layer_idx])
 
     # -------------------------------------------------------------------------------------------- memory
     def reserve(self, positions: int) -> None:

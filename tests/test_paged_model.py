@@ -147,6 +147,85 @@ def test_what_is_expected_belongs_to_the_sequences():
         assert cache.lengths == [20] * 3
 
 
+def _failing(at):
+    """A function that raises at its ``at``-th call, and the calls so far."""
+    calls = []
+
+    def wrap(real):
+        def fn(*a, **kw):
+            calls.append(1)
+            if len(calls) == at:
+                raise MemoryError("no room")
+            return real(*a, **kw)
+        return fn
+    return wrap
+
+
+@pytest.mark.parametrize("track", [False, True])
+def test_a_pass_that_fails_before_it_is_written_is_taken_back(track, monkeypatch):
+    """A first and a later pass fail in the write of the first layer, for all sequences and for some; passes of other lengths
+    follow."""
+    from sisa_amd import paged
+    model = _model64()
+    ids, counts = token_ids(3, 40, seed=12), [9, 30, 17]
+    want = [_logits(model, ids[i:i + 1], SISACache(), n)[:, n - 1:] for i, n in enumerate(counts)]
+    cache = SISAPagedCache(3, 60, page_size=16, track=track)
+    cache[2].reserve(40)
+    free = cache.free_pages
+
+    def fails(part, x):
+        before = cache.lengths, cache.free_pages
+        with monkeypatch.context() as m:
+            m.setattr(paged, "_write", _failing(1)(paged._write))
+            with pytest.raises(MemoryError):
+                model(x, cache=part)
+        assert (cache.lengths, cache.free_pages) == before
+
+    with torch.no_grad():
+        cache.expect(counts)
+        fails(cache, ids[:, :34])
+        assert cache.free_pages == free and cache.lengths == [0, 0, 0]
+        got = [model(ids[:, :30], cache=cache, logits_at=[n - 1 for n in counts]).logits]      # what was expected still is
+        assert cache.lengths == counts
+        for i, n in enumerate(counts):                       # from here on each at its own positions
+            fails(cache[i], ids[i:i + 1, n:n + 5])
+            y = model(ids[i:i + 1, n:n + 3], cache=cache[i]).logits
+            assert rel_err(torch.cat([got[0][i:i + 1], y], 1), want[i][:, :4]) <= GATES
+        fails(cache, ids[:, 30:31])
+        fails(cache[0:2], ids[:2, 30:33])
+        y = torch.cat([model(ids[i:i + 1, n + 3:n + 4], cache=cache[i]).logits for i, n in enumerate(counts)])
+        assert rel_err(y, torch.cat([w[:, 4:5] for w in want])) <= GATES
+    assert cache.lengths == [n + 4 for n in counts]
+
+
+@pytest.mark.parametrize("n_layer,name,at", [(2, "_write", 2), (1, "paged_attention", 1), (2, "paged_attention", 1),
+                                             (2, "paged_attention", 2), (1, "attention_weights", 1), (2, "attention_weights", 1)])
+def test_a_pass_that_fails_later_ends_its_sequences(n_layer, name, at, monkeypatch):
+    """It has reached some layers: no pass and no eviction goes on from there, others do, and release() mends it."""
+    from sisa_amd import paged
+    model = _model64(n_layer=n_layer)
+    ids = token_ids(2, 40, seed=13)
+    want = _logits(model, ids, SISACache(), 20)
+    cache = SISAPagedCache(2, 60, page_size=16, track=True, pages=20)
+    with torch.no_grad():
+        model(ids[1:, :20], cache=cache[1])
+        if name != "attention_weights":
+            model(ids[:1, :20], cache=cache[0])
+        with monkeypatch.context() as m:
+            m.setattr(paged, name, _failing(at)(getattr(paged, name)))
+            with pytest.raises(MemoryError):
+                model(ids[:1, 20:21] if cache.lengths[0] else ids[:1, :20], cache=cache[0])
+        for x in (ids[:1, 20:21], ids[:1, 20:24], ids[:1, :20]):
+            with pytest.raises(RuntimeError, match="release"):
+                model(x, cache=cache[0])
+        with pytest.raises(RuntimeError):
+            cache.evict(8, 2)
+        assert rel_err(model(ids[1:, 20:21], cache=cache[1]).logits, want[1:, 20:21]) <= GATES
+        cache[0].release()
+        got = [model(ids[:1, :20], cache=cache[0]).logits, model(ids[:1, 20:21], cache=cache[0]).logits]
+        assert rel_err(torch.cat(got, 1), want[:1, :21]) <= GATES and cache.lengths == [21, 21]
+
+
 def _dense(model, x, layer, kept):
     """Attention of the last row of ``x`` (1, n, d), the layer's normalised input, over the rows ``kept[h]``."""
     at = model.layers[layer].attn
@@ -478,3 +557,36 @@ def test_many_new_positions_in_parts(track, monkeypatch):
     if track:
         for layer in range(2):
             assert rel_err(caches[0].weights(layer).cpu(), caches[1].weights(layer).double()) <= 2e-5
+
+
+@pytest.mark.gpu
+def test_a_step_or_prompt_that_fails_is_taken_back_on_the_gpu(monkeypatch):
+    """The first layer's step, and a prompt's write, raise before anything is launched; then the same pass again, and one of
+    another length."""
+    from sisa_amd.kernels import paged as K
+    from sisa_amd.kernels import step
+    model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).to(torch.bfloat16).eval()
+    ids, counts = token_ids(2, 30, seed=14).to(DEV), [20, 11]
+    outs = []
+    for failing in (False, True):
+        cache = SISAPagedCache(2, 40, page_size=16, track=True)
+        with torch.no_grad():
+            cache.expect(counts)
+            if failing:
+                with monkeypatch.context() as m:
+                    m.setattr(K, "sisa_paged_write_hip", _failing(1)(K.sisa_paged_write_hip))
+                    with pytest.raises(MemoryError):
+                        model(ids[:, :25], cache=cache)
+                assert cache.lengths == [0, 0]
+            got = [model(ids[:, :20], cache=cache, logits_at=[n - 1 for n in counts]).logits]
+            for t in range(20, 24):
+                if failing:
+                    with monkeypatch.context() as m:
+                        m.setattr(step, "_step_paged", _failing(1)(step._step_paged))
+                        with pytest.raises(MemoryError):
+                            model(ids[:, t:t + 1], cache=cache)
+                    assert cache.lengths == [n + t - 20 for n in counts]
+                got.append(model(ids[:, t:t + 1], cache=cache).logits)
+            got.append(model(ids[:, 24:27], cache=cache).logits)
+        outs.append(torch.cat(got, 1))
+    assert torch.equal(*outs)
