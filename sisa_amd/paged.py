@@ -570,19 +570,24 @@ class SISAPagedCache:
             raise RuntimeError(f"SISAPagedCache.evict: {each} free pages are needed for a sequence's kept rows, "
                                f"{len(st.free)} are there")
         new = [[st.free.pop() for _ in range(each)] for _ in range(lo, hi)]
-        new_table = torch.tensor(new, dtype=torch.int32).to(st.table.device)
-        table, lengths, max_len = st.table[lo:hi], st.end[lo:hi], max(st.lengths[lo:hi])
-        for layer in st.layers.values():
-            w = layer.weights[lo:hi]
-            if isinstance(layer.pool, _Pages):
-                _, kept = _evict(layer.pool, table, lengths, w, keep, recent, new_table, max_len)
-            else:
-                from .kernels.paged import sisa_cache_evict_hip
+        table, lengths, max_len, kept = st.table[lo:hi], st.end[lo:hi], max(st.lengths[lo:hi]), []
+        try:                                               # the old pages and weights stay until every layer has its new ones
+            new_table = torch.tensor(new, dtype=torch.int32).to(table.device)
+            for layer in st.layers.values():
+                w = layer.weights[lo:hi]
+                if isinstance(layer.pool, _Pages):
+                    kept.append(_evict(layer.pool, table, lengths, w, keep, recent, new_table, max_len)[1])
+                else:
+                    from .kernels.paged import sisa_cache_evict_hip
 
-                kept = sisa_cache_evict_hip(layer.pool, table, lengths, w, keep, recent, layer.pool, new_table,
-                                            max_len=max_len).weights
-            w[:, :, :keep] = kept
-            w[:, :, keep:max_len].zero_()
+                    kept.append(sisa_cache_evict_hip(layer.pool, table, lengths, w, keep, recent, layer.pool, new_table,
+                                                     max_len=max_len).weights)
+        except BaseException:
+            st.free += [page for pages in reversed(new) for page in reversed(pages)]
+            raise
+        for layer, w in zip(st.layers.values(), kept):
+            layer.weights[lo:hi, :, :keep] = w
+            layer.weights[lo:hi, :, keep:max_len].zero_()
             layer.filled[lo:hi] = [keep] * (hi - lo)
         for n, pages in zip(range(lo, hi), new):
             st.free += reversed(st.held[n])

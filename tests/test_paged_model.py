@@ -297,6 +297,33 @@ def test_evict_with_few_free_pages_goes_sequence_by_sequence():
                                                 _logits(model, ids[:1], SISACache(), 63)[:, 63:]) <= GATES
 
 
+@pytest.mark.parametrize("at", [1, 2])
+def test_an_eviction_that_fails_leaves_the_cache_as_it_was(at, monkeypatch):
+    """In the first and in the second layer; lengths, pages, weights and what follows are those of a cache it never touched."""
+    from sisa_amd import paged
+    model = _model64()
+    ids = token_ids(2, 60, seed=16)
+    caches = [SISAPagedCache(2, 64, page_size=16, pages=12, track=True) for _ in range(2)]
+    outs = []
+    for cache, failing in zip(caches, (False, True)):
+        with torch.no_grad():
+            model(ids[:, :50], cache=cache)
+            if failing:
+                weights = [cache.weights(layer).clone() for layer in range(2)]
+                with monkeypatch.context() as m:
+                    m.setattr(paged, "_evict", _failing(at)(paged._evict))
+                    with pytest.raises(MemoryError):
+                        cache.evict(20, 5)
+                assert cache.lengths == [50, 50] and cache.free_pages == 4
+                assert all(torch.equal(cache.weights(layer), weights[layer]) for layer in range(2))
+            got = [model(ids[:, 50:51], cache=cache).logits]
+            cache.evict(20, 5)
+            got += [model(ids[:, t:t + 1], cache=cache).logits for t in range(51, 60)]
+        assert cache.lengths == [29, 29] and cache.free_pages == 8
+        outs.append(torch.cat(got, 1))
+    assert torch.equal(*outs) and all(torch.equal(*(c.weights(layer) for c in caches)) for layer in range(2))
+
+
 def test_refusals():
     model = _model64()
     ids = token_ids(2, 20, seed=7)
