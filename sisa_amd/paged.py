@@ -251,8 +251,9 @@ class _Writing:
 
 class SISAPagedCache:
     """Decode cache of ``sequences`` sequences of at most ``max_length`` positions each, in ``pages`` pages (default: what all
-    of them can need) of ``page_size`` positions per layer, a power of two of at least 16. ``track``: accumulate every
-    position's softmax weight, for :meth:`evict`.
+    of them can need, and with ``track`` as many more as one of them, for the rows that an eviction keeps) of ``page_size``
+    positions per layer, a power of two of at least 16. ``track``: accumulate every position's softmax weight, for
+    :meth:`evict`.
 
     The first pass of a sequence may be right-padded: ``cache.expect([5, 9])`` before it says how many of its positions are
     there. Later passes add the same number of positions to every sequence. ``cache[n]`` and ``cache[a:b]`` are the caches of
@@ -270,7 +271,8 @@ class SISAPagedCache:
         each = -(-max_length // page_size)
         if pages is not None and pages < 1:
             raise ValueError(f"SISAPagedCache: pages = {pages} must be positive")
-        self._store = _Store(sequences, max_length, sequences * each if pages is None else pages, page_size, track)
+        self._store = _Store(sequences, max_length, (sequences + bool(track)) * each if pages is None else pages, page_size,
+                             track)
         self._lo, self._hi = 0, sequences
 
     # -------------------------------------------------------------------------------------------- parts

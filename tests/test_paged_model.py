@@ -297,6 +297,21 @@ def test_evict_with_few_free_pages_goes_sequence_by_sequence():
                                                 _logits(model, ids[:1], SISACache(), 63)[:, 63:]) <= GATES
 
 
+@pytest.mark.parametrize("sequences,max_length,keep", [(1, 50, 40), (1, 16, 15), (3, 50, 49)])
+def test_evict_at_the_limit_of_a_default_cache(sequences, max_length, keep):
+    """Sequences of max_length positions, in as many pages as the cache comes with."""
+    model = _model64()
+    ids = token_ids(sequences, max_length + 1, seed=17)
+    with torch.no_grad():
+        cache, roomy = (SISAPagedCache(sequences, max_length, page_size=16, track=True, **kw) for kw in ({}, dict(pages=40)))
+        for c in (cache, roomy):
+            model(ids[:, :max_length], cache=c)
+            c.evict(keep, keep // 2)
+        assert cache.lengths == [keep] * sequences
+        a, b = (model(ids[:, max_length:], cache=c).logits for c in (cache, roomy))
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("at", [1, 2])
 def test_an_eviction_that_fails_leaves_the_cache_as_it_was(at, monkeypatch):
     """In the first and in the second layer; lengths, pages, weights and what follows are those of a cache it never touched."""
