@@ -114,7 +114,8 @@ int sisa_cache_evict(const sisa_cache_evict_args* a, void* stream);
 /* sisa_step (sisa_hip_step.h) with its cache in pages: one new token of each of B rows through a decoder layer, sequence n's
  * at position start[n], lengths[n] = start[n] + 1. The recurrences continue from g_last, f_last and phi, which are advanced in
  * place. weights: accumulated weights as sisa_paged_decode's, in place, or NULL. A sequence whose position has no page of the
- * pool, or whose length sisa_paged_decode does not take, gives NaN. */
+ * pool, or whose lengths[n] is not start[n] + 1, gives NaN, its weights are left as they are, and its g_last and f_last become
+ * NaN: so do its later steps, until these are set anew. A length above max_len gives NaN. */
 typedef struct {
     int32_t B, H, D, FF;       /* rows 1..SISA_STEP_MAX_ROWS, heads, width (64 H), hidden width of the FFN */
     int32_t dtype;             /* SISA_BF16 or SISA_F16, of the pool, too */

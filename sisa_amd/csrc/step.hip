@@ -228,18 +228,26 @@ SISA_DEV Place place_of(const AppendArgs& a, int b, int h) {
 }
 
 struct PagedAppendArgs : AppendArgs {  // phi_in, phi_out: the same memory
-    const int32_t *table, *start;
+    const int32_t *table, *start, *lengths;
     int64_t s_table;
     int W, shift, pages;
     float *g_last, *f_last;            // (B, H), advanced
+    int32_t* length;                   // (B): the lengths that the attention takes, -1 where the position has no place
 };
 SISA_DEV Place place_of(const PagedAppendArgs& a, int b, int h) {
     const int64_t pos = a.start[b];
     const int page = page_of(a.table + b * a.s_table, a.W, a.shift, a.pages, pos);
-    return Place{page, pos & ((1 << a.shift) - 1), a.g_last + b * a.H + h, a.f_last + b * a.H + h, page >= 0};
+    return Place{page, pos & ((1 << a.shift) - 1), a.g_last + b * a.H + h, a.f_last + b * a.H + h,
+                 page >= 0 && a.lengths[b] == pos + 1};
 }
-SISA_DEV void keep_last(const AppendArgs&, int, float*, float) {}
-SISA_DEV void keep_last(const PagedAppendArgs&, int bh, float* last, float v) { last[bh] = v; }
+// A position that is not in the cache ends its sequence: NaN here makes every later score NaN, whatever start and lengths
+// become (both counted on from -1, the next call would find an empty sequence).
+SISA_DEV void keep_last(const AppendArgs&, const Place&, int, float*, float) {}
+SISA_DEV void keep_last(const PagedAppendArgs&, const Place& at, int bh, float* last, float v) {
+    last[bh] = at.there ? v : __builtin_nanf("");
+}
+SISA_DEV void keep_length(const AppendArgs&, const Place&, int) {}
+SISA_DEV void keep_length(const PagedAppendArgs& a, const Place& at, int b) { a.length[b] = at.there ? a.lengths[b] : -1; }
 SISA_DEV float* g_last(const AppendArgs&) { return nullptr; }
 SISA_DEV float* f_last(const AppendArgs&) { return nullptr; }
 SISA_DEV float* g_last(const PagedAppendArgs& a) { return a.g_last; }
@@ -278,17 +286,19 @@ __global__ __launch_bounds__(64) void step_append_kernel(Args a) {
         const float v = *at.g - (al > 20.f ? al : log1pf(expf(al)));
         if (at.there) g[0] = v;
         a.gq[bh] = v;
-        keep_last(a, bh, g_last(a), v);
+        keep_last(a, at, bh, g_last(a), v);
     } else if (lane == 33) {           // F = F_prev + logsigmoid(z)
         float* f = (float*)a.f.ptr + at.b * a.f.sb + h * a.f.sh + at.slot * a.f.sl;
         const float z = a.z[bh];
         const float v = *at.f + ((z < 0.f ? z : (z != z ? z : 0.f)) - log1pf(expf(-fabsf(z))));
         if (at.there) f[0] = v;
         a.fq[bh] = v;
-        keep_last(a, bh, f_last(a), v);
+        keep_last(a, at, bh, f_last(a), v);
     } else if (lane == 34 && b == 0) {
         const float r = a.lambda_raw[h];
         a.lam[h] = r > 20.f ? r : log1pf(expf(r));
+    } else if (lane == 35 && h == 0) {
+        keep_length(a, at, b);
     }
 }
 
@@ -373,6 +383,7 @@ __global__ __launch_bounds__(64 * NORM_NWV) void step_gate_kernel(GateArgs a) {
 struct Ws {
     char *proj, *act, *c, *y, *h0;
     float *alpha, *z, *gq, *fq, *lam, *attn;
+    int32_t* length;
     int64_t bytes;
 };
 
@@ -397,6 +408,7 @@ Ws workspace(char* base, int64_t B, int64_t H, int64_t D, int64_t FF, int64_t at
     w.fq = (float*)take(B * H * 4);
     w.lam = (float*)take(H * 4);
     w.attn = (float*)take(attn_bytes);
+    w.length = (int32_t*)take(B * 4);
     w.bytes = at;
     return w;
 }
@@ -537,6 +549,8 @@ int launch_step_paged(const sisa_step_paged_args* a, hipStream_t st) {
                                                   ws.gq, ws.fq, ws.lam, ws.c, H, 0};
         ap.table = a->table;
         ap.start = a->start;
+        ap.lengths = a->lengths;
+        ap.length = ws.length;
         ap.s_table = a->s_table;
         ap.W = a->W;
         ap.shift = sisa::log2_of(p.page_size);
@@ -554,7 +568,7 @@ int launch_step_paged(const sisa_step_paged_args* a, hipStream_t st) {
         d.pool = p;
         d.table = a->table;
         d.s_table = a->s_table;
-        d.lengths = a->lengths;
+        d.lengths = ws.length;
         d.q = sisa_view{ws.proj, (int64_t)272 * H, DH, DH};
         d.c = sisa_view{ws.c, (int64_t)H * DS, DS, DS};
         d.gq = sisa_view{ws.gq, H, 1, 1};

@@ -632,3 +632,41 @@ def test_a_step_or_prompt_that_fails_is_taken_back_on_the_gpu(monkeypatch):
             got.append(model(ids[:, 24:27], cache=cache).logits)
         outs.append(torch.cat(got, 1))
     assert torch.equal(*outs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_step_without_a_place_ends_its_sequence(dtype, monkeypatch):
+    """Device tables and lengths that name no place for the new position: NaN, and NaN from then on, also where start and
+    lengths are counted on to valid ones; the other sequences as beside sequences that are well."""
+    from sisa_amd.kernels import step
+    model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).to(dtype).eval()
+    ids = token_ids(6, 45, seed=18).to(DEV)
+    calls, real = [], step.layer_step_paged
+    monkeypatch.setattr(step, "layer_step_paged", lambda *a: calls.append(1) or real(*a))
+    outs, held = [], []
+    for lost in (False, True):
+        cache = SISAPagedCache(6, 64, page_size=16, track=True)
+        with torch.no_grad():
+            model(ids[:, :40], cache=cache)
+            before = [cache.weights(layer).clone() for layer in range(2)]
+            st, got = cache._store, []
+            if lost:                       # the answer of a failed eviction; a length far below; no page; a page outside
+                st.end[1], st.end[2] = -1, -1000
+                st.table[3, 2], st.table[4, 2] = -1, st.pages
+            for t in range(40, 45):
+                if lost and t == 41:       # a place again, as if the caller had counted on, and mended the tables
+                    assert st.end.tolist()[1] == 0
+                    st.end[2] = 41
+                    st.table[3, 2], st.table[4, 2] = st.held[3][2], st.held[4][2]
+                got.append(model(ids[:, t:t + 1], cache=cache).logits)
+                if lost and t == 40:
+                    for layer in range(2):
+                        assert torch.equal(cache.weights(layer)[1:5], before[layer][1:5])
+        outs.append(torch.cat(got, 1))
+        held.append([cache.weights(layer) for layer in range(2)])
+    assert len(calls) == 20 and outs[0].isfinite().all()
+    assert outs[1][1:5].isnan().all()
+    for i in (0, 5):
+        assert torch.equal(outs[0][i], outs[1][i])
+        assert all(torch.equal(a[i], b[i]) for a, b in zip(*held))
