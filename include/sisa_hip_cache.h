@@ -94,8 +94,10 @@ int sisa_attn_weights(const sisa_attn_weights_args* a, void* stream);
  * sequence and, of the others, those with the largest weights (of equal ones the lowest position; NaN is above all). The
  * positions that are kept, -1 behind them, and their weights, 0 behind them, are written beside. new_lengths[n] is
  * min(lengths[n], keep), or -1 where the length is negative or above max_len or W pages, where new_table has too few
- * pages, or where a page of the sequence is not in its pool (what the new pages then hold is of no use). No page may be
- * both read and written. */
+ * pages, or where the old or the new page of a row that is kept is not in its pool (what the new pages then hold is of no
+ * use). The pages of rows that are not kept are not looked at. -1 is an answer, not a length to count on from: a caller who
+ * adds the next positions to it has an empty sequence, so negative lengths have to stay as they are (sisa_paged_decode then
+ * gives NaN). No page may be both read and written. */
 typedef struct {
     int32_t B, W, W_new, max_len;
     int32_t keep, recent;      /* 1 <= recent <= keep */

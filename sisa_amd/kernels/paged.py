@@ -227,7 +227,7 @@ def sisa_paged_decode_hip(q: Tensor, c: Tensor, g_q: Tensor, f_q: Tensor | None,
 
 
 class Evicted(NamedTuple):
-    """Result of :func:`sisa_cache_evict_hip`: ``lengths`` ``(B,)`` int32, and per head the kept positions' ``weights``
+    """Result of :func:`sisa_cache_evict_hip`: ``lengths`` ``(B,)`` int32 (-1: it could not be done), and per head the kept positions' ``weights``
     ``(B, H, keep)`` float32 (0 behind the last) and the ``positions`` ``(B, H, keep)`` int32 they had (-1 behind)."""
     lengths: Tensor
     weights: Tensor
@@ -242,8 +242,9 @@ def sisa_cache_evict_hip(pool: PagePool, table: Tensor, lengths: Tensor, weights
     and dtype); no page may be both read and written. The old pages are left as they are.
 
     The score of a SISA key depends on its own ``g`` and ``F``, not on how many keys lie between, so what follows attends
-    exactly as a softmax over the kept keys. Lengths that are negative or above ``max_len``, too few new pages, and pages
-    outside their pool answer with a new length of -1, which :func:`sisa_paged_decode_hip` turns into NaN."""
+    exactly as a softmax over the kept keys. Lengths that are negative or above ``max_len``, too few new pages, and pages of
+    kept rows outside their pool answer with a new length of -1, which :func:`sisa_paged_decode_hip` turns into NaN. It is not
+    a length to count on from, -1 and a new position being an empty sequence: ``held = torch.where(n < 0, n, n + 1)``."""
     name = "sisa_cache_evict_hip"
     if weights.requires_grad and torch.is_grad_enabled():
         inference_only(name)

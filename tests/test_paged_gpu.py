@@ -462,6 +462,47 @@ def test_evict_marks_lengths_and_pages_outside_the_pool():
     assert short.lengths.tolist() == [-1, 16, 15, 0, -1, -1]                     # one new page holds 16
 
 
+def test_tokens_after_an_eviction_that_could_not_be_done():
+    """Negative lengths are kept as they are: NaN for every later token of their sequences, nothing in their pages."""
+    from sisa_amd.kernels.paged import PagePool, sisa_cache_evict_hip, sisa_paged_decode_hip, sisa_paged_write_hip
+    cache = Cache([90] * 5, 2, 16, torch.bfloat16, seed=14)
+    table, keep = cache.table.clone(), 30
+    table[1, 5] = -1                                         # the page of the last, recent positions
+    w = torch.rand(5, 2, 96, generator=cache.gen, device=DEV)
+    w[4, :, 16:32] = -1.0                                    # none of these stays: their page is not looked at
+    table[4, 1] = cache.pool.pages
+    to = PagePool.empty(20, 2, 16, torch.bfloat16, DEV)
+    for t in (to.k, to.v, to.b, to.g, to.fgate):
+        t.zero_()
+    new = torch.arange(20, device=DEV, dtype=torch.int32).view(5, 4)
+    new[2, 1] = 20
+    got = sisa_cache_evict_hip(cache.pool, table, _ints(90, 90, 90, 97, 90), w, keep, 10, to, new, max_len=96)
+    assert got.lengths.tolist() == [keep, -1, -1, -1, keep]
+    whole = sisa_cache_evict_hip(cache.pool, cache.table, _ints(90, 90, 90, 90, 90), w, keep, 10,
+                                 PagePool.empty(10, 2, 16, torch.bfloat16, DEV),
+                                 torch.arange(10, device=DEV, dtype=torch.int32).view(5, 2), max_len=96)
+    assert torch.equal(got.positions[4], whole.positions[4]) and torch.equal(got.weights[4], whole.weights[4])
+    held, kept = got.lengths, got.positions.long()
+    rows = {n: x.gather(2, kept.clamp(min=0)[..., None].expand(-1, -1, -1, x.shape[3]) if x.dim() == 4 else kept.clamp(min=0))
+            for n, x in cache.rows.items()}
+    pages = {n: x.clone() for n, x in (("k", to.k), ("g", to.g))}
+    for step in range(3):
+        q, c, g, f = cache.queries()
+        g, f = g - 1 - step, f - 1 - step
+        k, v, b = (torch.randn(5, 2, 1, wd, generator=cache.gen, device=DEV).to(torch.bfloat16) for wd in (64, 64, 32))
+        sisa_paged_write_hip(to, new, held, k, v, b, g, f)
+        held = torch.where(held < 0, held, held + 1)
+        out = sisa_paged_decode_hip(q, c, g, f, cache.lam, to, new, held, max_len=64)
+        rows = {n: torch.cat([rows[n], x], 2) for n, x in dict(k=k, v=v, b=b, g=g, f=f).items()}
+        assert out[1:4].isnan().all()
+        near = Cache.__new__(Cache)
+        near.__dict__.update(cache.__dict__, rows=rows, lengths=[keep + step + 1] * 5)
+        want, _ = near.decode64(q, c, g, f)
+        for i in (0, 4):
+            assert _rel(out[i], want[i]) <= TOL
+    assert torch.equal(to.k[4:16], pages["k"][4:16]) and torch.equal(to.g[4:16], pages["g"][4:16])
+
+
 # ------------------------------------------------------------------------------------------------ received weights
 def _weights64(q, k, c, b, g, lam, f, lengths, window):
     out = torch.zeros(g.shape, device=DEV, dtype=torch.float64)
