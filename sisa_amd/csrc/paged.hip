@@ -380,7 +380,10 @@ int launch_decode(const sisa_paged_decode_args* a, TO* out, hipStream_t st) {
 namespace sisa {
 namespace detail {
 // The attention of 16-bit operands with the result rounded to their dtype, (B,H,M,64) contiguous (checked by the caller:
-// sisa_step_paged).
+// sisa_step_paged), and whether its launches take one new position of each of `rows` sequences and heads.
+__attribute__((visibility("hidden"))) bool paged_attn_fits(int64_t rows, int64_t max_len, bool tracked) {
+    return fits(rows, 1, max_len, 2, tracked);
+}
 __attribute__((visibility("hidden"))) int paged_attn_out16(const sisa_paged_decode_args* a, void* out, hipStream_t st) {
     return a->pool.dtype == SISA_BF16 ? launch_decode<__bf16>(a, (__bf16*)out, st) : launch_decode<_Float16>(a, (_Float16*)out, st);
 }

@@ -23,6 +23,7 @@ namespace sisa {
 namespace detail {
 __attribute__((visibility("hidden"))) int decode_attn_out16(const sisa_decode_args* a, void* out, hipStream_t st);   // decode.hip
 __attribute__((visibility("hidden"))) int paged_attn_out16(const sisa_paged_decode_args* a, void* out, hipStream_t st);  // paged.hip
+__attribute__((visibility("hidden"))) bool paged_attn_fits(int64_t rows, int64_t max_len, bool tracked);
 }
 }  // namespace sisa
 
@@ -676,6 +677,8 @@ extern "C" int sisa_step_paged(const sisa_step_paged_args* a, void* stream) {
     SISA_REQUIRE(a->W >= 1 && a->max_len >= 1 && a->max_len <= (int64_t)a->W * a->pool.page_size && a->max_len <= (1 << 30),
                  "sisa_step_paged: max_len=%d (at most W=%d pages of %d, and 2^30)", a->max_len, a->W, a->pool.page_size);
     SISA_REQUIRE(a->table && a->start && a->lengths && a->g_last && a->f_last && a->phi, "sisa_step_paged: null pointer");
+    SISA_REQUIRE(sisa::detail::paged_attn_fits((int64_t)a->B * a->H, a->max_len, a->weights.ptr != nullptr),
+                 "sisa_step_paged: B*H*max_len too large for one launch");
     hipStream_t st = (hipStream_t)stream;
     return a->dtype == SISA_BF16 ? launch_step_paged<__bf16>(a, st) : launch_step_paged<_Float16>(a, st);
 }

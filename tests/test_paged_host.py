@@ -174,3 +174,15 @@ def test_entry_points_refuse_more_than_a_launch_takes(lib):
         _refused(lib, "sisa_attn_weights", args, "too large")
     args = _lib.CacheEvictArgs(1 << 21, 1, 1, 16, 4, 2, _pool(lib), _pool(lib), 4096, 1, 4096, 1, 4096, gate, 4096, 4096, 4096)
     _refused(lib, "sisa_cache_evict", args, "2^22")
+
+
+@pytest.mark.parametrize("tracked", [False, True])
+@pytest.mark.parametrize("max_len", [1 << 22, 1 << 24, 1 << 30])
+def test_step_refuses_more_than_a_launch_takes(lib, max_len, tracked):
+    """Chunks of 256 positions of 64 rows of 16 heads: 2^32 threads and more."""
+    from sisa_amd.kernels import _lib
+    weights = _lib.View(4096, 1 << 30, 1 << 30, 1) if tracked else _lib.View(None, 0, 0, 0)
+    args = _lib.StepPagedArgs(64, 16, 1024, 256, _lib.BF16, max_len // 16, max_len, 0, 1e-6, 1e-6, 4096, 1024, None, 4096,
+                              *[4096] * 16, _pool(lib, heads=16), 4096, 1, 4096, 4096, 4096, 4096, 4096, weights, 4096, 4096,
+                              4096)
+    _refused(lib, "sisa_step_paged", args, "too large")
