@@ -186,3 +186,22 @@ def test_step_refuses_more_than_a_launch_takes(lib, max_len, tracked):
                               *[4096] * 16, _pool(lib, heads=16), 4096, 1, 4096, 4096, 4096, 4096, 4096, weights, 4096, 4096,
                               4096)
     _refused(lib, "sisa_step_paged", args, "too large")
+
+
+def test_both_steps_refuse_the_same(lib):
+    """What sisa_step and sisa_step_paged share is checked once; 64 H that passes 32 bits is no D."""
+    from sisa_amd.kernels import _lib
+    weights = {n: 4096 for n, t in _lib.StepPagedArgs._fields_ if t is ctypes.c_void_p and n != "res"}
+    pool = {n: _lib.View(4096, 1024, 64, 64) for n in ("k", "v", "b")} | {n: _lib.View(4096, 32, 16, 1) for n in ("g", "f")}
+    common = dict(B=1, H=2, D=128, FF=256, dtype=_lib.BF16, eps_attn=1e-6, eps_ffn=1e-6, sx=128)
+    for bad, word in ((dict(B=0), "B must be"), (dict(B=65), "B must be"), (dict(H=(1 << 26) + 2), "D = 64 H"),
+                      (dict(D=64), "D = 64 H"), (dict(H=17, D=1088, sx=1088), "D = 64 H"), (dict(FF=0), "FF positive"),
+                      (dict(dtype=_lib.F32), "bf16 or fp16"), (dict(w_gate=None), "given"), (dict(h=4104), "aligned"),
+                      (dict(w_down=4100), "w_down"), (dict(sx=120), "x rows"), (dict(res=4104), "x rows"),
+                      (dict(b_alpha=None), "null"), (dict(workspace=4112), "256-byte")):
+        given = common | weights | bad
+        names = {n for n, _ in _lib.StepArgs._fields_}
+        step = _lib.StepArgs(**{n: v for n, v in given.items() if n in names}, pos=3, phi_in=4096, phi_out=4096, **pool)
+        _refused(lib, "sisa_step", step, word)
+        paged = _lib.StepPagedArgs(**given, W=1, max_len=16, pool=_pool(lib))
+        _refused(lib, "sisa_step_paged", paged, word)
