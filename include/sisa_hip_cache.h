@@ -70,7 +70,8 @@ int sisa_paged_decode(const sisa_paged_decode_args* a, void* stream);
 
 /* The softmax weights that each position j of a prompt receives from the last `window` queries of its sequence (0: from
  * all of them), summed:  out_j = sum over i >= j, n - window <= i < n, of softmax_j(s_ij), with the score of sisa_attn_fwd
- * and n = lengths[b] (NULL: L; values outside 0 .. L count as the nearer of the two); 0 for j >= n. Workspace:
+ * and n = lengths[b] (NULL: L; values outside 0 .. L count as the nearer of the two); 0 for j >= n. g and f may rise, where a
+ * rise of more than 16 costs time. Workspace:
  * sisa_attn_weights_workspace_bytes(B, H, L, window). */
 #define SISA_ATTN_WEIGHTS_MAX_STRIDE (1 << 24)    /* of the positions of q, k, c and b, in elements */
 typedef struct {

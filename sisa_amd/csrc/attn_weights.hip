@@ -13,9 +13,11 @@
 // Bound by the vector unit: the products of a block take 48 cycles of the matrix pipe, its 256 scores' exponentials alone
 // 32 of issue. So blocks away from the diagonal factor the decay, exp(g_i - g_j) = exp(g_i - g_a) exp(g_a - g_j), and split
 // the forget term, (F_i - F_a) + (F_a - F_j), at an anchor a between the two: the wave's first query in the first pass,
-// its last key in the second. Both factors are at most 1 and both terms at most 0 there, so nothing overflows and rounding
-// grows with the differences of F, not with F. That leaves a product, two FMAs and one exponential for a score. Blocks
-// that meet the diagonal or the end of the sequence take the formula as it stands.
+// its last key in the second. Where g and F do not rise, both factors are at most 1 and both terms at most 0, so nothing
+// overflows and rounding grows with the differences of F, not with F. That leaves a product, two FMAs and one exponential for
+// a score. Blocks that meet the diagonal or the end of the sequence take the formula as it stands; so does every block of a
+// wave whose anchor is not finite, or on whose wrong side a g or F lies by more than RISE: the wave looks its gates through
+// first.
 #include "common.h"
 #include "host.h"
 #include "sisa_hip_cache.h"
@@ -26,6 +28,7 @@ constexpr int DH = 64, DS = 32;
 constexpr int FEW_ROWS = 256;         // query rows up to which, against four times as many keys, each wave has its own keys
 constexpr int MAX_SPLITS = 32;        // of the keys in the first pass
 constexpr float SCALE = LOG2E / 8;    // of q.k into log2 units
+constexpr float RISE = 16.f;          // e^16 at most in a factor: what the other one loses below 2^-126 is less than e^-71
 
 struct Rows {                         // queries of a sequence: first .. first + count - 1
     int n, first, count;
@@ -145,6 +148,32 @@ SISA_DEV Tile<T> turn(const Raw<T>& r, Buffer<T>* buf, int lane) {
                    lds4f(buf->gates + 32 + 4 * grp)};
 }
 
+// Whether a wave's anchor (ga, fa) serves it. `off`: it does not for the lane's own gates. SIGN 1: the gates of the keys in
+// `tiles` tiles from position `first` on, `step` positions from one to the next, must not lie below the anchor's; -1: those of
+// queries not above. NaN needs no care, every score that meets it is NaN in either form. Each quarter of the wave looks at E
+// tiles at a time. It costs 2 % of 4 x 2,048 positions of 12 heads and 3 % of the last 64 of 16,384 (76.6 -> 78.4 and 33.6 ->
+// 34.7 us); watching the gates that the loops load anyway, whose registers then spill, 22 % of both.
+template <int SIGN, bool FORGET, int E>
+SISA_DEV bool anchored(const sisa_attn_weights_args& a, int b, int h, float ga, float fa, bool off, int first, int tiles, int step,
+                       int lane) {
+    const float* g = (const float*)a.g.ptr + b * a.g.sb + h * a.g.sh;
+    const float* f = (const float*)a.f.ptr + b * a.f.sb + h * a.f.sh;
+    float w = 0.f;
+    for (int k = lane >> 4; k < tiles; k += 4 * E) {
+        float x[E], y[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {                  // behind the last tile the last again; positions are below 2^30
+            const unsigned at = first + step * (k + 4 * e < tiles ? k + 4 * e : tiles - 1) + (lane & 15);
+            x[e] = *(const float*)((const char*)g + 4 * at);
+            y[e] = FORGET ? *(const float*)((const char*)f + 4 * at) : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) w = fmaxf(w, fmaxf(SIGN * (ga - x[e]), FORGET ? SIGN * (fa - y[e]) : 0.f));
+    }
+    const float inf = __builtin_inff();
+    return !__any(off || w > RISE || !(fabsf(ga) < inf && (!FORGET || fabsf(fa) < inf)));
+}
+
 SISA_DEV float gate(const sisa_view& v, int b, int h, int r, int L) {
     return v.ptr ? ((const float*)v.ptr)[b * v.sb + h * v.sh + (r < L ? r : L - 1)] : 0.f;
 }
@@ -183,16 +212,6 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
     const int i0 = rows.first + r0;
     const float lam = a.lam[h * a.s_lam];
     Buffer<T>* buf = bufs + w;
-    Stream<T> keys(a.k, a.b, a, b, h, nullptr, lane);
-    Frags<T> q[U];
-    {
-        const Stream<T> own(a.q, a.c, a, b, h, nullptr, lane);
-        Raw<T> raw[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = own.load_edge(i0 + 16 * u, L);
-#pragma unroll
-        for (int u = 0; u < U; ++u) q[u] = turn<T, FORGET>(raw[u], buf, lane).x;
-    }
     float gi[U], fi[U], md[U], ld[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -203,11 +222,34 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
     }
     const int last = i0 + OWN < rows.n ? i0 + OWN : rows.n;          // keys 0 .. last - 1
     const int tiles = (last + 15) / 16;
-    // split s takes a contiguous range of the tiles, wave w every fourth; tiles up to `below` lie at or before i0
+    // split s takes a contiguous range of the tiles, wave w every NW-th; tiles up to `below` lie at or before i0
     const int per = (tiles + nsplit - 1) / nsplit;
     const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
     const int below = (i0 + 1) / 16 < t1 ? (i0 + 1) / 16 : t1;
-    for (int t = (below > t0 ? below : t0) + w; t < t1; t += NW) {   // meeting the diagonal
+    int far = 0;                                                     // whole tiles that the wave takes as those on the diagonal
+    Stream<T> keys(a.k, a.b, a, b, h, nullptr, lane);
+    Frags<T> q[U];
+    {
+        const Stream<T> own(a.q, a.c, a, b, h, nullptr, lane);
+        Raw<T> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = own.load_edge(i0 + 16 * u, L);
+        if (below - 1 - w >= t0) {
+            const float ga = gate(a.g, b, h, i0, L), fa = gate(a.f, b, h, i0, L);
+            bool off = false;
+#pragma unroll
+            for (int u = 0; u < U; ++u) off |= i0 + 16 * u + col < rows.n && (gi[u] - ga > RISE || fi[u] - fa > RISE);
+            const int whole = (below - 1 - t0 - w) / NW + 1;
+            // (eight waves with 64 rows: the keys are split, a wave has few tiles)
+            if (!anchored<1, FORGET, U == 4 && NW == 8 ? 2 : 8>(a, b, h, ga, fa, off, 16 * (below - 1 - w), whole, -16 * NW, lane))
+                far = whole;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = turn<T, FORGET>(raw[u], buf, lane).x;
+    }
+    for (int n = -far;; ++n) {                                       // meeting the diagonal
+        const int t = n < 0 ? below - 1 - w + NW * (n + 1) : (below > t0 ? below : t0) + w + NW * n;
+        if (t >= t1) break;
         const Tile<T> k = turn<T, FORGET>(keys.load_edge(16 * t, L), buf, lane);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -229,7 +271,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_lse_k
         }
     }
     int left = (below - 1 - t0 - w) / NW + 1;                        // whole tiles of this wave, from the diagonal down
-    if (below - 1 - w >= t0) {
+    if (far == 0 && below - 1 - w >= t0) {
         const float ga = gate(a.g, b, h, i0, L), fa = gate(a.f, b, h, i0, L);
         // y = 8 score - 8 (F_i - F_a); sums of 2^(y SCALE - ref), the maximum so far in mo
         float qg[U], mo[U], ref[U], lo[U];
@@ -392,9 +434,20 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
         int w0 = clear > 0 ? (clear + 15) / 16 : 0, w1 = rows.count / 16;
         w0 = w0 < from ? from : w0 < tiles ? w0 : tiles;
         w1 = w1 < w0 ? w0 : w1;
+        int left = w0 + ws < w1 ? (w1 - 1 - w0 - ws) / SHARE + 1 : 0;
+        int far = 0;                                                 // whole tiles that the wave takes as those on the edges
+        const float ga = gate(a.g, b, h, j0 + OWN - 1, L), fa = gate(a.f, b, h, j0 + OWN - 1, L);
+        if (left > 0) {
+            bool off = false;
+#pragma unroll
+            for (int u = 0; u < U; ++u) off |= ga - gj[u] > RISE || fa - fj[u] > RISE;
+            if (!anchored<-1, FORGET, FEW ? 2 : 8>(a, b, h, ga, fa, off, rows.first + 16 * (w0 + ws), left, 16 * SHARE, lane))
+                far = left, left = 0;
+        }
         const int edges = w0 - from + tiles - w1;
-        for (int e0 = ws; e0 < edges; e0 += SHARE) {
-            const int t = e0 < w0 - from ? from + e0 : w1 + e0 - (w0 - from), i0 = rows.first + 16 * t;
+        for (int e0 = ws - SHARE * far; e0 < edges; e0 += SHARE) {
+            const int t = e0 < 0 ? w0 + e0 + SHARE * far : e0 < w0 - from ? from + e0 : w1 + e0 - (w0 - from);
+            const int i0 = rows.first + 16 * t;
             Tile<T> q = turn<T, FORGET>(queries.load_edge(i0, L, 16 * t), buf, lane);
             if constexpr (FEW) q.st = lds4f(starts + 16 * t + 4 * grp);
 #pragma unroll
@@ -411,9 +464,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
                 }
             }
         }
-        int left = w0 + ws < w1 ? (w1 - 1 - w0 - ws) / SHARE + 1 : 0;
         if (left > 0) {
-            const float ga = gate(a.g, b, h, j0 + OWN - 1, L), fa = gate(a.f, b, h, j0 + OWN - 1, L);
             float kg[U], kf[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {

@@ -39,7 +39,8 @@ def sisa_attention_weights_hip(q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Te
     ``(H,)`` float32, as :func:`sisa_amd.kernels.attention.sisa_attention_hip` takes them. ``lengths`` ``(B,)`` int32: the
     positions of each sequence of a right-padded batch (default ``L``; values outside ``0 .. L`` count as the nearer of the
     two); what lies behind is not looked at and receives 0. Returns ``(B, H, L)`` float32. The scores are formed twice and
-    never stored."""
+    never stored. Gates that rise along the sequence are taken as they are (and more slowly where they rise by more than
+    16), not refused."""
     name = "sisa_attention_weights_hip"
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or c.requires_grad or b.requires_grad or g.requires_grad
                                     or lam.requires_grad or (fgate is not None and fgate.requires_grad)):

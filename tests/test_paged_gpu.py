@@ -576,6 +576,53 @@ def test_received_weights_with_steep_gates():
         assert _rel(got, _weights64(*x, g, lam, f, [L], None)) <= TOL
 
 
+# Gates that rise again, by more than a factor of the kernels' may hold. The scores' own decays stay moderate: where keys lie
+# below a query's g by `dip`, lam is e^-dip; F differences stay below 40, as the tolerance has them. A few heads (16 queries a
+# block), many, a window (its queries lie below every key, whose blocks rise and fall among themselves by more than 88).
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,L,window", [(1, 3, 300, None), (2, 24, 210, None), (2, 30, 700, None), (2, 3, 700, 64),
+                                          (1, 2, 1100, 300)])
+def test_received_weights_with_rising_gates(B, H, L, window, dtype):
+    from sisa_amd.kernels.weights import sisa_attention_weights_hip
+    gen = _gen(L + H)
+    rows = lambda w: torch.randn(B, L, H, w, generator=gen, device=DEV).to(dtype).transpose(1, 2)  # noqa: E731
+    x = [rows(64), rows(64), rows(32), rows(32)]
+    lengths = [L, 150][:B]
+    at = torch.arange(L, device=DEV)
+    for dip, f_dip in ((0.0, 30.0), (30.0, 0.0), (40.0, 30.0), (110.0, 0.0)):
+        if dip > 88 and window is None:
+            continue
+        lam = torch.rand(H, generator=gen, device=DEV) * math.exp(-min(dip, 40.0) if window is None else 0.0)
+        g, f = _gates(gen, B, H, L), _gates(gen, B, H, L)
+        for n, i in zip(lengths, range(B)):
+            low = ((at // 37) % 2 == 1) & (at < n - (window or 0))           # by turns, across every block's edges
+            g[i, :, low] -= dip
+            f[i, :, low] -= f_dip
+            if window is not None:                                           # the queries that count lie below all keys
+                g[i, :, max(0, n - window):] -= dip + 10
+                f[i, :, max(0, n - window):] -= f_dip
+        got = sisa_attention_weights_hip(*x, g, lam, f, lengths=_ints(*lengths), window=window)
+        assert _rel(got, _weights64(*x, g, lam, f, lengths, window)) <= TOL, (dip, f_dip)
+        if dip:
+            got = sisa_attention_weights_hip(*x, g, lam, lengths=_ints(*lengths), window=window)
+            assert _rel(got, _weights64(*x, g, lam, None, lengths, window)) <= TOL, (dip, f_dip)
+
+
+@pytest.mark.parametrize("window", [40, 300])
+@pytest.mark.parametrize("j", [63, 64, 127, 15, 16, 200])
+def test_received_weights_of_keys_that_are_forgotten(j, window):
+    """F or g of +inf at a key that no counted query is: it receives 0, the others what they would without it."""
+    from sisa_amd.kernels.weights import sisa_attention_weights_hip
+    gen, L, H = _gen(j), 700, 2
+    rows = lambda w: torch.randn(1, H, L, w, generator=gen, device=DEV)  # noqa: E731
+    x = [rows(64), rows(64), rows(32), rows(32)]
+    g, f, lam = _gates(gen, 1, H, L), _gates(gen, 1, H, L), torch.rand(H, generator=gen, device=DEV) + 0.1
+    f[0, 0, j] = g[0, 1, j] = math.inf
+    got = sisa_attention_weights_hip(*x, g, lam, f, window=window)
+    assert got.isfinite().all() and got[0, 0, j] == 0
+    assert _rel(got, _weights64(*x, g, lam, f, [L], window)) <= TOL
+
+
 def test_received_weights_of_other_layouts():
     """Positions far apart in memory, gates that are not neighbours, expanded ones, rows that begin off 16 bytes: copied."""
     from sisa_amd.kernels.weights import sisa_attention_weights_hip
