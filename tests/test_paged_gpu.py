@@ -151,6 +151,35 @@ def test_decode_of_many_chunks(M, dtype):
     test_decode([70_000, 200, 65_537], 1, 1024, M, dtype)
 
 
+@pytest.mark.parametrize("dtype,N", [(torch.bfloat16, 54560), (torch.bfloat16, 54561), (torch.float16, 60000), (torch.float32, 27700)])
+def test_decode_at_the_streaming_line(dtype, N):
+    """Caches just below and above 256 MiB (15 heads: 4,920 or 9,720 bytes a position) give each head what a pool of that head
+    alone, far below it, gives: the loads' cache policy is all that changes."""
+    from sisa_amd.kernels.paged import PagePool, sisa_paged_decode_hip
+    gen, H, S = _gen(N), 15, 64
+    W = -(-N // S)
+    new = lambda *w: torch.randn(W, H, S, *w, generator=gen, device=DEV)  # noqa: E731
+    k, v, b = new(64).to(dtype), new(64).to(dtype), new(32).to(dtype)
+    table = torch.randperm(W, generator=gen, device=DEV)[None].to(torch.int32)
+    g, f = (torch.empty(W, H, S, device=DEV) for _ in range(2))
+    for t in (g, f):
+        t[table[0].long()] = (0.02 * _gates(gen, 1, H, W * S)).view(H, W, S).transpose(0, 1)
+    q, c, lam = new(64)[:1, :, :1].to(dtype), new(32)[:1, :, :1].to(dtype), torch.rand(H, generator=gen, device=DEV)
+    page, slot = int(table[0, (N - 1) // S]), (N - 1) % S
+    gq, fq = (t[page, :, slot].reshape(1, H, 1).clone() for t in (g, f))
+    old, w = torch.rand(1, H, N, generator=gen, device=DEV), torch.zeros(1, H, N, device=DEV)
+    out = sisa_paged_decode_hip(q, c, gq, fq, lam, PagePool(k, v, b, g, f), table, _ints(N), max_len=N, weights=old, weights_out=w)
+    assert torch.equal(out, sisa_paged_decode_hip(q, c, gq, fq, lam, PagePool(k, v, b, g, f), table, _ints(N), max_len=N))
+    one = torch.zeros(1, 1, N, device=DEV)
+    for h in (0, 7, 14):
+        s = slice(h, h + 1)
+        pool = PagePool(*(t[:, s] for t in (k, v, b, g, f)))
+        alone = sisa_paged_decode_hip(q[:, s], c[:, s], gq[:, s], fq[:, s], lam[s], pool, table, _ints(N), max_len=N,
+                                      weights=old[:, s], weights_out=one)
+        assert torch.equal(out[:, s], alone) and torch.equal(w[:, s], one)
+    assert (w >= old).all() and (w > old).any(-1).all()
+
+
 def test_decode_continues_the_contiguous_cache():
     """The same rows through sisa_decode_hip, whose cache is one tensor."""
     from sisa_amd.kernels.decode import sisa_decode_hip
@@ -320,6 +349,29 @@ def test_write(starts, counts, H, S, M, dtype):
         assert torch.equal(x.nan_to_num(9.0), cache.t[name].nan_to_num(9.0)), name
 
 
+# 64 rows a wave: 134,400 rows, with waves that begin within a head, and 422,400, which are 256 MB and more read and written
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,M,S", [(3, 16, 2800, 64), (4, 16, 6600, 16)])
+def test_write_of_many_rows(B, H, M, S, dtype):
+    from sisa_amd.kernels.paged import PagePool, sisa_paged_write_hip
+    gen, starts, counts = _gen(M), [(37 * n) % 100 for n in range(B)], [M, M - 1, 1, M // 2 + 3][:B]
+    W = -(-(M + 100) // S)
+    pool = PagePool.empty(B * W + 5, H, S, dtype, DEV)
+    held = dict(k=pool.k, v=pool.v, b=pool.b, g=pool.g, f=pool.fgate)
+    for t in held.values():
+        t.fill_(7)
+    table = torch.randperm(pool.pages, generator=gen, device=DEV)[:B * W].view(B, W).to(torch.int32)
+    new = lambda *w: torch.randn(B, M, H, *w, generator=gen, device=DEV).transpose(1, 2)  # noqa: E731
+    rows = dict(k=new(64).to(dtype), v=new(64).to(dtype), b=new(32).to(dtype), g=new(), f=new())
+    want = {n: x.clone() for n, x in held.items()}
+    for i in range(B):
+        pos = starts[i] + torch.arange(counts[i], device=DEV)
+        for n, x in rows.items():
+            want[n][table[i].long()[pos // S], :, pos % S] = x[i, :, :counts[i]].transpose(0, 1)
+    sisa_paged_write_hip(pool, table, _ints(*starts), *rows.values(), _ints(*counts))
+    assert all(torch.equal(want[n], held[n]) for n in held)
+
+
 def test_write_leaves_out_what_has_no_page():
     """Rows before position 0, past the table and on pages outside the pool, and counts above M or below 0."""
     from sisa_amd.kernels.paged import sisa_paged_write_hip
@@ -426,6 +478,42 @@ def test_evict_where_a_digit_settles_it(high, low, more):
         w[..., 3:3 + 40 + more] = high
         return w
     _evict_case([300, 53, 51], 2, 16, 50, 10, torch.bfloat16, values)
+
+
+# 64 rows a wave: 134,400 kept rows, out of caches below and above 256 MB
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,S,S_new", [(4000, 64, 16), (17500, 128, 128)])
+def test_evict_of_many_rows(n, S, S_new, dtype):
+    from sisa_amd.kernels.paged import PagePool, sisa_cache_evict_hip
+    B, H, keep, recent, gen = 4, 12, 2800, 333, _gen(n)
+    lengths = [n, n - 1, keep - 5, n // 2 + 1000]
+    W, W_new = -(-n // S), -(-keep // S_new)
+    pool, to = PagePool.empty(B * W, H, S, dtype, DEV), PagePool.empty(B * W_new + 3, H, S_new, dtype, DEV)
+    old, new = (dict(k=p.k, v=p.v, b=p.b, g=p.g, f=p.fgate) for p in (pool, to))
+    for t in old.values():
+        t.copy_(torch.randn(t.shape, generator=gen, device=DEV, dtype=torch.float32))
+    for t in new.values():
+        t.fill_(7)
+    table = torch.randperm(pool.pages, generator=gen, device=DEV).view(B, W).to(torch.int32)
+    new_table = torch.randperm(to.pages, generator=gen, device=DEV)[:B * W_new].view(B, W_new).to(torch.int32)
+    w = _heavy(gen, B, H, n)
+    want, i = {x: t.clone() for x, t in new.items()}, torch.arange(keep, device=DEV)
+    got = sisa_cache_evict_hip(pool, table, _ints(*lengths), w, keep, recent, to, new_table, max_len=n)
+    assert got.lengths.tolist() == [min(m, keep) for m in lengths]
+    for m in range(B):
+        N, K = lengths[m], min(lengths[m], keep)
+        if N <= keep:
+            stay = i[:K].expand(H, K)
+        else:
+            order = w[m, :, :N - recent].sort(descending=True, stable=True).indices[:, :keep - recent]
+            stay = torch.cat([order.sort().values, torch.arange(N - recent, N, device=DEV).expand(H, recent)], 1)
+        assert torch.equal(got.positions[m, :, :K].long(), stay) and got.positions[m, :, K:].eq(-1).all()
+        assert torch.equal(got.weights[m, :, :K], w[m].gather(1, stay)) and got.weights[m, :, K:].eq(0).all()
+        h = torch.arange(H, device=DEV)[:, None].expand_as(stay)
+        for x in want:
+            want[x][new_table[m].long()[i[:K] // S_new].expand(H, K), h, (i[:K] % S_new).expand(H, K)] = \
+                old[x][table[m].long()[stay // S], h, stay % S]
+    assert all(torch.equal(want[x], new[x]) for x in new)
 
 
 def test_evict_of_a_long_cache():
@@ -558,6 +646,16 @@ def test_received_weights(lengths, L, H, window, dtype):
                                                 ([129, 97, 128, 32, 1, 79], 129, 20, None), ([400, 127], 400, 24, None),
                                                 ([130, 33, 31, 130, 7, 96, 64, 65], 130, 30, None)])
 def test_received_weights_of_many_heads(lengths, L, H, window, dtype):
+    test_received_weights(lengths, L, H, window, dtype)
+
+
+# windows whose first pass is split into 11, 32 and (256 blocks of 64 rows) no parts; and on either side of 256, where the
+# keys are no longer split
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,L,H,window", [([2600, 50], 2600, 2, 17), ([9000], 9000, 1, 64), ([8200, 3, 4100], 8200, 2, 65),
+                                                ([450, 449, 99, 300, 0, 1, 101, 400], 450, 16, 100), ([4000], 4000, 2, 256),
+                                                ([4000, 700], 4000, 2, 257), ([4001], 4001, 4, 1000)])
+def test_received_weights_of_windows_of_long_prompts(lengths, L, H, window, dtype):
     test_received_weights(lengths, L, H, window, dtype)
 
 
