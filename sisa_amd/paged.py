@@ -323,6 +323,7 @@ class SISAPagedCache:
     # -------------------------------------------------------------------------------------------- a forward pass
     def expect(self, counts: Sequence[int]) -> None:
         """How many positions of each row of the next, first pass are real; the others are padding on the right."""
+        self._store.undo()                                 # of a pass that was given up between two calls, as below
         counts = [int(c) for c in counts]
         if len(counts) != len(self) or any(c < 1 for c in counts):
             raise ValueError(f"SISAPagedCache.expect: {counts}: a positive count for each of the {len(self)} sequences")
@@ -354,7 +355,7 @@ class SISAPagedCache:
     def _begin(self, layer: _Layer, M: int) -> None:
         """The positions of a pass of ``M``, at its first layer; the later ones find them there."""
         st, lo, hi = self._store, self._lo, self._hi
-        st.undo()                                          # of a pass that was given up between two calls
+        st.undo()
         first = layer.filled[lo:hi] == st.lengths[lo:hi]
         if first:
             whole = all(x.filled[lo:hi] == st.lengths[lo:hi] for x in st.layers.values())
@@ -524,6 +525,7 @@ class SISAPagedCache:
     def reserve(self, positions: int) -> None:
         """Take the pages that ``positions`` more positions of every sequence need now, not as they come."""
         st = self._store
+        st.undo()
         ends = [min(n + positions, st.max_length) for n in self.lengths]
         if st.take(self._lo, ends) and st.table is not None:
             st.show(range(self._lo, self._hi))
@@ -531,6 +533,7 @@ class SISAPagedCache:
     def release(self) -> None:
         """Empty these sequences: their pages are free for others."""
         st, lo, hi = self._store, self._lo, self._hi
+        st.undo()
         for n in range(lo, hi):
             st.free += reversed(st.held[n])
             st.held[n] = []
@@ -549,6 +552,7 @@ class SISAPagedCache:
         those that have received the largest weight (each head its own). Sequences of at most ``keep`` are left alone. The
         kept rows move to other pages, of which there must be enough for one sequence."""
         st = self._store
+        st.undo()
         if not st.track:
             raise ValueError("SISAPagedCache.evict needs a cache made with track=True")
         if not 1 <= recent <= keep:

@@ -198,6 +198,33 @@ def test_a_pass_that_fails_before_it_is_written_is_taken_back(track, monkeypatch
     assert cache.lengths == [n + 4 for n in counts]
 
 
+def test_a_pass_that_is_given_up_between_two_calls_is_taken_back():
+    """Begun and never written, as by an interrupt outside of the cache's own functions: every entry finds the cache as before."""
+    model = _model64()
+    ids = token_ids(2, 30, seed=15)
+    want = _logits(model, ids, SISACache(), 20)
+    p = model.layers[0].attn._unfused_inputs(model.embed(ids[:, 20:29]).detach())
+    for entry in (lambda c: model(ids[:, 20:23], cache=c), lambda c: c.reserve(3), lambda c: c[1].release(),
+                  lambda c: c.evict(20, 5), lambda c: c[0].release()):
+        cache = SISAPagedCache(2, 60, page_size=16, track=True, pages=20)
+        with torch.no_grad():
+            model(ids[:, :20], cache=cache)
+            cache.begin(0, p.k, p.b, False)
+            entry(cache)
+            for i in range(2):
+                if not cache.lengths[i]:
+                    model(ids[i:i + 1, :20], cache=cache[i])
+                n = cache.lengths[i]
+                assert rel_err(model(ids[i:i + 1, n:n + 1], cache=cache[i]).logits, want[i:i + 1, n:n + 1]) <= GATES
+    cache = SISAPagedCache(2, 60)
+    cache.expect([9, 4])
+    with torch.no_grad():
+        cache.begin(0, p.k, p.b, False)
+        cache.expect([3, 8])                                # still the first pass
+        model(ids[:, :9], cache=cache)
+    assert cache.lengths == [3, 8]
+
+
 @pytest.mark.parametrize("n_layer,name,at", [(2, "_write", 2), (1, "paged_attention", 1), (2, "paged_attention", 1),
                                              (2, "paged_attention", 2), (1, "attention_weights", 1), (2, "attention_weights", 1)])
 def test_a_pass_that_fails_later_ends_its_sequences(n_layer, name, at, monkeypatch):
