@@ -139,7 +139,7 @@ def layer_step_paged(x: Tensor, res: Tensor | None, weights: list[int], d_ff: in
     B, _, D = x.shape
     H = D // HIP_D_HEAD
     at = cache.begin_step(layer_idx)
-    with cache.writing(layer_idx):
+    try:
         h, ffn = torch.empty((2, B, 1, D), device=x.device, dtype=x.dtype).unbind(0)
         tracked, dtype = at.weights is not None, _lib.dtype_code(x.dtype)
         size = _lib.load().sisa_step_paged_workspace_bytes(B, H, D, d_ff, at.max_len, dtype, tracked)
@@ -150,6 +150,9 @@ def layer_step_paged(x: Tensor, res: Tensor | None, weights: list[int], d_ff: in
                     at.table.stride(0), at.start.data_ptr(), at.end.data_ptr(), *(t.data_ptr() for t in at.last), *w,
                     h.data_ptr(), ffn.data_ptr(), ws.data_ptr())
         cache.end_step(layer_idx)
+    except BaseException:
+        cache.failed(layer_idx)
+        raise
     return h, ffn
 
 

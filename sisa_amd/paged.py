@@ -235,7 +235,7 @@ class _Store:
 
 
 class _Writing:
-    """Around what a layer does for a pass that has begun: an error in it takes the pass back, or marks the layer."""
+    """:meth:`SISAPagedCache.failed` on an error."""
     __slots__ = ("cache", "layer_idx")
 
     def __init__(self, cache: "SISAPagedCache", layer_idx: int) -> None:
@@ -246,7 +246,7 @@ class _Writing:
 
     def __exit__(self, kind, *_) -> None:
         if kind is not None:
-            self.cache._failed(self.layer_idx)
+            self.cache.failed(self.layer_idx)
 
 
 class SISAPagedCache:
@@ -345,7 +345,8 @@ class SISAPagedCache:
         """For a with statement around what a layer does between :meth:`begin` or :meth:`begin_step` and its end."""
         return _Writing(self, layer_idx)
 
-    def _failed(self, layer_idx: int) -> None:
+    def failed(self, layer_idx: int) -> None:
+        """An error in what a layer does for a pass that has begun: the pass is taken back, or the layer marked."""
         st = self._store
         if st.begun is not None:
             st.undo()
@@ -355,16 +356,14 @@ class SISAPagedCache:
     def _begin(self, layer: _Layer, M: int) -> None:
         """The positions of a pass of ``M``, at its first layer; the later ones find them there."""
         st, lo, hi = self._store, self._lo, self._hi
-        st.undo()
-        first = layer.filled[lo:hi] == st.lengths[lo:hi]
-        if first:
-            whole = all(x.filled[lo:hi] == st.lengths[lo:hi] for x in st.layers.values())
-        else:
-            whole = layer.filled[lo:hi] == st.starts[lo:hi] and st.widths[lo:hi] == [M] * len(self)
-        if not whole:
-            raise RuntimeError("SISAPagedCache: an earlier forward pass did not reach every layer; release() the sequences")
-        if not first:
+        if st.begun is not None:
+            st.undo()
+        filled = layer.filled[lo:hi]
+        first = filled == st.lengths[lo:hi]
+        if not first and filled == st.starts[lo:hi] and st.widths[lo:hi] == [M] * (hi - lo):
             return
+        if not first or any(x.filled[lo:hi] != filled for x in st.layers.values()):
+            raise RuntimeError("SISAPagedCache: an earlier forward pass did not reach every layer; release() the sequences")
         counts = [M if c is None else c for c in st.expected[lo:hi]]
         if max(counts) > M:
             raise ValueError(f"SISAPagedCache: {max(counts)} positions were expected, the pass has {M}")
