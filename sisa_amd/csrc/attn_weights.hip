@@ -536,7 +536,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 3 : 2) void weights_sum_k
 //   4 x 1,024 x 12,     768          64              45.7         37.3         33.1
 // Where few rows are counted against many keys, the keys of the first pass are split (256 keys at least, 32 splits at most),
 // the second joins the parts, and there each wave has its own keys (the last 64 of 16,384 positions of 16 heads: 43 -> 35.5 us,
-// 35 with four lanes to a row's join; 512 to 2,048 workgroups of splits in place of 256: first pass 15.6 -> 17 to 20.9).
+// 35 with four lanes to a row's join; 512 to 2,048 workgroups of splits in place of 256: first pass 15.6 -> 17 to 20.9). From
+// FEW_ROWS + 1 rows on nothing is split: the last 256 of 16,384 positions of 4 heads take 29 us, the last 257 80.
 struct Plan {
     int R, nsplit;
     bool few;
