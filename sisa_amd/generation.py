@@ -223,7 +223,7 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     ends when every row is finished. Returns ``(B, L + n)`` ids, ``n <= max_new_tokens``, with the rank of
     ``input_ids``.
 
-    ``prompt_lengths``: the prompts are right-padded rows of these lengths. A row's tokens follow its prompt, and what is
+    ``prompt_lengths``: the prompts are right-padded rows of these lengths (with anything). A row's tokens follow its prompt, and what is
     left of the row behind them is the first ``eos_token_id``, or 0 without one.
 
     ``cache_budget``: how many positions each layer and head keeps: the last ``cache_recent`` (default: a quarter) and those
@@ -260,11 +260,13 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
         if lengths is None:
             logits = model(rows, cache=cache, logits_to_keep=1).logits[:, -1]
         else:
-            cache.expect(lengths)
-            logits = model(rows, cache=cache, logits_at=[n - 1 for n in lengths]).logits[:, -1]
-            # rows are laid out from their own ends
+            # what pads the rows need not be a token; rows are laid out from their own ends
             n = torch.tensor(lengths, device=rows.device)
-            out[torch.arange(out.shape[1], device=rows.device) >= n[:, None]] = stops[0] if stops else 0
+            behind = torch.arange(out.shape[1], device=rows.device) >= n[:, None]
+            cache.expect(lengths)
+            logits = model(rows.masked_fill(behind[:, :prompt], 0), cache=cache,
+                           logits_at=[n - 1 for n in lengths]).logits[:, -1]
+            out[behind] = stops[0] if stops else 0
             ends = n[:, None]
         while True:
             token = _pick(logits, do_sample, temperature, top_k, generator).to(rows.dtype)

@@ -428,6 +428,18 @@ def test_generate_from_unequal_prompts():
             generate(model, ids, 2, prompt_lengths=bad)
 
 
+@pytest.mark.parametrize("pad", [-1, -100, 10 ** 6])
+def test_generate_from_prompts_padded_with_no_token(pad):
+    model = _model64()
+    ids, lengths = token_ids(3, 24, seed=8), torch.tensor([24, 3, 11])
+    padded = torch.where(torch.arange(24) < lengths[:, None], ids, pad)
+    before = padded.clone()
+    for kw in ({}, dict(eos_token_id=5), dict(cache_budget=8)):
+        want = generate(model, ids, 9, prompt_lengths=lengths, **kw)
+        assert torch.equal(generate(model, padded, 9, prompt_lengths=lengths, **kw), want)
+    assert torch.equal(padded, before)
+
+
 def test_generate_within_a_budget():
     model = _model64()
     ids = token_ids(2, 50, seed=9)
