@@ -9,6 +9,8 @@ works without a GPU or a built library; the attributes below are resolved on fir
 ``linear_cross_entropy(hidden, weight, labels, ignore_index=-100) -> loss``  (:mod:`.linear_ce`)
 ``PagePool``, ``sisa_paged_write_hip``, ``sisa_paged_decode_hip``, ``sisa_cache_evict_hip``: a generation cache in pages
 (:mod:`.paged`); ``sisa_attention_weights_hip``: what a prompt's positions have received (:mod:`.weights`)
+``PrefixGroups``, ``sisa_prefix_decode_hip``: attention of sequences with common first positions (:mod:`.prefix`);
+``sisa_verify_drafts_hip``: drafted tokens against the target's probabilities (:mod:`.verify`)
 """
 from __future__ import annotations
 
@@ -16,7 +18,8 @@ import importlib
 
 __all__ = ["sisa_attention_hip", "sisa_fused", "fused_layout", "concat_fused_weights", "linear_cross_entropy",
            "reference_linear_cross_entropy", "PagePool", "sisa_paged_write_hip", "sisa_paged_decode_hip",
-           "sisa_cache_evict_hip", "sisa_attention_weights_hip"]
+           "sisa_cache_evict_hip", "sisa_attention_weights_hip", "PrefixGroups", "sisa_prefix_decode_hip",
+           "sisa_verify_drafts_hip"]
 
 _LAZY = {
     "sisa_attention_hip": "attention",
@@ -30,6 +33,9 @@ _LAZY = {
     "sisa_paged_decode_hip": "paged",
     "sisa_cache_evict_hip": "paged",
     "sisa_attention_weights_hip": "weights",
+    "PrefixGroups": "prefix",
+    "sisa_prefix_decode_hip": "prefix",
+    "sisa_verify_drafts_hip": "verify",
 }
 
 

@@ -193,6 +193,22 @@ class StepPagedArgs(Structure):
                 ("weights", View), ("h", c_void_p), ("ffn", c_void_p), ("workspace", c_void_p)]
 
 
+class PrefixDecodeArgs(Structure):
+    _fields_ = [("B", c_int32), ("M", c_int32), ("W", c_int32), ("G", c_int32), ("max_len", c_int32),
+                ("max_shared", c_int32), ("out_dtype", c_int32), ("reserved", c_int32), ("pool", PagePoolArgs),
+                ("table", c_void_p), ("s_table", c_int64), ("lengths", c_void_p), ("first", c_void_p),
+                ("group", c_void_p), ("shared", c_void_p), ("q", View), ("c", View), ("gq", View), ("fq", View),
+                ("lam", c_void_p), ("s_lam", c_int64), ("out", c_void_p), ("workspace", c_void_p)]
+
+
+class VerifyArgs(Structure):
+    _fields_ = [("B", c_int32), ("K", c_int32), ("V", c_int32), ("p_dtype", c_int32), ("q_dtype", c_int32),
+                ("reserved", c_int32), ("p", c_void_p), ("p_b", c_int64), ("p_k", c_int64), ("q", c_void_p),
+                ("q_b", c_int64), ("q_k", c_int64), ("drafts", c_void_p), ("d_b", c_int64), ("d_k", c_int64),
+                ("u", c_void_p), ("u_b", c_int64), ("u_k", c_int64), ("counts", c_void_p), ("tokens", c_void_p),
+                ("accepted", c_void_p), ("workspace", c_void_p)]
+
+
 class Round16Args(Structure):
     _fields_ = [("n", c_int64), ("dtype", c_int32), ("x", c_void_p), ("y", c_void_p), ("back", c_void_p)]
 
@@ -261,6 +277,14 @@ CACHE_SIGNATURES = {
     "sisa_step_paged": ([POINTER(StepPagedArgs), c_void_p], c_int),
 }
 
+# branched and drafted generation (include/sisa_hip_branch.h)
+BRANCH_SIGNATURES = {
+    "sisa_prefix_decode_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32, c_int32, c_int32], c_int64),
+    "sisa_prefix_decode": ([POINTER(PrefixDecodeArgs), c_void_p], c_int),
+    "sisa_verify_workspace_bytes": ([c_int32, c_int32], c_int64),
+    "sisa_verify": ([POINTER(VerifyArgs), c_void_p], c_int),
+}
+
 _LOCK = threading.Lock()
 _LIB = None
 
@@ -277,7 +301,8 @@ def load() -> ctypes.CDLL:
             raise RuntimeError(f"SISA HIP library not built: {LIB_PATH} is missing (run sisa_amd.build.build())")
         lib = ctypes.CDLL(LIB_PATH)
         for name, (argtypes, restype) in (*SIGNATURES.items(), *STEP_SIGNATURES.items(),
-                                           *CE_SIGNATURES.items(), *CACHE_SIGNATURES.items()):
+                                           *CE_SIGNATURES.items(), *CACHE_SIGNATURES.items(),
+                                           *BRANCH_SIGNATURES.items()):
             fn = getattr(lib, name)
             fn.argtypes = argtypes
             fn.restype = restype
