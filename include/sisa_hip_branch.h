@@ -22,7 +22,8 @@ extern "C" {
  * to B and group[n] is the group of sequence n: where they do not agree no memory outside the arguments' is touched, and the
  * rows are of no use. An infinite v that a row sees may give NaN. The lengths of a group may be anything, below shared[r],
  * too. max_len bounds the lengths and max_shared the common positions, each at most W * page_size; the launch is sized by
- * them. Workspace: sisa_prefix_decode_workspace_bytes(B, H, M, G, max_len, max_shared). */
+ * them. The positions of a page of the pool are at least a row apart and those of a head within 2 GiB. Workspace:
+ * sisa_prefix_decode_workspace_bytes(B, H, M, G, max_len, max_shared). */
 typedef struct {
     int32_t B, M, W, G;
     int32_t max_len, max_shared;

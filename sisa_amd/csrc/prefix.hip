@@ -3,13 +3,15 @@
 //   s_mj = q_m.k_j / 8 + lam exp(g_m - g_j) (c_m.b_j) + (F_m - F_j);   out_m = softmax_j(s_mj) v_j
 //
 // The softmax over a sequence's positions is joined from its parts: the common positions, which the query rows of a group see
-// alike and which are read once for 16 NR of them, and its own. Both parts are the same work: up to 16 NR query rows against
-// a range of positions in the pages of one table row, 32 positions (a tile) of a wave at a time on the matrix cores.
+// alike, and its own. Both are the same work for a wave: up to 16 query rows against a range of positions in the pages of one
+// table row, 32 positions (a tile) at a time on the matrix cores. Of a group of more than 16 rows, two or four waves of a
+// workgroup have rows of their own and go through the same positions side by side, so that the cached rows come from memory
+// once and from the nearest cache for the others; the remaining ones split the positions.
 //
 // Scores are computed transposed (S^T = K Q^T), so that a lane has one query row's softmax and the weights are the operand of
-// O^T += V^T P^T as they are. K and b~ go from memory to the operand registers, each used by one wave only; v passes through
-// LDS, which transposes it. The weights enter their product as a sum of two (fp16) or three (bf16) operands, so that the
-// result is an fp32 one: rounded once to bf16 they would be off by 2^-9.
+// O^T += V^T P^T as they are. K and b~ go from memory to the operand registers; v passes through LDS, which transposes it. The
+// weights enter their product as a sum of two (fp16) or three (bf16) operands, so that the result is an fp32 one: rounded once
+// to bf16 they would be off by 2^-9.
 #include "pages.h"
 #include "sisa_hip_branch.h"
 
@@ -20,15 +22,15 @@ constexpr int KT = 32;                // positions of a tile
 constexpr int NW = 4;                 // waves of a workgroup
 constexpr int MOST = 64;              // most parts of a range: the join has a lane for each
 
-// How a call is cut into workgroups: the query rows of all groups into tiles of 16 NR, a group's common positions into `parts`
-// workgroups, a sequence's own ones into `own_parts` waves.
+// How a call is cut: the query rows of all groups into tiles of 16 << log_rw, 16 to a wave; a group's common positions into
+// `parts` workgroups of 4 >> log_rw waves a row, a sequence's own ones into `own_parts` waves.
 struct Plan {
-    int nr;
+    int log_rw;
     unsigned tiles, own_tiles, parts, own_parts, own_rows;
     int64_t items, own_items;         // workgroups, waves
 };
 
-// Tile t of all groups' query rows: group r's tiles begin at r + first[r] M / (16 NR), which leaves room for each.
+// Tiles of all groups' query rows: group r's begin at r + floor(first[r] M / rows of a tile), which leaves room for each.
 SISA_DEV int64_t tile_base(const sisa_prefix_decode_args& a, int r, int log_per) {
     const int64_t n = a.first[r];
     return r + ((n < 0 ? 0 : n > a.B ? a.B : n) * a.M >> log_per);
@@ -72,10 +74,9 @@ struct __attribute__((aligned(16))) WaveLds {
     float g[KT], f[KT];
 };
 
-// Up to 16 NR query rows, counted from sequence n0's first, against positions lo <= j < hi of a table row.
+// Up to 16 query rows, counted from sequence n0's first, against positions lo <= j < hi of a table row.
 struct Work {
     int h, n0, r0, rows, lo, hi;
-    const int32_t* row;
 };
 
 // What a wave loads of a tile: K and b~ as operands, v in 16-byte pieces, g and F of the position lane % 16 of either half.
@@ -87,100 +88,93 @@ struct Tile {
     float g[2], f[2];
 };
 
-// 16-byte loads relative to a scalar base, 0 for the offset NOWHERE.
-constexpr int NOWHERE = (int)0x80000000;
-template <class V> SISA_DEV V load_at(const char* base, int voff, int soff) {
-    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, 0x7fffffff);
+// Loads at a lane's offset from a scalar base, 0 where it is not below `bytes`.
+template <class V> SISA_DEV V load_at(const char* base, int bytes, int voff, int soff) {
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(base, bytes);
     if constexpr (sizeof(V) == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0));
     else return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
 }
-template <class T> SISA_DEV frag8<T> load_frag(const char* base, int voff, int soff) {
-    if constexpr (sizeof(T) == 2) return load_at<frag8<T>>(base, voff, soff);
-    else return join<T>(load_at<f32x4>(base, voff, soff), load_at<f32x4>(base, voff, soff + 16));
+template <class T> SISA_DEV frag8<T> load_frag(const char* base, int bytes, int voff, int soff) {
+    if constexpr (sizeof(T) == 2) return load_at<frag8<T>>(base, bytes, voff, soff);
+    else return join<T>(load_at<f32x4>(base, bytes, voff, soff), load_at<f32x4>(base, bytes, voff, soff + 16));
 }
 
-// A wave's view of the positions of one head: where the 16 from 16 i on begin in each tensor (lane i % 64), and what a lane
-// adds to that.
-template <class T>
-struct Places {
-    const sisa_page_pool* P;
-    const int32_t* row;
-    int W, shift, h, lo, hi, base;
-    int page;                          // of 16-block base + lane; -1: none of the pool's
-    int64_t k, v, b, g, f;
-    int ok, ov, ob, og, of;            // byte offsets of the lane in a block of 16 positions
+// A scalar in registers of its own: as part of the wide load of the kernel's arguments it would keep all of that alive.
+template <class X> SISA_DEV X apart(X x) {
+    asm("" : "+s"(x));
+    return x;
+}
 
-    SISA_DEV void init(const sisa_page_pool& pool, const Work& w, int W_, int shift_, int lane) {
-        constexpr int es = sizeof(T);
-        P = &pool;
-        row = w.row, W = W_, shift = shift_, h = w.h, lo = w.lo, hi = w.hi;
-        const int grp = lane >> 4, lc = lane & 15, ch = lane % Tile<T>::CPR, r = lane / Tile<T>::CPR;
-        ok = (lc * (int)pool.k.sl + 8 * grp) * es;
-        ob = (lc * (int)pool.b.sl + 8 * grp) * es;
-        ov = (r * (int)pool.v.sl + Tile<T>::E * ch) * es;
-        og = lc * (int)pool.g.sl * 4;
-        of = lc * (int)pool.f.sl * 4;
-    }
-    SISA_DEV void look_up(int tile, int lane) {
-        constexpr int es = sizeof(T);
-        base = 2 * tile;
-        const int j = 16 * (base + lane), slot = j & (P->page_size - 1);
-        page = j < hi ? page_of(row, W, shift, P->pages, j) : -1;
-        const int64_t at = page < 0 ? 0 : page;
-        auto place = [&](const sisa_view& x, int size) { return (at * x.sb + h * x.sh + slot * x.sl) * size; };
-        k = place(P->k, es);
-        v = place(P->v, es);
-        b = place(P->b, es);
-        g = place(P->g, 4);
-        f = place(P->f, 4);
-    }
-    SISA_DEV static const char* at(const void* p, int64_t place, int i) {
-        const unsigned lo = __builtin_amdgcn_readlane((int)place, i), hi = __builtin_amdgcn_readlane((int)(place >> 32), i);
-        return (const char*)p + (int64_t)((uint64_t)hi << 32 | lo);
-    }
-    // The tile of positions 32 tile ..
-    SISA_DEV void load(int tile, int lane, Tile<T>& x) {
-        if (2 * tile - base >= 64) look_up(tile, lane);
-        const int lc = lane & 15, r = lane / Tile<T>::CPR;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const int i = 2 * tile + kb - base, j0 = 16 * (2 * tile + kb);
-            const bool there = __builtin_amdgcn_readlane(page, i) >= 0;
-            const char *pk = at(P->k.ptr, k, i), *pv = at(P->v.ptr, v, i), *pb = at(P->b.ptr, b, i), *pg = at(P->g.ptr, g, i),
-                       *pf = at(P->f.ptr, f, i);
-            const bool in = there && j0 + lc >= lo && j0 + lc < hi;
-            const int vk = in ? ok : NOWHERE, vb = in ? ob : NOWHERE;
-            x.k[kb][0] = load_frag<T>(pk, vk, 0);
-            x.k[kb][1] = load_frag<T>(pk, vk, 32 * (int)sizeof(T));
-            x.b[kb] = load_frag<T>(pb, vb, 0);
-            x.g[kb] = load_at<float>(pg, in ? og : NOWHERE, 0);
-            x.f[kb] = load_at<float>(pf, in && P->f.ptr ? of : NOWHERE, 0);
-            if (!there) x.f[kb] = __builtin_nanf("");
-            constexpr int HALF = Tile<T>::PASS / 2, ROWS = 64 / Tile<T>::CPR;
-#pragma unroll
-            for (int p = 0; p < HALF; ++p) {
-                const int jv = j0 + ROWS * p + r;
-                x.v[HALF * kb + p] = load_at<u32x4>(pv, there && jv >= lo && jv < hi ? ov : NOWHERE,
-                                                    ROWS * p * (int)P->v.sl * (int)sizeof(T));
-            }
-        }
+// One tensor of the pool as a head's waves see it: where the head begins, bytes from page to page and from row to row, and
+// what a lane adds to the first of 16 rows.
+struct Stream {
+    const char* base;
+    int64_t page;
+    int row, lane;
+    SISA_DEV void init(const sisa_view& x, int h, int size, int lane_row, int lane_col) {
+        base = apart((const char*)x.ptr + h * x.sh * size);
+        page = apart(x.sb * size);
+        row = apart((int)x.sl * size);
+        lane = lane_row * row + lane_col;
     }
 };
+struct Streams {
+    Stream k, v, b, g, f;
+};
+
+// 16 positions of a tile from slot `slot` of page p on, `n` of them (0 without a page); the other rows are 0.
+template <class T>
+SISA_DEV void load_half(const Streams& s, int p, int slot, int n, int kb, Tile<T>& x) {
+    constexpr int HALF = Tile<T>::PASS / 2, ROWS = 64 / Tile<T>::CPR;
+    const int end = slot + n;
+    const char *pk = s.k.base + p * s.k.page, *pv = s.v.base + p * s.v.page, *pb = s.b.base + p * s.b.page;
+    x.k[kb][0] = load_frag<T>(pk, n ? end * s.k.row : 0, s.k.lane, slot * s.k.row);
+    x.k[kb][1] = load_frag<T>(pk, n ? end * s.k.row : 0, s.k.lane, slot * s.k.row + 32 * (int)sizeof(T));
+    x.b[kb] = load_frag<T>(pb, n ? end * s.b.row : 0, s.b.lane, slot * s.b.row);
+    x.g[kb] = load_at<float>(s.g.base + p * s.g.page, n ? end * s.g.row : 0, s.g.lane, slot * s.g.row);
+    x.f[kb] = load_at<float>(s.f.base + p * s.f.page, n ? end * s.f.row : 0, s.f.lane, slot * s.f.row);
+#pragma unroll
+    for (int i = 0; i < HALF; ++i)
+        x.v[HALF * kb + i] = load_at<u32x4>(pv, n ? end * s.v.row : 0, s.v.lane, (slot + ROWS * i) * s.v.row);
+}
+
+struct Space {
+    f32x2 *stat, *own_stat;
+    float *part, *own;
+    int64_t bytes;
+};
+struct PartArgs {
+    sisa_prefix_decode_args a;
+    Plan plan;
+    int shift;
+    Space ws;
+};
+// A kernel's argument read again where it is needed: kept from the beginning they do not fit the scalar registers.
+template <class X> SISA_DEV X again(size_t offset) {
+    typedef const __attribute__((address_space(4))) char* Const;
+    Const p = (Const)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const __attribute__((address_space(4))) X*)(p + offset);
+}
+#define AGAIN(field) again<decltype(PartArgs::field)>(offsetof(PartArgs, field))
 
 // The workgroups of the common parts, then those of the own ones, whose waves are on their own. Unnormalised outputs go to
-// `part`, 16 NR rows an item, and `own`; each row's reference (log2) and sum to `stat` and `own_stat`.
-template <class T, int NR>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) void prefix_part_kernel(sisa_prefix_decode_args a, Plan plan, int shift, f32x2* stat,
-                                                              float* part, f32x2* own_stat, float* own_part) {
-    constexpr int PER = 16 * NR, LOG = NR == 1 ? 4 : NR == 2 ? 5 : 6, LD = DH + 4;
+// `part`, a tile of rows an item, and `own_part`; each row's reference (log2) and sum to `stat` and `own_stat`.
+template <class T>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 4 : 3))) void prefix_part_kernel(
+    PartArgs args) {
+    constexpr int LD = DH + 4;
     __shared__ WaveLds<T> lds[NW];
-    __shared__ __attribute__((aligned(16))) float ms[NW][PER], ls[NW][PER], os[NW][16][LD];
+    __shared__ __attribute__((aligned(16))) float ms[NW][16], ls[NW][16], os[NW][16][LD];
+    const sisa_prefix_decode_args& a = args.a;
+    const Plan& plan = args.plan;
     const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4, lc = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const bool own = blockIdx.x >= (unsigned)plan.items;
-    const int64_t held = (int64_t)a.W << shift;
+    const int64_t held = (int64_t)a.W << args.shift;
     const unsigned H = a.pool.heads;
-    unsigned item = own ? (blockIdx.x - (unsigned)plan.items) * NW + w : blockIdx.x;
+    const int log_rw = plan.log_rw, rw = 1 << log_rw, log_per = 4 + log_rw;
+    const unsigned item = own ? (blockIdx.x - (unsigned)plan.items) * NW + w : blockIdx.x;
     Work k;
     Range t;                                             // the wave's tiles
     if (own) {
@@ -201,207 +195,204 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         t.from += first;
         t.to += first;
     } else {
-        const unsigned ph = item / plan.tiles, tile = item - ph * plan.tiles, p = ph / H;
-        k.h = ph - p * H;
+        // tile by tile: those that no group needs come last, and the others spread over all XCDs
+        const unsigned tp = item / H, tile = tp / plan.parts, p = tp - tile * plan.parts;
+        k.h = item - tp * H;
         int r = 0;                                       // the last group whose tiles begin at or before this one
         if (a.G > 1) {
             r = -1;
-            for (int i = 0; i < a.G; i += 64) r += __popcll(__ballot(i + lane < a.G && tile_base(a, i + lane, LOG) <= tile));
+            for (int i = 0; i < a.G; i += 64) r += __popcll(__ballot(i + lane < a.G && tile_base(a, i + lane, log_per) <= tile));
             if (r < 0) return;
         }
         const int f0 = a.first[r], f1 = a.first[r + 1];
         k.hi = common(a, held, r);
         if (f0 < 0 || f1 > a.B || f1 <= f0 || k.hi <= 0) return;
-        const int64_t all = (int64_t)(f1 - f0) * a.M, nth = (int64_t)tile - tile_base(a, r, LOG), at = nth * PER;
-        if (nth < 0 || at >= all) return;
+        const int64_t all = (int64_t)(f1 - f0) * a.M, nth = (int64_t)tile - tile_base(a, r, log_per);
+        const int64_t at = (nth << log_per) + 16 * (w & (rw - 1));
+        if (nth < 0 || nth << log_per >= all) return;
         k.n0 = f0;
         k.r0 = at;
-        k.rows = all - at < PER ? all - at : PER;
+        k.rows = at >= all ? 0 : all - at < 16 ? all - at : 16;
         k.lo = 0;
-        const int n = (k.hi + KT - 1) / KT;
-        if (part_of(n, plan.parts * NW, p * NW).from >= n) return;
-        t = part_of(n, plan.parts * NW, p * NW + w);
+        const int n = (k.hi + KT - 1) / KT, kw = NW >> log_rw;
+        if (part_of(n, plan.parts * kw, p * kw).from >= n) return;
+        t = part_of(n, plan.parts * kw, p * kw + (w >> log_rw));
+        if (!k.rows) t.to = t.from;
     }
-    k.row = a.table + k.n0 * a.s_table;
-    const int nr = (k.rows + 15) >> 4;
-    Places<T> at;
-    at.init(a.pool, k, a.W, shift, lane);
-    at.look_up(t.from, lane);
+    const int32_t* table = apart(a.table + k.n0 * a.s_table);
 
-    // Query rows: lane i finds row i's; column lc of each group of 16 is a lane's, in all four groups of lanes.
-    frag8<T> q[NR][2], c[NR];
-    float gq[NR], fq[NR], m2[NR], l[NR];                 // l: the lane's part
-    int lim[NR];                                         // positions below it are seen
-    f32x4 o[NR][4];                                      // output features 16 db + 4 grp + i
-    int least = k.hi;                                    // every row sees what lies before it
+    // Column lc of the operand is query row lc, in all four groups of lanes; behind the last row the last again.
+    frag8<T> q[2], c;
+    float gq, fq = 0.f, m2 = LEAST, l = 0.f;             // l: the lane's part
+    int len, back, lim = 0, least = 0;                   // positions that the row sees, and that every row does
+    f32x4 o[4] = {zero4(), zero4(), zero4(), zero4()};   // output features 16 db + 4 grp + i
     {
-        int n = k.n0, m = k.r0 + lane, seen = 0;
+        const int r = k.r0 + (lc < k.rows ? lc : k.rows - 1);
+        int n = k.n0, m = r;
         if (!own) {
-            const unsigned d = a.M == 1 ? m : (unsigned)m / (unsigned)a.M;
+            const unsigned d = a.M == 1 ? r : (unsigned)r / (unsigned)a.M;
             n += d;
             m -= d * a.M;
         }
-        float g = 0.f, f = 0.f;
-        int64_t pq = 0, pc = 0;
-        if (lane < k.rows) {
-            g = ((const float*)a.gq.ptr)[n * a.gq.sb + k.h * a.gq.sh + m * a.gq.sl];
-            if (a.fq.ptr) f = ((const float*)a.fq.ptr)[n * a.fq.sb + k.h * a.fq.sh + m * a.fq.sl];
-            pq = n * a.q.sb + k.h * a.q.sh + m * a.q.sl;
-            pc = n * a.c.sb + k.h * a.c.sh + m * a.c.sl;
-            seen = visible(a, held, n, m);
-            seen = seen < k.hi ? seen : k.hi;
-            if (seen >= 0) least = seen;                 // the join answers for the others
-        }
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) {
-            const int y = __shfl_xor(least, s);
-            least = y < least ? y : least;
-        }
-        least = __builtin_amdgcn_readfirstlane(least);
-#pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const int from = 16 * i + lc;
-            gq[i] = __shfl(g, from);
-            fq[i] = __shfl(f, from);
-            lim[i] = __shfl(seen, from);
-            const T *rq = (const T*)a.q.ptr + lane_value(pq, from) + 8 * grp, *rc = (const T*)a.c.ptr + lane_value(pc, from) + 8 * grp;
-            q[i][0] = q[i][1] = c[i] = zero8<T>();
-            if (from < k.rows) q[i][0] = load8<T>(rq), q[i][1] = load8<T>(rq + 32), c[i] = load8<T>(rc);
-            if (from >= k.rows) gq[i] = -__builtin_inff();
-            l[i] = 0.f;
-            m2[i] = LEAST;
-#pragma unroll
-            for (int db = 0; db < 4; ++db) o[i][db] = zero4();
-        }
+        if (!k.rows) n = m = 0;
+        len = a.lengths[n];
+        back = a.M - 1 - m;
+        gq = ((const float*)a.gq.ptr)[n * a.gq.sb + k.h * a.gq.sh + m * a.gq.sl];
+        if (a.fq.ptr) fq = ((const float*)a.fq.ptr)[n * a.fq.sb + k.h * a.fq.sh + m * a.fq.sl];
+        const T *rq = (const T*)a.q.ptr + (n * a.q.sb + k.h * a.q.sh + m * a.q.sl) + 8 * grp;
+        q[0] = load8<T>(rq);
+        q[1] = load8<T>(rq + 32);
+        c = load8<T>((const T*)a.c.ptr + (n * a.c.sb + k.h * a.c.sh + m * a.c.sl) + 8 * grp);
     }
     const float lam = a.lam[k.h * a.s_lam] * LOG2E;
-
+    const int mask = apart(a.pool.page_size - 1), pages = apart(a.pool.pages), W = apart(a.W), shift = apart(args.shift);
+    const int max_len = apart(a.max_len), row_f = a.pool.f.ptr ? 1 : 0;
     using X = Tile<T>;
+    Streams ss;
+    {
+        const int row = lane / X::CPR, col = 16 * (lane % X::CPR), part = 8 * grp * (int)sizeof(T);
+        ss.k.init(a.pool.k, k.h, sizeof(T), lc, part);
+        ss.v.init(a.pool.v, k.h, sizeof(T), row, col);
+        ss.b.init(a.pool.b, k.h, sizeof(T), lc, part);
+        ss.g.init(a.pool.g, k.h, 4, lc, 0);
+        ss.f.init(a.pool.f, k.h, 4, lc, 0);
+        if (!row_f) ss.f.row = 0;                        // no forget term: every F is 0
+    }
+
     WaveLds<T>& sm = lds[w];
-    X x;
     bool odd = false;
-    for (int tile = t.from < t.to ? t.from - 1 : t.to; tile < t.to; ++tile) {
+    int near_pages = -1, base = t.from - 32;             // lane i: the page of the 16 positions from 16 (2 base + i) on
+    for (int tile = t.from; tile < t.to; ++tile) {
         const int jt = tile * KT;
-        const bool mixed = jt + KT > least || jt < k.lo;               // some row does not see all of the tile
-        frag8<T> kf[2][2], bf[2];
-        bool fast = false;
-        float ge = 0.f, fe = 0.f;
-        if (tile >= t.from) {
-            if (mixed) {
-                // Values that are not finite, at positions that some row does not see: 0 in the product (0 times them would
-                // be NaN there), and added to the rows that see them at the end.
-                asm volatile("");      // a branch, not selects
-#pragma unroll
-                for (int i = 0; i < X::PASS; ++i) {
-                    T e[X::E];
-                    __builtin_memcpy(e, &x.v[i], 16);
-#pragma unroll
-                    for (int j = 0; j < X::E; ++j) {
-                        const float y = (float)e[j];
-                        if (!(y - y == 0.f)) e[j] = (T)0.f, odd = true;
-                    }
-                    __builtin_memcpy(&x.v[i], e, 16);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < X::PASS; ++i)
-                *reinterpret_cast<u32x4*>(sm.v + toff<T, DH>((64 * i + lane) / X::CPR, lane % X::CPR)) = x.v[i];
-            // Where every row sees the tile: exp(g_m - g_j) as exp(g_m - g_e) exp(g_e - g_j) and F_m - F_j as (F_m - F_e) +
-            // (F_e - F_j), e the tile's last position, one factor a row and one a position. Both are at most 1 where g
-            // falls; where it rises too far for them, or F_e is not finite, the tile is taken pair by pair.
-            ge = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x.g[1]), 15));
-            fe = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x.f[1]), 15));
-            const float d0 = (ge - x.g[0]) * LOG2E, d1 = (ge - x.g[1]) * LOG2E;
-            bool near = fabsf(d0) <= FACTORED && fabsf(d1) <= FACTORED && fe - fe == 0.f;
-#pragma unroll
-            for (int g = 0; g < NR; ++g) near = near && (gq[g] - ge) * LOG2E <= FACTORED;
-            fast = !mixed && __ballot(!near) == 0;
-            if (grp == 0) {
-                sm.g[lc] = fast ? fast_exp2(d0) : x.g[0];
-                sm.g[16 + lc] = fast ? fast_exp2(d1) : x.g[1];
-                sm.f[lc] = fast ? (fe - x.f[0]) * LOG2E : x.f[0];
-                sm.f[16 + lc] = fast ? (fe - x.f[1]) * LOG2E : x.f[1];
-            }
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) kf[kb][0] = x.k[kb][0], kf[kb][1] = x.k[kb][1], bf[kb] = x.b[kb];
+        if (tile - base >= 32) {
+            base = tile;
+            const int j = 16 * (2 * base + lane);
+            near_pages = j < k.hi && j + 16 > k.lo ? page_of(table, W, shift, pages, j) : -1;
         }
-        if (tile + 1 < t.to) at.load(tile + 1, lane, x);               // under way meanwhile
-        if (tile < t.from) continue;
+        X x;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int page = __builtin_amdgcn_readlane(near_pages, 2 * (tile - base) + kb), j0 = jt + 16 * kb;
+            const int left = k.hi - j0 < 16 ? k.hi - j0 : 16;
+            load_half<T>(ss, page < 0 ? 0 : page, j0 & mask, page < 0 || left < 0 ? 0 : left, kb, x);
+            if (page < 0) x.f[kb] = __builtin_nanf("");
+        }
+        if (tile == t.from) {                            // the first loads are under way: what has come of the query rows
+            const int seen = len - back;
+            lim = len < 0 || len > max_len || len > held ? -1 : seen > 0 ? seen : 0;
+            lim = lim < k.hi ? lim : k.hi;
+            least = lim < 0 ? k.hi : lim;                // the join answers for rows that see nothing defined
+            if (lc >= k.rows) lim = 0, least = k.hi, gq = -__builtin_inff();
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) {
+                const int y = __shfl_xor(least, d);
+                least = y < least ? y : least;
+            }
+            least = __builtin_amdgcn_readfirstlane(least);
+        }
+        const bool mixed = jt + KT > least || jt < k.lo;               // some row does not see all of the tile
+        if (mixed) {
+            // Values that are not finite, at positions that some row does not see: 0 in the product (0 times them would be
+            // NaN there), and added to the rows that see them at the end.
+#pragma unroll
+            for (int i = 0; i < X::PASS; ++i) {
+                T e[X::E];
+                __builtin_memcpy(e, &x.v[i], 16);
+#pragma unroll
+                for (int j = 0; j < X::E; ++j) {
+                    const float y = (float)e[j];
+                    if (!(y - y == 0.f)) e[j] = (T)0.f, odd = true;
+                }
+                __builtin_memcpy(&x.v[i], e, 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < X::PASS; ++i)
+            *reinterpret_cast<u32x4*>(sm.v + toff<T, DH>((64 * i + lane) / X::CPR, lane % X::CPR)) = x.v[i];
+        // Where every row sees the tile: exp(g_m - g_j) as exp(g_m - g_e) exp(g_e - g_j) and F_m - F_j as (F_m - F_e) +
+        // (F_e - F_j), e the tile's last position, one factor a row and one a position. Both are at most 1 where g falls;
+        // where it rises too far for them, or F_e is not finite, the tile is taken pair by pair.
+        const float ge = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x.g[1]), 15));
+        const float fe = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x.f[1]), 15));
+        const float d0 = (ge - x.g[0]) * LOG2E, d1 = (ge - x.g[1]) * LOG2E, dq = (gq - ge) * LOG2E;
+        const bool near = fabsf(d0) <= FACTORED && fabsf(d1) <= FACTORED && dq <= FACTORED && fe - fe == 0.f;
+        const bool fast = !mixed && __ballot(!near) == 0;
+        if (grp == 0) {
+            sm.g[lc] = fast ? fast_exp2(d0) : x.g[0];
+            sm.g[16 + lc] = fast ? fast_exp2(d1) : x.g[1];
+            sm.f[lc] = fast ? (fe - x.f[0]) * LOG2E : x.f[0];
+            sm.f[16 + lc] = fast ? (fe - x.f[1]) * LOG2E : x.f[1];
+        }
+        f32x4 s[2], cb[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            s[kb] = mma(x.k[kb][1], q[1], mma(x.k[kb][0], q[0], zero4()));
+            cb[kb] = mma(x.b[kb], c, zero4());
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int g = 0; g < NR; ++g) {
-            if (g >= nr) break;
-            f32x4 s[2];
-            float more = 0.f;                            // to be added to the scores
-            f32x4 qk[2], cb[2];
+        float more = 0.f;                                // to be added to the scores
+        if (fast) {
+            more = (fq - fe) * LOG2E;
+            const float rowf = lam * fast_exp2(dq);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                qk[kb] = mma(kf[kb][1], q[g][1], mma(kf[kb][0], q[g][0], zero4()));
-                cb[kb] = mma(bf[kb], c[g], zero4());
+                const f32x4 gk = lds4f(sm.g + 16 * kb + 4 * grp), fk = lds4f(sm.f + 16 * kb + 4 * grp);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[kb][e] = fmaf(cb[kb][e] * gk[e], rowf, fmaf(s[kb][e], 0.125f * LOG2E, fk[e]));
             }
-            if (fast) {
-                more = (fq[g] - fe) * LOG2E;
-                const float rowf = lam * fast_exp2((gq[g] - ge) * LOG2E);
+        } else {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const f32x4 gk = lds4f(sm.g + 16 * kb + 4 * grp), fk = lds4f(sm.f + 16 * kb + 4 * grp);
+            for (int kb = 0; kb < 2; ++kb) {
+                const f32x4 gk = lds4f(sm.g + 16 * kb + 4 * grp), fk = lds4f(sm.f + 16 * kb + 4 * grp);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) s[kb][e] = fmaf(cb[kb][e] * gk[e], rowf, fmaf(qk[kb][e], 0.125f * LOG2E, fk[e]));
-                }
-            } else {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const f32x4 gk = lds4f(sm.g + 16 * kb + 4 * grp), fk = lds4f(sm.f + 16 * kb + 4 * grp);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int j = jt + 16 * kb + 4 * grp + e;
-                        const float dec = lam * fast_exp2((gq[g] - gk[e]) * LOG2E);
-                        s[kb][e] = fmaf(fq[g] - fk[e], LOG2E, fmaf(qk[kb][e], 0.125f * LOG2E, dec * cb[kb][e]));
-                        s[kb][e] = j >= k.lo && j < lim[g] ? s[kb][e] : -__builtin_inff();
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    const int j = jt + 16 * kb + 4 * grp + e;
+                    const float dec = lam * fast_exp2((gq - gk[e]) * LOG2E);
+                    s[kb][e] = fmaf(fq - fk[e], LOG2E, fmaf(s[kb][e], 0.125f * LOG2E, dec * cb[kb][e]));
+                    s[kb][e] = j >= k.lo && j < lim ? s[kb][e] : -__builtin_inff();
                 }
             }
-            f32x4 p[2];
-            float sum;
-            auto weights = [&]() {
-                const float off = more - m2[g] + UP<T>;
-                sum = 0.f;
+        }
+        f32x4 p[2];
+        float sum;
+        auto weights = [&]() {
+            const float off = more - m2 + UP<T>;
+            sum = 0.f;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        p[kb][e] = fast_exp2(s[kb][e] + off);
-                        sum += p[kb][e];
-                    }
-            };
+                for (int e = 0; e < 4; ++e) {
+                    p[kb][e] = fast_exp2(s[kb][e] + off);
+                    sum += p[kb][e];
+                }
+        };
+        weights();
+        const bool over = sum > __builtin_exp2f(RAISE + UP<T>);
+        if (__ballot(over)) {
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kb][e]);
+            mx = group_max(mx) + more;
+            const float to = group_max(over ? 1.f : 0.f) > 0.f ? fmaxf(m2, mx) : m2, corr = fast_exp2(m2 - to);
+            m2 = to;
+            l *= corr;
+#pragma unroll
+            for (int db = 0; db < 4; ++db) o[db] *= corr;
             weights();
-            const bool over = sum > __builtin_exp2f(RAISE + UP<T>);
-            if (__ballot(over)) {
-                float mx = -__builtin_inff();
+        }
+        l += sum;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+        for (int i = 0; i < Split<T>::terms; ++i) {
+            const frag8<T> pf = pack8<T>(p[0], p[1]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[kb][e]);
-                mx = group_max(mx) + more;
-                const float to = group_max(over ? 1.f : 0.f) > 0.f ? fmaxf(m2[g], mx) : m2[g], corr = fast_exp2(m2[g] - to);
-                m2[g] = to;
-                l[g] *= corr;
+            for (int db = 0; db < 4; ++db) o[db] = mma(frag_tr<T, DH>(sm.v, 16 * db, 0, lane), pf, o[db]);
+            if (i + 1 < Split<T>::terms) {
+                const f32x8 back = __builtin_convertvector(pf, f32x8);
 #pragma unroll
-                for (int db = 0; db < 4; ++db) o[g][db] *= corr;
-                weights();
-            }
-            l[g] += sum;
-#pragma unroll
-            for (int i = 0; i < Split<T>::terms; ++i) {
-                const frag8<T> pf = pack8<T>(p[0], p[1]);
-#pragma unroll
-                for (int db = 0; db < 4; ++db) o[g][db] = mma(frag_tr<T, DH>(sm.v, 16 * db, 0, lane), pf, o[g][db]);
-                if (i + 1 < Split<T>::terms) {
-                    const f32x8 back = __builtin_convertvector(pf, f32x8);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) p[0][e] -= back[e], p[1][e] -= back[4 + e];
-                }
+                for (int e = 0; e < 4; ++e) p[0][e] -= back[e], p[1][e] -= back[4 + e];
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -411,68 +402,59 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2))) vo
         const int from = t.from * KT > k.lo ? t.from * KT : k.lo, to = t.to * KT < k.hi ? t.to * KT : k.hi;
         for (int j = from; j < to; ++j) {
             if ((j / KT + 1) * KT <= least && j / KT * KT >= k.lo) continue;       // its tile was taken whole
-            const int page = page_of(k.row, a.W, shift, a.pool.pages, j);
+            const int page = page_of(table, W, shift, pages, j);
             if (page < 0) continue;
-            const T* v = (const T*)a.pool.v.ptr + page * a.pool.v.sb + k.h * a.pool.v.sh + (j & (a.pool.page_size - 1)) * a.pool.v.sl;
-#pragma unroll 1
+            const T* v = (const T*)(ss.v.base + page * ss.v.page + (j & mask) * ss.v.row) + 4 * grp;
+#pragma unroll
             for (int db = 0; db < 4; ++db)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float y = (float)v[16 * db + 4 * grp + e];
-                    const bool bad = !(y - y == 0.f);
-#pragma unroll
-                    for (int g = 0; g < NR; ++g)
-#pragma unroll
-                        for (int d = 0; d < 4; ++d)
-                            if (d == db && bad && j < lim[g]) o[g][d][e] += y;
+                    const float y = (float)v[16 * db + e];
+                    if (!(y - y == 0.f) && j < lim) o[db][e] += y;
                 }
         }
     }
-
-    if (own) {
-        const float sum = group_sum(l[0]);
+    l = group_sum(l);
+    f32x2 *const stat = AGAIN(ws.stat), *const own_stat = AGAIN(ws.own_stat);
+    float *const part = AGAIN(ws.part), *const own_part = AGAIN(ws.own);
+    const unsigned own_rows = AGAIN(plan.own_rows);
+    // a row's output and sum, where no other wave of the workgroup has it
+    auto alone = [&](f32x2* to_stat, float* to_part, int64_t r) {
         if (lc >= k.rows) return;
-        const int64_t to = (int64_t)item * plan.own_rows + lc;
-        if (grp == 0) own_stat[to] = f32x2{m2[0] - UP<T>, sum};
+        if (grp == 0) to_stat[r] = f32x2{m2 - UP<T>, l};
 #pragma unroll
-        for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(own_part + to * DH + 16 * db + 4 * grp) = o[0][db];
+        for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(to_part + r * DH + 16 * db + 4 * grp) = o[db];
+    };
+    if (own) {
+        alone(own_stat, own_part, (int64_t)item * own_rows + lc);
         return;
     }
-    // the waves' parts of common positions joined, in order
+    const int64_t to = (int64_t)item << log_per;
+    if (log_rw == 2) {
+        alone(stat, part, to + 16 * w + lc);
+        return;
+    }
+    // the parts of the waves that have the same rows (every rw-th) joined, in order
+    if (grp == 0) ms[w][lc] = m2 - UP<T>, ls[w][lc] = l;
+    __syncthreads();
+    const int g0 = w & (rw - 1);
+    float cm = ms[g0][lc];
+    for (int i = g0 + rw; i < NW; i += rw) cm = fmaxf(cm, ms[i][lc]);
+    const float mine = fast_exp2(m2 - UP<T> - cm);
 #pragma unroll
-    for (int g = 0; g < NR; ++g) {
-        const float sum = group_sum(l[g]);
-        if (grp == 0) ms[w][16 * g + lc] = m2[g] - UP<T>, ls[w][16 * g + lc] = sum;
+    for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&os[w][lc][16 * db + 4 * grp]) = o[db] * mine;
+    if (w < rw && grp == 0 && lc < k.rows) {
+        float cl = 0.f;
+        for (int i = g0; i < NW; i += rw) cl = fmaf(ls[i][lc], fast_exp2(ms[i][lc] - cm), cl);
+        stat[to + 16 * w + lc] = f32x2{cm, cl};
     }
     __syncthreads();
-#pragma unroll
-    for (int g = 0; g < NR; ++g) {
-        if (g >= nr) break;
-        const int row = 16 * g + lc;
-        float cm = ms[0][row];
-#pragma unroll
-        for (int i = 1; i < NW; ++i) cm = fmaxf(cm, ms[i][row]);
-        auto factor = [&](float y) { return fast_exp2(y - cm); };
-        const float mine = factor(ms[w][row]);
-#pragma unroll
-        for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(&os[w][lc][16 * db + 4 * grp]) = o[g][db] * mine;
-        __syncthreads();
-        const int64_t to = (int64_t)item * PER + 16 * g;
-        {
-            static_assert(64 * NW == 16 * (DH / 4), "a thread per 4 features");
-            const int rr = tid / (DH / 4), d = 4 * (tid % (DH / 4));
-            f32x4 y = lds4f(&os[0][rr][d]);
-#pragma unroll
-            for (int i = 1; i < NW; ++i) y += lds4f(&os[i][rr][d]);
-            if (16 * g + rr < k.rows) *reinterpret_cast<f32x4*>(part + (to + rr) * DH + d) = y;
-        }
-        if (w == 0 && grp == 0) {
-            float cl = 0.f;
-#pragma unroll
-            for (int i = 0; i < NW; ++i) cl = fmaf(ls[i][row], factor(ms[i][row]), cl);
-            stat[to + lc] = f32x2{cm, cl};
-        }
-        __syncthreads();
+    static_assert(64 * NW == 16 * (DH / 4), "a thread per row of 16 and 4 features");
+    const int rr = tid / (DH / 4), d = 4 * (tid % (DH / 4));
+    for (int g = 0; g < rw; ++g) {
+        f32x4 y = lds4f(&os[g][rr][d]);
+        for (int i = g + rw; i < NW; i += rw) y += lds4f(&os[i][rr][d]);
+        *reinterpret_cast<f32x4*>(part + (to + 16 * g + rr) * DH + d) = y;
     }
 }
 
@@ -511,9 +493,9 @@ __global__ __launch_bounds__(64 * NW) void prefix_join_kernel(sisa_prefix_decode
     };
     auto each_of = [](int n, unsigned parts) { return (int)(((unsigned)n + parts - 1) / parts); };
     const int first = lo / KT, tiles = (lo + KT - 1) / KT, own_tiles = (end + KT - 1) / KT - first;
-    const int nc = active(tiles, NW * each_of(tiles, plan.parts * NW), 0);
+    const int kw = NW << 4 >> log_per, nc = active(tiles, kw * each_of(tiles, plan.parts * kw), 0);
     const int no = vis > lo ? active(own_tiles, each_of(own_tiles, plan.own_parts), first) : 0;
-    const int64_t at = (((int64_t)h * plan.tiles + tile) << log_per) + (mine & (per - 1)), step = ((int64_t)H * plan.tiles) << log_per;
+    const int64_t at = ((tile * plan.parts * H + h) << log_per) + (mine & (per - 1)), step = (int64_t)H << log_per;
     const int64_t own_at = (((int64_t)n * plan.own_tiles + (m >> 4)) * H + h) * plan.own_rows + (m & 15),
                   own_step = (int64_t)a.B * plan.own_tiles * H * plan.own_rows;
     const f32x2 s0 = lane < nc ? stat[at + lane * step] : f32x2{LEAST, 0.f};
@@ -558,8 +540,8 @@ __global__ __launch_bounds__(64 * NW) void prefix_join_kernel(sisa_prefix_decode
 Plan plan_of(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64_t max_shared) {
     Plan p{};
     const int64_t rows = sisa::cdiv(B, G) * M;           // of a group, on average
-    p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const int64_t per = 16 * p.nr;
+    p.log_rw = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
+    const int64_t per = (int64_t)16 << p.log_rw;
     p.tiles = (unsigned)(max_shared > 0 ? G + B * M / per : 0);
     p.own_tiles = (unsigned)sisa::cdiv(M, 16);
     p.own_rows = (unsigned)(M < 16 ? M : 16);
@@ -568,20 +550,15 @@ Plan plan_of(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64_
         const int64_t n = want < most ? want : most;
         return (unsigned)(n < 1 ? 1 : n > MOST ? MOST : n);
     };
-    p.parts = parts(p.tiles * H, 1024, max_shared, KT * NW);
+    p.parts = parts(p.tiles * H, 1024, max_shared, KT * NW >> p.log_rw);
     p.own_parts = parts(B * p.own_tiles * H, 4096, max_len, KT);
     p.items = (int64_t)p.parts * p.tiles * H;
     p.own_items = (int64_t)p.own_parts * B * p.own_tiles * H;
     return p;
 }
 
-struct Space {
-    f32x2 *stat, *own_stat;
-    float *part, *own;
-    int64_t bytes;
-};
 Space space_of(char* base, const Plan& p) {
-    const int64_t rows = p.items * 16 * p.nr, own = p.own_items * p.own_rows;
+    const int64_t rows = p.items * 16 << p.log_rw, own = p.own_items * p.own_rows;
     Space s{};
     char* at = base;
     auto take = [&](int64_t bytes) {
@@ -602,7 +579,7 @@ int64_t workgroups(const Plan& p) { return p.items + sisa::cdiv(p.own_items, NW)
 template <class T, class TO>
 int launch_join(const sisa_prefix_decode_args* a, const Plan& p, int shift, const Space& ws, hipStream_t st) {
     const int64_t rows = (int64_t)a->B * a->pool.heads * a->M;
-    const int log_per = p.nr == 1 ? 4 : p.nr == 2 ? 5 : 6;
+    const int log_per = 4 + p.log_rw;
     if (rows < 2048)
         prefix_join_kernel<TO, NW><<<(unsigned)rows, 64 * NW, 0, st>>>(*a, p, shift, log_per, ws.stat, ws.part, ws.own_stat, ws.own);
     else prefix_join_kernel<TO, 1><<<(unsigned)sisa::cdiv(rows, NW), 64 * NW, 0, st>>>(*a, p, shift, log_per, ws.stat, ws.part, ws.own_stat, ws.own);
@@ -614,14 +591,15 @@ int launch(const sisa_prefix_decode_args* a, const Plan& p, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size);
     const Space ws = space_of((char*)a->workspace, p);
     const unsigned grid = (unsigned)workgroups(p);
-    switch (p.nr) {
-        case 1: prefix_part_kernel<T, 1><<<grid, 64 * NW, 0, st>>>(*a, p, shift, ws.stat, ws.part, ws.own_stat, ws.own); break;
-        case 2: prefix_part_kernel<T, 2><<<grid, 64 * NW, 0, st>>>(*a, p, shift, ws.stat, ws.part, ws.own_stat, ws.own); break;
-        default: prefix_part_kernel<T, 4><<<grid, 64 * NW, 0, st>>>(*a, p, shift, ws.stat, ws.part, ws.own_stat, ws.own);
-    }
+    prefix_part_kernel<T><<<grid, 64 * NW, 0, st>>>(PartArgs{*a, p, shift, ws});
     const int rc = sisa::launch_status("sisa_prefix_decode");
     if (rc) return rc;
     return a->out_dtype == SISA_F32 ? launch_join<T, float>(a, p, shift, ws, st) : launch_join<T, T>(a, p, shift, ws, st);
+}
+
+// Rows of a page that 32-bit offsets reach, each behind the last.
+bool rows_ok(const sisa_page_pool& p, const sisa_view& x, int width, int size) {
+    return x.sl >= width && (int64_t)p.page_size * x.sl * size <= 0x7fffff00;
 }
 
 bool sizes_ok(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64_t max_shared) {
@@ -651,6 +629,11 @@ extern "C" int sisa_prefix_decode(const sisa_prefix_decode_args* a, void* stream
                  "sisa_prefix_decode: null pointer");
     SISA_REQUIRE(a->workspace && sisa::aligned16(a->workspace), "sisa_prefix_decode: null workspace, or not 16-byte aligned");
     SISA_REQUIRE(a->out_dtype == SISA_F32 || a->out_dtype == a->pool.dtype, "sisa_prefix_decode: out_dtype");
+    const sisa_page_pool& P = a->pool;
+    const int es = sisa::elem_size(P.dtype);
+    SISA_REQUIRE(rows_ok(P, P.k, DH, es) && rows_ok(P, P.v, DH, es) && rows_ok(P, P.b, DS, es) && rows_ok(P, P.g, 1, 4) &&
+                     (!P.f.ptr || rows_ok(P, P.f, 1, 4)),
+                 "sisa_prefix_decode: the positions of a page must be at least a row apart, and all of a head's within 2 GiB");
     SISA_REQUIRE(sisa::view_ok(a->q, a->pool.dtype) && sisa::view_ok(a->c, a->pool.dtype),
                  "sisa_prefix_decode: q and c rows must be 16-byte aligned");
     SISA_REQUIRE(a->gq.ptr && (a->fq.ptr == nullptr) == (a->pool.f.ptr == nullptr),
