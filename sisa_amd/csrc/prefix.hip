@@ -27,7 +27,8 @@ constexpr int MOST = 64;              // most parts of a range: the join has a l
 struct Plan {
     int log_rw;
     unsigned tiles, own_tiles, parts, own_parts, own_rows;
-    int64_t items, own_items;         // workgroups, waves
+    unsigned items, own_items;        // workgroups and waves of a head
+    unsigned blocks;                  // workgroups of the common parts, of all heads
 };
 
 // Tiles of all groups' query rows: group r's begin at r + floor(first[r] M / rows of a tile), which leaves room for each.
@@ -88,7 +89,18 @@ struct Tile {
     float g[2], f[2];
 };
 
-// Loads at a lane's offset from a scalar base, 0 where it is not below `bytes`.
+// A scalar in registers of its own: as part of the wide load of the kernel's arguments it would keep all of that alive.
+template <class X> SISA_DEV X apart(X x) {
+    asm("" : "+s"(x));
+    return x;
+}
+
+// The exponents of a 32-bit word of T, 1 in their lowest places, and the signs.
+template <class T> constexpr unsigned EXPONENT = sizeof(T) == 4 ? 0x7f800000 : __is_same(T, __bf16) ? 0x7f807f80 : 0x7c007c00;
+template <class T> constexpr unsigned EXPONENT_ONE = sizeof(T) == 4 ? 0x00800000 : __is_same(T, __bf16) ? 0x00800080 : 0x04000400;
+template <class T> constexpr unsigned SIGN = sizeof(T) == 4 ? 0x80000000 : 0x80008000;
+
+// Loads at a lane's offset from a scalar base and a scalar one, 0 from `bytes` on.
 template <class V> SISA_DEV V load_at(const char* base, int bytes, int voff, int soff) {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(base, bytes);
     if constexpr (sizeof(V) == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0));
@@ -97,12 +109,6 @@ template <class V> SISA_DEV V load_at(const char* base, int bytes, int voff, int
 template <class T> SISA_DEV frag8<T> load_frag(const char* base, int bytes, int voff, int soff) {
     if constexpr (sizeof(T) == 2) return load_at<frag8<T>>(base, bytes, voff, soff);
     else return join<T>(load_at<f32x4>(base, bytes, voff, soff), load_at<f32x4>(base, bytes, voff, soff + 16));
-}
-
-// A scalar in registers of its own: as part of the wide load of the kernel's arguments it would keep all of that alive.
-template <class X> SISA_DEV X apart(X x) {
-    asm("" : "+s"(x));
-    return x;
 }
 
 // One tensor of the pool as a head's waves see it: where the head begins, bytes from page to page and from row to row, and
@@ -117,26 +123,8 @@ struct Stream {
         row = apart((int)x.sl * size);
         lane = lane_row * row + lane_col;
     }
+    SISA_DEV const char* at(int p) const { return base + p * page; }
 };
-struct Streams {
-    Stream k, v, b, g, f;
-};
-
-// 16 positions of a tile from slot `slot` of page p on, `n` of them (0 without a page); the other rows are 0.
-template <class T>
-SISA_DEV void load_half(const Streams& s, int p, int slot, int n, int kb, Tile<T>& x) {
-    constexpr int HALF = Tile<T>::PASS / 2, ROWS = 64 / Tile<T>::CPR;
-    const int end = slot + n;
-    const char *pk = s.k.base + p * s.k.page, *pv = s.v.base + p * s.v.page, *pb = s.b.base + p * s.b.page;
-    x.k[kb][0] = load_frag<T>(pk, n ? end * s.k.row : 0, s.k.lane, slot * s.k.row);
-    x.k[kb][1] = load_frag<T>(pk, n ? end * s.k.row : 0, s.k.lane, slot * s.k.row + 32 * (int)sizeof(T));
-    x.b[kb] = load_frag<T>(pb, n ? end * s.b.row : 0, s.b.lane, slot * s.b.row);
-    x.g[kb] = load_at<float>(s.g.base + p * s.g.page, n ? end * s.g.row : 0, s.g.lane, slot * s.g.row);
-    x.f[kb] = load_at<float>(s.f.base + p * s.f.page, n ? end * s.f.row : 0, s.f.lane, slot * s.f.row);
-#pragma unroll
-    for (int i = 0; i < HALF; ++i)
-        x.v[HALF * kb + i] = load_at<u32x4>(pv, n ? end * s.v.row : 0, s.v.lane, (slot + ROWS * i) * s.v.row);
-}
 
 struct Space {
     f32x2 *stat, *own_stat;
@@ -170,19 +158,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     const Plan& plan = args.plan;
     const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4, lc = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const bool own = blockIdx.x >= (unsigned)plan.items;
-    const int64_t held = (int64_t)a.W << args.shift;
+    // The heads of an item, whose rows are neighbours in memory, follow each other.
     const unsigned H = a.pool.heads;
+    const bool own = blockIdx.x >= plan.blocks;
+    const unsigned nth = own ? (blockIdx.x - plan.blocks) * NW + w : blockIdx.x, item = nth / H;
+    const int64_t held = (int64_t)a.W << args.shift;
     const int log_rw = plan.log_rw, rw = 1 << log_rw, log_per = 4 + log_rw;
-    const unsigned item = own ? (blockIdx.x - (unsigned)plan.items) * NW + w : blockIdx.x;
     Work k;
+    k.h = nth - item * H;
     Range t;                                             // the wave's tiles
     if (own) {
         if (item >= plan.own_items) return;
-        const unsigned nm = item / H, pn = plan.own_tiles == 1 ? nm : nm / plan.own_tiles, p = pn / (unsigned)a.B, n = pn - p * a.B;
-        k.h = item - nm * H;
+        const unsigned pn = plan.own_tiles == 1 ? item : item / plan.own_tiles, p = pn / (unsigned)a.B, n = pn - p * a.B;
         k.n0 = n;
-        k.r0 = 16 * (nm - pn * plan.own_tiles);
+        k.r0 = 16 * (item - pn * plan.own_tiles);
         k.rows = a.M - k.r0 < 16 ? a.M - k.r0 : 16;
         const int r = a.group[n];
         k.hi = visible(a, held, n, k.r0 + k.rows - 1);
@@ -195,9 +184,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         t.from += first;
         t.to += first;
     } else {
-        // tile by tile: those that no group needs come last, and the others spread over all XCDs
-        const unsigned tp = item / H, tile = tp / plan.parts, p = tp - tile * plan.parts;
-        k.h = item - tp * H;
+        // tile by tile: those that no group needs come last
+        const unsigned tile = item / plan.parts, p = item - tile * plan.parts;
         int r = 0;                                       // the last group whose tiles begin at or before this one
         if (a.G > 1) {
             r = -1;
@@ -207,9 +195,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         const int f0 = a.first[r], f1 = a.first[r + 1];
         k.hi = common(a, held, r);
         if (f0 < 0 || f1 > a.B || f1 <= f0 || k.hi <= 0) return;
-        const int64_t all = (int64_t)(f1 - f0) * a.M, nth = (int64_t)tile - tile_base(a, r, log_per);
-        const int64_t at = (nth << log_per) + 16 * (w & (rw - 1));
-        if (nth < 0 || nth << log_per >= all) return;
+        const int64_t all = (int64_t)(f1 - f0) * a.M, past = (int64_t)tile - tile_base(a, r, log_per);
+        const int64_t at = (past << log_per) + 16 * (w & (rw - 1));
+        if (past < 0 || past << log_per >= all) return;
         k.n0 = f0;
         k.r0 = at;
         k.rows = at >= all ? 0 : all - at < 16 ? all - at : 16;
@@ -219,7 +207,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         t = part_of(n, plan.parts * kw, p * kw + (w >> log_rw));
         if (!k.rows) t.to = t.from;
     }
-    const int32_t* table = apart(a.table + k.n0 * a.s_table);
+    const auto table = apart((const __attribute__((address_space(1))) int32_t*)a.table + k.n0 * a.s_table);
 
     // Column lc of the operand is query row lc, in all four groups of lanes; behind the last row the last again.
     frag8<T> q[2], c;
@@ -246,36 +234,64 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     }
     const float lam = a.lam[k.h * a.s_lam] * LOG2E;
     const int mask = apart(a.pool.page_size - 1), pages = apart(a.pool.pages), W = apart(a.W), shift = apart(args.shift);
-    const int max_len = apart(a.max_len), row_f = a.pool.f.ptr ? 1 : 0;
+    const int max_len = apart(a.max_len);
+    const bool has_f = a.pool.f.ptr != nullptr;
     using X = Tile<T>;
-    Streams ss;
+    Stream sk, sv, sb, sg, sf;
     {
         const int row = lane / X::CPR, col = 16 * (lane % X::CPR), part = 8 * grp * (int)sizeof(T);
-        ss.k.init(a.pool.k, k.h, sizeof(T), lc, part);
-        ss.v.init(a.pool.v, k.h, sizeof(T), row, col);
-        ss.b.init(a.pool.b, k.h, sizeof(T), lc, part);
-        ss.g.init(a.pool.g, k.h, 4, lc, 0);
-        ss.f.init(a.pool.f, k.h, 4, lc, 0);
-        if (!row_f) ss.f.row = 0;                        // no forget term: every F is 0
+        sk.init(a.pool.k, k.h, sizeof(T), lc, part);
+        sv.init(a.pool.v, k.h, sizeof(T), row, col);
+        sb.init(a.pool.b, k.h, sizeof(T), lc, part);
+        sg.init(a.pool.g, k.h, 4, lc, 0);
+        sf.init(has_f ? a.pool.f : a.pool.g, k.h, 4, lc, 0);
     }
 
+    auto page_at = [&](int j) {                          // -1: none of the pool's
+        const int i = j >> shift, p = i < W ? table[i] : -1;
+        return p < pages ? p : -1;
+    };
     WaveLds<T>& sm = lds[w];
     bool odd = false;
     int near_pages = -1, base = t.from - 32;             // lane i: the page of the 16 positions from 16 (2 base + i) on
+#pragma unroll 1
     for (int tile = t.from; tile < t.to; ++tile) {
         const int jt = tile * KT;
         if (tile - base >= 32) {
             base = tile;
             const int j = 16 * (2 * base + lane);
-            near_pages = j < k.hi && j + 16 > k.lo ? page_of(table, W, shift, pages, j) : -1;
+            near_pages = j < k.hi ? page_at(j) : -1;
         }
+        // Rows from hi on are 0, and so are those of pages that are not there, whose F is NaN. The second half lies in the
+        // first one's page but for pages of 16.
         X x;
+        {
+            const int i = 2 * (tile - base), p0 = __builtin_amdgcn_readlane(near_pages, i), p1 = __builtin_amdgcn_readlane(near_pages, i + 1);
+            const int left = k.hi - jt, at0 = p0 < 0 ? 0 : p0, at1 = p1 < 0 ? 0 : p1;
+            int slot = jt & mask, end = slot + (left < KT ? left : KT);
+            end = p0 < 0 ? 0 : end;
+            const char *bk = sk.at(at0), *bv = sv.at(at0), *bb = sb.at(at0), *bg = sg.at(at0), *bf = sf.at(at0);
+            constexpr int ROWS = 64 / X::CPR, HALF = X::PASS / 2;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const int page = __builtin_amdgcn_readlane(near_pages, 2 * (tile - base) + kb), j0 = jt + 16 * kb;
-            const int left = k.hi - j0 < 16 ? k.hi - j0 : 16;
-            load_half<T>(ss, page < 0 ? 0 : page, j0 & mask, page < 0 || left < 0 ? 0 : left, kb, x);
-            if (page < 0) x.f[kb] = __builtin_nanf("");
+            for (int kb = 0; kb < 2; ++kb) {
+                if (kb) {
+                    if (mask < 16) {
+                        bk = sk.at(at1), bv = sv.at(at1), bb = sb.at(at1), bg = sg.at(at1), bf = sf.at(at1);
+                        slot = -16;
+                        end = p1 < 0 || left < 16 ? 0 : left - 16;
+                    }
+                    slot += 16;
+                }
+                x.k[kb][0] = load_frag<T>(bk, end * sk.row, sk.lane, slot * sk.row);
+                x.k[kb][1] = load_frag<T>(bk, end * sk.row, sk.lane, slot * sk.row + 32 * (int)sizeof(T));
+                x.b[kb] = load_frag<T>(bb, end * sb.row, sb.lane, slot * sb.row);
+                x.g[kb] = load_at<float>(bg, end * sg.row, sg.lane, slot * sg.row);
+                x.f[kb] = load_at<float>(bf, has_f ? end * sf.row : 0, sf.lane, slot * sf.row);
+#pragma unroll
+                for (int r = 0; r < HALF; ++r) x.v[HALF * kb + r] = load_at<u32x4>(bv, end * sv.row, sv.lane, (slot + ROWS * r) * sv.row);
+            }
+            if (p0 < 0) x.f[0] = __builtin_nanf("");
+            if (p1 < 0) x.f[1] = __builtin_nanf("");
         }
         if (tile == t.from) {                            // the first loads are under way: what has come of the query rows
             const int seen = len - back;
@@ -293,17 +309,25 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         const bool mixed = jt + KT > least || jt < k.lo;               // some row does not see all of the tile
         if (mixed) {
             // Values that are not finite, at positions that some row does not see: 0 in the product (0 times them would be
-            // NaN there), and added to the rows that see them at the end.
+            // NaN there), and added to the rows that see them at the end. An exponent of ones carries into the sign's place.
+            unsigned ones = 0;
 #pragma unroll
-            for (int i = 0; i < X::PASS; ++i) {
-                T e[X::E];
-                __builtin_memcpy(e, &x.v[i], 16);
+            for (int i = 0; i < X::PASS; ++i)
 #pragma unroll
-                for (int j = 0; j < X::E; ++j) {
-                    const float y = (float)e[j];
-                    if (!(y - y == 0.f)) e[j] = (T)0.f, odd = true;
+                for (int e = 0; e < 4; ++e) ones |= (x.v[i][e] & EXPONENT<T>) + EXPONENT_ONE<T>;
+            if (__ballot((ones & SIGN<T>) != 0)) {
+                odd = true;
+#pragma unroll
+                for (int i = 0; i < X::PASS; ++i) {
+                    T e[X::E];
+                    __builtin_memcpy(e, &x.v[i], 16);
+#pragma unroll
+                    for (int j = 0; j < X::E; ++j) {
+                        const float y = (float)e[j];
+                        if (!(y - y == 0.f)) e[j] = (T)0.f;
+                    }
+                    __builtin_memcpy(&x.v[i], e, 16);
                 }
-                __builtin_memcpy(&x.v[i], e, 16);
             }
         }
 #pragma unroll
@@ -398,13 +422,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();                 // the tile has been read
     }
-    if (__ballot(odd)) {
+    if (odd) {
         const int from = t.from * KT > k.lo ? t.from * KT : k.lo, to = t.to * KT < k.hi ? t.to * KT : k.hi;
         for (int j = from; j < to; ++j) {
             if ((j / KT + 1) * KT <= least && j / KT * KT >= k.lo) continue;       // its tile was taken whole
-            const int page = page_of(table, W, shift, pages, j);
+            const int page = page_at(j);
             if (page < 0) continue;
-            const T* v = (const T*)(ss.v.base + page * ss.v.page + (j & mask) * ss.v.row) + 4 * grp;
+            const T* v = (const T*)(sv.at(page) + (j & mask) * sv.row) + 4 * grp;
 #pragma unroll
             for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -417,7 +441,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
     l = group_sum(l);
     f32x2 *const stat = AGAIN(ws.stat), *const own_stat = AGAIN(ws.own_stat);
     float *const part = AGAIN(ws.part), *const own_part = AGAIN(ws.own);
-    const unsigned own_rows = AGAIN(plan.own_rows);
+    const unsigned own_rows = AGAIN(plan.own_rows), own_items = AGAIN(plan.own_items), items = AGAIN(plan.items);
     // a row's output and sum, where no other wave of the workgroup has it
     auto alone = [&](f32x2* to_stat, float* to_part, int64_t r) {
         if (lc >= k.rows) return;
@@ -426,10 +450,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         for (int db = 0; db < 4; ++db) *reinterpret_cast<f32x4*>(to_part + r * DH + 16 * db + 4 * grp) = o[db];
     };
     if (own) {
-        alone(own_stat, own_part, (int64_t)item * own_rows + lc);
+        alone(own_stat, own_part, ((int64_t)k.h * own_items + item) * own_rows + lc);
         return;
     }
-    const int64_t to = (int64_t)item << log_per;
+    const int64_t to = ((int64_t)k.h * items + item) << log_per;
     if (log_rw == 2) {
         alone(stat, part, to + 16 * w + lc);
         return;
@@ -495,9 +519,9 @@ __global__ __launch_bounds__(64 * NW) void prefix_join_kernel(sisa_prefix_decode
     const int first = lo / KT, tiles = (lo + KT - 1) / KT, own_tiles = (end + KT - 1) / KT - first;
     const int kw = NW << 4 >> log_per, nc = active(tiles, kw * each_of(tiles, plan.parts * kw), 0);
     const int no = vis > lo ? active(own_tiles, each_of(own_tiles, plan.own_parts), first) : 0;
-    const int64_t at = ((tile * plan.parts * H + h) << log_per) + (mine & (per - 1)), step = (int64_t)H << log_per;
-    const int64_t own_at = (((int64_t)n * plan.own_tiles + (m >> 4)) * H + h) * plan.own_rows + (m & 15),
-                  own_step = (int64_t)a.B * plan.own_tiles * H * plan.own_rows;
+    const int64_t at = (((int64_t)h * plan.items + tile * plan.parts) << log_per) + (mine & (per - 1)), step = per;
+    const int64_t own_at = ((int64_t)h * plan.own_items + (int64_t)n * plan.own_tiles + (m >> 4)) * plan.own_rows + (m & 15),
+                  own_step = (int64_t)a.B * plan.own_tiles * plan.own_rows;
     const f32x2 s0 = lane < nc ? stat[at + lane * step] : f32x2{LEAST, 0.f};
     const f32x2 s1 = lane < no ? own_stat[own_at + lane * own_step] : f32x2{LEAST, 0.f};
     float mx = fmaxf(s0[0], s1[0]);
@@ -545,20 +569,27 @@ Plan plan_of(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64_
     p.tiles = (unsigned)(max_shared > 0 ? G + B * M / per : 0);
     p.own_tiles = (unsigned)sisa::cdiv(M, 16);
     p.own_rows = (unsigned)(M < 16 ? M : 16);
-    auto parts = [](int64_t items, int64_t total, int64_t positions, int64_t each) {
-        const int64_t most = sisa::cdiv(positions, each), want = items > 0 ? sisa::cdiv(total, items) : 1;
-        const int64_t n = want < most ? want : most;
+    // As many parts as fill the chip while a wave keeps a tile, or, for longer ranges, more of them of eight tiles to a wave,
+    // which even out: `few` and `many` workgroups, or waves, in all. us of the first launch, few alone / many alone / the larger
+    // of both: 16 rows of 2,000 common positions of 12 heads 9.4 / 14.1 / 9.4; 24 x 8 drafts of up to 6,000 53 / 41 / 41.
+    auto parts = [](int64_t items, int64_t positions, int64_t tile, int64_t few, int64_t many) {
+        auto of = [&](int64_t total, int64_t each) {
+            const int64_t most = sisa::cdiv(positions, each), want = items > 0 ? sisa::cdiv(total, items) : 1;
+            return want < most ? want : most;
+        };
+        const int64_t a = of(few, tile), b = of(many, 8 * tile), n = a > b ? a : b;
         return (unsigned)(n < 1 ? 1 : n > MOST ? MOST : n);
     };
-    p.parts = parts(p.tiles * H, 1024, max_shared, KT * NW >> p.log_rw);
-    p.own_parts = parts(B * p.own_tiles * H, 4096, max_len, KT);
-    p.items = (int64_t)p.parts * p.tiles * H;
-    p.own_items = (int64_t)p.own_parts * B * p.own_tiles * H;
+    p.parts = parts(p.tiles * H, max_shared, KT * NW >> p.log_rw, 512, 2048);
+    p.own_parts = parts(B * p.own_tiles * H, max_len, KT, 2048, 16384);
+    p.items = p.parts * p.tiles;
+    p.own_items = (unsigned)(p.own_parts * B * p.own_tiles);
+    p.blocks = (unsigned)(H * p.items);
     return p;
 }
 
-Space space_of(char* base, const Plan& p) {
-    const int64_t rows = p.items * 16 << p.log_rw, own = p.own_items * p.own_rows;
+Space space_of(char* base, const Plan& p, int64_t H) {
+    const int64_t rows = H * p.items * 16 << p.log_rw, own = H * p.own_items * p.own_rows;
     Space s{};
     char* at = base;
     auto take = [&](int64_t bytes) {
@@ -574,7 +605,7 @@ Space space_of(char* base, const Plan& p) {
     return s;
 }
 
-int64_t workgroups(const Plan& p) { return p.items + sisa::cdiv(p.own_items, NW); }
+int64_t workgroups(const Plan& p, int64_t H) { return H * p.items + sisa::cdiv(H * p.own_items, NW); }
 
 template <class T, class TO>
 int launch_join(const sisa_prefix_decode_args* a, const Plan& p, int shift, const Space& ws, hipStream_t st) {
@@ -589,8 +620,8 @@ int launch_join(const sisa_prefix_decode_args* a, const Plan& p, int shift, cons
 template <class T>
 int launch(const sisa_prefix_decode_args* a, const Plan& p, hipStream_t st) {
     const int shift = sisa::log2_of(a->pool.page_size);
-    const Space ws = space_of((char*)a->workspace, p);
-    const unsigned grid = (unsigned)workgroups(p);
+    const Space ws = space_of((char*)a->workspace, p, a->pool.heads);
+    const unsigned grid = (unsigned)workgroups(p, a->pool.heads);
     prefix_part_kernel<T><<<grid, 64 * NW, 0, st>>>(PartArgs{*a, p, shift, ws});
     const int rc = sisa::launch_status("sisa_prefix_decode");
     if (rc) return rc;
@@ -612,7 +643,7 @@ bool sizes_ok(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64
 extern "C" int64_t sisa_prefix_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t G, int32_t max_len,
                                                       int32_t max_shared) {
     if (!sizes_ok(B, H, M, G, max_len, max_shared)) return 0;
-    return space_of(nullptr, plan_of(B, H, M, G, max_len, max_shared)).bytes;
+    return space_of(nullptr, plan_of(B, H, M, G, max_len, max_shared), H).bytes;
 }
 
 extern "C" int sisa_prefix_decode(const sisa_prefix_decode_args* a, void* stream) {
@@ -639,7 +670,7 @@ extern "C" int sisa_prefix_decode(const sisa_prefix_decode_args* a, void* stream
     SISA_REQUIRE(a->gq.ptr && (a->fq.ptr == nullptr) == (a->pool.f.ptr == nullptr),
                  "sisa_prefix_decode: gq must be given, and fq where the pool has f");
     const Plan p = plan_of(a->B, a->pool.heads, a->M, a->G, a->max_len, a->max_shared);
-    SISA_REQUIRE(workgroups(p) * 64 * NW <= sisa::MAX_THREADS && (int64_t)a->B * a->M * a->pool.heads * 64 <= sisa::MAX_THREADS - 64 * NW,
+    SISA_REQUIRE(workgroups(p, a->pool.heads) * 64 * NW <= sisa::MAX_THREADS && (int64_t)a->B * a->M * a->pool.heads * 64 <= sisa::MAX_THREADS - 64 * NW,
                  "sisa_prefix_decode: too large for one launch");
     hipStream_t st = (hipStream_t)stream;
     switch (a->pool.dtype) {
