@@ -92,6 +92,7 @@ def test_verification_refuses_bad_arguments(lib):
         return _lib.VerifyArgs(B, K, V, p_dtype, q_dtype, 0, p, 16, 8, q, 8, 8, drafts, 1, 1, u, 2, 1, None, tokens, accepted, ws)
     for bad, word in ((dict(B=-1), "bad shape"), (dict(K=-1), "bad shape"), (dict(V=0), "bad shape"), (dict(V=(1 << 24) + 1), "2^24"),
                       (dict(B=(1 << 21) + 1), "2^21"), (dict(p_dtype=_lib.F64), "fp32, bf16 or fp16"), (dict(q_dtype=7), "fp32, bf16 or fp16"),
+                      (dict(ws=None), "workspace"), (dict(ws=4104), "workspace"), (dict(B=1 << 20, V=1 << 20), "too large"),
                       *((dict([(x, None)]), "null pointer") for x in ("p", "drafts", "u", "tokens", "accepted"))):
         _refused(lib, "sisa_verify", args(**bad), word)
     assert lib.sisa_verify(ctypes.byref(args(B=0)), None) == 0
@@ -101,6 +102,12 @@ def test_workspaces(lib):
     size = lib.sisa_prefix_decode_workspace_bytes
     assert size(0, 1, 1, 1, 1, 0) == size(1, 1, 1, 2, 1, 0) == size(1, 1, 1, 1, 0, 0) == size(1, 1, 1, 1, 1, -1) == 0
     assert size(16, 12, 1, 1, 3000, 2000) > size(16, 12, 1, 1, 3000, 0) > 0
+
+
+def test_verification_workspace(lib):
+    size = lib.sisa_verify_workspace_bytes
+    assert size(0, 8) == size(1, 0) == size(1, (1 << 24) + 1) == 0
+    assert size(3, 50277) >= 3 * 50 * 16 and size(1, 1) > 0
 
 
 def test_python_calls_refuse_tensors_off_the_gpu(lib):
