@@ -38,12 +38,30 @@ typedef struct {
     sisa_view q, c;            /* (B,H,M,64|32) in the pool's dtype */
     sisa_view gq, fq;          /* (B,H,M) fp32; fq.ptr NULL exactly where the pool's f is */
     const float* lam; int64_t s_lam;           /* (H) fp32 */
-    void* out;                 /* (B,H,M,64) contiguous in out_dtype */
-    void* workspace;           /* 16-byte aligned; NULL where none is needed */
+    sisa_view out;             /* (B,H,M,64) in out_dtype, unit last stride */
+    void* workspace;           /* 16-byte aligned */
 } sisa_prefix_decode_args;
 
 int64_t sisa_prefix_decode_workspace_bytes(int32_t B, int32_t H, int32_t M, int32_t G, int32_t max_len, int32_t max_shared);
 int sisa_prefix_decode(const sisa_prefix_decode_args* a, void* stream);
+
+/* sisa_step_paged for M new positions of each of step.B sequences in groups: x, res, h and ffn are of step.B * M rows (at most
+ * SISA_STEP_MAX_ROWS), row m of sequence n at n * M + m, at position step.start[n] + m; step.lengths[n] = start[n] + M. The
+ * attention is sisa_prefix_decode's, first, group, shared and max_shared as there; step.weights is not used (NULL). A sequence
+ * one of whose positions has no page of the pool ends with NaN from that row on, all of its attention with it. rows, or NULL:
+ * what the recurrences continue from, (B,H,.) of 18 fp32 values (g, F, 16 phases) each s_rows values apart for a sequence
+ * and head: before this call at row0, after position m at row0 + 1 + m. */
+#define SISA_BRANCH_ROW 18
+typedef struct {
+    sisa_step_paged_args step;
+    int32_t M, G, max_shared, row0;
+    const int32_t *first, *group, *shared;     /* (G + 1), (B), (G) */
+    float* rows; int64_t s_rows;
+} sisa_step_branch_args;
+
+int64_t sisa_step_branch_workspace_bytes(int32_t B, int32_t H, int32_t D, int32_t FF, int32_t M, int32_t G, int32_t max_len,
+                                         int32_t max_shared);
+int sisa_step_branch(const sisa_step_branch_args* a, void* stream);
 
 /* Drafted tokens against the target's probabilities, by given random numbers. p[n,i] are the target's probabilities of what
  * follows i drafts of row n, q[n,i] those that draft i was drawn from. Draft i < counts[n] is accepted while all before it
@@ -65,7 +83,7 @@ typedef struct {
     const int32_t* counts;     /* (B), or NULL: K of each row */
     int64_t* tokens;           /* (B, K+1) contiguous */
     int32_t* accepted;         /* (B) */
-    void* workspace;           /* 16-byte aligned; NULL where none is needed */
+    void* workspace;           /* 16-byte aligned */
 } sisa_verify_args;
 
 #define SISA_VERIFY_MAX_V (1 << 24)

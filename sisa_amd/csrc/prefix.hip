@@ -495,7 +495,7 @@ __global__ __launch_bounds__(64 * NW) void prefix_join_kernel(sisa_prefix_decode
     if (WPR == 1 && row >= (unsigned)a.B * H * M) return;
     const unsigned nh = M == 1 ? row : row / M, m = row - nh * M, n = nh / H, h = nh - n * H;
     const int64_t held = (int64_t)a.W << shift;
-    TO* out = (TO*)a.out + (int64_t)row * DH + lane;
+    TO* out = (TO*)a.out.ptr + n * a.out.sb + h * a.out.sh + m * a.out.sl + lane;
     const int r = a.group[n], vis = visible(a, held, n, m), last = (m | 15) < M ? m | 15 : M - 1;
     const int end = visible(a, held, n, last);
     int lo = -1, f0 = 0, f1 = 0;
@@ -656,7 +656,7 @@ extern "C" int sisa_prefix_decode(const sisa_prefix_decode_args* a, void* stream
                  "sisa_prefix_decode: bad shape B=%d M=%d W=%d G=%d max_len=%d max_shared=%d (1 to B groups; at most W pages of "
                  "%d, and 2^30 positions; B*M*H at most 2^28)",
                  a->B, a->M, a->W, a->G, a->max_len, a->max_shared, a->pool.page_size);
-    SISA_REQUIRE(a->table && a->lengths && a->first && a->group && a->shared && a->lam && a->out,
+    SISA_REQUIRE(a->table && a->lengths && a->first && a->group && a->shared && a->lam && a->out.ptr,
                  "sisa_prefix_decode: null pointer");
     SISA_REQUIRE(a->workspace && sisa::aligned16(a->workspace), "sisa_prefix_decode: null workspace, or not 16-byte aligned");
     SISA_REQUIRE(a->out_dtype == SISA_F32 || a->out_dtype == a->pool.dtype, "sisa_prefix_decode: out_dtype");

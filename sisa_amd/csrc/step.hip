@@ -17,6 +17,7 @@
 // recomputed by every workgroup (B short rows, served by L2) while its first weights are on their way: one launch and
 // one dependent round trip less than a norm of its own.
 #include "pages.h"
+#include "sisa_hip_branch.h"
 #include "sisa_hip_step.h"
 
 namespace sisa {
@@ -303,6 +304,78 @@ __global__ __launch_bounds__(64) void step_append_kernel(Args a) {
     }
 }
 
+// M positions of each sequence, one wave per (sequence, head): step_append_kernel's work position by position, with the state
+// of the recurrences in registers between them.
+struct RowsAppendArgs {
+    PagedAppendArgs p;                 // phi_in, phi_out: the same memory
+    int M, row0;
+    float* rows;                       // or null: the state before, and after each position
+    int64_t s_rows;
+};
+
+template <class T>
+__global__ __launch_bounds__(64) void step_append_rows_kernel(RowsAppendArgs a) {
+    const PagedAppendArgs& p = a.p;
+    const int lane = threadIdx.x, H = p.H, bh = blockIdx.x, b = bh / H, h = bh % H, M = a.M;
+    const int64_t start = p.start[b];
+    const bool whole = p.lengths[b] == start + M;
+    float phi = lane < DS / 2 ? p.phi_in[(int64_t)bh * (DS / 2) + lane] : 0.f;
+    float last = lane == 32 ? p.g_last[bh] : lane == 33 ? p.f_last[bh] : 0.f;
+    float* rows = a.rows ? a.rows + bh * a.s_rows + (int64_t)a.row0 * SISA_BRANCH_ROW : nullptr;
+    auto note = [&](int row) {
+        if (!rows) return;
+        if (lane < DS / 2) rows[row * SISA_BRANCH_ROW + 2 + lane] = phi;
+        else if (lane == 32 || lane == 33) rows[row * SISA_BRANCH_ROW + lane - 32] = last;
+    };
+    note(0);
+    bool all = whole;
+    for (int m = 0; m < M; ++m) {
+        const int64_t row = (int64_t)b * M + m, pos = start + m, slot = pos & ((1 << p.shift) - 1);
+        const int64_t page = page_of(p.table + b * p.s_table, p.W, p.shift, p.pages, pos);
+        const T* P = (const T*)p.proj + row * 272 * H;
+        all = all && page >= 0;
+        if (all) {
+            ((T*)p.k.ptr)[page * p.k.sb + h * p.k.sh + slot * p.k.sl + lane] = P[(H + h) * DH + lane];
+            ((T*)p.v.ptr)[page * p.v.sb + h * p.v.sh + slot * p.v.sl + lane] = P[(2 * H + h) * DH + lane];
+        }
+        if (lane < DS / 2) {
+            phi += (float)P[256 * H + h * (DS / 2) + lane];
+            const float cs = cosf(phi), sn = sinf(phi);
+            const T* bp = P + 192 * H + h * DS + 2 * lane;
+            const T* cp = P + 224 * H + h * DS + 2 * lane;
+            const float b0 = (float)bp[0], b1 = (float)bp[1], c0 = (float)cp[0], c1 = (float)cp[1];
+            T* co = (T*)p.c + (row * H + h) * DS + 2 * lane;
+            if (all) {
+                T* bo = (T*)p.b.ptr + page * p.b.sb + h * p.b.sh + slot * p.b.sl + 2 * lane;
+                bo[0] = cvt<T>(b0 * cs - b1 * sn);
+                bo[1] = cvt<T>(b1 * cs + b0 * sn);
+            }
+            co[0] = cvt<T>(c0 * cs - c1 * sn);
+            co[1] = cvt<T>(c1 * cs + c0 * sn);
+        } else if (lane == 32) {
+            const float al = p.alpha[row * H + h];
+            last = all ? last - (al > 20.f ? al : log1pf(expf(al))) : __builtin_nanf("");
+            if (all) ((float*)p.g.ptr)[page * p.g.sb + h * p.g.sh + slot * p.g.sl] = last;
+            p.gq[row * H + h] = last;
+        } else if (lane == 33) {
+            const float z = p.z[row * H + h];
+            last = all ? last + ((z < 0.f ? z : (z != z ? z : 0.f)) - log1pf(expf(-fabsf(z)))) : __builtin_nanf("");
+            if (all) ((float*)p.f.ptr)[page * p.f.sb + h * p.f.sh + slot * p.f.sl] = last;
+            p.fq[row * H + h] = last;
+        }
+        note(1 + m);
+    }
+    if (lane < DS / 2) p.phi_out[(int64_t)bh * (DS / 2) + lane] = phi;
+    else if (lane == 32) p.g_last[bh] = last;
+    else if (lane == 33) p.f_last[bh] = last;
+    else if (lane == 34 && b == 0) {
+        const float r = p.lambda_raw[h];
+        p.lam[h] = r > 20.f ? r : log1pf(expf(r));
+    } else if (lane == 35 && h == 0) {
+        p.length[b] = all ? p.lengths[b] : -1;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ W_O, down
 // y = x W^T for W (rows, K), row stride K; OUT = add + y when `add` is given (both rounded to T in turn).
 struct LinArgs {
@@ -501,6 +574,24 @@ int launch_step(const sisa_step_args* a, hipStream_t st) {
     }, st);
 }
 
+PagedAppendArgs paged_append(const sisa_step_paged_args* a, const Ws& ws) {
+    const sisa_page_pool& p = a->pool;
+    PagedAppendArgs ap{};
+    static_cast<AppendArgs&>(ap) = AppendArgs{ws.proj, ws.alpha, ws.z, a->phi, a->lambda_raw, p.k, p.v, p.b, p.g, p.f, a->phi,
+                                              ws.gq, ws.fq, ws.lam, ws.c, a->H, 0};
+    ap.table = a->table;
+    ap.start = a->start;
+    ap.lengths = a->lengths;
+    ap.length = ws.length;
+    ap.s_table = a->s_table;
+    ap.W = a->W;
+    ap.shift = sisa::log2_of(p.page_size);
+    ap.pages = p.pages;
+    ap.g_last = a->g_last;
+    ap.f_last = a->f_last;
+    return ap;
+}
+
 // The fields that a step with the cache in pages shares with sisa_step.
 sisa_step_args common_of(const sisa_step_paged_args* a) {
     sisa_step_args c{};
@@ -545,20 +636,7 @@ int launch_step_paged(const sisa_step_paged_args* a, hipStream_t st) {
     const Ws ws = workspace((char*)a->workspace, B, H, a->D, a->FF,
                             sisa_paged_decode_workspace_bytes(B, H, 1, a->max_len, a->dtype, a->weights.ptr != nullptr));
     return launch_rows<T>(&c, ws, [&]() -> int {
-        PagedAppendArgs ap{};
-        static_cast<AppendArgs&>(ap) = AppendArgs{ws.proj, ws.alpha, ws.z, a->phi, a->lambda_raw, p.k, p.v, p.b, p.g, p.f, a->phi,
-                                                  ws.gq, ws.fq, ws.lam, ws.c, H, 0};
-        ap.table = a->table;
-        ap.start = a->start;
-        ap.lengths = a->lengths;
-        ap.length = ws.length;
-        ap.s_table = a->s_table;
-        ap.W = a->W;
-        ap.shift = sisa::log2_of(p.page_size);
-        ap.pages = p.pages;
-        ap.g_last = a->g_last;
-        ap.f_last = a->f_last;
-        step_append_kernel<T><<<(unsigned)(B * H), 64, 0, st>>>(ap);
+        step_append_kernel<T><<<(unsigned)(B * H), 64, 0, st>>>(paged_append(a, ws));
         const int rc = sisa::launch_status("sisa_step_paged (append)");
         if (rc) return rc;
         sisa_paged_decode_args d{};
@@ -579,6 +657,50 @@ int launch_step_paged(const sisa_step_paged_args* a, hipStream_t st) {
         d.w_in = d.w_out = a->weights;
         d.workspace = ws.attn;
         return sisa::detail::paged_attn_out16(&d, ws.y, st);
+    }, st);
+}
+
+// The layer's products see B M rows; the workspace, too, is of as many.
+Ws branch_space(char* base, int64_t B, int64_t H, int64_t D, int64_t FF, int64_t M, int64_t G, int64_t max_len, int64_t max_shared) {
+    return workspace(base, B * M, H, D, FF,
+                     sisa_prefix_decode_workspace_bytes((int)B, (int)H, (int)M, (int)G, (int)max_len, (int)max_shared));
+}
+
+template <class T>
+int launch_step_branch(const sisa_step_branch_args* a, hipStream_t st) {
+    const sisa_step_paged_args* s = &a->step;
+    const int B = s->B, H = s->H, M = a->M;
+    sisa_step_args c = common_of(s);
+    c.B = B * M;
+    const Ws ws = branch_space((char*)s->workspace, B, H, s->D, s->FF, M, a->G, s->max_len, a->max_shared);
+    return launch_rows<T>(&c, ws, [&]() -> int {
+        step_append_rows_kernel<T><<<(unsigned)(B * H), 64, 0, st>>>(RowsAppendArgs{paged_append(s, ws), M, a->row0, a->rows, a->s_rows});
+        const int rc = sisa::launch_status("sisa_step_branch (append)");
+        if (rc) return rc;
+        sisa_prefix_decode_args d{};
+        d.B = B;
+        d.M = M;
+        d.W = s->W;
+        d.G = a->G;
+        d.max_len = s->max_len;
+        d.max_shared = a->max_shared;
+        d.out_dtype = s->dtype;
+        d.pool = s->pool;
+        d.table = s->table;
+        d.s_table = s->s_table;
+        d.lengths = ws.length;
+        d.first = a->first;
+        d.group = a->group;
+        d.shared = a->shared;
+        d.q = sisa_view{ws.proj, (int64_t)M * 272 * H, DH, (int64_t)272 * H};
+        d.c = sisa_view{ws.c, (int64_t)M * H * DS, DS, (int64_t)H * DS};
+        d.gq = sisa_view{ws.gq, (int64_t)M * H, 1, H};
+        d.fq = sisa_view{ws.fq, (int64_t)M * H, 1, H};
+        d.lam = ws.lam;
+        d.s_lam = 1;
+        d.out = sisa_view{ws.y, (int64_t)M * H * DH, DH, (int64_t)H * DH};
+        d.workspace = ws.attn;
+        return sisa_prefix_decode(&d, st);
     }, st);
 }
 
@@ -670,6 +792,40 @@ extern "C" int sisa_step_paged(const sisa_step_paged_args* a, void* stream) {
                  "sisa_step_paged: B*H*max_len too large for one launch");
     hipStream_t st = (hipStream_t)stream;
     return a->dtype == SISA_BF16 ? launch_step_paged<__bf16>(a, st) : launch_step_paged<_Float16>(a, st);
+}
+
+extern "C" int64_t sisa_step_branch_workspace_bytes(int32_t B, int32_t H, int32_t D, int32_t FF, int32_t M, int32_t G,
+                                                    int32_t max_len, int32_t max_shared) {
+    if (B < 1 || H < 1 || D < 1 || FF < 1 || M < 1 || B > SISA_STEP_MAX_ROWS || M > SISA_STEP_MAX_ROWS || G < 1 || max_len < 1 ||
+        max_shared < 0)
+        return 0;
+    return branch_space(nullptr, B, H, D, FF, M, G, max_len, max_shared).bytes;
+}
+
+extern "C" int sisa_step_branch(const sisa_step_branch_args* a, void* stream) {
+    SISA_REQUIRE(a != nullptr, "sisa_step_branch: null args");
+    const sisa_step_paged_args* s = &a->step;
+    SISA_REQUIRE(a->M >= 1 && s->B >= 1 && s->B <= SISA_STEP_MAX_ROWS && a->M <= SISA_STEP_MAX_ROWS &&
+                     s->B * a->M <= SISA_STEP_MAX_ROWS,
+                 "sisa_step_branch: B=%d sequences of M=%d rows: 1 .. 64 in all", s->B, a->M);
+    const sisa_step_args c = common_of(s);
+    const char* fault = step_fault(&c);
+    SISA_REQUIRE(fault == nullptr, "sisa_step_branch: %s (B=%d H=%d D=%d FF=%d dtype=%d)", fault, s->B, s->H, s->D, s->FF, s->dtype);
+    SISA_REQUIRE_POOL("sisa_step_branch", s->pool);
+    SISA_REQUIRE(s->pool.heads == s->H && s->pool.dtype == s->dtype && s->pool.f.ptr,
+                 "sisa_step_branch: the pool must have the layer's heads and dtype, and f");
+    const int64_t held = (int64_t)s->W * s->pool.page_size;
+    SISA_REQUIRE(s->W >= 1 && s->max_len >= 1 && s->max_len <= held && s->max_len <= (1 << 30) && a->max_shared >= 0 &&
+                     a->max_shared <= held && a->max_shared <= (1 << 30) && a->G >= 1 && a->G <= s->B,
+                 "sisa_step_branch: max_len=%d max_shared=%d (at most W=%d pages of %d, and 2^30), G=%d of 1 .. B groups", s->max_len,
+                 a->max_shared, s->W, s->pool.page_size, a->G);
+    SISA_REQUIRE(s->table && s->start && s->lengths && s->g_last && s->f_last && s->phi && a->first && a->group && a->shared,
+                 "sisa_step_branch: null pointer");
+    SISA_REQUIRE(s->weights.ptr == nullptr, "sisa_step_branch: no weights are tracked");
+    SISA_REQUIRE(!a->rows || (a->row0 >= 0 && a->s_rows >= (int64_t)(a->row0 + 1 + a->M) * SISA_BRANCH_ROW),
+                 "sisa_step_branch: row0=%d and M=%d rows do not fit s_rows=%lld", a->row0, a->M, (long long)a->s_rows);
+    hipStream_t st = (hipStream_t)stream;
+    return s->dtype == SISA_BF16 ? launch_step_branch<__bf16>(a, st) : launch_step_branch<_Float16>(a, st);
 }
 
 extern "C" int sisa_cache_fill(const sisa_cache_fill_args* a, void* stream) {

@@ -23,12 +23,13 @@ from typing import TYPE_CHECKING, Iterable
 import torch
 from torch import Tensor
 
+from .backends import hip_status
 from .paged import SISAPagedCache
 
 if TYPE_CHECKING:  # pragma: no cover
     from .modeling import SISAForCausalLM
 
-__all__ = ["LayerState", "SISACache", "generate"]
+__all__ = ["LayerState", "SISACache", "generate", "verify_drafts"]
 
 
 
@@ -166,14 +167,37 @@ def _pick(logits: Tensor, do_sample: bool, temperature: float, top_k: int | None
     with every logit below the row's ``top_k``-th largest set to -inf (the reference's sampling rule,
     src/sisa/generation.py:126-135: ties at the k-th value stay candidates, and a seeded generator yields the same
     draws as the reference's)."""
-    scores = logits.float()
     if not do_sample:
-        return scores.argmax(dim=-1)
-    scores = scores / temperature
+        return logits.float().argmax(dim=-1)
+    return torch.multinomial(_probabilities(logits, temperature, top_k), 1, generator=generator).squeeze(-1)
+
+
+def _probabilities(logits: Tensor, temperature: float, top_k: int | None) -> Tensor:
+    """What :func:`_pick` draws from."""
+    scores = logits.float() / temperature
     if top_k is not None and top_k < scores.shape[-1]:
         floor = scores.topk(top_k, dim=-1).values[..., -1:]
         scores = torch.where(scores < floor, torch.full_like(scores, float("-inf")), scores)
-    return torch.multinomial(scores.softmax(-1), 1, generator=generator).squeeze(-1)
+    return scores.softmax(-1)
+
+
+def verify_drafts(p: Tensor, drafts: Tensor, u: Tensor, q: Tensor) -> tuple[Tensor, Tensor]:
+    """:func:`sisa_amd.kernels.verify.sisa_verify_drafts_hip` in plain PyTorch, on any device: ``(tokens, accepted)``."""
+    B, K = drafts.shape
+    row, i = torch.arange(B, device=p.device), torch.arange(K + 1, device=p.device)
+    at, u = drafts[..., None], u.double()
+    took = u[:, :K] * q.gather(2, at)[..., 0].double() < p[:, :K].gather(2, at)[..., 0].double()
+    accepted = took.long().cumprod(1).sum(1)
+    target = p[row, accepted].double()
+    rest = (target - q[row, accepted.clamp(max=K - 1)].double()).clamp(min=0.0)
+    weights = torch.where(((accepted < K) & (rest.sum(1) > 0))[:, None], rest, target)
+    upto = weights.cumsum(1)
+    over = (upto > u[:, K:] * upto[:, -1:]) & (weights > 0)
+    last = weights.shape[1] - 1 - (weights > 0).flip(1).int().argmax(1)
+    token = torch.where(over.any(1), over.int().argmax(1), last)
+    padded = torch.cat([drafts, drafts.new_full((B, 1), -1)], 1)
+    behind, here = i > accepted[:, None], i == accepted[:, None]
+    return torch.where(behind, -1, torch.where(here, token[:, None], padded)), accepted.to(torch.int32)
 
 
 def _prompt_lengths(prompt_lengths, rows: Tensor) -> list[int] | None:
@@ -215,7 +239,8 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
              top_k: int | None = None, eos_token_id: int | Iterable[int] | Tensor | None = None,
              do_sample: bool = False, *, generator: torch.Generator | None = None,
              prompt_lengths: Iterable[int] | Tensor | None = None, cache_budget: int | None = None,
-             cache_recent: int | None = None) -> Tensor:
+             cache_recent: int | None = None, samples: int = 1, draft: "SISAForCausalLM | None" = None,
+             draft_tokens: int = 4) -> Tensor:
     """Continue the prompts ``input_ids`` (``(B, L)`` of equal-length rows, or ``(L,)``) by up to ``max_new_tokens``
     tokens: greedy, or sampled at ``temperature`` from the ``top_k`` most likely tokens with ``do_sample``.
 
@@ -229,6 +254,15 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     ``cache_budget``: how many positions each layer and head keeps: the last ``cache_recent`` (default: a quarter) and those
     that have received the largest softmax weight. The cache is cut after the prompt, and whenever it has grown by an eighth
     (at least 16) over its budget; until a cut nothing is left out.
+
+    ``samples``: every prompt is read once and continued that many times; the rows of a prompt are neighbours, ``(B * samples,
+    L + n)`` (``(samples, L + n)`` for one prompt of rank 1). Their attention reads the prompt's cached positions once for all
+    of them.
+
+    ``draft``: a smaller model with the same vocabulary, which proposes ``draft_tokens`` tokens at a time; the model reads them
+    in one pass and keeps those that it would have taken: with ``do_sample``, by random numbers such that what comes out is
+    distributed as without the draft (not the same draws from a seed), else those that are its own likeliest. Neither goes with
+    ``cache_budget``, and not with the other.
     """
     if max_new_tokens < 0:
         raise ValueError(f"max_new_tokens = {max_new_tokens} is negative")
@@ -242,22 +276,46 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
                          f"{tuple(input_ids.shape)}")
     if cache_recent is not None and cache_budget is None:
         raise ValueError("cache_recent goes with cache_budget")
+    if samples < 1 or draft_tokens < 1:
+        raise ValueError(f"samples = {samples}, draft_tokens = {draft_tokens}: both must be positive")
+    if (samples > 1) + (draft is not None) + (cache_budget is not None) > 1:
+        raise ValueError("samples, draft and cache_budget do not go together")
+    if draft is not None and draft.config.vocab_size != model.config.vocab_size:
+        raise ValueError(f"the draft has {draft.config.vocab_size} tokens, the model {model.config.vocab_size}")
     lengths = _prompt_lengths(prompt_lengths, rows)
     budget = None if cache_budget is None else _Budget(cache_budget, cache_recent)
     stops = _eos_ids(eos_token_id)
+    if draft is not None:
+        result = _generate_drafted(model, draft, draft_tokens, rows, lengths, max_new_tokens, stops,
+                                   (temperature, top_k) if do_sample else None, generator)
+        return result if input_ids.dim() == 2 else result.squeeze(0)
     stop_ids = torch.tensor(stops, device=rows.device, dtype=rows.dtype) if stops else None
-    prompt = rows.shape[1]
+    prompt, prompts = rows.shape[1], rows.shape[0]
+    if samples > 1:
+        rows = rows.repeat_interleave(samples, 0)
+        lengths = None if lengths is None else [n for n in lengths for _ in range(samples)]
     out = rows.new_empty((rows.shape[0], prompt + max_new_tokens))
     out[:, :prompt] = rows
     length = prompt
     if max_new_tokens:
-        if lengths is None and budget is None:
+        if lengths is None and budget is None and samples == 1:
             cache = SISACache(capacity=prompt + max_new_tokens)
         else:
             cache = _paged_cache(rows.shape[0], max(lengths or [prompt]), max_new_tokens, budget)
         finished = torch.zeros(rows.shape[0], dtype=torch.bool, device=rows.device)
         ends = None
-        if lengths is None:
+        if samples > 1:
+            some = cache[:prompts]
+            first = [prompt] * prompts if lengths is None else lengths[::samples]
+            n = torch.tensor(first, device=rows.device)
+            some.expect(first)
+            ids = rows[::samples].masked_fill(torch.arange(prompt, device=rows.device) >= n[:, None], 0)
+            logits = model(ids, cache=some, logits_at=[m - 1 for m in first]).logits[:, -1].repeat_interleave(samples, 0)
+            cache.branch(samples)
+            if lengths is not None:
+                ends = n.repeat_interleave(samples)[:, None]
+                out[torch.arange(out.shape[1], device=rows.device) >= ends] = stops[0] if stops else 0
+        elif lengths is None:
             logits = model(rows, cache=cache, logits_to_keep=1).logits[:, -1]
         else:
             # what pads the rows need not be a token; rows are laid out from their own ends
@@ -284,4 +342,79 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
                 cache.evict(budget.keep, budget.recent)
             logits = model(token[:, None], cache=cache, logits_to_keep=1).logits[:, -1]
     result = out[:, :length].contiguous()
-    return result if input_ids.dim() == 2 else result.squeeze(0)
+    return result if input_ids.dim() == 2 or samples > 1 else result.squeeze(0)
+
+
+def _generate_drafted(model, draft, K: int, rows: Tensor, lengths: list[int] | None, new: int, stops: list[int],
+                      sampling: tuple[float, int | None] | None, generator: torch.Generator | None) -> Tensor:
+    """:func:`generate` with a draft. In each round the draft reads its last token and its own proposals, one by one, and the
+    model all of them at once; both caches keep what was accepted. Rows that are done keep nothing more."""
+    B, prompt = rows.shape
+    first = [prompt] * B if lengths is None else lengths
+    fill = stops[0] if stops else 0
+    if not new:
+        return rows.clone()
+    n = torch.tensor(first, device=rows.device)
+    ids = rows.masked_fill(torch.arange(prompt, device=rows.device) >= n[:, None], 0)
+    caches = [SISAPagedCache(B, max(first) + new + K + 1) for _ in range(2)]
+    logits = []
+    for m, cache in zip((model, draft), caches):
+        cache.expect(first)
+        logits.append(m(ids, cache=cache, logits_at=[i - 1 for i in first]).logits[:, -1])
+    target, proposals = caches
+    token = _pick(logits[0], sampling is not None, *(sampling or (1.0, None)), generator).to(rows.dtype)
+    out = [[t] for t in token.tolist()]
+    done = [new == 1 or t[0] in stops for t in out]
+    while not all(done):
+        proposals.tentative(K + 1)
+        target.tentative(K + 1)
+        said, q, last = [token], [], token
+        for i in range(K + 1):
+            logits = draft(last[:, None], cache=proposals, logits_to_keep=1).logits[:, -1]
+            if i == K:                                     # the last proposal is read for the draft's cache alone
+                break
+            if sampling is None:
+                last = logits.float().argmax(dim=-1).to(rows.dtype)
+            else:
+                q.append(_probabilities(logits, *sampling))
+                last = torch.multinomial(q[-1], 1, generator=generator).squeeze(-1).to(rows.dtype)
+            said.append(last)
+        logits = model(torch.stack(said, 1), cache=target).logits
+        drafts = torch.stack(said[1:], 1).long()
+        if sampling is None:
+            own = logits.float().argmax(dim=-1)
+            accepted = (own[:, :K] == drafts).long().cumprod(1).sum(1)
+            tokens = torch.where(torch.arange(K + 1, device=rows.device) <= accepted[:, None], own, -1)
+        else:
+            p = _probabilities(logits, *sampling)
+            u = torch.rand((B, K + 1), device=p.device, generator=generator)
+            if p.is_cuda and hip_status(p.device)[0]:
+                from .kernels.verify import sisa_verify_drafts_hip
+
+                tokens, accepted = sisa_verify_drafts_hip(p, drafts, u, torch.stack(q, 1))
+            else:
+                tokens, accepted = verify_drafts(p, drafts, u, torch.stack(q, 1))
+        got, took = tokens.tolist(), accepted.tolist()
+        counts = []
+        for i, row in enumerate(out):
+            if done[i]:
+                counts.append(0)
+                got[i][0], took[i] = fill, 0
+                continue
+            if got[i][took[i]] < 0:
+                raise RuntimeError("generate: the model's probabilities are not finite, or 0 everywhere")
+            for t in got[i][:took[i] + 1]:
+                row.append(t)
+                done[i] = len(row) == new or t in stops
+                if done[i]:
+                    break
+            counts.append(0 if done[i] else took[i] + 1)
+        target.keep(counts)
+        proposals.keep(counts)
+        token = torch.tensor([row[a] for row, a in zip(got, took)], device=rows.device, dtype=rows.dtype)
+    longest = max(len(row) for row in out)
+    result = rows.new_full((B, prompt + longest), fill)
+    result[:, :prompt] = torch.where(torch.arange(prompt, device=rows.device) < n[:, None], rows, fill)
+    at = n[:, None] + torch.arange(longest, device=rows.device)
+    return result.scatter_(1, at, torch.tensor([row + [fill] * (longest - len(row)) for row in out], device=rows.device,
+                                               dtype=rows.dtype))

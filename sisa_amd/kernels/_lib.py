@@ -198,7 +198,12 @@ class PrefixDecodeArgs(Structure):
                 ("max_shared", c_int32), ("out_dtype", c_int32), ("reserved", c_int32), ("pool", PagePoolArgs),
                 ("table", c_void_p), ("s_table", c_int64), ("lengths", c_void_p), ("first", c_void_p),
                 ("group", c_void_p), ("shared", c_void_p), ("q", View), ("c", View), ("gq", View), ("fq", View),
-                ("lam", c_void_p), ("s_lam", c_int64), ("out", c_void_p), ("workspace", c_void_p)]
+                ("lam", c_void_p), ("s_lam", c_int64), ("out", View), ("workspace", c_void_p)]
+
+
+class StepBranchArgs(Structure):
+    _fields_ = [*StepPagedArgs._fields_, ("M", c_int32), ("G", c_int32), ("max_shared", c_int32), ("row0", c_int32),
+                ("first", c_void_p), ("group", c_void_p), ("shared", c_void_p), ("rows", c_void_p), ("s_rows", c_int64)]
 
 
 class VerifyArgs(Structure):
@@ -281,6 +286,8 @@ CACHE_SIGNATURES = {
 BRANCH_SIGNATURES = {
     "sisa_prefix_decode_workspace_bytes": ([c_int32, c_int32, c_int32, c_int32, c_int32, c_int32], c_int64),
     "sisa_prefix_decode": ([POINTER(PrefixDecodeArgs), c_void_p], c_int),
+    "sisa_step_branch_workspace_bytes": ([c_int32] * 8, c_int64),
+    "sisa_step_branch": ([POINTER(StepBranchArgs), c_void_p], c_int),
     "sisa_verify_workspace_bytes": ([c_int32, c_int32], c_int64),
     "sisa_verify": ([POINTER(VerifyArgs), c_void_p], c_int),
 }

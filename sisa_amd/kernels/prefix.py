@@ -98,5 +98,5 @@ def sisa_prefix_decode_hip(q: Tensor, c: Tensor, g_q: Tensor, f_q: Tensor | None
     ws = lam.new_empty((_lib.floats("sisa_prefix_decode_workspace_bytes", B, H, M, G, max_len, max_shared),))
     _decode(q, B, M, W, G, max_len, max_shared, _lib.F32, 0, pool.packed, table.data_ptr(), table.stride(0),
             lengths.data_ptr(), groups.first.data_ptr(), groups.group.data_ptr(), shared.data_ptr(), *vq, *vc, *vg, *vf,
-            lam.data_ptr(), lam.stride(0), out.data_ptr(), ws.data_ptr())
+            lam.data_ptr(), lam.stride(0), out.data_ptr(), *out.stride()[:3], ws.data_ptr())
     return out

@@ -21,7 +21,7 @@ from . import attention as A
 from . import fused_prep as P
 
 __all__ = ["unobserved", "plain", "plain_linears", "rows_ok", "whole", "prefill_takes", "step_weights",
-           "layer_step", "layer_step_paged", "prefill_paged", "layer_prefill", "prefill", "MAX_ROWS", "MAX_WIDTH", "PREFILL_ROWS", "PREFILL_WORK"]
+           "layer_step", "layer_step_paged", "layer_step_branch", "prefill_paged", "layer_prefill", "prefill", "MAX_ROWS", "MAX_WIDTH", "PREFILL_ROWS", "PREFILL_WORK"]
 
 MAX_ROWS, MAX_WIDTH = 64, 1024          # SISA_STEP_MAX_ROWS, SISA_STEP_MAX_D
 #: Prompts of at most this many tokens (all rows together) take ``sisa_prefill``, and at most PREFILL_WORK / width of them
@@ -149,6 +149,35 @@ def layer_step_paged(x: Tensor, res: Tensor | None, weights: list[int], d_ff: in
                     0 if res is None else res.data_ptr(), *weights, lambda_raw.data_ptr(), at.pool.packed, at.table.data_ptr(),
                     at.table.stride(0), at.start.data_ptr(), at.end.data_ptr(), *(t.data_ptr() for t in at.last), *w,
                     h.data_ptr(), ffn.data_ptr(), ws.data_ptr())
+        cache.end_step(layer_idx)
+    except BaseException:
+        cache.failed(layer_idx)
+        raise
+    return h, ffn
+
+
+_step_branch = _lib.Packed("sisa_step_branch", _lib.StepBranchArgs)
+
+
+def layer_step_branch(x: Tensor, res: Tensor | None, weights: list[int], d_ff: int, lambda_raw: Tensor,
+                      eps: tuple[float, float], cache, layer_idx: int) -> tuple[Tensor, Tensor]:
+    """:func:`layer_step_paged` for the new positions ``x`` ``(B, M, D)``, contiguous where ``M > 1``, of a cache that
+    :meth:`sisa_amd.paged.SISAPagedCache.shares`: what the sequences, or the positions, have in common is read once."""
+    B, M, D = x.shape
+    H = D // HIP_D_HEAD
+    at, sharing, noted = cache.begin_rows(layer_idx, M)
+    try:
+        h, ffn = torch.empty((2, B, M, D), device=x.device, dtype=x.dtype).unbind(0)
+        G = len(sharing.groups)
+        size = _lib.floats("sisa_step_branch_workspace_bytes", B, H, D, d_ff, M, G, at.max_len, sharing.most)
+        ws = torch.empty((size,), device=x.device, dtype=torch.float32)
+        rows, row0 = (None, 0) if noted is None else noted
+        _step_branch(x, B, H, D, d_ff, _lib.dtype_code(x.dtype), at.table.shape[1], at.max_len, 0, *eps, x.data_ptr(),
+                     x.stride(0) if M == 1 else D, 0 if res is None else res.data_ptr(), *weights, lambda_raw.data_ptr(),
+                     at.pool.packed, at.table.data_ptr(), at.table.stride(0), at.start.data_ptr(), at.end.data_ptr(),
+                     *(t.data_ptr() for t in at.last), 0, 0, 0, 0, h.data_ptr(), ffn.data_ptr(), ws.data_ptr(), M, G,
+                     sharing.most, row0, sharing.groups.first.data_ptr(), sharing.groups.group.data_ptr(),
+                     sharing.shared.data_ptr(), 0 if rows is None else rows.data_ptr(), 0 if rows is None else rows.stride(1))
         cache.end_step(layer_idx)
     except BaseException:
         cache.failed(layer_idx)

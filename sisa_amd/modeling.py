@@ -347,7 +347,8 @@ class SISABlock(nn.Module):
         """Generation on HIP kernels, or None where it does not apply. A prompt (empty cache entry) takes
         ``sisa_prefill`` in a 16-bit model while it is short, else :meth:`_forward_hip` with the cache filled from the
         fused projections; one new position of at most 64 rows of a 16-bit model takes ``sisa_step``, or with a cache in
-        pages, whose prompts all go by :meth:`_forward_hip`, ``sisa_step_paged``. All return
+        pages, whose prompts all go by :meth:`_forward_hip`, ``sisa_step_paged``, or, for branches of a prompt and drafted
+        positions, of which there may be several, ``sisa_step_branch``. All return
         ``(h, f)`` as :meth:`_forward_hip` with ``defer``. Only for inference with nothing watching the modules in
         between: other calls take the module path."""
         from .generation import SISACache
@@ -377,7 +378,8 @@ class SISABlock(nn.Module):
             slab = cache
         else:
             return None
-        if slab is not None and (autocast or L != 1 or B > step.MAX_ROWS or D > step.MAX_WIDTH):
+        shares = paged and slab is not None and cache.shares()
+        if slab is not None and (autocast or (L != 1 and not shares) or B * L > step.MAX_ROWS or D > step.MAX_WIDTH):
             return None
         if not (step.unobserved(x) and step.plain(self, SISABlock) and step.plain(ffn, SwiGLU) and step.plain(n1, RMSNorm)
                 and step.plain(n2, RMSNorm)):
@@ -386,7 +388,7 @@ class SISABlock(nn.Module):
         native = (not autocast and lam.dtype == torch.float32 and lam.shape == (H,)
                   and lam.get_device() == x.get_device() and lam.is_contiguous())
         if paged and slab is not None:
-            if not native or not step.rows_ok(x) or not step.whole(res):
+            if not native or not (step.rows_ok(x) if L == 1 else step.whole(x)) or not step.whole(res):
                 return None
         elif slab is not None:
             buf = slab.buffers
@@ -408,7 +410,8 @@ class SISABlock(nn.Module):
         if weights is None:
             return None
         if paged:
-            return step.layer_step_paged(x, res, *weights, lam, (n1.eps, n2.eps), cache, at.layer_idx)
+            run = step.layer_step_branch if shares else step.layer_step_paged
+            return run(x, res, *weights, lam, (n1.eps, n2.eps), cache, at.layer_idx)
         slab = cache.room(at.layer_idx, 1, buf, slab.phi)
         h, f, phi = step.layer_step(x, res, *weights, lam, (n1.eps, n2.eps), slab, slab.phi.contiguous())
         slab.filled, slab.phi = slab.filled + 1, phi

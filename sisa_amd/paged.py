@@ -1,6 +1,7 @@
-"""A decode cache in pages: sequences of unequal lengths in one batch, and a bound on how many positions are kept.
+"""A decode cache in pages: sequences of unequal lengths in one batch, a bound on how many positions are kept, several
+continuations of one prompt, and positions that can be taken back.
 
-:class:`SISAPagedCache` stands where :class:`sisa_amd.generation.SISACache` does (``model(ids, cache=cache)``), with two
+:class:`SISAPagedCache` stands where :class:`sisa_amd.generation.SISACache` does (``model(ids, cache=cache)``), with four
 things that one has not:
 
 * every sequence has its own length and takes its memory in pages from a common pool, so prompts of different lengths are
@@ -8,9 +9,13 @@ things that one has not:
   alone, to fill while the others stay;
 * with ``track=True`` every position's softmax weight is accumulated over the queries that saw it, and :meth:`evict` cuts
   the sequences down to their last and their most attended positions. The score of a SISA key depends on its own ``g``,
-  ``F`` and rotated ``b``, not on its distance, so what follows is exactly the softmax over the kept keys.
+  ``F`` and rotated ``b``, not on its distance, so what follows is exactly the softmax over the kept keys;
+* :meth:`branch` continues every prompt several times: the branches hold the prompt's pages together, and their attention
+  reads them once;
+* after :meth:`tentative`, :meth:`keep` takes back what a draft proposed in vain.
 
-On the GPU the operators are the HIP kernels of :mod:`sisa_amd.kernels.paged` and :mod:`sisa_amd.kernels.weights`;
+On the GPU the operators are the HIP kernels of :mod:`sisa_amd.kernels.paged`, :mod:`sisa_amd.kernels.weights` and
+:mod:`sisa_amd.kernels.prefix`;
 elsewhere, and for head or state sizes those do not take, the plain PyTorch forms below, in float32 (float64 inputs:
 float64). Inference only. The reference has no such cache.
 """
@@ -158,6 +163,27 @@ class _Step(NamedTuple):
     max_len: int
 
 
+class _Sharing(NamedTuple):
+    """What :func:`sisa_amd.kernels.prefix.sisa_prefix_decode_hip` is told of the sequences: their groups, the positions that each
+    has in common, and the most of them."""
+    groups: object
+    shared: Tensor
+    most: int
+
+
+#: What the recurrences continue from, of a sequence and head: g, F and the phases.
+_ROW = 2 + HIP_D_STATE // 2
+
+
+class _Trial:
+    """Positions that may be taken back: the sequences, how many positions there can be, where they begin, and per layer
+    ``(sequences, H, room + 1, 2 + d_state // 2)`` what the recurrences continue from before the first and after each."""
+
+    def __init__(self, lo: int, hi: int, room: int, starts: list[int]) -> None:
+        self.lo, self.hi, self.room, self.starts = lo, hi, room, starts
+        self.rows: dict[int, Tensor] = {}
+
+
 class _Begun(NamedTuple):
     """A pass whose first layer is not written yet: its sequences, and what the store held for them before."""
     lo: int
@@ -188,6 +214,11 @@ class _Store:
         self.widths = [0] * sequences                                  # that pass's positions, padding included
         self.expected: list[int | None] = [None] * sequences           # real positions of the next pass, if not all
         self.begun: _Begun | None = None
+        self.trial: _Trial | None = None
+        self.family: list[tuple[int, int] | None] = [None] * sequences    # a prompt's number, and its pages that are shared
+        self.families = 0
+        self.others: dict[int, int] = {}                   # of a shared page: how many sequences hold it beside one
+        self.sharing: dict[tuple[int, int], _Sharing | None] = {}
         self.layers: dict[int, _Layer] = {}
         self.table = self.start = self.end = None          # on the model's device, made by the first pass
 
@@ -212,6 +243,47 @@ class _Store:
         for n, pages in enumerate(need, lo):
             self.held[n] += [self.free.pop() for _ in range(pages)]
         return [n for n, pages in enumerate(need, lo) if pages]
+
+    def give(self, pages) -> None:
+        """Pages of a sequence that holds them no more: free, where no other does."""
+        for page in pages:
+            left = self.others.pop(page, 0)
+            if not left:
+                self.free.append(page)
+            elif left > 1:
+                self.others[page] = left - 1
+
+    def runs(self, lo: int, hi: int) -> list[tuple[int, int]]:
+        """Neighbours that continue the same prompt: how many, and the positions that they share."""
+        out, last = [], None
+        for family in self.family[lo:hi]:
+            if family is not None and family == last:
+                out[-1] = (out[-1][0] + 1, out[-1][1])
+            else:
+                out.append((1, 0 if family is None else family[1] * self.page_size))
+            last = family
+        return out
+
+    def grouped(self, lo: int, hi: int) -> _Sharing | None:
+        """The sequences' groups for the kernels, or None where no two have pages in common."""
+        if (lo, hi) not in self.sharing:
+            runs, found = self.runs(lo, hi), None
+            if any(size > 1 and shared for size, shared in runs):
+                from .kernels.prefix import PrefixGroups
+
+                shared = torch.tensor([n for _, n in runs], dtype=torch.int32).to(self.table.device)
+                found = _Sharing(PrefixGroups([size for size, _ in runs], self.table.device), shared, max(n for _, n in runs))
+            self.sharing[lo, hi] = found
+        return self.sharing[lo, hi]
+
+    def singles(self, lo: int, hi: int) -> object:
+        """Every sequence a group of its own."""
+        from .kernels.prefix import PrefixGroups
+
+        key = (lo, hi, "singles")
+        if key not in self.sharing:
+            self.sharing[key] = PrefixGroups([1] * (hi - lo), self.table.device)
+        return self.sharing[key]
 
     def undo(self) -> None:
         """Take back the pass that has begun and written nothing: the cache is as it was before."""
@@ -370,6 +442,12 @@ class SISAPagedCache:
         ends = [n + c for n, c in zip(self.lengths, counts)]
         if max(ends) > st.max_length:
             raise ValueError(f"SISAPagedCache: {max(ends)} positions exceed max_length = {st.max_length}")
+        trial = st.trial
+        if trial is not None and lo < trial.hi and trial.lo < hi:
+            if (lo, hi) != (trial.lo, trial.hi):
+                raise ValueError("SISAPagedCache: a pass of tentative sequences takes all of them")
+            if ends[0] - trial.starts[0] > trial.room:
+                raise ValueError(f"SISAPagedCache: more than the {trial.room} positions that tentative() was told of")
         st.begun = _Begun(lo, hi, [len(pages) for pages in st.held[lo:hi]], st.starts[lo:hi], st.lengths[lo:hi],
                           st.expected[lo:hi])
         try:
@@ -454,7 +532,38 @@ class SISAPagedCache:
             raise RuntimeError("SISAPagedCache is for inference: run the model under torch.no_grad()")
         count = self.begin(layer_idx, p.k, p.b, hip)
         with self.writing(layer_idx):
+            self._note(layer_idx, p)
             self.put(layer_idx, (p.k, p.v, p.b, p.g.float(), p.fgate.float()), at_last(p.phi, count)[:, :, 0], count, hip)
+
+    def _rows(self, layer_idx: int) -> tuple[Tensor, int] | None:
+        """Of a pass of tentative positions that has begun: the layer's states, and the place of the one before it."""
+        st = self._store
+        trial = st.trial
+        if trial is None or (trial.lo, trial.hi) != (self._lo, self._hi):
+            return None
+        rows, last = trial.rows.get(layer_idx), st.layers[layer_idx].last
+        if rows is None:
+            rows = trial.rows[layer_idx] = last.phi.new_empty((len(self), last.phi.shape[1], trial.room + 1,
+                                                               2 + last.phi.shape[2]))
+        return rows, st.starts[self._lo] - trial.starts[0]
+
+    def _note(self, layer_idx: int, p) -> None:
+        found = self._rows(layer_idx)
+        if found is None:
+            return
+        (rows, at), M = found, p.k.shape[2]
+        before = _Last(*(t[self._lo:self._hi] for t in self._store.layers[layer_idx].last))
+        rows[:, :, at] = torch.cat([before.g, before.fgate, before.phi], -1)
+        rows[:, :, at + 1:at + 1 + M] = torch.cat([p.g[..., None], p.fgate[..., None], p.phi], -1)
+
+    def _sharing(self) -> _Sharing | None:
+        """Which positions the sequences' new rows have in common: a prompt's with its other branches, or, for positions that may
+        be taken back, all that lies before them with each other."""
+        st, lo, hi = self._store, self._lo, self._hi
+        found = st.grouped(lo, hi)
+        if found is None and st.trial is not None and (st.trial.lo, st.trial.hi) == (lo, hi):
+            found = _Sharing(st.singles(lo, hi), st.start[lo:hi], max(st.starts[lo:hi]))
+        return found
 
     def attend(self, layer_idx: int, p, lam: Tensor, hip: bool) -> Tensor:
         """The attention of the rows that :meth:`extend` has just written, ``(B, H, M, d_head)`` float32 (float64 rows:
@@ -473,6 +582,12 @@ class SISAPagedCache:
 
         st, lo, hi = self._store, self._lo, self._hi
         table, lengths, longest, (B, H, M, _) = st.table[lo:hi], st.end[lo:hi], self.seq_len, p.q.shape
+        sharing = None if weights is not None else self._sharing()
+        if sharing is not None:
+            from .kernels.prefix import sisa_prefix_decode_hip
+
+            return sisa_prefix_decode_hip(p.q, p.c, p.g, p.fgate, lam, pool, table, lengths, sharing.groups, sharing.shared,
+                                          max_len=longest, max_shared=sharing.most)
         rows = max(1, MAX_SCORES // (B * H * longest))
         if rows >= M:
             return sisa_paged_decode_hip(p.q, p.c, p.g, p.fgate, lam, pool, table, lengths, max_len=longest, weights=weights)
@@ -520,6 +635,129 @@ class SISAPagedCache:
     def end_step(self, layer_idx: int) -> None:
         self._written(self._store.layers[layer_idx])
 
+    def shares(self) -> bool:
+        """Whether the sequences of a :meth:`kernel_layer` are for the kernels of common positions: branches of a prompt, or
+        positions that may be taken back."""
+        st, lo, hi = self._store, self._lo, self._hi
+        trial = st.trial
+        return (trial is not None and (trial.lo, trial.hi) == (lo, hi)) or st.grouped(lo, hi) is not None
+
+    def begin_rows(self, layer_idx: int, M: int) -> tuple["_Step", _Sharing, tuple[Tensor, int] | None]:
+        """:meth:`begin_step` for ``M`` positions of every sequence of a cache that :meth:`shares`, with what they share and where
+        their states go."""
+        st, lo, hi = self._store, self._lo, self._hi
+        layer = st.layers[layer_idx]
+        self._begin(layer, M)
+        with self.writing(layer_idx):
+            at = _Step(layer.pool, st.table[lo:hi], st.start[lo:hi], st.end[lo:hi], _Last(*(t[lo:hi] for t in layer.last)), None,
+                       self.seq_len)
+            return at, self._sharing(), self._rows(layer_idx)
+
+    # -------------------------------------------------------------------------------------------- branches and drafts
+    def _settled(self, what: str) -> None:
+        """A call between whole passes of a cache that is not tracked."""
+        st = self._store
+        st.undo()
+        if st.track:
+            raise ValueError(f"SISAPagedCache.{what}: a cache with track=True accumulates weights, which cannot be shared or taken "
+                             f"back")
+        if st.trial is not None and self._lo < st.trial.hi and st.trial.lo < self._hi:
+            raise RuntimeError(f"SISAPagedCache.{what}: keep() the tentative positions first")
+        for layer in st.layers.values():
+            if layer.filled[self._lo:self._hi] != self.lengths:
+                raise RuntimeError(f"SISAPagedCache.{what}: a forward pass has not reached every layer")
+
+    def branch(self, n: int) -> None:
+        """Continue every prompt ``n`` times. The first ``len(self) // n`` of these sequences hold the prompts, the others are
+        empty; afterwards sequences ``i n .. i n + n - 1`` continue prompt ``i``. Its whole pages belong to all of them, and are
+        read once for all of them by their attention; what lies in a page that is not full is copied."""
+        st, lo, hi = self._store, self._lo, self._hi
+        self._settled("branch")
+        if n < 1 or len(self) % n:
+            raise ValueError(f"SISAPagedCache.branch: {len(self)} sequences are not prompts of n = {n} each")
+        k = len(self) // n
+        lengths = self.lengths
+        if not all(lengths[:k]) or any(lengths[k:]):
+            raise ValueError(f"SISAPagedCache.branch: the first {k} sequences hold the prompts, the others must be empty; lengths "
+                             f"are {lengths}")
+        if n == 1:
+            return
+        S = st.page_size
+        whole, old = [m // S for m in lengths[:k]], [st.held[lo + i] for i in range(k)]
+        src = [old[i][whole[i]] for i in range(k) if lengths[i] % S for _ in range(n - 1)]
+        free = [*st.free, *(page for i in range(lo + k, hi) for page in st.held[i])]       # some that reserve() has taken
+        if len(src) > len(free):
+            raise RuntimeError(f"SISAPagedCache.branch: {len(src)} pages are needed for the copies of pages that are not full, "
+                               f"{len(free)} are free")
+        dst = [free.pop() for _ in src]
+        states = [[t[lo:lo + k].repeat_interleave(n, 0) for t in layer.last] for layer in st.layers.values()]
+        if src:                                            # no sequence holds what is written yet
+            a, b = (torch.tensor(x).to(st.table.device) for x in (src, dst))
+            for layer in st.layers.values():
+                pool = layer.pool
+                for t in (pool.k, pool.v, pool.b, pool.g, pool.fgate):
+                    t[b] = t[a]
+        for layer, state in zip(st.layers.values(), states):
+            for t, x in zip(layer.last, state):
+                t[lo:hi] = x
+        copies, held = iter(dst), []
+        for i in range(k):
+            for page in old[i][:whole[i]]:
+                st.others[page] = st.others.get(page, 0) + n - 1
+            held.append(old[i])
+            held += [old[i][:whole[i]] + ([next(copies)] if lengths[i] % S else []) for _ in range(n - 1)]
+        st.free[:], st.held[lo:hi] = free, held
+        ends = [m for m in lengths[:k] for _ in range(n)]
+        st.starts[lo:hi], st.lengths[lo:hi] = list(ends), list(ends)
+        for i in range(k):
+            st.families += 1
+            st.family[lo + i * n:lo + i * n + n] = [(st.families, whole[i])] * n
+        st.sharing.clear()
+        for layer in st.layers.values():
+            layer.filled[lo:hi] = list(ends)
+        st.expected[lo:hi] = [None] * len(self)
+        st.end[lo:hi].copy_(torch.tensor(ends, dtype=torch.int32))
+        st.show(range(lo, hi))
+
+    def tentative(self, positions: int) -> None:
+        """The next passes, of up to ``positions`` positions of every sequence, are proposals, of which :meth:`keep` says what
+        stays. They take all of these sequences together."""
+        self._settled("tentative")
+        if positions < 1:
+            raise ValueError(f"SISAPagedCache.tentative: positions = {positions} must be positive")
+        if not all(self.lengths):
+            raise ValueError("SISAPagedCache.tentative: an empty sequence has nothing to go back to")
+        if self._store.trial is not None:
+            raise RuntimeError("SISAPagedCache.tentative: other sequences' positions are tentative; keep() them first")
+        self._store.trial = _Trial(self._lo, self._hi, positions, self.lengths)
+
+    def keep(self, counts: Sequence[int]) -> None:
+        """Keep the first ``counts[n]`` positions of every sequence since :meth:`tentative`, and go on from there."""
+        st, lo, hi = self._store, self._lo, self._hi
+        st.undo()
+        trial, counts = st.trial, [int(c) for c in counts]
+        if trial is None or (trial.lo, trial.hi) != (lo, hi):
+            raise RuntimeError("SISAPagedCache.keep: tentative() comes first, for the same sequences")
+        added = self.lengths[0] - trial.starts[0]
+        if len(counts) != len(self) or any(not 0 <= c <= added for c in counts):
+            raise ValueError(f"SISAPagedCache.keep: {counts}: for each of the {len(self)} sequences 0 .. {added} positions")
+        for layer in st.layers.values():
+            if layer.filled[lo:hi] != self.lengths:
+                raise RuntimeError("SISAPagedCache.keep: a forward pass has not reached every layer; release() the sequences")
+        if min(counts) < added:
+            ends = [n + c for n, c in zip(trial.starts, counts)]
+            row = torch.arange(len(self), device=st.table.device)
+            at = torch.tensor(counts).to(st.table.device)
+            for i, layer in st.layers.items():
+                state = trial.rows[i][row, :, at]
+                for t, x in zip(layer.last, (state[..., 0:1], state[..., 1:2], state[..., 2:])):
+                    t[lo:hi] = x
+            st.end[lo:hi].copy_(torch.tensor(ends, dtype=torch.int32))
+            st.starts[lo:hi], st.lengths[lo:hi] = list(ends), list(ends)
+            for layer in st.layers.values():
+                layer.filled[lo:hi] = list(ends)
+        st.trial = None
+
     # -------------------------------------------------------------------------------------------- memory
     def reserve(self, positions: int) -> None:
         """Take the pages that ``positions`` more positions of every sequence need now, not as they come."""
@@ -534,8 +772,12 @@ class SISAPagedCache:
         st, lo, hi = self._store, self._lo, self._hi
         st.undo()
         for n in range(lo, hi):
-            st.free += reversed(st.held[n])
+            st.give(reversed(st.held[n]))
             st.held[n] = []
+        st.family[lo:hi] = [None] * len(self)
+        st.sharing.clear()
+        if st.trial is not None and lo < st.trial.hi and st.trial.lo < hi:
+            st.trial = None
         st.starts[lo:hi] = st.lengths[lo:hi] = [0] * (hi - lo)
         for layer in st.layers.values():
             layer.filled[lo:hi] = [0] * (hi - lo)

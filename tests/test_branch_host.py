@@ -30,7 +30,8 @@ def test_header_functions_are_exported(lib):
 
 def test_struct_layout_matches_c(tmp_path):
     from sisa_amd.kernels import _lib
-    pairs = {"PrefixDecodeArgs": "sisa_prefix_decode_args", "VerifyArgs": "sisa_verify_args"}
+    pairs = {"PrefixDecodeArgs": "sisa_prefix_decode_args", "VerifyArgs": "sisa_verify_args",
+             "StepBranchArgs": "sisa_step_branch_args"}
     lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "sisa_hip_branch.h"', "int main(void) {"]
     expect = []
     for py, c in pairs.items():
@@ -38,7 +39,8 @@ def test_struct_layout_matches_c(tmp_path):
         lines.append(f'printf("%zu\\n", sizeof({c}));')
         expect.append(ctypes.sizeof(cls))
         for name, _ in cls._fields_:
-            lines.append(f'printf("%zu\\n", offsetof({c}, {name}));')
+            inner = py == "StepBranchArgs" and name in dict(_lib.StepPagedArgs._fields_)
+            lines.append(f'printf("%zu\\n", offsetof({c}, {"step." * inner}{name}));')
             expect.append(getattr(cls, name).offset)
     lines += ["return 0;", "}"]
     (tmp_path / "layout.c").write_text("\n".join(lines))
@@ -68,7 +70,7 @@ def test_attention_refuses_bad_arguments(lib):
     assert lib.sisa_prefix_decode(None, None) == 1 and lib.sisa_last_error().decode().startswith("sisa_prefix_decode")
 
     def args(B=2, M=1, W=1, G=1, max_len=16, max_shared=16, out_dtype=0, pool=None, table=4096, lengths=4096, first=4096,
-             group=4096, shared=4096, q=row, c=row, gq=gate, fq=gate, lam=4096, out=4096, ws=4096):
+             group=4096, shared=4096, q=row, c=row, gq=gate, fq=gate, lam=4096, out=row, ws=4096):
         return _lib.PrefixDecodeArgs(B, M, W, G, max_len, max_shared, out_dtype, 0, pool or _pool(), table, W, lengths, first,
                                      group, shared, q, c, gq, fq, lam, 1, out, ws)
     for bad, word in ((dict(pool=_pool(page_size=24)), "power of two"), (dict(pool=_pool(g=none)), "no g"), (dict(W=0), "bad shape"),
@@ -76,12 +78,36 @@ def test_attention_refuses_bad_arguments(lib):
                       (dict(max_len=0), "max_len=0"), (dict(max_shared=17), "max_shared=17"), (dict(max_shared=-1), "max_shared=-1"),
                       (dict(out_dtype=_lib.F16), "out_dtype"), (dict(q=crooked), "aligned"), (dict(c=crooked), "aligned"),
                       (dict(gq=none), "gq"), (dict(fq=none), "fq"), (dict(ws=None), "workspace"), (dict(ws=4104), "workspace"),
-                      *((dict([(x, None)]), "null pointer") for x in ("table", "lengths", "first", "group", "shared", "lam", "out")),
+                      *((dict([(x, None)]), "null pointer") for x in ("table", "lengths", "first", "group", "shared", "lam")),
+                      (dict(out=none), "null pointer"),
                       # threads of a launch are counted in 32 bits
                       (dict(B=1 << 27), "too large"), (dict(B=1 << 26, W=1 << 20, max_len=1 << 24, max_shared=0), "too large"),
                       (dict(B=1 << 20, M=128), "too large"), (dict(B=1 << 20, M=1 << 10), "2^28")):
         _refused(lib, "sisa_prefix_decode", args(**bad), word)
     assert lib.sisa_prefix_decode(ctypes.byref(args(B=0)), None) == 0
+
+
+def test_step_refuses_bad_arguments(lib):
+    from sisa_amd.kernels import _lib
+    assert lib.sisa_step_branch(None, None) == 1 and lib.sisa_last_error().decode().startswith("sisa_step_branch")
+    none = _lib.View(None, 0, 0, 0)
+
+    def args(B=2, M=3, G=1, H=2, D=128, dtype=_lib.BF16, W=1, max_len=16, max_shared=16, row0=0, w_q=4096, pool=None, phi=4096,
+             weights=none, first=4096, group=4096, shared=4096, rows=4096, s_rows=4 * 18, ws=4096):
+        return _lib.StepBranchArgs(B, H, D, 256, dtype, W, max_len, 0, 1e-6, 1e-6, 4096, D, None, 4096, w_q, *[4096] * 15,
+                                   pool or _pool(), 4096, W, 4096, 4096, 4096, 4096, phi, weights, 4096, 4096, ws, M, G, max_shared,
+                                   row0, first, group, shared, rows, s_rows)
+    for bad, word in ((dict(B=0), "1 .. 64"), (dict(M=0), "1 .. 64"), (dict(B=13, M=5), "1 .. 64"), (dict(B=1 << 30, M=4), "1 .. 64"),
+                      (dict(D=192), "B must be"), (dict(dtype=_lib.F32), "bf16 or fp16"), (dict(w_q=None), "given"), (dict(ws=4112), "256-byte"),
+                      (dict(pool=_pool(dtype=_lib.F16)), "heads and dtype"), (dict(pool=_pool(heads=3)), "heads and dtype"),
+                      (dict(pool=_pool(f=none)), "and f"), (dict(pool=_pool(page_size=20)), "power of two"), (dict(max_len=17), "max_len"),
+                      (dict(max_shared=17), "max_shared"), (dict(max_shared=-1), "max_shared"), (dict(G=0), "G=0"), (dict(G=3), "G=3"),
+                      (dict(weights=_lib.View(4096, 32, 16, 1)), "tracked"), (dict(row0=-1), "row0"), (dict(s_rows=71), "row0"),
+                      (dict(row0=1), "row0"), *((dict([(x, None)]), "null pointer") for x in ("phi", "first", "group", "shared"))):
+        _refused(lib, "sisa_step_branch", args(**bad), word)
+    size = lib.sisa_step_branch_workspace_bytes
+    assert size(0, 2, 128, 256, 1, 1, 16, 0) == size(1, 2, 128, 256, 65, 1, 16, 0) == size(1, 2, 128, 256, 1, 1, 16, -1) == 0
+    assert size(2, 2, 128, 256, 4, 1, 600, 500) > size(2, 2, 128, 256, 1, 1, 600, 500) > 0
 
 
 def test_verification_refuses_bad_arguments(lib):
