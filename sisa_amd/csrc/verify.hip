@@ -159,7 +159,7 @@ __global__ __launch_bounds__(NTH) void verify_find_kernel(sisa_verify_args a, un
             double run = ahead + up - own;
             for (unsigned c = c0; c < c1; ++c) {
                 const double x = sum_of(c);
-                if (run + x > goal) {
+                if (x > 0. && run + x > goal) {
                     atomicMin(&owner, (int)c);
                     break;
                 }

@@ -549,3 +549,17 @@ def test_another_stream():
         got, verified = case.run(*rows), _verify(p, drafts, u, q)
     side.synchronize()
     assert torch.equal(got, plain) and torch.equal(verified.tokens, want.tokens)
+
+
+@pytest.mark.parametrize("empty", [3, 5, 6])
+def test_a_border_that_rounding_moves_past_tokens_without_weight(empty):
+    """Sums of 1,024 tokens whose total up to a chunk depends on the order of its additions, 1 or 1 + 2^-52 for weights 2^-53,
+    2^-53 and 1, with the goal 0.5 * 2 between them, and a chunk behind them that holds nothing: the token is one that has a
+    weight, on either side of the border."""
+    chunk = 1024
+    p = torch.zeros((1, 1, 8 * chunk), device=DEV)
+    weights = {empty - 3: 2.0 ** -53, empty - 2: 2.0 ** -53, empty - 1: 1.0, empty + 1: 1.0}
+    for c, x in weights.items():
+        p[0, 0, c * chunk + 17] = x
+    got = _verify(p, torch.empty((1, 0), dtype=torch.int64, device=DEV), torch.tensor([[0.5]], device=DEV))
+    assert got.tokens.item() in ((empty - 1) * chunk + 17, (empty + 1) * chunk + 17)
