@@ -12,6 +12,13 @@
 // O^T += V^T P^T as they are. K and b~ go from memory to the operand registers; v passes through LDS, which transposes it. The
 // weights enter their product as a sum of two (fp16) or three (bf16) operands, so that the result is an fp32 one: rounded once
 // to bf16 they would be off by 2^-9.
+//
+// Both launches, from a kernel trace, bf16: 64 rows against 16,384 common positions of 12 heads 41 us (114 MB at 2.8 TB/s; a
+// copy reaches 4.8), 24 x 8 drafts against up to 6,000 46 us (169 MB, 3.7 TB/s), 256 rows against 1,500 and up to 1,000 of
+// their own 60 us. What a wave holds is kept few enough for four waves a SIMD, strides and bases in scalar registers. The first
+// launch for the 64 rows: 64 rows to a wave, 256 registers 91 us; 16 rows to a wave, 168 registers 41; this form 34. A head's
+// positions are read beside the other heads', whose rows follow in memory: with each head by itself an earlier form of the
+// loads took 47 us there, against 36.
 #include "pages.h"
 #include "sisa_hip_branch.h"
 
@@ -151,7 +158,7 @@ template <class X> SISA_DEV X again(size_t offset) {
 template <class T>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 4 : 3))) void prefix_part_kernel(
     PartArgs args) {
-    constexpr int LD = DH + 4;
+    constexpr int LD = DH + 4;         // rows apart by 4 banks
     __shared__ WaveLds<T> lds[NW];
     __shared__ __attribute__((aligned(16))) float ms[NW][16], ls[NW][16], os[NW][16][LD];
     const sisa_prefix_decode_args& a = args.a;
@@ -294,8 +301,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
             if (p1 < 0) x.f[1] = __builtin_nanf("");
         }
         if (tile == t.from) {                            // the first loads are under way: what has come of the query rows
-            const int seen = len - back;
-            lim = len < 0 || len > max_len || len > held ? -1 : seen > 0 ? seen : 0;
+            lim = len < 0 || len > max_len || len > held ? -1 : len > back ? len - back : 0;
             lim = lim < k.hi ? lim : k.hi;
             least = lim < 0 ? k.hi : lim;                // the join answers for rows that see nothing defined
             if (lc >= k.rows) lim = 0, least = k.hi, gq = -__builtin_inff();
@@ -566,18 +572,19 @@ Plan plan_of(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64_
     const int64_t rows = sisa::cdiv(B, G) * M;           // of a group, on average
     p.log_rw = rows <= 16 ? 0 : rows <= 32 ? 1 : 2;
     const int64_t per = (int64_t)16 << p.log_rw;
-    p.tiles = (unsigned)(max_shared > 0 ? G + B * M / per : 0);
+    p.tiles = (unsigned)(max_shared > 0 ? G - 1 + sisa::cdiv(B * M, per) : 0);
     p.own_tiles = (unsigned)sisa::cdiv(M, 16);
     p.own_rows = (unsigned)(M < 16 ? M : 16);
-    // As many parts as fill the chip while a wave keeps a tile, or, for longer ranges, more of them of eight tiles to a wave,
-    // which even out: `few` and `many` workgroups, or waves, in all. us of the first launch, few alone / many alone / the larger
-    // of both: 16 rows of 2,000 common positions of 12 heads 9.4 / 14.1 / 9.4; 24 x 8 drafts of up to 6,000 53 / 41 / 41.
+    // As many parts as fill the chip while a wave keeps a tile, or, for longer ranges, more of them of twelve tiles to a wave,
+    // which even out: `few` and `many` workgroups, or waves, in all. us of the first launch with `few` alone / `many` alone /
+    // the larger of both: 16 rows of 2,000 common positions of 12 heads 9.9 / 17.5 / 10.7, 64 of 16,384 33 / 34 / 34, 24 x 8
+    // drafts of up to 6,000 53 / 40 / 40, 256 rows of 1,500 and up to 1,000 of their own 69 / 49 / 52.
     auto parts = [](int64_t items, int64_t positions, int64_t tile, int64_t few, int64_t many) {
         auto of = [&](int64_t total, int64_t each) {
             const int64_t most = sisa::cdiv(positions, each), want = items > 0 ? sisa::cdiv(total, items) : 1;
             return want < most ? want : most;
         };
-        const int64_t a = of(few, tile), b = of(many, 8 * tile), n = a > b ? a : b;
+        const int64_t a = of(few, tile), b = of(many, 12 * tile), n = a > b ? a : b;
         return (unsigned)(n < 1 ? 1 : n > MOST ? MOST : n);
     };
     p.parts = parts(p.tiles * H, max_shared, KT * NW >> p.log_rw, 512, 2048);
