@@ -11,8 +11,8 @@ writes its rows in place and the layer state handed to the attention is a view o
 the new rows' bytes, not a copy of the whole cache. ``generate`` sizes the slabs for the prompt plus every new token
 up front; a cache made without a capacity grows by doubling. When the appended rows carry autograd history the slab
 is rebuilt out of place instead, so gradients still flow. Batched decoding with this cache assumes equal-length prompts
-(there is no padding mask); prompts of unequal lengths, and a bound on the positions that are kept, go through
-:class:`sisa_amd.paged.SISAPagedCache`.
+(there is no padding mask); prompts of unequal lengths, a bound on the positions that are kept, several continuations of a
+prompt and tokens that a draft model proposes go through :class:`sisa_amd.paged.SISAPagedCache`.
 """
 from __future__ import annotations
 

@@ -721,7 +721,8 @@ class SISAPagedCache:
 
     def tentative(self, positions: int) -> None:
         """The next passes, of up to ``positions`` positions of every sequence, are proposals, of which :meth:`keep` says what
-        stays. They take all of these sequences together."""
+        stays. They take all of these sequences together; :meth:`release` of any of them ends the trial, and what the others have
+        taken stays."""
         self._settled("tentative")
         if positions < 1:
             raise ValueError(f"SISAPagedCache.tentative: positions = {positions} must be positive")
