@@ -182,19 +182,22 @@ def _probabilities(logits: Tensor, temperature: float, top_k: int | None) -> Ten
 
 
 def verify_drafts(p: Tensor, drafts: Tensor, u: Tensor, q: Tensor) -> tuple[Tensor, Tensor]:
-    """:func:`sisa_amd.kernels.verify.sisa_verify_drafts_hip` in plain PyTorch, on any device: ``(tokens, accepted)``."""
-    B, K = drafts.shape
+    """:func:`sisa_amd.kernels.verify.sisa_verify_drafts_hip` in plain PyTorch, on any device, for rows that all have ``K`` drafts
+    drawn from ``q``: ``(tokens, accepted)``."""
+    (B, K), V = drafts.shape, p.shape[2]
     row, i = torch.arange(B, device=p.device), torch.arange(K + 1, device=p.device)
-    at, u = drafts[..., None], u.double()
+    at, u = drafts.clamp(0, V - 1)[..., None], u.double()
     took = u[:, :K] * q.gather(2, at)[..., 0].double() < p[:, :K].gather(2, at)[..., 0].double()
+    took &= (drafts >= 0) & (drafts < V)
     accepted = took.long().cumprod(1).sum(1)
     target = p[row, accepted].double()
-    rest = (target - q[row, accepted.clamp(max=K - 1)].double()).clamp(min=0.0)
-    weights = torch.where(((accepted < K) & (rest.sum(1) > 0))[:, None], rest, target)
-    upto = weights.cumsum(1)
-    over = (upto > u[:, K:] * upto[:, -1:]) & (weights > 0)
-    last = weights.shape[1] - 1 - (weights > 0).flip(1).int().argmax(1)
-    token = torch.where(over.any(1), over.int().argmax(1), last)
+    behind_all = torch.cat([q, q.new_zeros((B, 1, V))], 1)         # after the last draft nothing is taken off
+    rest = (target - behind_all[row, accepted].double()).clamp(min=0.0)
+    weights = torch.where((rest.sum(1) == 0)[:, None], target.clamp(min=0.0), rest)
+    total, upto, some = weights.sum(1), weights.cumsum(1), weights > 0
+    over = (upto > u[:, K:] * upto[:, -1:]) & some
+    token = torch.where(over.any(1), over.int().argmax(1), V - 1 - some.flip(1).int().argmax(1))
+    token = torch.where(total.isfinite() & (total > 0), token, -1)
     padded = torch.cat([drafts, drafts.new_full((B, 1), -1)], 1)
     behind, here = i > accepted[:, None], i == accepted[:, None]
     return torch.where(behind, -1, torch.where(here, token[:, None], padded)), accepted.to(torch.int32)

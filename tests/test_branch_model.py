@@ -246,6 +246,50 @@ def test_plain_verification(V):
     assert torch.equal(accepted, want[1])
 
 
+def test_plain_verification_edges():
+    """What test_verify_edges asks of the kernel: weights that are 0 everywhere, sums that are not finite, values below 0, drafts
+    outside the vocabulary, random numbers at the ends of their range and outside it; and no drafts at all."""
+    nan, inf, V = float("nan"), float("inf"), 100
+    gen = torch.Generator().manual_seed(5)
+    p, q = (torch.randn(19, k, V, generator=gen).mul(3).softmax(-1) for k in (3, 2))
+    drafts = torch.multinomial(q.flatten(0, 1), 1, generator=gen).view(19, 2)
+    u = torch.full((19, 3), 0.99999994)
+    drafts[0, 0], drafts[1, 0], drafts[2, 1] = -1, V, 1 << 40
+    p[3, 0], u[3] = q[3, 0], 1.0                          # refused with nothing left of p - q
+    p[4] = 0.0                                            # nothing to draw from
+    for n in range(5, 9):
+        p[n, 0, drafts[n, 0]] = 0.0                       # the first draft is refused
+    for n, (x, y) in enumerate(((nan, 0.1), (inf, 0.1), (0.1, nan), (inf, inf)), 5):
+        at = 7 if int(drafts[n, 0]) != 7 else 8
+        p[n, 0, at], q[n, 0, at] = x, y
+    u[9, 2], u[10, 2], u[11, 2], u[12, 2], u[13, 2] = 0.0, 1.0, -1.0, 2.0, nan
+    p[9:14, :, :5] = p[9:14, :, 95:] = 0.0                # first and last tokens that cannot be
+    u[14, 0] = nan
+    p[15] = -0.25                                         # not probabilities: below 0 counts as 0
+    p[16], u[17, :2], p[17, 2], u[18, :2] = nan, 0.0, 0.0, 0.0
+    p[18, 2, 50:] = -1.0                                  # after the last draft, too
+    tokens, accepted = verify_drafts(p, drafts, u, q)
+    want = _want(p, drafts, u, q)
+    assert accepted.tolist() == want[1].tolist() and tokens.tolist() == want[0].tolist()
+    assert all(tokens[n, accepted[n]] == -1 for n in (4, 5, 6, 7, 8, 15, 16, 17)) and accepted[17] == accepted[18] == 2
+    none = verify_drafts(p[:, :1], drafts[:, :0], u[:, 2:], q[:, :0])
+    assert none[0].tolist() == _want(p[:, :1], drafts[:, :0], u[:, 2:], q[:, :0])[0].tolist() and not none[1].any()
+
+
+def test_generate_with_a_draft_ends_where_probabilities_are_not_finite():
+    model, small, ids = _model64(), tiny_model(seed=5, n_layer=1).double().eval(), token_ids(2, 9, seed=8)
+    kw = dict(do_sample=True, draft=small, draft_tokens=3, generator=torch.Generator().manual_seed(3))
+    for value in (float("nan"), float("inf"), float("-inf")):
+        def later(module, args, kwargs, out):             # all but the prompt's pass
+            if kwargs["cache"].seq_len > 9:
+                out.logits.fill_(value)
+        hook = model.register_forward_hook(later, with_kwargs=True)
+        with pytest.raises(RuntimeError, match="not finite"):
+            generate(model, ids, 8, **kw)
+        hook.remove()
+    assert generate(model, ids, 8, **kw).shape == (2, 17)
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,bound", [(torch.float32, 2e-5), (torch.bfloat16, 5e-2), (torch.float16, 1e-2)])
