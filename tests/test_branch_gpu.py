@@ -563,3 +563,23 @@ def test_a_border_that_rounding_moves_past_tokens_without_weight(empty):
         p[0, 0, c * chunk + 17] = x
     got = _verify(p, torch.empty((1, 0), dtype=torch.int64, device=DEV), torch.tensor([[0.5]], device=DEV))
     assert got.tokens.item() in ((empty - 1) * chunk + 17, (empty + 1) * chunk + 17)
+
+
+def test_verify_infinities_on_both_sides():
+    """Where p and q are infinite at one token their difference is not a number, and so is the sum: no token, in the first
+    1,024 tokens, behind them and at the end; beside an infinite p or q alone."""
+    inf, V = math.inf, 2600
+    for types in ((torch.float32, None), (torch.bfloat16, torch.float16)):
+        p, drafts, u, q = _drafted(6, 2, V, *types, seed=14)
+        u[:, 2] = torch.tensor([0.0, 0.3, 0.6, 0.9, 0.99999994, 0.5], device=DEV)
+        for n, at in enumerate((5, 1030, V - 1, 700, 2047, 2048)):
+            x = int(drafts[n, 0])
+            p[n, 0, x] = 0.0                              # the first draft is refused
+            at += at == x
+            if at == V:
+                at = V - 2
+            p[n, 0, at] = inf if n != 4 else 0.1
+            q[n, 0, at] = inf if n != 3 else 0.1
+        want = _want(p, drafts, u, q)
+        assert want[1].tolist() == [0] * 6 and [int(t) < 0 for t in want[0][:, 0]] == [True, True, True, True, False, True]
+        _same(_verify(p, drafts, u, q), want)
