@@ -274,9 +274,9 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(sizeof(
         X x;
         {
             const int i = 2 * (tile - base), p0 = __builtin_amdgcn_readlane(near_pages, i), p1 = __builtin_amdgcn_readlane(near_pages, i + 1);
-            const int left = k.hi - jt, at0 = p0 < 0 ? 0 : p0, at1 = p1 < 0 ? 0 : p1;
-            int slot = jt & mask, end = slot + (left < KT ? left : KT);
-            end = p0 < 0 ? 0 : end;
+            const int left = k.hi - jt < KT ? k.hi - jt : KT, at0 = p0 < 0 ? 0 : p0, at1 = p1 < 0 ? 0 : p1;
+            int slot = jt & mask, end = slot + left;     // a row of the page, so that end times a row's bytes fits 32 bits
+            end = p0 < 0 ? 0 : end <= mask ? end : mask + 1;
             const char *bk = sk.at(at0), *bv = sv.at(at0), *bb = sb.at(at0), *bg = sg.at(at0), *bf = sf.at(at0);
             constexpr int ROWS = 64 / X::CPR, HALF = X::PASS / 2;
 #pragma unroll

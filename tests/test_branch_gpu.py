@@ -583,3 +583,26 @@ def test_verify_infinities_on_both_sides():
         want = _want(p, drafts, u, q)
         assert want[1].tolist() == [0] * 6 and [int(t) < 0 for t in want[0][:, 0]] == [True, True, True, True, False, True]
         _same(_verify(p, drafts, u, q), want)
+
+
+@pytest.mark.parametrize("wide", ["k", "v", "b", "g", "f"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_far_apart_in_pages_of_16(wide, dtype):
+    """Pages of 16 positions whose rows lie 2^20 bytes apart, every page's and head's beside each other, more than 4,096
+    positions of them: the bytes of what is left of a range pass 2^32, those of a page do not."""
+    from sisa_amd.kernels.paged import PagePool
+    case = Grouped([2, 1, 1], [4119, 4112, 0], [9, 70, 5, 4125], 2, 16, dtype, seed=15)
+    for x in (case.rows, case.t):
+        for gate in "gf":
+            x[gate] *= 0.01                               # flat enough for the first positions to weigh as much as the last
+    rows = case.queries(2)
+    plain = case.run(*rows)
+    assert _rel(plain, case.want(*rows)) <= TOL
+    t = case.t[wide]
+    P, H, S = t.shape[:3]
+    width = t[0, 0, 0].numel()
+    far = torch.zeros(S * (1 << 20) // t.element_size(), device=DEV, dtype=t.dtype)
+    assert P * H * width * t.element_size() <= 1 << 20
+    far = far.as_strided(t.shape, (H * width, width, (1 << 20) // t.element_size(), *t.stride()[3:])).copy_(t)
+    case.pool = PagePool(*(far if x == wide else case.t[x] for x in ("k", "v", "b", "g", "f")))
+    assert torch.equal(case.run(*rows), plain)
