@@ -228,12 +228,17 @@ class _Budget:
         self.slack = max(16, keep // 8)
 
 
-def _paged_cache(rows: int, longest: int, new: int, budget: _Budget | None) -> SISAPagedCache:
-    """A cache for prompts of up to ``longest`` positions and ``new`` more, or for what a budget lets them grow to."""
+def _paged_cache(lengths: list[int], new: int, budget: _Budget | None, samples: int = 1) -> SISAPagedCache:
+    """A cache for prompts of these lengths and ``new`` more positions of each of their samples, or for what a budget lets them
+    grow to. The whole pages of a prompt are held once."""
+    rows, longest = len(lengths) * samples, max(lengths)
+    size, each = 64, lambda n: -(-n // 64)  # noqa: E731
+    if samples > 1:
+        pages = sum(n // size + samples * (each(n + new) - n // size) for n in lengths)
+        return SISAPagedCache(rows, longest + new, pages=pages, page_size=size)
     if budget is None:
         return SISAPagedCache(rows, longest + new)
     top = max(longest + 1, min(longest + new, budget.keep + budget.slack) + 1)
-    size, each = 64, lambda n: -(-n // 64)  # noqa: E731
     return SISAPagedCache(rows, top, pages=rows * (each(top) + each(budget.keep)), page_size=size, track=True)
 
 
@@ -294,9 +299,9 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
         return result if input_ids.dim() == 2 else result.squeeze(0)
     stop_ids = torch.tensor(stops, device=rows.device, dtype=rows.dtype) if stops else None
     prompt, prompts = rows.shape[1], rows.shape[0]
+    first = [prompt] * prompts if lengths is None else lengths
     if samples > 1:
         rows = rows.repeat_interleave(samples, 0)
-        lengths = None if lengths is None else [n for n in lengths for _ in range(samples)]
     out = rows.new_empty((rows.shape[0], prompt + max_new_tokens))
     out[:, :prompt] = rows
     length = prompt
@@ -304,12 +309,11 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
         if lengths is None and budget is None and samples == 1:
             cache = SISACache(capacity=prompt + max_new_tokens)
         else:
-            cache = _paged_cache(rows.shape[0], max(lengths or [prompt]), max_new_tokens, budget)
+            cache = _paged_cache(first, max_new_tokens, budget, samples)
         finished = torch.zeros(rows.shape[0], dtype=torch.bool, device=rows.device)
         ends = None
         if samples > 1:
             some = cache[:prompts]
-            first = [prompt] * prompts if lengths is None else lengths[::samples]
             n = torch.tensor(first, device=rows.device)
             some.expect(first)
             ids = rows[::samples].masked_fill(torch.arange(prompt, device=rows.device) >= n[:, None], 0)

@@ -199,6 +199,26 @@ def test_generate_samples():
     assert drawn.shape == (9, 36) and not torch.equal(drawn[0], drawn[1])
 
 
+def test_generate_samples_holds_what_is_shared_once(monkeypatch):
+    """The pool is of a prompt's whole pages once, and of each sample's own: enough for all, and all taken at the end (but for
+    the last token, which is not cached)."""
+    from sisa_amd import generation
+    made = []
+    monkeypatch.setattr(generation, "SISAPagedCache", lambda *a, **kw: made.append(SISAPagedCache(*a, **kw)) or made[-1])
+    model = _model64()
+    for lengths, n, new in (([300], 16, 5), ([64, 200, 1, 129], 3, 70), ([63, 128], 2, 1), ([128], 4, 65), ([130, 63], 5, 2)):
+        ids = token_ids(len(lengths), max(lengths), seed=9)
+        got = generate(model, ids, new, prompt_lengths=lengths, samples=n)
+        assert torch.equal(got, generate(model, ids, new, prompt_lengths=lengths).repeat_interleave(n, 0))
+        cache = next(c for c in made if len(c) == n * len(lengths))
+        made.clear()
+        most = sum(m // 64 + n * (-(-(m + new) // 64) - m // 64) for m in lengths)
+        held = sum(m // 64 + n * (-(-(m + new - 1) // 64) - m // 64) for m in lengths)
+        assert cache._store.pages == most and cache._store.pages - cache.free_pages == held
+    generate(model, ids, 3, samples=2)
+    assert made[0]._store.pages == 2 * (2 + 2 * 1)
+
+
 def test_generate_with_a_draft():
     model, ids, lengths = _model64(), token_ids(3, 24, seed=8), [24, 3, 11]
     small = tiny_model(seed=5, n_layer=1).double().eval()
