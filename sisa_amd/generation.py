@@ -298,6 +298,7 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
                                    (temperature, top_k) if do_sample else None, generator)
         return result if input_ids.dim() == 2 else result.squeeze(0)
     stop_ids = torch.tensor(stops, device=rows.device, dtype=rows.dtype) if stops else None
+    pad_unread = bool(stops) and not 0 <= stops[0] < model.config.vocab_size       # what finished rows are padded with is no token
     prompt, prompts = rows.shape[1], rows.shape[0]
     first = [prompt] * prompts if lengths is None else lengths
     if samples > 1:
@@ -347,6 +348,8 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
                 break
             if budget is not None and (length == prompt + 1 or cache.seq_len >= budget.keep + budget.slack):
                 cache.evict(budget.keep, budget.recent)
+            if pad_unread:
+                token = token.masked_fill(finished, 0)
             logits = model(token[:, None], cache=cache, logits_to_keep=1).logits[:, -1]
     result = out[:, :length].contiguous()
     return result if input_ids.dim() == 2 or samples > 1 else result.squeeze(0)
@@ -406,7 +409,7 @@ def _generate_drafted(model, draft, K: int, rows: Tensor, lengths: list[int] | N
         for i, row in enumerate(out):
             if done[i]:
                 counts.append(0)
-                got[i][0], took[i] = fill, 0
+                got[i][0], took[i] = 0, 0                  # read and not kept (the fill need not be a token)
                 continue
             if got[i][took[i]] < 0:
                 raise RuntimeError("generate: the model's probabilities are not finite, or 0 everywhere")

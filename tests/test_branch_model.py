@@ -296,6 +296,27 @@ def test_plain_verification_edges():
     assert none[0].tolist() == _want(p[:, :1], drafts[:, :0], u[:, 2:], q[:, :0])[0].tolist() and not none[1].any()
 
 
+@pytest.mark.parametrize("first", [-1, 300, 1 << 40])
+def test_ends_that_are_no_tokens(first):
+    """An end that is no token of the vocabulary (a tokenizer without one says -1) pads the rows that are done, and is never read:
+    neither where a draft lets some rows end before others, nor behind an end that is a token."""
+    model, ids, lengths = _model64(), token_ids(3, 24, seed=8), [24, 3, 11]
+    small = tiny_model(seed=5, n_layer=1).double().eval()
+    plain = generate(model, ids, 13)
+    for eos in (first, [first, int(plain[1, 28])]):
+        want = plain.clone()
+        if eos is not first:
+            for row in want:
+                hits = (row[24:] == eos[1]).nonzero()
+                if hits.numel():
+                    row[24 + int(hits[0]) + 1:] = first
+        for kw in ({}, dict(samples=2), dict(draft=small), dict(draft=model, draft_tokens=3), dict(cache_budget=200)):
+            got = generate(model, ids, 13, eos_token_id=eos, **kw)
+            assert torch.equal(got, want.repeat_interleave(kw.get("samples", 1), 0)), kw
+    ended = dict(prompt_lengths=lengths, eos_token_id=first)
+    assert torch.equal(generate(model, ids, 13, draft=small, **ended), generate(model, ids, 13, **ended))
+
+
 def test_generate_with_a_draft_ends_where_probabilities_are_not_finite():
     model, small, ids = _model64(), tiny_model(seed=5, n_layer=1).double().eval(), token_ids(2, 9, seed=8)
     kw = dict(do_sample=True, draft=small, draft_tokens=3, generator=torch.Generator().manual_seed(3))
