@@ -134,6 +134,15 @@ inline const char* pool_fault(const sisa_page_pool& p) {
     return nullptr;
 }
 
+// What attention over common positions asks of a pool beside: rows of a page behind each other, within 32-bit offsets.
+inline bool near_rows(const sisa_page_pool& p) {
+    auto ok = [&](const sisa_view& x, int width, int size) {
+        return x.sl >= width && x.sl <= 0x7fffff00 / ((int64_t)p.page_size * size);
+    };
+    const int es = elem_size(p.dtype);
+    return ok(p.k, 64, es) && ok(p.v, 64, es) && ok(p.b, 32, es) && ok(p.g, 1, 4) && (!p.f.ptr || ok(p.f, 1, 4));
+}
+
 }  // namespace sisa
 
 #define SISA_REQUIRE_POOL(name, pool)                                       \
@@ -141,3 +150,5 @@ inline const char* pool_fault(const sisa_page_pool& p) {
         const char* fault_ = ::sisa::pool_fault(pool);                      \
         SISA_REQUIRE(fault_ == nullptr, "%s: %s", name, fault_);            \
     } while (0)
+#define SISA_REQUIRE_NEAR_ROWS(name, pool)                                  \
+    SISA_REQUIRE(::sisa::near_rows(pool), "%s: the positions of a page must be at least a row apart, and all of a head's within 2 GiB", name)

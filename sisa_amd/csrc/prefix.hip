@@ -635,11 +635,6 @@ int launch(const sisa_prefix_decode_args* a, const Plan& p, hipStream_t st) {
     return a->out_dtype == SISA_F32 ? launch_join<T, float>(a, p, shift, ws, st) : launch_join<T, T>(a, p, shift, ws, st);
 }
 
-// Rows of a page that 32-bit offsets reach, each behind the last.
-bool rows_ok(const sisa_page_pool& p, const sisa_view& x, int width, int size) {
-    return x.sl >= width && (int64_t)p.page_size * x.sl * size <= 0x7fffff00;
-}
-
 bool sizes_ok(int64_t B, int64_t H, int64_t M, int64_t G, int64_t max_len, int64_t max_shared) {
     return B >= 1 && H >= 1 && M >= 1 && G >= 1 && G <= B && max_len >= 1 && max_len <= (1 << 30) && max_shared >= 0 &&
            max_shared <= (1 << 30) && B * M <= (1 << 28) / H;
@@ -667,11 +662,7 @@ extern "C" int sisa_prefix_decode(const sisa_prefix_decode_args* a, void* stream
                  "sisa_prefix_decode: null pointer");
     SISA_REQUIRE(a->workspace && sisa::aligned16(a->workspace), "sisa_prefix_decode: null workspace, or not 16-byte aligned");
     SISA_REQUIRE(a->out_dtype == SISA_F32 || a->out_dtype == a->pool.dtype, "sisa_prefix_decode: out_dtype");
-    const sisa_page_pool& P = a->pool;
-    const int es = sisa::elem_size(P.dtype);
-    SISA_REQUIRE(rows_ok(P, P.k, DH, es) && rows_ok(P, P.v, DH, es) && rows_ok(P, P.b, DS, es) && rows_ok(P, P.g, 1, 4) &&
-                     (!P.f.ptr || rows_ok(P, P.f, 1, 4)),
-                 "sisa_prefix_decode: the positions of a page must be at least a row apart, and all of a head's within 2 GiB");
+    SISA_REQUIRE_NEAR_ROWS("sisa_prefix_decode", a->pool);
     SISA_REQUIRE(sisa::view_ok(a->q, a->pool.dtype) && sisa::view_ok(a->c, a->pool.dtype),
                  "sisa_prefix_decode: q and c rows must be 16-byte aligned");
     SISA_REQUIRE(a->gq.ptr && (a->fq.ptr == nullptr) == (a->pool.f.ptr == nullptr),

@@ -814,6 +814,7 @@ extern "C" int sisa_step_branch(const sisa_step_branch_args* a, void* stream) {
     SISA_REQUIRE_POOL("sisa_step_branch", s->pool);
     SISA_REQUIRE(s->pool.heads == s->H && s->pool.dtype == s->dtype && s->pool.f.ptr,
                  "sisa_step_branch: the pool must have the layer's heads and dtype, and f");
+    SISA_REQUIRE_NEAR_ROWS("sisa_step_branch", s->pool);   // else the attention refuses once the rows are appended
     const int64_t held = (int64_t)s->W * s->pool.page_size;
     SISA_REQUIRE(s->W >= 1 && s->max_len >= 1 && s->max_len <= held && s->max_len <= (1 << 30) && a->max_shared >= 0 &&
                      a->max_shared <= held && a->max_shared <= (1 << 30) && a->G >= 1 && a->G <= s->B,

@@ -147,3 +147,16 @@ def test_python_calls_refuse_tensors_off_the_gpu(lib):
         sisa_verify_drafts_hip(p, drafts, u)
     with pytest.raises(ValueError, match="K \\+ 1"):
         sisa_verify_drafts_hip(p[:, :2], drafts, u)
+
+
+def test_step_refuses_what_its_attention_does(lib):
+    """A pool that the attention refuses is refused before the layer's rows are written, not after."""
+    from sisa_amd.kernels import _lib
+    none, far = _lib.View(None, 0, 0, 0), _lib.View(4096, 1 << 32, 1 << 31, 1 << 26)
+
+    def args(pool):
+        return _lib.StepBranchArgs(2, 2, 128, 256, _lib.BF16, 1, 16, 0, 1e-6, 1e-6, 4096, 128, None, 4096, 4096, *[4096] * 15, pool,
+                                   4096, 1, 4096, 4096, 4096, 4096, 4096, none, 4096, 4096, 4096, 3, 1, 16, 0, 4096, 4096, 4096, None, 0)
+    for bad in (dict(k=far), dict(v=far), dict(b=far), dict(g=_lib.View(4096, 32, 16, 1 << 25)), dict(f=_lib.View(4096, 32, 16, 0)),
+                dict(k=_lib.View(4096, 2048, 1024, 56)), dict(b=_lib.View(4096, 2048, 1024, 24))):
+        _refused(lib, "sisa_step_branch", args(_pool(**bad)), "a row apart")
