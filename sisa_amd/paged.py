@@ -34,6 +34,8 @@ __all__ = ["SISAPagedCache", "attention_weights", "paged_attention"]
 
 #: Scores of a call of the attention kernel over pages that several new positions take: about 5 bytes of workspace each.
 MAX_SCORES = 1 << 26
+#: Rows, of every head, of a call of the one over common positions: about 530 bytes of workspace each, at most 420 MB in all.
+MAX_ROWS = 1 << 19
 
 
 # ------------------------------------------------------------------------------------------------ plain forms
@@ -582,19 +584,22 @@ class SISAPagedCache:
 
         st, lo, hi = self._store, self._lo, self._hi
         table, lengths, longest, (B, H, M, _) = st.table[lo:hi], st.end[lo:hi], self.seq_len, p.q.shape
+
+        def parts(rows: int, attend) -> Tensor:
+            """Some of the new rows at a time, for which the sequences end with the last of them."""
+            if rows >= M:
+                return attend(p.q, p.c, p.g, p.fgate, lengths)
+            return torch.cat([attend(*(t[:, :, m:m + rows] for t in (p.q, p.c, p.g, p.fgate)), lengths - max(0, M - m - rows))
+                              for m in range(0, M, rows)], 2)
+
         sharing = None if weights is not None else self._sharing()
         if sharing is not None:
             from .kernels.prefix import sisa_prefix_decode_hip
 
-            return sisa_prefix_decode_hip(p.q, p.c, p.g, p.fgate, lam, pool, table, lengths, sharing.groups, sharing.shared,
-                                          max_len=longest, max_shared=sharing.most)
-        rows = max(1, MAX_SCORES // (B * H * longest))
-        if rows >= M:
-            return sisa_paged_decode_hip(p.q, p.c, p.g, p.fgate, lam, pool, table, lengths, max_len=longest, weights=weights)
-        # the workspace grows with the rows' scores: some rows at a time, for which the sequences end with the last of them
-        return torch.cat([sisa_paged_decode_hip(*(t[:, :, m:m + rows] for t in (p.q, p.c, p.g, p.fgate)), lam, pool, table,
-                                                lengths - max(0, M - m - rows), max_len=longest, weights=weights)
-                          for m in range(0, M, rows)], 2)
+            return parts(max(1, MAX_ROWS // (B * H)), lambda q, c, g, f, ends: sisa_prefix_decode_hip(
+                q, c, g, f, lam, pool, table, ends, sharing.groups, sharing.shared, max_len=longest, max_shared=sharing.most))
+        return parts(max(1, MAX_SCORES // (B * H * longest)), lambda q, c, g, f, ends: sisa_paged_decode_hip(
+            q, c, g, f, lam, pool, table, ends, max_len=longest, weights=weights))
 
     def receive(self, layer_idx: int, q: Tensor, k: Tensor, c: Tensor, b: Tensor, g: Tensor, lam: Tensor, fgate: Tensor,
                 hip: bool) -> None:

@@ -484,3 +484,32 @@ def test_a_step_that_fails_is_taken_back(monkeypatch):
         monkeypatch.setattr(step, "_step_branch", real)
         got = [model(tokens[:, t:t + 1], cache=caches[1]).logits for t in range(3)]
     assert torch.equal(torch.cat(got, 1), torch.cat(want, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tentative", [False, True])
+def test_many_new_positions_in_parts(tentative, monkeypatch):
+    """Twenty positions behind branches of ragged prompts, and behind single sequences that can go back, three at a time, against
+    the model's float64 copy; the bound as above."""
+    from sisa_amd import paged
+    from sisa_amd.kernels import prefix
+    model = tiny_model(seed=3, theta_scale=0.25, attn_impl="auto").to(DEV).eval()
+    ref = tiny_model(seed=3, theta_scale=0.25).eval()
+    ref.load_state_dict({n: t.cpu() for n, t in model.state_dict().items()})
+    ref = ref.double()
+    prompts, more, lengths, n = token_ids(2, 40, seed=11), token_ids(4, 20, seed=12), [40, 17], 1 if tentative else 2
+    monkeypatch.setattr(paged, "MAX_ROWS", 3 * 2 * n * model.config.n_head + 1)
+    calls, real = [], prefix.sisa_prefix_decode_hip
+    monkeypatch.setattr(prefix, "sisa_prefix_decode_hip", lambda q, *a, **kw: calls.append(q.shape[2]) or real(q, *a, **kw))
+    outs = []
+    with torch.no_grad():
+        for m, dev in ((model, DEV), (ref, "cpu")):
+            cache, _ = _branched(m, prompts.to(dev), lengths, n)
+            if tentative:
+                cache.tentative(20)
+            outs.append(m(more[:2 * n].to(dev), cache=cache).logits.cpu())
+            if tentative:
+                cache.keep([11, 20])
+            outs.append(m(more[:2 * n, :1].to(dev), cache=cache).logits.cpu())
+    assert calls[:14] == [3, 3, 3, 3, 3, 3, 2] * 2 and set(calls[14:]) <= {1}
+    assert rel_err(outs[0], outs[2]) <= 2e-5 and rel_err(outs[1], outs[3]) <= 2e-5
