@@ -173,10 +173,6 @@ class _Sharing(NamedTuple):
     most: int
 
 
-#: What the recurrences continue from, of a sequence and head: g, F and the phases.
-_ROW = 2 + HIP_D_STATE // 2
-
-
 class _Trial:
     """Positions that may be taken back: the sequences, how many positions there can be, where they begin, and per layer
     ``(sequences, H, room + 1, 2 + d_state // 2)`` what the recurrences continue from before the first and after each."""
