@@ -606,3 +606,46 @@ def test_rows_far_apart_in_pages_of_16(wide, dtype):
     far = far.as_strided(t.shape, (H * width, width, (1 << 20) // t.element_size(), *t.stride()[3:])).copy_(t)
     case.pool = PagePool(*(far if x == wide else case.t[x] for x in ("k", "v", "b", "g", "f")))
     assert torch.equal(case.run(*rows), plain)
+
+
+def test_two_graphs_and_eager_calls():
+    """Two graphs of the same calls on the same tensors, one over fewer groups, replayed in either order with eager calls between and
+    beside them: each one's answers are those of the eager calls on what the tensors hold then, after the other's replay, too."""
+    case = Grouped([3, 2], [70, 20], [10, 20, 30, 6, 50], 2, 16, torch.bfloat16, seed=16)
+    q, c, g, f = case.queries(4)
+    p, drafts, u, draft_p = _drafted(case.B, 3, 2500, torch.float32, None, seed=17)
+    shared, fewer, lengths = _ints([70, 20]), _ints([70, 16]), _ints(case.lengths)
+    from sisa_amd.kernels.prefix import sisa_prefix_decode_hip
+
+    def step(common, n):
+        got = _verify(p[:n], drafts[:n], u[:n], draft_p[:n])
+        out = sisa_prefix_decode_hip(q, c, g, f, case.lam, case.pool, case.table, lengths, case.groups, common)
+        return out, got.tokens, got.accepted
+    calls = [(shared, case.B), (fewer, 2)]
+    for x, t in case.t.items():                           # positions 16 .. 19 of the last sequence in its own page, too
+        t[int(case.table[4, 1]), :, :4] = case.rows[x][4, :, 16:20]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for call in calls:
+            step(*call)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in calls], []
+    for graph, call in zip(graphs, calls):
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step(*call))
+    seen = []
+    for turn in range(4):
+        q.copy_(torch.randn(q.shape, generator=case.gen, device=DEV))
+        u.uniform_(generator=case.gen)
+        lengths.copy_(_ints([n - turn for n in case.lengths]))
+        for i in (0, 1) if turn % 2 else (1, 0):
+            graphs[i].replay()
+            step(*calls[1 - i])
+        want = [step(*call) for call in calls]
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert got[0].isfinite().all() and all(torch.equal(x, y) for x, y in zip(got, ref))
+        seen.append(outs[0][0].clone())
+    assert not any(torch.equal(x, y) for x, y in zip(seen, seen[1:]))
