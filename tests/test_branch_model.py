@@ -296,6 +296,28 @@ def test_plain_verification_edges():
     assert none[0].tolist() == _want(p[:, :1], drafts[:, :0], u[:, 2:], q[:, :0])[0].tolist() and not none[1].any()
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param(DEV, marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("k", [1, 3])
+def test_drafted_samples_are_the_models(k, device):
+    """Three tokens of 4,000 rows behind one prompt, drawn with a draft that thinks otherwise, against the model's probabilities
+    of all 125 continuations. A share x of n rows has the standard deviation sqrt(x (1 - x) / n): six of them (chances of 2e-9 a
+    cell), and a row for cells of next to no weight."""
+    n, V = 4000, 5
+    model = tiny_model(seed=3, theta_scale=0.25, vocab_size=V, attn_impl="auto").to(device).eval()
+    small = tiny_model(seed=5, n_layer=1, vocab_size=V, attn_impl="auto").to(device).eval()
+    prompt = torch.tensor([[1, 4, 0, 2, 2, 3, 1]], device=device)
+    every = torch.cartesian_prod(*[torch.arange(V, device=device)] * 3)
+    with torch.no_grad():
+        behind = torch.cat([prompt.expand(len(every), -1), every], 1)
+        p, other = (m(behind).logits[:, -4:-1].float().div(0.7).softmax(-1).gather(2, every[..., None])[..., 0] for m in (model, small))
+    assert (p[:, 0] - other[:, 0]).abs().max() > 0.05     # else nothing would be refused
+    want = p.prod(1)
+    got = generate(model, prompt.expand(n, -1), 3, do_sample=True, temperature=0.7, draft=small, draft_tokens=k,
+                   generator=torch.Generator(device).manual_seed(4))[:, 7:]
+    share = torch.bincount((got * torch.tensor([V * V, V, 1], device=device)).sum(1), minlength=V ** 3) / n
+    assert ((share - want).abs() <= 6 * (want * (1 - want) / n).sqrt() + 1 / n).all()
+
+
 @pytest.mark.parametrize("first", [-1, 300, 1 << 40])
 def test_ends_that_are_no_tokens(first):
     """An end that is no token of the vocabulary (a tokenizer without one says -1) pads the rows that are done, and is never read:
