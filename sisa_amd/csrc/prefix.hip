@@ -13,9 +13,11 @@
 // weights enter their product as a sum of two (fp16) or three (bf16) operands, so that the result is an fp32 one: rounded once
 // to bf16 they would be off by 2^-9.
 //
-// Both launches, from a kernel trace, bf16: 64 rows against 16,384 common positions of 12 heads 41 us (114 MB at 2.8 TB/s; a
-// copy reaches 4.8), 24 x 8 drafts against up to 6,000 46 us (169 MB, 3.7 TB/s), 256 rows against 1,500 and up to 1,000 of
-// their own 60 us. What a wave holds is kept few enough for four waves a SIMD, strides and bases in scalar registers. The first
+// Both launches, from a kernel trace, bf16: 64 rows against 16,384 common positions of 12 heads 41 us (114 MB at 2.8 TB/s; reading
+// alone reaches 7.1), 24 x 8 drafts against up to 6,000 46 us (169 MB, 3.7 TB/s), 256 rows against 1,500 and up to 1,000 of
+// their own 60 us. What bounds the first launch of the 64 rows is the L1, which serves four waves that each load the same rows
+// (52,000 accesses a CU in 67,000 cycles; VALU 46 %, matrix cores 12 %); that of the drafts, waves that wait for their one tile
+// (45 % of their cycles). What a wave holds is kept few enough for four waves a SIMD, strides and bases in scalar registers. The first
 // launch for the 64 rows: 64 rows to a wave, 256 registers 91 us; 16 rows to a wave, 168 registers 41; this form 34. A head's
 // positions are read beside the other heads', whose rows follow in memory: with each head by itself an earlier form of the
 // loads took 47 us there, against 36.

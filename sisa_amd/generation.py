@@ -252,8 +252,8 @@ def generate(model: "SISAForCausalLM", input_ids: Tensor, max_new_tokens: int, t
     """Continue the prompts ``input_ids`` (``(B, L)`` of equal-length rows, or ``(L,)``) by up to ``max_new_tokens``
     tokens: greedy, or sampled at ``temperature`` from the ``top_k`` most likely tokens with ``do_sample``.
 
-    A row that emits an ``eos_token_id`` is finished and padded with the first such id from then on; generation
-    ends when every row is finished. Returns ``(B, L + n)`` ids, ``n <= max_new_tokens``, with the rank of
+    A row that emits an ``eos_token_id`` is finished and padded with the first such id (which need not be a token) from then on;
+    generation ends when every row is finished. Returns ``(B, L + n)`` ids, ``n <= max_new_tokens``, with the rank of
     ``input_ids``.
 
     ``prompt_lengths``: the prompts are right-padded rows of these lengths (with anything). A row's tokens follow its prompt, and what is
